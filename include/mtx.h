@@ -315,6 +315,87 @@ int mtx_decode_qkv_attn_f32(int B, int H, int D, const float* x, int64_t ldx, co
                             float scale, float* o, int64_t ldo, void* stream);
 
 /*
+ * Keys and values in pages.  A pool holds n_pages pages of `page` rows for each
+ * of Hkv K/V heads: k_pages and v_pages are (n_pages, Hkv, page, D) views (four
+ * element strides each, unit d stride, the others multiples of 16 bytes), so
+ * pools stored by heads and by rows ((n_pages, page, Hkv, D)) both pass.  table
+ * is device int32 (B, max_pages), row stride table_ld: row j of sequence b lies
+ * in page table[b][j / page] at row j % page.  lengths is device int32 (B); a
+ * length counts at most max_pages * page rows.  Page ids and lengths are read on
+ * the device (a recorded launch follows them): a row whose page id is outside
+ * [0, n_pages) is not there -- attention does not see it and nothing is written
+ * to it.  D in {16, 32, 64, 128}.  dtype is that of the rows outside the cache
+ * (new rows, q, o), cache_dtype the pool's: fp32 over fp32 or bf16, bf16 over
+ * bf16.  (The reference has no cache: GPT.generate recomputes the whole context
+ * per token, transformer.py:93-104.)
+ */
+/*
+ * Append: rows of T new tokens, k and v (B, Hkv, T, D) views, to the end of each
+ * sequence's pages.  lengths[b] counts the new rows already; with counts (device
+ * int32 (B), may be NULL: T) sequence b appends its first min(counts[b], T) rows
+ * and the others are skipped: new row i goes to cached row lengths[b] - n_b + i.
+ * Rows that fall before row 0 or behind the sequence's pages are skipped.  Two
+ * sequences that list one page both write to it: shared pages belong before the
+ * rows that are appended.  fp32 rows are rounded to nearest even into a bf16
+ * pool.  Replaces, for paged decoding, mtx_kv_append_f32.
+ */
+int mtx_kv_append_paged(int dtype, int cache_dtype, int B, int T, int Hkv, int D, const void* k,
+                        const int64_t* k_strides, const void* v, const int64_t* v_strides, int64_t n_pages,
+                        int page, void* k_pages, const int64_t* kp_strides, void* v_pages,
+                        const int64_t* vp_strides, const int* table, int64_t table_ld, int max_pages,
+                        const int* lengths, const int* counts, void* stream);
+
+/*
+ * Attention of one new token per sequence over its cached rows (the
+ * sub-graph of transformer.py:36-44 at the last position): q and o are
+ * (B, H, 1, D) views, H a multiple of Hkv; query head h reads K/V head
+ * h / (H / Hkv).  s_j = scale * q.k_j, lse = log sum_j exp(s_j) (fp32 (B, H)
+ * contiguous, may be NULL), o = sum_j exp(s_j - lse) v_j over the rows
+ * j < lengths[b] that are there; a sequence without any gets o = 0 and
+ * lse = -inf.  Rows that are not seen may hold anything, NaN included.
+ * weights (may be NULL): fp32 (B, Hkv, weights_ld) contiguous, weights_ld >=
+ * max_pages * page; for j < lengths[b]
+ *   weights[b][hk][j] = weights_in[b][hk][j] + sum over hk's query heads of
+ *                       exp(s_j - lse)
+ * and the other entries are left as they were.  weights_in NULL counts as 0; it
+ * may be `weights` itself, which then accumulates over calls (what
+ * mtx_kv_evict_paged goes by).  A workspace of
+ * mtx_attn_decode_paged_workspace_bytes() bytes, 16-byte aligned, is written by
+ * the call and free after it; calls that overlap need their own.  Deterministic.
+ */
+size_t mtx_attn_decode_paged_workspace_bytes(int B, int H, int Hkv, int D, int page, int max_pages,
+                                             int with_weights);
+int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, int Hkv, int D, const void* q,
+                          const int64_t* q_strides, int64_t n_pages, int page, const void* k_pages,
+                          const int64_t* kp_strides, const void* v_pages, const int64_t* vp_strides,
+                          const int* table, int64_t table_ld, int max_pages, const int* lengths, void* o,
+                          const int64_t* o_strides, float* lse, const float* weights_in, float* weights,
+                          int64_t weights_ld, void* workspace, size_t workspace_bytes, float scale, void* stream);
+
+/*
+ * Eviction: each sequence longer than `keep` rows keeps, for each K/V head by
+ * itself, its last `recent` rows and the keep - recent rows of greatest weight
+ * among the others (ties: the lowest row; NaN counts above every number); a
+ * shorter one keeps all its rows.  The kept rows are written, in their order, to
+ * rows 0, 1, ... of the pages of to_table (int32 (B, to_pages), row stride
+ * to_ld; to_pages * page >= min(keep, max_pages * page)), which must not be
+ * among the pages the tables of the call read: the old pages stay as they are
+ * and may be shared.  The order of cached rows does not matter to attention, and
+ * a head's row i need not be another head's token.  Written besides:
+ *   lengths_out[b] = min(lengths[b], keep);
+ *   weights_out (laid out as weights): the kept rows' weights, then 0;
+ *   slots (B, Hkv, keep): the rows they came from, ascending, then -1.
+ * lengths_out, weights_out and to_table are other memory than lengths, weights
+ * and table.  A kept row that is not there becomes zeros; one whose new page is
+ * not there is dropped.
+ */
+int mtx_kv_evict_paged(int cache_dtype, int B, int Hkv, int D, int64_t n_pages, int page, void* k_pages,
+                       const int64_t* kp_strides, void* v_pages, const int64_t* vp_strides, const int* table,
+                       int64_t table_ld, int max_pages, const int* lengths, const float* weights,
+                       int64_t weights_ld, const int* to_table, int64_t to_ld, int to_pages, int keep, int recent,
+                       int* lengths_out, float* weights_out, int* slots, void* stream);
+
+/*
  * Greedy pick over rows of x (rows, cols; row stride ld): idx[r * idx_stride]
  * = first index of the row maximum (np.argmax, the build's greedy harness over
  * the logits of transformer.py:97-98) and, if margin != NULL,
@@ -718,6 +799,37 @@ int mtx_xent_fwd_f32(const float* logits, int64_t ld, const int64_t* labels, flo
 int mtx_xent_bwd_f32(const float* logits, int64_t ld, const int64_t* labels, const float* lse,
                      const float* gscalar, float scale, float* dlogits, int64_t ldd, int64_t rows, int V,
                      int accumulate, void* stream);
+
+/*
+ * Log probabilities of given tokens (log_softmax, functional.py:81-97, at the
+ * tokens; generation samples from softmax(logits / temperature),
+ * transformer.py:97-100, scale = 1 / temperature).  With x = scale * logits[r]
+ * (rows x V, row stride ld, fp32 or bf16):
+ *   lse = log sum exp x;  logprob = x[token] - lse;  entropy = -sum p log p;
+ *   top_ids, top_logprobs (rows, top): the `top` <= 64 largest logits, largest
+ *   first, ties to the lowest id (NaN counts above every number), and their log
+ *   probabilities.  top may be 0.
+ * A logit of -inf has probability 0 and adds nothing to the entropy; a row of
+ * nothing else gets lse, log probabilities -inf and entropy 0.  A row whose token
+ * is outside [0, V) has no token: logprob 0.  Workspace:
+ * mtx_token_logprobs_workspace_bytes() bytes, 16-byte aligned, free after the
+ * call; calls that overlap need their own.  Deterministic.
+ */
+size_t mtx_token_logprobs_workspace_bytes(int64_t rows, int V, int top);
+int mtx_token_logprobs(int dtype, int64_t rows, int V, const void* logits, int64_t ld, const int64_t* tokens,
+                       float scale, float* logprob, float* lse, float* entropy, int top, int64_t* top_ids,
+                       float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * Its gradient, from the upstream gradients of logprob and entropy (fp32 (rows),
+ * either may be NULL: 0) and the forward's lse and entropy:
+ *   dlogits[r][v] = scale * (g_logprob (1[v = token] - p_v)
+ *                            - g_entropy p_v (log p_v + entropy))   (fp32)
+ * added to dlogits when accumulate != 0.  Rows without a token have no
+ * g_logprob term, entries of probability 0 no gradient but the token's own.
+ */
+int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void* logits, int64_t ld, const int64_t* tokens,
+                           const float* lse, const float* entropy, const float* g_logprob, const float* g_entropy,
+                           float scale, float* dlogits, int64_t ldd, int accumulate, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Embedding and optimizer                                                  */

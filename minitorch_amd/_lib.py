@@ -92,6 +92,13 @@ SIGNATURES = {
     "mtx_attn_decode": (_I, [_I, _I, _I, _I, _I,
                              _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P,
                              _P, _P, _F, _P]),
+    "mtx_kv_append_paged": (_I, [_I] * 6 + [_P, _I64P, _P, _I64P, _I64, _I, _P, _I64P, _P, _I64P, _P, _I64, _I,
+                                            _P, _P, _P]),
+    "mtx_attn_decode_paged_workspace_bytes": (_SZ, [_I] * 7),
+    "mtx_attn_decode_paged": (_I, [_I] * 6 + [_P, _I64P, _I64, _I, _P, _I64P, _P, _I64P, _P, _I64, _I, _P,
+                                              _P, _I64P, _P, _P, _P, _I64, _P, _SZ, _F, _P]),
+    "mtx_kv_evict_paged": (_I, [_I] * 4 + [_I64, _I, _P, _I64P, _P, _I64P, _P, _I64, _I, _P, _P, _I64, _P, _I64,
+                                           _I, _I, _I, _P, _P, _P, _P]),
     "mtx_argmax_f32": (_I, [_I, _I, _P, _I64, _P, _I64, _P, _I64, _P]),
     "mtx_kv_append_f32": (_I, [_I, _I, _I, _P, _I64, _P, _I64, _I64, _P, _P]),
     "mtx_decode_advance": (_I, [_I, _P, _P, _P]),
@@ -145,6 +152,9 @@ SIGNATURES = {
     "mtx_gelu_bwd_f32": (_I, [_P, _P, _P, _I64, _I, _P]),
     "mtx_xent_fwd_f32": (_I, [_P, _I64, _P, _P, _P, _I64, _I, _P]),
     "mtx_xent_bwd_f32": (_I, [_P, _I64, _P, _P, _P, _F, _P, _I64, _I64, _I, _I, _P]),
+    "mtx_token_logprobs_workspace_bytes": (_SZ, [_I64, _I, _I]),
+    "mtx_token_logprobs": (_I, [_I, _I64, _I, _P, _I64, _P, _F, _P, _P, _P, _I, _P, _P, _P, _SZ, _P]),
+    "mtx_token_logprobs_bwd": (_I, [_I, _I64, _I, _P, _I64, _P, _P, _P, _P, _P, _F, _P, _I64, _I, _P]),
     "mtx_embedding_fwd_f32": (_I, [_P, _I64, _I64, _P, _I64, _P, _I64, _I, _P]),
     "mtx_embedding_bwd_f32": (_I, [_P, _I64, _P, _I64, _P, _I64, _I64, _I, _I, _P]),
     "mtx_adam_blocks": (_I, [_I64P, _I, _I64P, _I64P]),

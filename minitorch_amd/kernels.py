@@ -160,6 +160,144 @@ def attn_decode(q, k, v, scale: float, out=None, lse=None, lengths=None):
     return out, lse
 
 
+# ---------------------------------------------------------------------------
+# keys and values in pages
+# ---------------------------------------------------------------------------
+
+def _paged(k_pages, v_pages, table, lengths):
+    """(n_pages, Hkv, page, D, B) of a paged cache, checked: two
+    (n_pages, Hkv, page, D) views of one dtype, an int32 (B, max_pages) table
+    with contiguous rows and int32 (B,) lengths."""
+    _need_cuda(k_pages, v_pages, table, lengths)
+    if len(k_pages.shape) != 4 or tuple(k_pages.shape) != tuple(v_pages.shape) or _dt(k_pages) != _dt(v_pages):
+        raise ValueError("k_pages and v_pages must be (n_pages, Hkv, page, D) views of one shape and dtype")
+    if _dt(table) != "int32" or len(table.shape) != 2 or table.stride(1) != 1:
+        raise ValueError("table must be int32 (B, max_pages) with contiguous rows")
+    B = table.shape[0]
+    if _dt(lengths) != "int32" or tuple(lengths.shape) != (B,) or not lengths.is_contiguous():
+        raise ValueError(f"lengths must be contiguous int32 ({B},)")
+    return (*k_pages.shape, B)
+
+
+def _row_weights(name, w, B, Hkv, cap):
+    """Checks weights of cached rows: contiguous fp32 (B, Hkv, >= cap)."""
+    _need_cuda(w)
+    if _dt(w) != "float32" or len(w.shape) != 3 or tuple(w.shape[:2]) != (B, Hkv) or w.shape[2] < cap \
+            or not w.is_contiguous():
+        raise ValueError(f"{name} must be contiguous fp32 ({B}, {Hkv}, >= {cap})")
+
+
+def kv_append_paged(k, v, k_pages, v_pages, table, lengths, counts=None):
+    """Write the keys and values of T new tokens per sequence, k and v
+    (B, Hkv, T, D) views, to the end of its pages (mtx_kv_append_paged).
+    lengths (B,) counts them already; counts (int32 (B,)): sequence b appends
+    only its first counts[b] rows.  fp32 rows may go to a bf16 pool."""
+    n_pages, Hkv, page, D, B = _paged(k_pages, v_pages, table, lengths)
+    _need_cuda(k, v)
+    _bhtd("k", k)
+    _bhtd("v", v)
+    T = k.shape[2]
+    if tuple(k.shape) != (B, Hkv, T, D) or tuple(v.shape) != (B, Hkv, T, D) or _dt(k) != _dt(v):
+        raise ValueError(f"k and v must be ({B}, {Hkv}, T, {D}) of one dtype (got {tuple(k.shape)}, {tuple(v.shape)})")
+    if counts is not None:
+        _need_cuda(counts)
+        if _dt(counts) != "int32" or tuple(counts.shape) != (B,) or not counts.is_contiguous():
+            raise ValueError(f"counts must be contiguous int32 ({B},)")
+    L.call("mtx_kv_append_paged", L.dtype_code(k), L.dtype_code(k_pages), B, T, Hkv, D, L.ptr(k), L.strides(k),
+           L.ptr(v), L.strides(v), n_pages, page, L.ptr(k_pages), L.strides(k_pages), L.ptr(v_pages),
+           L.strides(v_pages), L.ptr(table), table.stride(0), table.shape[1], L.ptr(lengths),
+           L.ptr(counts) if counts is not None else None, L.stream_handle())
+
+
+@functools.lru_cache(maxsize=512)
+def _decode_paged_workspace_bytes(*sizes):
+    """mtx_attn_decode_paged_workspace_bytes, a function of the sizes alone."""
+    return L.lib().mtx_attn_decode_paged_workspace_bytes(*sizes)
+
+
+def attn_decode_paged(q, k_pages, v_pages, table, lengths, scale: float, out=None, lse=None, weights=None,
+                      weights_in=None):
+    """Attention of one new token per sequence over its pages
+    (mtx_attn_decode_paged): q (B, H, 1, D), H a multiple of the pool's Hkv,
+    fp32 or bf16 over a pool of the same dtype or fp32 over bf16.  weights
+    (B, Hkv, >= max_pages * page) fp32: receives weights_in (0 without it; it
+    may be weights itself) plus the attention each cached row got.  Returns
+    (out like q, lse or None)."""
+    n_pages, Hkv, page, D, B = _paged(k_pages, v_pages, table, lengths)
+    _need_cuda(q)
+    _bhtd("q", q)
+    H = q.shape[1]
+    if tuple(q.shape) != (B, H, 1, D):
+        raise ValueError(f"q must be ({B}, H, 1, {D}) (got {tuple(q.shape)})")
+    if out is None:
+        out = dev.empty_buf((B, H, 1, D), _dt(q))
+    _need_cuda(out)
+    _bhtd("out", out)
+    if tuple(out.shape) != (B, H, 1, D) or _dt(out) != _dt(q):
+        raise ValueError("out must have q's shape and dtype")
+    if lse is not None:
+        _need_cuda(lse)
+        if not lse.is_contiguous() or tuple(lse.shape) != (B, H) or _dt(lse) != "float32":
+            raise ValueError("lse must be a contiguous fp32 (B,H) tensor")
+    width = table.shape[1]
+    wld = 0
+    if weights is not None:
+        _row_weights("weights", weights, B, Hkv, width * page)
+        wld = weights.shape[2]
+        if weights_in is not None:
+            _row_weights("weights_in", weights_in, B, Hkv, width * page)
+            if tuple(weights_in.shape) != tuple(weights.shape):
+                raise ValueError("weights_in must have weights' shape")
+    elif weights_in is not None:
+        raise ValueError("weights_in without weights")
+    ws_bytes = _decode_paged_workspace_bytes(B, H, Hkv, D, page, width, int(weights is not None))
+    ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
+    L.call("mtx_attn_decode_paged", L.dtype_code(q), L.dtype_code(k_pages), B, H, Hkv, D, L.ptr(q), L.strides(q),
+           n_pages, page, L.ptr(k_pages), L.strides(k_pages), L.ptr(v_pages), L.strides(v_pages), L.ptr(table),
+           table.stride(0), width, L.ptr(lengths), L.ptr(out), L.strides(out),
+           L.ptr(lse) if lse is not None else None, L.ptr(weights_in) if weights_in is not None else None,
+           L.ptr(weights) if weights is not None else None, wld, L.ptr(ws) if ws is not None else None, ws_bytes,
+           float(scale), L.stream_handle())
+    return out, lse
+
+
+def kv_evict_paged(k_pages, v_pages, table, lengths, weights, to_table, keep: int, recent: int, lengths_out=None,
+                   weights_out=None, slots=None):
+    """Cut each sequence and K/V head down to its last `recent` rows and the
+    keep - recent others of greatest weight, written in order to the pages of
+    to_table (mtx_kv_evict_paged): int32 (B, to_pages), pages of the same pool
+    that no table of the call reads.  weights as attn_decode_paged accumulates
+    them.  Returns (lengths_out (B,), weights_out like weights, slots
+    (B, Hkv, keep) int32: the rows kept, then -1)."""
+    n_pages, Hkv, page, D, B = _paged(k_pages, v_pages, table, lengths)
+    width, keep = table.shape[1], int(keep)
+    _row_weights("weights", weights, B, Hkv, width * page)
+    _need_cuda(to_table)
+    if _dt(to_table) != "int32" or len(to_table.shape) != 2 or to_table.shape[0] != B or to_table.stride(1) != 1:
+        raise ValueError(f"to_table must be int32 ({B}, to_pages) with contiguous rows")
+    if keep < 1:
+        raise ValueError("keep must be at least 1")
+    if lengths_out is None:
+        lengths_out = dev.empty_buf((B,), "int32")
+    if weights_out is None:
+        weights_out = dev.empty_buf(weights.shape, "float32")
+    if slots is None:
+        slots = dev.empty_buf((B, Hkv, keep), "int32")
+    _need_cuda(lengths_out, slots)
+    _row_weights("weights_out", weights_out, B, Hkv, width * page)
+    if tuple(weights_out.shape) != tuple(weights.shape):
+        raise ValueError("weights_out must have weights' shape")
+    if _dt(lengths_out) != "int32" or tuple(lengths_out.shape) != (B,) or not lengths_out.is_contiguous():
+        raise ValueError(f"lengths_out must be contiguous int32 ({B},)")
+    if _dt(slots) != "int32" or tuple(slots.shape) != (B, Hkv, keep) or not slots.is_contiguous():
+        raise ValueError(f"slots must be contiguous int32 ({B}, {Hkv}, {keep})")
+    L.call("mtx_kv_evict_paged", L.dtype_code(k_pages), B, Hkv, D, n_pages, page, L.ptr(k_pages),
+           L.strides(k_pages), L.ptr(v_pages), L.strides(v_pages), L.ptr(table), table.stride(0), width,
+           L.ptr(lengths), L.ptr(weights), weights.shape[2], L.ptr(to_table), to_table.stride(0), to_table.shape[1],
+           keep, int(recent), L.ptr(lengths_out), L.ptr(weights_out), L.ptr(slots), L.stream_handle())
+    return lengths_out, weights_out, slots
+
+
 DECODE_STEP_WIDTHS = (128, 256, 384, 512)
 _DECODE_LAYER_KEYS = ("ln1_gamma", "ln1_beta", "w_qkv", "b_qkv", "w_out", "b_out", "ln2_gamma", "ln2_beta",
                       "w_fc1", "b_fc1", "w_fc2", "b_fc2", "k_cache", "v_cache")
@@ -940,6 +1078,85 @@ def xent_bwd(logits, labels, lse, gscalar, scale, dlogits, accumulate=False):
     _, _, ldd = _rows(dlogits)
     L.call("mtx_xent_bwd_f32", L.ptr(logits), ld, L.ptr(labels), L.ptr(lse), L.ptr(gscalar),
            float(scale), L.ptr(dlogits), ldd, r, V, int(bool(accumulate)), L.stream_handle())
+
+
+TOP_MAX = 64  # alternatives per row of token_logprobs
+
+
+@functools.lru_cache(maxsize=512)
+def _logprobs_workspace_bytes(rows, V, top):
+    """mtx_token_logprobs_workspace_bytes, a function of the sizes alone."""
+    return L.lib().mtx_token_logprobs_workspace_bytes(rows, V, top)
+
+
+def _logits_rows(logits, tokens, **vectors):
+    """(rows, V, ld) of (rows, V) logits, checked with the int64 (rows,)
+    tokens and fp32 (rows,) vectors (None: not there) that go with them."""
+    _need_cuda(logits, tokens)
+    if len(logits.shape) != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be (rows, V) with contiguous rows")
+    rows, V = logits.shape
+    if _dt(tokens) != "int64" or tuple(tokens.shape) != (rows,) or not tokens.is_contiguous():
+        raise ValueError(f"tokens must be contiguous int64 ({rows},)")
+    for name, t in vectors.items():
+        if t is None:
+            continue
+        _need_cuda(t)
+        if _dt(t) != "float32" or tuple(t.shape) != (rows,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous fp32 ({rows},)")
+    return rows, V, logits.stride(0)
+
+
+def token_logprobs(logits, tokens, top: int = 0, scale: float = 1.0, logprob=None, entropy=None, lse=None,
+                   top_ids=None, top_logprobs=None):
+    """Log probabilities of one token per row of logits (rows, V), fp32 or
+    bf16, at scale * logits, the entropy, and the `top` (<= 64) most likely
+    tokens with theirs, ties to the lowest id (mtx_token_logprobs).  A token
+    outside [0, V) means the row has none (logprob 0).  Returns (logprob,
+    entropy, lse) fp32 (rows,), top_ids int64 and top_logprobs fp32
+    (rows, top)."""
+    top = int(top)
+    rows, V, ld = _logits_rows(logits, tokens, logprob=logprob, entropy=entropy, lse=lse)
+    logprob, entropy, lse = (dev.empty_buf((rows,), "float32") if t is None else t for t in (logprob, entropy, lse))
+    if not 0 <= top <= min(V, TOP_MAX):
+        raise ValueError(f"top must be between 0 and {min(V, TOP_MAX)} (got {top})")
+    if top_ids is None:
+        top_ids = dev.empty_buf((rows, top), "int64")
+    if top_logprobs is None:
+        top_logprobs = dev.empty_buf((rows, top), "float32")
+    for name, t, dt in (("top_ids", top_ids, "int64"), ("top_logprobs", top_logprobs, "float32")):
+        _need_cuda(t)
+        if _dt(t) != dt or tuple(t.shape) != (rows, top) or (top and rows and not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {dt} ({rows}, {top})")
+    if rows:
+        ws_bytes = _logprobs_workspace_bytes(rows, V, top)
+        ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
+        L.call("mtx_token_logprobs", L.dtype_code(logits), rows, V, L.ptr(logits), ld, L.ptr(tokens), float(scale),
+               L.ptr(logprob), L.ptr(lse), L.ptr(entropy), top, L.ptr(top_ids) if top else None,
+               L.ptr(top_logprobs) if top else None, L.ptr(ws) if ws is not None else None, ws_bytes,
+               L.stream_handle())
+    return logprob, entropy, lse, top_ids, top_logprobs
+
+
+def token_logprobs_bwd(logits, tokens, lse, entropy, g_logprob, g_entropy, scale: float = 1.0, dlogits=None,
+                       accumulate: bool = False):
+    """The logits' gradient from those of logprob and entropy (fp32 (rows,),
+    None: 0) and the forward's lse and entropy (mtx_token_logprobs_bwd):
+    fp32 (rows, V), added to dlogits with accumulate."""
+    rows, V, ld = _logits_rows(logits, tokens, lse=lse, entropy=entropy, g_logprob=g_logprob, g_entropy=g_entropy)
+    if dlogits is None:
+        if accumulate:
+            raise ValueError("accumulate needs dlogits")
+        dlogits = dev.empty_buf((rows, V), "float32")
+    _need_cuda(dlogits)
+    if _dt(dlogits) != "float32" or tuple(dlogits.shape) != (rows, V) or dlogits.stride(1) != 1:
+        raise ValueError(f"dlogits must be fp32 ({rows}, {V}) with contiguous rows")
+    if rows:
+        L.call("mtx_token_logprobs_bwd", L.dtype_code(logits), rows, V, L.ptr(logits), ld, L.ptr(tokens), L.ptr(lse),
+               L.ptr(entropy), L.ptr(g_logprob) if g_logprob is not None else None,
+               L.ptr(g_entropy) if g_entropy is not None else None, float(scale), L.ptr(dlogits), dlogits.stride(0),
+               int(bool(accumulate)), L.stream_handle())
+    return dlogits
 
 
 def embedding_fwd(weight, idx, out):
