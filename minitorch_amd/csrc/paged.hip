@@ -15,6 +15,7 @@
 #include "mtx_common.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace mtx {
@@ -31,15 +32,31 @@ struct Table {
   int width;        // pages per sequence
   int page;         // rows per page
   int64_t n_pages;  // pages in the pool
+  uint32_t mul;     // j / page = (mulhi(j, mul) + j) >> shift for j < 2^31
+  int shift;
+
+  // the index of the page that holds row j
+  __device__ __forceinline__ int div(int j) const { return (int)((__umulhi((uint32_t)j, mul) + (uint32_t)j) >> shift); }
+  // the id at index i of sequence b's pages, or -1
+  __device__ __forceinline__ int id(int b, int i) const {
+    const int x = ids[b * ld + i];
+    return (unsigned)x < (unsigned)n_pages ? x : -1;
+  }
 };
 
-// page id of row j, or -1
-__device__ __forceinline__ int page_of(const Table& t, int b, int j) {
-  const int id = t.ids[b * t.ld + j / t.page];
-  return (unsigned)id < (unsigned)t.n_pages ? id : -1;
+// rows of `page` a page: the smallest shift with 2^shift >= page, and
+// 2^32 (2^shift - page) / page + 1 (Granlund and Montgomery's division by an
+// invariant integer)
+Table make_table(const int* ids, int64_t ld, int width, int page, int64_t n_pages) {
+  int shift = 0;
+  while ((1 << shift) < page) ++shift;
+  const uint32_t mul = (uint32_t)((((uint64_t)(1u << shift) - page) << 32) / page + 1);
+  return Table{ids, ld, width, page, n_pages, mul, shift};
 }
-__device__ __forceinline__ int64_t row_at(const Pages& g, const Table& t, int id, int h, int j) {
-  return id * g.sp + h * g.sh + (j % t.page) * g.sr;
+
+// offset of row j, whose page's index is i and id is `id`
+__device__ __forceinline__ int64_t row_at(const Pages& g, const Table& t, int id, int i, int j) {
+  return id * g.sp + (j - i * t.page) * g.sr;
 }
 
 // ---------------------------------------------------------------------------
@@ -65,10 +82,10 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
   const int n = a.counts != nullptr ? min(a.counts[b], a.T) : a.T;
   const int j = a.lengths[b] - n + t;
   if (t >= n || j < 0 || j >= a.tab.width * a.tab.page) return;
-  const int id = page_of(a.tab, b, j);
+  const int pi = a.tab.div(j), id = a.tab.id(b, pi);
   if (id < 0) return;
   const TX* __restrict__ x = static_cast<const TX*>(a.x[z]) + b * a.sb[z] + h * a.sh[z] + t * a.st[z] + 8 * c;
-  TC* __restrict__ y = static_cast<TC*>(a.g[z].p) + row_at(a.g[z], a.tab, id, h, j) + 8 * c;
+  TC* __restrict__ y = static_cast<TC*>(a.g[z].p) + row_at(a.g[z], a.tab, id, pi, j) + h * a.g[z].sh + 8 * c;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     if constexpr (sizeof(TX) == sizeof(TC)) y[e] = x[e];
@@ -79,6 +96,34 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
 // ---------------------------------------------------------------------------
 // decode
 // ---------------------------------------------------------------------------
+// One query against n cached rows reads 2 n D values a K/V head and does 4 G n D
+// flops on them (G = H / Hkv heads share the rows): 2 G flops a value, bound by
+// the memory for every G here.  So K and V go from memory straight into the
+// registers the matrix instructions read, each value once:
+//
+//   scores, S^T = K Q^T: A = K (16 keys, lane l holds key l % 16 and the d values
+//   of its quarter l / 16), B = Q (16 heads, the same d values); lane l then has
+//   the scores of head l % 16 and keys 4 (l / 16) + r;
+//   output, O^T = V^T P^T: B = P is those registers as they are, keys
+//   16 t + 4 (l / 16) + r for k; A = V^T takes the same keys' rows, of which lane
+//   l loads values VD (l % 16) .. + VD - 1 (VD = D / 16): its matrix row of
+//   product n is d = VD (l % 16) + n.
+//
+// Nothing passes through LDS or across lanes but the rare update of the running
+// maximum: it is raised only when a score exceeds it by more than 2^8 in the
+// exponent (probabilities stay below 2^8, the sums in fp32), which in practice
+// happens in a wave's first tile.
+//
+// fp32 pools use fp32 matrix instructions.  Over bf16 pools the weights enter the
+// products as two bf16 pieces (16 bits; the output is rounded to 8) for bf16 rows,
+// and q and the weights as three (24 bits) for fp32 rows.
+//
+// A workgroup takes `chunk` rows of one sequence and K/V head, its four waves in
+// turn tiles of 16 NT rows, and joins them in LDS; several chunks of a sequence
+// are joined by finish_kernel.
+constexpr int kMaxChunk = 2048;
+constexpr float kRaise = 8.f;
+
 struct DecodeArgs {
   const void* q;
   int64_t qb, qh;
@@ -91,79 +136,417 @@ struct DecodeArgs {
   const float* win;
   float* w;
   int64_t wld;
-  float* ws;
-  int B, H, Hkv, D, cap;
-  float scale;
+  float* part_o;  // [B H][S][D] sums, relative to part_ml's maximum
+  float* part_ml; // [B H][S][2] maximum (log2 units) and sum
+  float* s;       // [B H][sld] scores (log2 units), with weights
+  int64_t sld;
+  int B, H, Hkv, G, S, HT, chunk, cap;
+  int direct;     // the workgroup's result is final: no finish_kernel
+  float c;        // scale * log2(e)
 };
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+template <typename TQ, typename TC, int D> struct DecodeTile;
+
+// bf16 pools
+template <typename TQ, int D>
+struct DecodeTile<TQ, bf16_t, D> {
+  static constexpr int NT = 2, VD = D / 16, NC = D >= 32 ? D / 32 : 1, VW = VD >= 2 ? VD / 2 : 1;
+  static constexpr int QP = sizeof(TQ) == 4 ? 3 : 1, PP = sizeof(TQ) == 4 ? 3 : 2;
+  bf16x8 q[QP][NC];
+  uint4 k[NT][NC];
+  uint32_t v[4 * NT][VW];
+
+  __device__ __forceinline__ void load_q(const TQ* row, int quarter) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const bool in = row != nullptr && 32 * c + 8 * quarter < D;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = in ? Elem<TQ>::to_f(row[32 * c + 8 * quarter + e]) : 0.f;
+#pragma unroll
+      for (int p = 0; p < QP; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = pk_bf16(x[2 * i], x[2 * i + 1]);
+          x[2 * i] -= __uint_as_float(w[i] << 16);
+          x[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+        }
+        q[p][c] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+      }
+    }
+  }
+  __device__ __forceinline__ void load_k(int t, const bf16_t* row, int quarter) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      k[t][c] = *reinterpret_cast<const uint4*>(row + 32 * c + (D >= 32 ? 8 * quarter : 8 * (quarter & 1)));
+  }
+  __device__ __forceinline__ void load_v(int e, const bf16_t* row) {
+    if constexpr (VD == 8) {
+      const uint4 u = *reinterpret_cast<const uint4*>(row);
+      v[e][0] = u.x, v[e][1] = u.y, v[e][2] = u.z, v[e][3] = u.w;
+    } else if constexpr (VD == 4) {
+      const uint2 u = *reinterpret_cast<const uint2*>(row);
+      v[e][0] = u.x, v[e][1] = u.y;
+    } else if constexpr (VD == 2) {
+      v[e][0] = *reinterpret_cast<const uint32_t*>(row);
+    } else {
+      v[e][0] = *row;
+    }
+  }
+  __device__ __forceinline__ void clear_v(int e) {
+#pragma unroll
+    for (int i = 0; i < VW; ++i) v[e][i] = 0;
+  }
+  __device__ __forceinline__ f32x4 scores(int t, int quarter) const {
+    f32x4 s = zero4();
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      uint4 u = k[t][c];
+      if (D < 32 && quarter >= 2) u = make_uint4(0, 0, 0, 0);  // 16 values fill half the product
+      const bf16x8 a = __builtin_bit_cast(bf16x8, u);
+#pragma unroll
+      for (int p = QP - 1; p >= 0; --p) s = Mfma<bf16_t>::mma(a, q[p][c], s);
+    }
+    return s;
+  }
+  __device__ __forceinline__ void add_v(float (&p)[4 * NT], f32x4 (&o)[VD]) const {
+    bf16x8 b[PP];
+#pragma unroll
+    for (int i = 0; i < PP; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = pk_bf16(p[2 * j], p[2 * j + 1]);
+        p[2 * j] -= __uint_as_float(w[j] << 16);
+        p[2 * j + 1] -= __uint_as_float(w[j] & 0xffff0000u);
+      }
+      b[i] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+    }
+#pragma unroll
+    for (int n = 0; n < VD; ++n) {
+      uint32_t w[4];  // column n of the eight rows
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = __builtin_amdgcn_perm(v[2 * j + 1][n / 2], v[2 * j][n / 2], n & 1 ? 0x07060302 : 0x05040100);
+      const bf16x8 a = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+      for (int i = PP - 1; i >= 0; --i) o[n] = Mfma<bf16_t>::mma(a, b[i], o[n]);
+    }
+  }
+};
+
+// fp32 pools
+template <typename TQ, int D>
+struct DecodeTile<TQ, float, D> {
+  static constexpr int NT = D >= 128 ? 1 : 2, VD = D / 16, NC = D / 16;
+  f32x4 q[NC];
+  f32x4 k[NT][NC];
+  float v[4 * NT][VD];
+
+  __device__ __forceinline__ void load_q(const TQ* row, int quarter) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      q[c] = row != nullptr ? *reinterpret_cast<const f32x4*>(row + 16 * c + 4 * quarter) : zero4();
+  }
+  __device__ __forceinline__ void load_k(int t, const float* row, int quarter) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) k[t][c] = *reinterpret_cast<const f32x4*>(row + 16 * c + 4 * quarter);
+  }
+  __device__ __forceinline__ void load_v(int e, const float* row) {
+    if constexpr (VD >= 4) {
+#pragma unroll
+      for (int i = 0; i < VD; i += 4) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(row + i);
+        v[e][i] = x[0], v[e][i + 1] = x[1], v[e][i + 2] = x[2], v[e][i + 3] = x[3];
+      }
+    } else if constexpr (VD == 2) {
+      const f32x2 x = *reinterpret_cast<const f32x2*>(row);
+      v[e][0] = x[0], v[e][1] = x[1];
+    } else {
+      v[e][0] = *row;
+    }
+  }
+  __device__ __forceinline__ void clear_v(int e) {
+#pragma unroll
+    for (int i = 0; i < VD; ++i) v[e][i] = 0.f;
+  }
+  __device__ __forceinline__ f32x4 scores(int t, int) const {
+    f32x4 s = zero4();
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = Mfma<float>::mma(k[t][c][e], q[c][e], s);
+    return s;
+  }
+  __device__ __forceinline__ void add_v(float (&p)[4 * NT], f32x4 (&o)[VD]) const {
+#pragma unroll
+    for (int e = 0; e < 4 * NT; ++e)
+#pragma unroll
+      for (int n = 0; n < VD; ++n) o[n] = Mfma<float>::mma(v[e][n], p[e], o[n]);
+  }
+};
+
+__device__ __forceinline__ float lane_max4(float v) {  // over the four quarters
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float lane_sum4(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
 }
 
-// one workgroup per sequence and query head, the scores in the workspace
-template <typename TQ, typename TC>
-__global__ __launch_bounds__(256) void decode_kernel(const DecodeArgs a) {
-  __shared__ float q[128], red[4];
-  const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hkv);
-  const int tid = threadIdx.x, len = min(max(a.lengths[b], 0), a.cap);
-  const TQ* __restrict__ qp = static_cast<const TQ*>(a.q) + b * a.qb + h * a.qh;
-  if (tid < a.D) q[tid] = Elem<TQ>::to_f(qp[tid]);
+// EVEN: pages of a multiple of 16 rows and row strides that fit 32-bit lane
+// offsets, so 16 rows have one page and one uniform address; otherwise each lane
+// looks up its rows
+template <typename TQ, typename TC, int D, bool EVEN>
+__global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
+  using Tile = DecodeTile<TQ, TC, D>;
+  constexpr int NT = Tile::NT, VD = Tile::VD, KT = 16 * NT, LD = D + 4;
+  __shared__ union {
+    int ids[kMaxChunk + 2];
+    struct { float o[4][16][LD], m[4][16], l[4][16]; } j;
+  } sh;
+  __shared__ float lse2[16];
+
+  const int split = blockIdx.x % a.S, rest = blockIdx.x / a.S;
+  const int ht = rest % a.HT, bh = rest / a.HT, b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
+  const int heads = min(16, a.G - 16 * ht), h0 = hk * a.G + 16 * ht;
+  const int n = min(max(a.lengths[b], 0), a.cap);
+  const int c0 = split * a.chunk, c1 = min(n, c0 + a.chunk);
+  if (c0 >= n && !(a.direct && split == 0)) return;  // finish_kernel knows which chunks there are
+
+  Tile tile;
+  tile.load_q(col < heads ? static_cast<const TQ*>(a.q) + b * a.qb + (h0 + col) * a.qh : nullptr, quarter);
+  const int p0 = a.tab.div(c0);
+  const int np = c1 > c0 ? a.tab.div(c1 - 1) - p0 + 1 : 0;
+  for (int i = tid; i < np; i += 256) sh.ids[i] = a.tab.id(b, p0 + i);
   __syncthreads();
-  float* __restrict__ s = a.ws + (int64_t)blockIdx.x * a.cap;
-  float m = -INFINITY;
-  for (int j = tid; j < len; j += 256) {
-    const int id = page_of(a.tab, b, j);
-    float x = -INFINITY;
-    if (id >= 0) {
-      const TC* __restrict__ k = static_cast<const TC*>(a.k.p) + row_at(a.k, a.tab, id, hk, j);
-      x = 0.f;
-      for (int d = 0; d < a.D; ++d) x = fmaf(q[d], Elem<TC>::to_f(k[d]), x);
-      x *= a.scale;
+
+  const TC* __restrict__ kp = static_cast<const TC*>(a.k.p) + hk * a.k.sh;
+  const TC* __restrict__ vp = static_cast<const TC*>(a.v.p) + hk * a.v.sh;
+  uint32_t there = 0;  // which of the lane's rows 16 t + 4 quarter + r (bit 4 t + r) are seen
+
+  // row j of the chunk: its offset in a pool, or -1
+  auto look = [&](const Pages& g, int j) -> int64_t {
+    if (j >= c1) return -1;
+    const int pi = a.tab.div(j), id = sh.ids[pi - p0];
+    return id < 0 ? -1 : row_at(g, a.tab, id, pi, j);
+  };
+  // the same of a row that is one for the whole wave
+  auto look1 = [&](const Pages& g, int j) -> int64_t {
+    if (j >= c1) return -1;
+    const int pi = a.tab.div(j), id = __builtin_amdgcn_readfirstlane(sh.ids[pi - p0]);
+    return id < 0 ? -1 : row_at(g, a.tab, id, pi, j);
+  };
+  auto load_k = [&](int j0) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if constexpr (EVEN) {
+        const int64_t at = look1(a.k, __builtin_amdgcn_readfirstlane(j0 + 16 * t));
+        const TC* base = kp + (at < 0 ? 0 : at);
+        tile.load_k(t, base + col * (int)a.k.sr, quarter);
+      } else {
+        const int64_t at = look(a.k, j0 + 16 * t + col);
+        tile.load_k(t, kp + (at < 0 ? 0 : at), quarter);
+      }
     }
-    s[j] = x;
-    m = fmaxf(m, x);
+  };
+  auto load_v = [&](int j0) {
+    there = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if constexpr (EVEN) {
+        const int j = __builtin_amdgcn_readfirstlane(j0 + 16 * t);
+        const int64_t at = look1(a.v, j);
+        const TC* base = vp + (at < 0 ? 0 : at);
+        const int seen = at < 0 ? 0 : c1 - j;  // rows from j on
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          tile.load_v(4 * t + r, base + (4 * quarter + r) * (int)a.v.sr + VD * col);
+          there |= (uint32_t)(4 * quarter + r < seen) << (4 * t + r);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t at = look(a.v, j0 + 16 * t + 4 * quarter + r);
+          tile.load_v(4 * t + r, vp + (at < 0 ? 0 : at) + VD * col);
+          there |= (uint32_t)(at >= 0) << (4 * t + r);
+        }
+      }
+    }
+  };
+
+  f32x4 o[VD];
+#pragma unroll
+  for (int i = 0; i < VD; ++i) o[i] = zero4();
+  float mu = -FLT_MAX, l = 0.f;
+  int j0 = c0 + KT * wave;
+  if (j0 < c1) {
+    load_k(j0);
+    load_v(j0);
   }
+  for (; j0 < c1; j0 += 4 * KT) {
+    const int next = j0 + 4 * KT;
+    float p[4 * NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const f32x4 s = tile.scores(t, quarter);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[4 * t + r] = s[r] * a.c;
+    }
+    if (next < c1) load_k(next);
+    if (__ballot(there != (1u << (4 * NT)) - 1)) {  // a hidden row: no weight, and its V is not used
+#pragma unroll
+      for (int e = 0; e < 4 * NT; ++e)
+        if (!((there >> e) & 1)) {
+          p[e] = -INFINITY;
+          tile.clear_v(e);
+        }
+    }
+    if (a.w != nullptr && col < heads) {
+      float* s = a.s + (int64_t)(b * a.H + h0 + col) * a.sld + j0 + 4 * quarter;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        *reinterpret_cast<f32x4*>(s + 16 * t) = f32x4{p[4 * t], p[4 * t + 1], p[4 * t + 2], p[4 * t + 3]};
+    }
+    float mx = p[0];
+#pragma unroll
+    for (int e = 1; e < 4 * NT; ++e) mx = fmaxf(mx, p[e]);
+    if (__ballot(mx > mu + kRaise)) {
+      const float m = fmaxf(mu, lane_max4(mx)), f = __builtin_amdgcn_exp2f(mu - m);
+      mu = m;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < VD; ++i) o[i] *= f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4 * NT; ++e) {
+      p[e] = __builtin_amdgcn_exp2f(p[e] - mu);
+      l += p[e];
+    }
+    tile.add_v(p, o);
+    if (next < c1) load_v(next);
+  }
+
+  // join the waves: head col's values VD (4 quarter + r) + n in o[n][r]
+  l = lane_sum4(l);
+  __syncthreads();  // the page ids are read
+  if (col < heads) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < VD; ++i) sh.j.o[wave][col][VD * (4 * quarter + r) + i] = o[i][r];
+    if (quarter == 0) {
+      sh.j.m[wave][col] = mu;
+      sh.j.l[wave][col] = l;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < heads * D; i += 256) {
+    const int h = i / D, d = i % D;
+    const float m = fmaxf(fmaxf(sh.j.m[0][h], sh.j.m[1][h]), fmaxf(sh.j.m[2][h], sh.j.m[3][h]));
+    float x = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sh.j.m[w][h] - m);
+      x += f * sh.j.o[w][h][d];
+      sum += f * sh.j.l[w][h];
+    }
+    const int64_t row = (int64_t)b * a.H + h0 + h;
+    if (a.direct) {
+      const bool some = sum > 0.f || sum != sum;
+      static_cast<TQ*>(a.o)[b * a.ob + (h0 + h) * a.oh + d] = Elem<TQ>::from_f(some ? x / sum : 0.f);
+      if (d == 0) {
+        if (a.lse != nullptr) a.lse[row] = some ? m * kLn2 + logf(sum) : -INFINITY;
+        lse2[h] = some ? m + log2f(sum) : 0.f;
+      }
+    } else {
+      a.part_o[(row * a.S + split) * D + d] = x;
+      if (d == 0) {
+        a.part_ml[(row * a.S + split) * 2] = m;
+        a.part_ml[(row * a.S + split) * 2 + 1] = sum;
+      }
+    }
+  }
+  if (a.direct && a.w != nullptr) {
+    __syncthreads();  // this workgroup's scores and lse2 are written
+    const float* s = a.s + ((int64_t)b * a.H + h0) * a.sld;
+    for (int j = tid; j < n; j += 256) {
+      float w = 0.f;
+      for (int g = 0; g < heads; ++g) w += __builtin_amdgcn_exp2f(s[g * a.sld + j] - lse2[g]);
+      if (a.win != nullptr) w += a.win[bh * a.wld + j];
+      a.w[bh * a.wld + j] = w;
+    }
+  }
+}
+
+// maximum and sum of one head over its chunks, by one wave
+__device__ __forceinline__ void chunk_total(const float* ml, int chunks, int lane, float& m, float& l) {
+  m = -FLT_MAX;
+  l = 0.f;
+  for (int i = lane; i < chunks; i += 64) m = fmaxf(m, ml[2 * i]);
   m = wave_max(m);
-  if ((tid & 63) == 0) red[tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  if (m == -INFINITY) m = 0.f;
-  float l = 0.f;
-  for (int j = tid; j < len; j += 256) l += expf(s[j] - m);
-  l = block_sum(l, red);
-  if (a.lse != nullptr && tid == 0) a.lse[blockIdx.x] = m + logf(l);
-  __syncthreads();
-  TQ* __restrict__ op = static_cast<TQ*>(a.o) + b * a.ob + h * a.oh;
-  if (tid < a.D) {
-    float acc = 0.f;
-    for (int j = 0; j < len; ++j) {
-      const int id = page_of(a.tab, b, j);
-      if (id < 0) continue;
-      acc = fmaf(expf(s[j] - m), Elem<TC>::to_f((static_cast<const TC*>(a.v.p) + row_at(a.v, a.tab, id, hk, j))[tid]),
-                 acc);
-    }
-    op[tid] = Elem<TQ>::from_f(l > 0.f || l != l ? acc / l : 0.f);
-  }
-  if (a.w != nullptr) {
-    __syncthreads();  // the scores are read above
-    const float lse = m + logf(l);
-    for (int j = tid; j < len; j += 256) s[j] = s[j] == -INFINITY ? 0.f : expf(s[j] - lse);
-  }
+  for (int i = lane; i < chunks; i += 64) l += ml[2 * i + 1] * __builtin_amdgcn_exp2f(ml[2 * i] - m);
+  l = wave_sum(l);
 }
 
-__global__ __launch_bounds__(256) void weights_kernel(const DecodeArgs a) {
-  const int bh = blockIdx.y, b = bh / a.Hkv, G = a.H / a.Hkv;
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= min(a.lengths[b], a.cap)) return;
-  const float* __restrict__ s = a.ws + (int64_t)bh * G * a.cap + j;
-  float w = 0.f;
-  for (int g = 0; g < G; ++g) w += s[(int64_t)g * a.cap];
-  if (a.win != nullptr) w += a.win[bh * a.wld + j];
-  a.w[bh * a.wld + j] = w;
+// Joins the chunks of decode_kernel: the first B H workgroups each one head's
+// output, the others kFinishRows rows' weights of one sequence and K/V head
+constexpr int kFinishRows = 1024;
+template <typename TQ, int D>
+__global__ __launch_bounds__(256) void finish_kernel(const DecodeArgs a) {
+  constexpr int DL = D / 4, NG = 256 / DL;  // lanes over d, groups of chunks
+  __shared__ union {
+    f32x4 x[NG][DL];
+    float lse2[256];
+  } sh;
+  const int tid = threadIdx.x, lane = tid & 63;
+  if ((int)blockIdx.x < a.B * a.H) {
+    const int64_t row = blockIdx.x;
+    const int b = blockIdx.x / a.H, h = blockIdx.x % a.H;
+    const int chunks = (min(max(a.lengths[b], 0), a.cap) + a.chunk - 1) / a.chunk;
+    const float* ml = a.part_ml + row * a.S * 2;
+    float m, l;
+    chunk_total(ml, chunks, lane, m, l);
+    const int d = tid % DL, g = tid / DL;
+    const f32x4* po = reinterpret_cast<const f32x4*>(a.part_o + row * a.S * D) + d;
+    f32x4 x = zero4();
+    for (int i = g; i < chunks; i += NG) x += po[i * DL] * __builtin_amdgcn_exp2f(ml[2 * i] - m);
+    sh.x[g][d] = x;
+    __syncthreads();
+    const bool some = l > 0.f || l != l;
+    if (g == 0) {
+      x = sh.x[0][d];
+#pragma unroll
+      for (int i = 1; i < NG; ++i) x += sh.x[i][d];
+      TQ* o = static_cast<TQ*>(a.o) + b * a.ob + h * a.oh + 4 * d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = Elem<TQ>::from_f(some ? x[e] / l : 0.f);
+    }
+    if (tid == 0 && a.lse != nullptr) a.lse[row] = some ? m * kLn2 + logf(l) : -INFINITY;
+    return;
+  }
+  const int i = blockIdx.x - a.B * a.H, blocks = (a.cap + kFinishRows - 1) / kFinishRows;
+  const int bh = i / blocks, b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int n = min(max(a.lengths[b], 0), a.cap), j0 = (i % blocks) * kFinishRows, j1 = min(n, j0 + kFinishRows);
+  if (j0 >= n) return;
+  const int chunks = (n + a.chunk - 1) / a.chunk;
+  const int64_t row = (int64_t)b * a.H + hk * a.G;
+  for (int g = tid >> 6; g < a.G; g += 4) {
+    float m, l;
+    chunk_total(a.part_ml + (row + g) * a.S * 2, chunks, lane, m, l);
+    if (lane == 0) sh.lse2[g] = l > 0.f || l != l ? m + log2f(l) : 0.f;
+  }
+  __syncthreads();
+  const float* s = a.s + row * a.sld;
+  for (int j = j0 + tid; j < j1; j += 256) {
+    float w = 0.f;
+    for (int g = 0; g < a.G; ++g) w += __builtin_amdgcn_exp2f(s[g * a.sld + j] - sh.lse2[g]);
+    if (a.win != nullptr) w += a.win[bh * a.wld + j];
+    a.w[bh * a.wld + j] = w;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -261,11 +644,12 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a, int bloc
   if (r >= a.keep) return;
   const int j = a.slots[(int64_t)bh * a.keep + r];
   if (j < 0) return;
-  const int from = page_of(a.from, b, j), to = page_of(a.to, b, r);
+  const int fi = a.from.div(j), ti = a.to.div(r);
+  const int from = a.from.id(b, fi), to = a.to.id(b, ti);
   if (to < 0) return;
   const Pages& g = blockIdx.y ? a.v : a.k;
-  const TC* __restrict__ x = static_cast<const TC*>(g.p) + row_at(g, a.from, from < 0 ? 0 : from, h, j) + 8 * c;
-  TC* __restrict__ y = static_cast<TC*>(g.p) + row_at(g, a.to, to, h, r) + 8 * c;
+  const TC* __restrict__ x = static_cast<const TC*>(g.p) + row_at(g, a.from, from < 0 ? 0 : from, fi, j) + h * g.sh + 8 * c;
+  TC* __restrict__ y = static_cast<TC*>(g.p) + row_at(g, a.to, to, ti, r) + h * g.sh + 8 * c;
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = from < 0 ? (TC)0 : x[e];
 }
@@ -321,6 +705,49 @@ int check_cache(int B, int H, int D, int64_t n_pages, int page, const int* table
   return MTX_OK;
 }
 
+// How a decode call is cut: chunks of rows, a multiple of what four waves take
+// in turn, enough of them for two workgroups a CU where the cache is long, and
+// the workspace [part_o | part_ml | scores].
+struct DecodePlan {
+  int chunk, S, HT, direct;
+  int64_t n_o, n_ml, n_s, sld;
+  size_t bytes() const { return (size_t)(n_o + n_ml + n_s) * sizeof(float); }
+};
+DecodePlan make_plan(int B, int H, int Hkv, int D, int cap, bool weights) {
+  DecodePlan p;
+  p.HT = cdiv(H / Hkv, 16);
+  const int64_t want = ((int64_t)cap * B * Hkv * p.HT / 512 + 127) / 128 * 128;
+  p.chunk = (int)std::min<int64_t>(std::max<int64_t>(want, 256), kMaxChunk);
+  p.S = cdiv(cap, p.chunk);
+  p.direct = p.S == 1 && (!weights || p.HT == 1);
+  p.sld = ((int64_t)cap + 31) / 32 * 32;
+  p.n_o = p.direct ? 0 : (int64_t)B * H * p.S * D;
+  p.n_ml = p.direct ? 0 : ((int64_t)B * H * p.S * 2 + 3) / 4 * 4;
+  p.n_s = weights ? (int64_t)B * H * p.sld : 0;
+  return p;
+}
+
+template <typename TQ, typename TC, int D>
+int launch_decode(bool even, unsigned groups, unsigned finish, const DecodeArgs& a, hipStream_t st) {
+  if (even) hipLaunchKernelGGL((decode_kernel<TQ, TC, D, true>), dim3(groups), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((decode_kernel<TQ, TC, D, false>), dim3(groups), dim3(256), 0, st, a);
+  MTX_LAUNCHED();
+  if (!a.direct) {
+    hipLaunchKernelGGL((finish_kernel<TQ, D>), dim3(finish), dim3(256), 0, st, a);
+    MTX_LAUNCHED();
+  }
+  return MTX_OK;
+}
+template <typename TQ, typename TC>
+int dispatch_decode(int D, bool even, unsigned groups, unsigned finish, const DecodeArgs& a, hipStream_t st) {
+  switch (D) {
+    case 16: return launch_decode<TQ, TC, 16>(even, groups, finish, a, st);
+    case 32: return launch_decode<TQ, TC, 32>(even, groups, finish, a, st);
+    case 64: return launch_decode<TQ, TC, 64>(even, groups, finish, a, st);
+    default: return launch_decode<TQ, TC, 128>(even, groups, finish, a, st);
+  }
+}
+
 }  // namespace
 }  // namespace mtx
 
@@ -348,7 +775,7 @@ extern "C" int mtx_kv_append_paged(int dtype, int cache_dtype, int B, int T, int
                {k_strides[2], v_strides[2]},
                {{k_pages, kp_strides[0], kp_strides[1], kp_strides[2]},
                 {v_pages, vp_strides[0], vp_strides[1], vp_strides[2]}},
-               {table, table_ld, max_pages, page, n_pages},
+               make_table(table, table_ld, max_pages, page, n_pages),
                lengths,
                counts,
                T,
@@ -367,8 +794,10 @@ extern "C" int mtx_kv_append_paged(int dtype, int cache_dtype, int B, int T, int
 
 extern "C" size_t mtx_attn_decode_paged_workspace_bytes(int B, int H, int Hkv, int D, int page, int max_pages,
                                                         int with_weights) {
-  if (B < 1 || H < 1 || page < 1 || max_pages < 1) return 0;
-  return (size_t)B * H * page * max_pages * sizeof(float);
+  if (B < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || page < 1 || max_pages < 1 ||
+      (int64_t)page * max_pages > (1 << 28))
+    return 0;
+  return make_plan(B, H, Hkv, D, page * max_pages, with_weights != 0).bytes();
 }
 
 extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, int Hkv, int D, const void* q,
@@ -381,7 +810,8 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
   int rc;
   if ((rc = check_dtypes(dtype, cache_dtype))) return rc;
   if ((rc = check_cache(B, H, D, n_pages, page, table, table_ld, max_pages, lengths))) return rc;
-  MTX_CHECK_SHAPE(Hkv >= 1 && H % Hkv == 0, "H=%d query heads must be a multiple of Hkv=%d K/V heads", H, Hkv);
+  MTX_CHECK_SHAPE(Hkv >= 1 && H % Hkv == 0 && H / Hkv <= 256,
+                  "H=%d query heads must be a multiple of Hkv=%d K/V heads, at most 256 times", H, Hkv);
   const int es = dtype == MTX_F32 ? 4 : 2, ec = cache_dtype == MTX_F32 ? 4 : 2;
   if ((rc = check_view("q", q, q_strides, es))) return rc;
   if ((rc = check_view("k_pages", k_pages, kp_strides, ec))) return rc;
@@ -394,26 +824,27 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
   MTX_CHECK_ARG(weights != nullptr || weights_in == nullptr, "weights_in without weights");
   MTX_CHECK_ARG(weights == nullptr || weights_ld >= cap, "weights: rows of %lld values for %d cached rows",
                 (long long)weights_ld, cap);
-  const size_t need = mtx_attn_decode_paged_workspace_bytes(B, H, Hkv, D, page, max_pages, weights != nullptr);
-  MTX_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small (%zu < %zu)",
-                workspace_bytes, need);
+  const DecodePlan plan = make_plan(B, H, Hkv, D, cap, weights != nullptr);
+  const size_t need = plan.bytes();
+  MTX_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need && ((uintptr_t)workspace & 15u) == 0),
+                "workspace: %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
+  const int64_t groups = (int64_t)B * Hkv * plan.HT * plan.S;
+  const int64_t finish = (int64_t)B * H + (weights != nullptr ? (int64_t)B * Hkv * cdiv(cap, kFinishRows) : 0);
+  MTX_CHECK_SHAPE(groups <= INT32_MAX && finish <= INT32_MAX, "decode: too many sequences, heads and rows in one call");
+  float* ws = static_cast<float*>(workspace);
   DecodeArgs a{q, q_strides[0], q_strides[1],
                {const_cast<void*>(k_pages), kp_strides[0], kp_strides[1], kp_strides[2]},
                {const_cast<void*>(v_pages), vp_strides[0], vp_strides[1], vp_strides[2]},
-               {table, table_ld, max_pages, page, n_pages},
+               make_table(table, table_ld, max_pages, page, n_pages),
                lengths, o, o_strides[0], o_strides[1], lse, weights_in, weights, weights_ld,
-               static_cast<float*>(workspace), B, H, Hkv, D, cap, scale};
+               ws, ws + plan.n_o, ws + plan.n_o + plan.n_ml, plan.sld,
+               B, H, Hkv, H / Hkv, plan.S, plan.HT, plan.chunk, cap, plan.direct, scale * kLog2e};
+  // 16 rows at lane offsets of 32 bits from one address
+  const bool even = page % 16 == 0 && std::max(kp_strides[2], vp_strides[2]) < (1 << 24);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache_dtype == MTX_F32) hipLaunchKernelGGL((decode_kernel<float, float>), dim3(B * H), dim3(256), 0, st, a);
-  else if (dtype == MTX_F32) hipLaunchKernelGGL((decode_kernel<float, bf16_t>), dim3(B * H), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((decode_kernel<bf16_t, bf16_t>), dim3(B * H), dim3(256), 0, st, a);
-  MTX_LAUNCHED();
-  if (weights != nullptr) {
-    MTX_CHECK_SHAPE(B * Hkv <= 65535, "weights: at most 65535 sequences times K/V heads");
-    hipLaunchKernelGGL(weights_kernel, dim3(cdiv(cap, 256), B * Hkv), dim3(256), 0, st, a);
-    MTX_LAUNCHED();
-  }
-  return MTX_OK;
+  if (cache_dtype == MTX_F32) return dispatch_decode<float, float>(D, even, (unsigned)groups, (unsigned)finish, a, st);
+  if (dtype == MTX_F32) return dispatch_decode<float, bf16_t>(D, even, (unsigned)groups, (unsigned)finish, a, st);
+  return dispatch_decode<bf16_t, bf16_t>(D, even, (unsigned)groups, (unsigned)finish, a, st);
 }
 
 extern "C" int mtx_kv_evict_paged(int cache_dtype, int B, int H, int D, int64_t n_pages, int page, void* k_pages,
@@ -443,8 +874,8 @@ extern "C" int mtx_kv_evict_paged(int cache_dtype, int B, int H, int D, int64_t 
   const int rows = std::min(keep, cap);
   EvictArgs a{{k_pages, kp_strides[0], kp_strides[1], kp_strides[2]},
               {v_pages, vp_strides[0], vp_strides[1], vp_strides[2]},
-              {table, table_ld, max_pages, page, n_pages},
-              {to_table, to_ld, to_pages, page, n_pages},
+              make_table(table, table_ld, max_pages, page, n_pages),
+              make_table(to_table, to_ld, to_pages, page, n_pages),
               lengths, weights, weights_ld, lengths_out, weights_out, slots, B, H, D, cap, keep, recent};
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(select_kernel, dim3(B * H), dim3(256), 0, st, a);
