@@ -9,6 +9,7 @@
 #include "mtx_common.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace mtx {
@@ -35,66 +36,281 @@ __device__ __forceinline__ uint64_t rank_key(float v, int i) {
   return ((uint64_t)u << 32) | (uint32_t)~i;
 }
 
+// E values from any address that their type allows: global loads need no more
+// alignment than that
+template <typename T, int E>
+struct __attribute__((packed, aligned(sizeof(T)))) Unaligned {
+  T x[E];
+};
+template <int E>
+__device__ __forceinline__ void load_values(const float* p, float (&x)[E]) {
+  const auto u = *reinterpret_cast<const Unaligned<float, E>*>(p);
+#pragma unroll
+  for (int i = 0; i < E; ++i) x[i] = u.x[i];
+}
+template <int E>
+__device__ __forceinline__ void load_values(const bf16_t* p, float (&x)[E]) {
+  const auto u = *reinterpret_cast<const Unaligned<bf16_t, E>*>(p);
+#pragma unroll
+  for (int i = 0; i < E; ++i) x[i] = bf2f(u.x[i]);
+}
+
+// values of -inf add 0, not 0 * inf; NaN stays
+constexpr float kFarBelow = -1e30f;
+__device__ __forceinline__ float below(float d) { return __builtin_elementwise_maximum(d, kFarBelow); }
+
+// 64 values of a wave, largest in lane 0 (bitonic)
+__device__ __forceinline__ float wave_sort(float v, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int m = size >> 1; m >= 1; m >>= 1) {
+      const float o = __shfl_xor(v, m, 64);
+      v = ((lane & size) == 0) == ((lane & m) == 0) ? fmaxf(v, o) : fminf(v, o);
+    }
+  return v;
+}
+// the 64 largest of two sorted waves' values, sorted
+__device__ __forceinline__ float wave_merge(float v, float w, int lane) {
+  v = fmaxf(v, __shfl(w, 63 - lane, 64));
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    const float o = __shfl_xor(v, m, 64);
+    v = (lane & m) == 0 ? fmaxf(v, o) : fminf(v, o);
+  }
+  return v;
+}
+
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+
+// A row's outputs but the alternatives, by one thread: maximum m (at least
+// -FLT_MAX), sums l of exp((x - m) scale) and t of that times (x - m)
 template <typename T>
-__global__ __launch_bounds__(256) void logprobs_kernel(const LpArgs a) {
-  __shared__ float red[4];
-  __shared__ uint64_t best[4];
-  const int tid = threadIdx.x;
-  const int64_t r = blockIdx.x;
+__device__ __forceinline__ void row_result(const LpArgs& a, int64_t r, const T* x, float m, float l, float t) {
+  const float logl = logf(l);
+  const int64_t k = a.tok[r];
+  float lp = 0.f;
+  if (k >= 0 && k < a.V) lp = l == 0.f ? -INFINITY : fmaf(Elem<T>::to_f(x[k]) - m, a.scale, -logl);
+  a.logprob[r] = lp;
+  a.lse[r] = l == 0.f ? -INFINITY : fmaf(m, a.scale, logl);
+  a.entropy[r] = l == 0.f ? 0.f : fmaf(-t / l, a.scale, logl);
+}
+__device__ __forceinline__ void put_top(const LpArgs& a, int64_t r, int rank, uint64_t key, float v, float m, float l) {
+  a.ids[r * a.top + rank] = (int)~(uint32_t)key;
+  a.tops[r * a.top + rank] = l == 0.f ? -INFINITY : fmaf(v - m, a.scale, -logf(l));
+}
+
+// Alternatives of a row: the top-th largest of the lanes' (threads') largest
+// values bounds the wanted ones from below, so only values from that bound on,
+// about `top` of them, are collected and ranked by counting.  Rows that hold NaN,
+// and rows where too many values reach the bound (ties), take `top` rounds over
+// all values instead.
+
+// ---- rows of up to 64 VPL values: one wave each, the row in registers ----
+constexpr int kSmallCap = 256;
+template <typename T, int VPL>
+__global__ __launch_bounds__(256) void logprobs_small_kernel(const LpArgs a, int64_t rows) {
+  __shared__ uint64_t cands[4][kSmallCap];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r = (int64_t)blockIdx.x * 4 + wave;
+  if (r >= rows) return;
   const T* __restrict__ x = static_cast<const T*>(a.x) + r * a.ld;
-  float m = -INFINITY;
-  for (int i = tid; i < a.V; i += 256) m = fmaxf(m, Elem<T>::to_f(x[i]) * a.scale);
-  m = wave_max(m);
-  if ((tid & 63) == 0) red[tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float m0 = m == -INFINITY ? 0.f : m;
+  float v[VPL], best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) v[i] = lane + 64 * i < a.V ? Elem<T>::to_f(x[lane + 64 * i]) : -INFINITY;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) best = fmaxf(best, v[i]);
+  const float m = fmaxf(wave_max(best), -FLT_MAX), c = a.scale * kLog2e;
   float l = 0.f, t = 0.f;
-  for (int i = tid; i < a.V; i += 256) {
-    const float d = Elem<T>::to_f(x[i]) * a.scale - m0, e = expf(d);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const float d = below(v[i] - m), e = __builtin_amdgcn_exp2f(d * c);
     l += e;
-    t -= e == 0.f ? 0.f : e * d;
+    t = fmaf(e, d, t);
   }
   l = wave_sum(l);
-  __syncthreads();
-  if ((tid & 63) == 0) red[tid >> 6] = l;
-  __syncthreads();
-  l = (red[0] + red[1]) + (red[2] + red[3]);
   t = wave_sum(t);
-  __syncthreads();
-  if ((tid & 63) == 0) red[tid >> 6] = t;
-  __syncthreads();
-  t = (red[0] + red[1]) + (red[2] + red[3]);
-  const float lse = m0 + logf(l);
-  if (tid == 0) {
-    const int64_t k = a.tok[r];
-    float lp = 0.f;
-    if (k >= 0 && k < a.V) lp = l == 0.f ? -INFINITY : Elem<T>::to_f(x[k]) * a.scale - lse;
-    a.logprob[r] = lp;
-    a.lse[r] = lse;
-    a.entropy[r] = l == 0.f ? 0.f : logf(l) + t / l;
+  if (lane == 0) row_result(a, r, x, m, l, t);
+  if (a.top == 0) return;
+  uint64_t* buf = cands[wave];
+  int n = 0;
+  if (l == l) {
+    const float bound = __shfl(wave_sort(best, lane), a.top - 1, 64);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const bool in = v[i] >= bound && lane + 64 * i < a.V;
+      const uint64_t mask = __ballot(in);
+      const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, n));
+      if (in && at < kSmallCap) buf[at] = rank_key(v[i], lane + 64 * i);
+      n += __popcll(mask);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  if (n >= a.top && n <= kSmallCap) {
+    for (int i = lane; i < n; i += 64) {
+      const uint64_t mine = buf[i];
+      int rank = 0;
+      for (int k = 0; k < n; ++k) rank += buf[k] > mine;
+      if (rank < a.top) put_top(a, r, rank, mine, key_value(mine), m, l);
+    }
+    return;
   }
   uint64_t last = ~0ull;
   for (int k = 0; k < a.top; ++k) {
     uint64_t mine = 0;
-    for (int i = tid; i < a.V; i += 256) {
-      const uint64_t key = rank_key(Elem<T>::to_f(x[i]), i);
-      if (key < last || k == 0) mine = key > mine ? key : mine;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const uint64_t key = rank_key(v[i], lane + 64 * i);
+      if (lane + 64 * i < a.V && (key < last || k == 0) && key > mine) mine = key;
     }
 #pragma unroll
     for (int s = 32; s >= 1; s >>= 1) {
       const uint64_t o = __shfl_xor(mine, s, 64);
       mine = o > mine ? o : mine;
     }
-    __syncthreads();
-    if ((tid & 63) == 0) best[tid >> 6] = mine;
-    __syncthreads();
-    last = std::max(std::max(best[0], best[1]), std::max(best[2], best[3]));
-    if (tid == 0) {
-      const int i = (int)~(uint32_t)last;
-      a.ids[r * a.top + k] = i;
-      a.tops[r * a.top + k] = l == 0.f ? -INFINITY : Elem<T>::to_f(x[i]) * a.scale - lse;
+    last = mine;
+    if (lane == 0) put_top(a, r, k, last, Elem<T>::to_f(x[(int)~(uint32_t)last]), m, l);
+  }
+}
+
+// ---- longer rows: a workgroup of NT threads each, one pass with the running
+// maximum and sums, E values (16 bytes) a load and kLoads of them in flight ----
+constexpr int kLoads = 4, kCap = 1024;
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
+  constexpr int E = Elem<T>::kVec, W = NT / 64, STEP = NT * E;
+  __shared__ uint64_t cands[kCap];
+  __shared__ float sorted[W][64], red[3][W];
+  __shared__ int count;
+  __shared__ uint64_t bests[W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r = blockIdx.x;
+  const T* __restrict__ x = static_cast<const T*>(a.x) + r * a.ld;
+  const float c = a.scale * kLog2e;
+  float m = -FLT_MAX, l = 0.f, t = 0.f;
+  auto raise = [&](float top) {  // the sums relative to a larger maximum
+    const float n = fmaxf(m, top), d = fmaxf(m - n, kFarBelow), f = __builtin_amdgcn_exp2f(d * c);
+    t = f * fmaf(l, d, t);
+    l *= f;
+    m = n;
+  };
+  auto add = [&](float v) {
+    const float d = below(v - m), e = __builtin_amdgcn_exp2f(d * c);
+    l += e;
+    t = fmaf(e, d, t);
+  };
+  int i = tid * E;
+  for (; i + (kLoads - 1) * STEP + E <= a.V; i += kLoads * STEP) {
+    float v[kLoads][E];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) load_values<E>(x + i + u * STEP, v[u]);
+    float top = v[0][0];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = fmaxf(top, v[u][e]);
+    raise(top);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) add(v[u][e]);
+  }
+  for (; i < a.V; i += STEP) {
+    float v[E];
+    if (i + E <= a.V) {
+      load_values<E>(x + i, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = i + e < a.V ? Elem<T>::to_f(x[i + e]) : -INFINITY;
     }
+    float top = v[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);
+    raise(top);
+#pragma unroll
+    for (int e = 0; e < E; ++e) add(v[e]);
+  }
+  const float mine = m;  // the thread's largest value
+  raise(wave_max(m));
+  l = wave_sum(l);
+  t = wave_sum(t);
+  if (lane == 0) red[0][wave] = m, red[1][wave] = l, red[2][wave] = t;
+  if (a.top) {
+    sorted[wave][lane] = wave_sort(mine, lane);
+    if (tid == 0) count = 0;
+  }
+  __syncthreads();
+  // every thread joins the waves' sums in the same order
+  const int w0 = lane % W;
+  m = red[0][w0], l = red[1][w0], t = red[2][w0];
+  float all = red[0][0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) all = fmaxf(all, red[0][w]);
+  raise(all);
+#pragma unroll
+  for (int s = 1; s < W; s <<= 1) {
+    l += __shfl_xor(l, s, 64);
+    t += __shfl_xor(t, s, 64);
+  }
+  if (tid == 0) row_result(a, r, x, m, l, t);
+  if (a.top == 0) return;
+#pragma unroll
+  for (int s = 1; s < W; s <<= 1) {
+    if (wave % (2 * s) == 0) sorted[wave][lane] = wave_merge(sorted[wave][lane], sorted[wave + s][lane], lane);
+    __syncthreads();
+  }
+  const float bound = sorted[0][a.top - 1];
+  if (l == l && mine >= bound) {
+    for (int i = tid * E; i < a.V; i += STEP) {
+      float v[E];
+      if (i + E <= a.V) {
+        load_values<E>(x + i, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = i + e < a.V ? Elem<T>::to_f(x[i + e]) : -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (v[e] >= bound && i + e < a.V) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kCap) cands[at] = rank_key(v[e], i + e);
+        }
+    }
+  }
+  __syncthreads();
+  const int n = count;
+  if (n >= a.top && n <= kCap) {
+    for (int i = tid; i < n; i += NT) {
+      const uint64_t key = cands[i];
+      int rank = 0;
+      for (int k = 0; k < n; ++k) rank += cands[k] > key;
+      if (rank < a.top) put_top(a, r, rank, key, key_value(key), m, l);
+    }
+    return;
+  }
+  uint64_t last = ~0ull;
+  for (int k = 0; k < a.top; ++k) {
+    uint64_t best = 0;
+    for (int i = tid; i < a.V; i += NT) {
+      const uint64_t key = rank_key(Elem<T>::to_f(x[i]), i);
+      if ((key < last || k == 0) && key > best) best = key;
+    }
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) {
+      const uint64_t o = __shfl_xor(best, s, 64);
+      best = o > best ? o : best;
+    }
+    __syncthreads();
+    if (lane == 0) bests[wave] = best;
+    __syncthreads();
+    last = bests[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) last = bests[w] > last ? bests[w] : last;
+    if (tid == 0) put_top(a, r, k, last, Elem<T>::to_f(x[(int)~(uint32_t)last]), m, l);
   }
 }
 
@@ -107,34 +323,74 @@ struct LpBwdArgs {
   const float* g;
   const float* gh;
   float* dx;
-  int64_t ldd;
-  int V;
+  int64_t ldd, rows;
+  int V, per;  // threads per row
   float scale;
   int accumulate;
 };
 
+// dx = p (A + B log p) with A = -scale (g + gh H), B = -scale gh, and scale g at
+// the token: one pass, 4 values a load and store, up to kUnroll of them a thread
+constexpr int kUnroll = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const LpBwdArgs a) {
-  const int64_t r = blockIdx.x;
+  const int64_t r = (int64_t)blockIdx.x * (256 / a.per) + threadIdx.x / a.per;
+  if (r >= a.rows) return;
+  const T* __restrict__ x = static_cast<const T*>(a.x) + r * a.ld;
+  float* __restrict__ o = a.dx + r * a.ldd;
   const float lse = a.lse[r];
   const int64_t tok = a.tok[r];
-  const float g = a.g != nullptr && tok >= 0 && tok < a.V ? a.g[r] : 0.f;
-  const float gh = a.gh != nullptr ? a.gh[r] : 0.f;
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < a.V; i += gridDim.y * 256) {
-    const float lp = Elem<T>::to_f(static_cast<const T*>(a.x)[r * a.ld + i]) * a.scale - lse;
-    const float p = lse == -INFINITY ? 0.f : expf(lp);
-    float d = p == 0.f ? 0.f : -p * (g + gh * (lp + a.entropy[r]));
-    if (i == tok && lse != -INFINITY) d += g;
-    d *= a.scale;
-    float* o = a.dx + r * a.ldd + i;
-    *o = a.accumulate ? *o + d : d;
+  const bool none = lse == -INFINITY;
+  const float g = a.g != nullptr && tok >= 0 && tok < a.V && !none ? a.g[r] : 0.f;
+  const float gh = a.gh != nullptr && !none ? a.gh[r] : 0.f;
+  const float A = -a.scale * fmaf(gh, none ? 0.f : a.entropy[r], g), Bf = -a.scale * gh, own = a.scale * g;
+  const float off = none ? 0.f : lse;
+  const int step = 4 * a.per;
+  const int i0 = (int)(blockIdx.y * kUnroll * step + 4 * (threadIdx.x % a.per));
+  float v[kUnroll][4];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int i = i0 + u * step;
+    if (i + 4 <= a.V) {
+      load_values<4>(x + i, v[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[u][e] = i + e < a.V ? Elem<T>::to_f(x[i + e]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int i = i0 + u * step;
+    if (i >= a.V) break;
+    float d[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float lp = below(fmaf(v[u][e], a.scale, -off)), p = __builtin_amdgcn_exp2f(lp * kLog2e);
+      d[e] = p * fmaf(Bf, lp, A);
+      if (i + e == tok) d[e] += own;
+    }
+    if (i + 4 <= a.V) {
+      auto* q = reinterpret_cast<Unaligned<float, 4>*>(o + i);
+      Unaligned<float, 4> w;
+      if (a.accumulate) {
+        w = *q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.x[e] += d[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.x[e] = d[e];
+      }
+      *q = w;
+    } else {
+      for (int e = 0; e < 4 && i + e < a.V; ++e) o[i + e] = a.accumulate ? o[i + e] + d[e] : d[e];
+    }
   }
 }
 
 int check_rows(int dtype, int64_t rows, int V, const void* logits, int64_t ld, const int64_t* tokens, float scale) {
   if (dtype != MTX_F32 && dtype != MTX_BF16) return fail(MTX_ERR_DTYPE, "unsupported dtype %d", dtype);
-  MTX_CHECK_SHAPE(rows >= 1 && rows <= (1 << 30) && V >= 1 && V <= (1 << 28),
-                  "token_logprobs: needs rows >= 1 and 1 <= V <= 2^28 (got %lld, %d)", (long long)rows, V);
+  MTX_CHECK_SHAPE(rows >= 1 && rows <= (1 << 30) && V >= 1 && V <= (1 << 27),
+                  "token_logprobs: needs rows >= 1 and 1 <= V <= 2^27 (got %lld, %d)", (long long)rows, V);
   MTX_CHECK_ARG(logits != nullptr && tokens != nullptr, "logits, tokens: null pointer");
   MTX_CHECK_ARG(((uintptr_t)logits & (dtype == MTX_F32 ? 3u : 1u)) == 0, "logits: pointer must be aligned to its type");
   MTX_CHECK_ARG(ld >= V || (rows == 1 && ld >= 0), "logits: row stride %lld < V=%d", (long long)ld, V);
@@ -143,6 +399,20 @@ int check_rows(int dtype, int64_t rows, int V, const void* logits, int64_t ld, c
 }
 
 constexpr int kMostTop = 64;
+
+template <typename T>
+int launch_logprobs(const LpArgs& a, int64_t rows, hipStream_t st) {
+  const dim3 four((unsigned)((rows + 3) / 4));
+  if (a.V <= 64) hipLaunchKernelGGL((logprobs_small_kernel<T, 1>), four, dim3(256), 0, st, a, rows);
+  else if (a.V <= 128) hipLaunchKernelGGL((logprobs_small_kernel<T, 2>), four, dim3(256), 0, st, a, rows);
+  else if (a.V <= 256) hipLaunchKernelGGL((logprobs_small_kernel<T, 4>), four, dim3(256), 0, st, a, rows);
+  else if (a.V <= 512) hipLaunchKernelGGL((logprobs_small_kernel<T, 8>), four, dim3(256), 0, st, a, rows);
+  else if (a.V <= 1024) hipLaunchKernelGGL((logprobs_small_kernel<T, 16>), four, dim3(256), 0, st, a, rows);
+  else if (a.V <= 8192) hipLaunchKernelGGL((logprobs_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((logprobs_kernel<T, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, a);
+  MTX_LAUNCHED();
+  return MTX_OK;
+}
 
 }  // namespace
 }  // namespace mtx
@@ -163,10 +433,7 @@ extern "C" int mtx_token_logprobs(int dtype, int64_t rows, int V, const void* lo
   MTX_CHECK_ARG(top == 0 || (top_ids && top_logprobs), "top_ids, top_logprobs: null pointer");
   LpArgs a{logits, ld, tokens, logprob, lse, entropy, top_ids, top_logprobs, V, top, scale};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == MTX_F32) hipLaunchKernelGGL(logprobs_kernel<float>, dim3((unsigned)rows), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(logprobs_kernel<bf16_t>, dim3((unsigned)rows), dim3(256), 0, st, a);
-  MTX_LAUNCHED();
-  return MTX_OK;
+  return dtype == MTX_F32 ? launch_logprobs<float>(a, rows, st) : launch_logprobs<bf16_t>(a, rows, st);
 }
 
 extern "C" int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void* logits, int64_t ld,
@@ -178,9 +445,12 @@ extern "C" int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void
   MTX_CHECK_ARG(lse && entropy && dlogits, "lse, entropy, dlogits: null pointer");
   MTX_CHECK_ARG(((uintptr_t)dlogits & 3u) == 0 && (ldd >= V || (rows == 1 && ldd >= 0)),
                 "dlogits: row stride %lld < V=%d", (long long)ldd, V);
-  LpBwdArgs a{logits, ld, tokens, lse, entropy, g_logprob, g_entropy, dlogits, ldd, V, scale, accumulate};
+  int per = 16;
+  while (per < 256 && per * 4 < V) per *= 2;
+  LpBwdArgs a{logits, ld, tokens, lse, entropy, g_logprob, g_entropy, dlogits, ldd, rows, V, per, scale, accumulate};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)rows, std::min(cdiv(V, 1024), 65535));
+  const int64_t groups = (rows + 256 / per - 1) / (256 / per);
+  const dim3 grid((unsigned)groups, (unsigned)cdiv(V, 4 * per * kUnroll));
   if (dtype == MTX_F32) hipLaunchKernelGGL(logprobs_bwd_kernel<float>, grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL(logprobs_bwd_kernel<bf16_t>, grid, dim3(256), 0, st, a);
   MTX_LAUNCHED();
