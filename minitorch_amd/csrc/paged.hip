@@ -69,27 +69,35 @@ struct AppendArgs {
   Table tab;
   const int* lengths;
   const int* counts;
-  int T, H, D, blocks;
+  int T, H, C, blocks;  // C: 16-byte chunks of a cached row
 };
 
+// 16 bytes of a cached row from the values of a new one
+__device__ __forceinline__ uint4 cache_chunk(const float* x, float*) { return *reinterpret_cast<const uint4*>(x); }
+__device__ __forceinline__ uint4 cache_chunk(const bf16_t* x, bf16_t*) { return *reinterpret_cast<const uint4*>(x); }
+__device__ __forceinline__ uint4 cache_chunk(const float* x, bf16_t*) {
+  const f32x4 u = reinterpret_cast<const f32x4*>(x)[0], v = reinterpret_cast<const f32x4*>(x)[1];
+  return make_uint4(pack_bf2(u[0], u[1]), pack_bf2(u[2], u[3]), pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+}
+
+// A thread writes 16 bytes of a row's key and of its value, found by one lookup
 template <typename TX, typename TC>
 __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
-  const int z = blockIdx.y, b = blockIdx.x / a.blocks;
-  const int c8 = a.D >> 3;  // chunks of 8 values a row
+  constexpr int E = 16 / sizeof(TC);
+  const int b = blockIdx.x / a.blocks;
   const int i = (blockIdx.x % a.blocks) * 256 + threadIdx.x;
-  if (i >= a.T * a.H * c8) return;
-  const int c = i % c8, h = (i / c8) % a.H, t = i / (c8 * a.H);
+  const int c = i & (a.C - 1), row = i / a.C, h = row % a.H, t = row / a.H;
+  if (t >= a.T) return;
   const int n = a.counts != nullptr ? min(a.counts[b], a.T) : a.T;
-  const int j = a.lengths[b] - n + t;
-  if (t >= n || j < 0 || j >= a.tab.width * a.tab.page) return;
-  const int pi = a.tab.div(j), id = a.tab.id(b, pi);
+  const int64_t j = (int64_t)a.lengths[b] - n + t;
+  if (t >= n || j < 0 || j >= (int64_t)a.tab.width * a.tab.page) return;
+  const int pi = a.tab.div((int)j), id = a.tab.id(b, pi);
   if (id < 0) return;
-  const TX* __restrict__ x = static_cast<const TX*>(a.x[z]) + b * a.sb[z] + h * a.sh[z] + t * a.st[z] + 8 * c;
-  TC* __restrict__ y = static_cast<TC*>(a.g[z].p) + row_at(a.g[z], a.tab, id, pi, j) + h * a.g[z].sh + 8 * c;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if constexpr (sizeof(TX) == sizeof(TC)) y[e] = x[e];
-    else y[e] = Elem<TC>::from_f(Elem<TX>::to_f(x[e]));
+  for (int z = 0; z < 2; ++z) {
+    const TX* x = static_cast<const TX*>(a.x[z]) + b * a.sb[z] + h * a.sh[z] + t * a.st[z] + E * c;
+    TC* y = static_cast<TC*>(a.g[z].p) + row_at(a.g[z], a.tab, id, pi, (int)j) + h * a.g[z].sh + E * c;
+    *reinterpret_cast<uint4*>(y) = cache_chunk(x, y);
   }
 }
 
@@ -561,7 +569,8 @@ struct EvictArgs {
   int* lengths_out;
   float* w_out;
   int* slots;
-  int B, H, D, cap, keep, recent;
+  int B, H, cap, keep, recent;
+  int C, es;  // 16-byte chunks of a row, bytes of a value
 };
 
 // order of weights as unsigned numbers: NaN above everything, -0 equal to 0
@@ -571,87 +580,221 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
-__device__ __forceinline__ int block_count(int v, int* red) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
-}
+// Selection, one workgroup of NT threads per sequence and K/V head: the key of
+// the last kept row (of the cand rows that are not recent, `want` are kept), then
+// the kept rows in order.  The range of keys [lo, hi] is cut into up to 2048 equal
+// bins, counted in LDS; the bin in which the want-th largest key lies is the next
+// range: at most three rounds, fewer where the weights are spread less (equal
+// weights: none).  Rows are held in registers, R a thread (rows 4 (NT i + tid) + e
+// in v[i][e]), where they fit (SINGLE), so that they are read once; otherwise each
+// round reads them again, NT R at a time.
+constexpr int kBins = 2048;
 
-// one workgroup per sequence and K/V head: the smallest key that is kept, bit
-// by bit, then the kept slots in order
-__global__ __launch_bounds__(256) void select_kernel(const EvictArgs a) {
-  __shared__ int red[4], scan[256];
-  const int bh = blockIdx.x, b = bh / a.H, tid = threadIdx.x;
+template <int NT, int R, bool SINGLE>
+__global__ __launch_bounds__(NT) void select_kernel(const EvictArgs a) {
+  constexpr int W = NT / 64, NI = R / 4, BLOCK = NT * R;
+  __shared__ int bins[kBins], part[W], gts[NI * W], ties[NI * W], total[2];
+  __shared__ uint32_t mins[W], maxs[W], found[3];
+  const int bh = blockIdx.x, b = bh / a.H, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int len = min(max(a.lengths[b], 0), a.cap);
   const float* __restrict__ w = a.w + bh * a.wld;
   int* __restrict__ slots = a.slots + (int64_t)bh * a.keep;
   float* __restrict__ wo = a.w_out + bh * a.wld;
   if (tid == 0 && bh % a.H == 0) a.lengths_out[b] = min(len, a.keep);
-  const int cand = len > a.keep ? len - a.recent : 0, want = a.keep - a.recent;
-  uint32_t bound = 0;
-  if (cand > 0) {
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t t = bound | (1u << bit);
-      int n = 0;
-      for (int j = tid; j < cand; j += 256) n += weight_key(w[j]) >= t;
-      if (block_count(n, red) >= want) bound = t;
+  const int cand = len > a.keep ? len - a.recent : 0;
+  int want = a.keep - a.recent;
+
+  uint32_t key[R];  // 0, which no weight has, where there is no candidate
+  auto load = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int j = base + 4 * (NT * i + tid);
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = j + e < cand ? w[j + e] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) key[4 * i + e] = j + e < cand ? weight_key(x[e]) : 0u;
     }
+  };
+  if (SINGLE) load(0);
+  auto each = [&](auto f) {
+    for (int base = 0; base < cand; base += BLOCK) {
+      if (!SINGLE) load(base);
+#pragma unroll
+      for (int i = 0; i < R; ++i) f(key[i]);
+    }
+  };
+
+  uint32_t bound = 0;  // smallest kept key; `want` of the rows that have it are kept
+  if (cand > 0 && want > 0) {
+    uint32_t lo = 0xffffffffu, hi = 0;
+    each([&](uint32_t k) {
+      lo = min(lo, k - 1u);
+      hi = max(hi, k);
+    });
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+      lo = min(lo, (uint32_t)__shfl_xor((int)lo, m, 64));
+      hi = max(hi, (uint32_t)__shfl_xor((int)hi, m, 64));
+    }
+    if (lane == 0) mins[wave] = lo, maxs[wave] = hi;
+    __syncthreads();
+    for (int i = 0; i < W; ++i) lo = min(lo, mins[i]), hi = max(hi, maxs[i]);
+    ++lo;
+    while (lo < hi) {
+      const int shift = max(0, 21 - __clz((int)(hi - lo)));  // (hi - lo) >> shift < kBins
+      for (int i = tid; i < kBins; i += NT) bins[i] = 0;
+      __syncthreads();
+      each([&](uint32_t k) {
+        if (k - lo <= hi - lo) atomicAdd(&bins[(k - lo) >> shift], 1);
+      });
+      __syncthreads();
+      // from the top bin down: a thread's bins, its wave's, the waves above
+      constexpr int PB = kBins / NT;
+      const int top = kBins - 1 - PB * tid;
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < PB; ++i) mine += bins[top - i];
+      int upto = mine;
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const int x = __shfl_up(upto, m, 64);
+        if (lane >= m) upto += x;
+      }
+      if (lane == 63) part[wave] = upto;
+      __syncthreads();
+      for (int i = 0; i < wave; ++i) upto += part[i];
+      if (upto - mine < want && upto >= want) {
+        int above = upto - mine, i = 0;
+        while (above + bins[top - i] < want) above += bins[top - i++];
+        const uint32_t l = lo + ((uint32_t)(top - i) << shift);
+        found[0] = l;
+        found[1] = l + min(hi - l, (1u << shift) - 1);
+        found[2] = (uint32_t)(want - above);
+      }
+      __syncthreads();
+      lo = found[0], hi = found[1], want = (int)found[2];
+    }
+    bound = lo;
+  } else {
+    bound = 0xffffffffu;  // no candidate, or none of them
+    want = 0;
   }
-  int above = 0;
-  for (int j = tid; j < cand; j += 256) above += weight_key(w[j]) > bound;
-  int ties = want - block_count(above, red);  // of those equal to the bound, the first ones
-  int at = 0;
-  for (int j0 = 0; j0 < len; j0 += 256) {
-    const int j = j0 + tid;
-    const uint32_t key = j < cand ? weight_key(w[j]) : 0u;
-    const bool tie = j < cand && key == bound;
-    scan[tid] = tie;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < 256; ++i) {
-      before += i < tid ? scan[i] : 0;
-      all += scan[i];
+
+  // positions: rows above the bound and recent ones before a row, and of those
+  // at the bound the first `want`
+  int gat = 0, tat = 0;  // of the blocks before
+  for (int base = 0; base < len; base += BLOCK) {
+    if (!SINGLE) load(base);
+    auto above = [&](int i, int e) {
+      const int j = base + 4 * (NT * i + tid) + e;
+      return key[4 * i + e] > bound || (j >= cand && j < len);
+    };
+    auto equal = [&](int i, int e) { return key[4 * i + e] == bound && want > 0; };
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      int ng = 0, nt = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ng += __popcll(__ballot(above(i, e)));
+        nt += __popcll(__ballot(equal(i, e)));
+      }
+      if (lane == 0) gts[i * W + wave] = ng, ties[i * W + wave] = nt;
     }
     __syncthreads();
-    const bool kept = j < len && (j >= cand || key > bound || (tie && before < ties));
-    ties = max(0, ties - all);
-    scan[tid] = kept;
-    __syncthreads();
-    before = 0, all = 0;
-    for (int i = 0; i < 256; ++i) {
-      before += i < tid ? scan[i] : 0;
-      all += scan[i];
+    if (wave == 0) {  // exclusive sums in order of rows
+      int g0 = gat, t0 = tat;
+      for (int x0 = 0; x0 < NI * W; x0 += 64) {
+        const int x = x0 + lane;
+        const int g = x < NI * W ? gts[x] : 0, t = x < NI * W ? ties[x] : 0;
+        int gs = g, ts = t;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+          const int gx = __shfl_up(gs, m, 64), tx = __shfl_up(ts, m, 64);
+          if (lane >= m) gs += gx, ts += tx;
+        }
+        if (x < NI * W) gts[x] = g0 + gs - g, ties[x] = t0 + ts - t;
+        g0 += __shfl(gs, 63, 64);
+        t0 += __shfl(ts, 63, 64);
+      }
+      if (lane == 0) total[0] = g0, total[1] = t0;
     }
     __syncthreads();
-    if (kept && at + before < a.keep) {
-      slots[at + before] = j;
-      wo[at + before] = w[j];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      // within the wave: lanes below, then this lane's rows in order
+      int ga = gts[i * W + wave], ta = ties[i * W + wave];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t bg = __ballot(above(i, e)), bt = __ballot(equal(i, e));
+        ga = __builtin_amdgcn_mbcnt_hi((uint32_t)(bg >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bg, ga));
+        ta = __builtin_amdgcn_mbcnt_hi((uint32_t)(bt >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bt, ta));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = base + 4 * (NT * i + tid) + e, pos = ga + min(ta, want);
+        const bool isg = above(i, e), ist = equal(i, e);
+        if ((isg || (ist && ta < want)) && pos < a.keep) {
+          slots[pos] = j;
+          wo[pos] = w[j];
+        }
+        ga += isg;
+        ta += ist;
+      }
     }
-    at += all;
+    gat = total[0], tat = total[1];
+    __syncthreads();
   }
-  for (int j = at + tid; j < a.keep; j += 256) slots[j] = -1;
-  for (int j = at + tid; j < a.cap; j += 256) wo[j] = 0.f;
 }
 
-template <typename TC>
-__global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a, int blocks) {
-  const int bh = blockIdx.x / blocks, b = bh / a.H, h = bh % a.H;
-  const int c8 = a.D >> 3, i = (blockIdx.x % blocks) * 256 + threadIdx.x;
-  const int r = i / c8, c = i % c8;
-  if (r >= a.keep) return;
-  const int j = a.slots[(int64_t)bh * a.keep + r];
-  if (j < 0) return;
-  const int fi = a.from.div(j), ti = a.to.div(r);
-  const int from = a.from.id(b, fi), to = a.to.id(b, ti);
-  if (to < 0) return;
-  const Pages& g = blockIdx.y ? a.v : a.k;
-  const TC* __restrict__ x = static_cast<const TC*>(g.p) + row_at(g, a.from, from < 0 ? 0 : from, fi, j) + h * g.sh + 8 * c;
-  TC* __restrict__ y = static_cast<TC*>(g.p) + row_at(g, a.to, to, ti, r) + h * g.sh + 8 * c;
+// Copies the kept rows, a thread 16 bytes of the keys and the values of kRows
+// rows; the last blocks of a sequence and head clear the weights behind them
+constexpr int kRows = 4;
+__global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a, int blocks, int fills) {
+  const int bh = blockIdx.x / (blocks + fills), block = blockIdx.x % (blocks + fills);
+  const int b = bh / a.H, h = bh % a.H;
+  const int new_len = min(min(max(a.lengths[b], 0), a.cap), a.keep);
+  if (block >= blocks) {
+    float* wo = a.w_out + bh * a.wld;
+    int* slots = a.slots + (int64_t)bh * a.keep;
+    for (int j = new_len + (block - blocks) * 256 + threadIdx.x; j < max(a.cap, a.keep); j += fills * 256) {
+      if (j < a.cap) wo[j] = 0.f;
+      if (j < a.keep) slots[j] = -1;
+    }
+    return;
+  }
+  const int c = threadIdx.x & (a.C - 1), per = 256 / a.C, r0 = block * per * kRows + threadIdx.x / a.C;
+  const int* __restrict__ slots = a.slots + (int64_t)bh * a.keep;
+  int j[kRows], fi[kRows], from[kRows], to[kRows], ti[kRows];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = from < 0 ? (TC)0 : x[e];
+  for (int i = 0; i < kRows; ++i) j[i] = r0 + per * i < new_len ? slots[r0 + per * i] : -1;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    fi[i] = a.from.div(max(j[i], 0));
+    ti[i] = a.to.div(r0 + per * i);
+    from[i] = j[i] < 0 ? -1 : a.from.id(b, fi[i]);
+    to[i] = j[i] < 0 ? -1 : a.to.id(b, ti[i]);
+  }
+  uint4 x[kRows], y[kRows];
+  const int64_t es = a.es;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    x[i] = y[i] = make_uint4(0, 0, 0, 0);
+    if (from[i] < 0) continue;
+    x[i] = reinterpret_cast<const uint4*>(static_cast<const char*>(a.k.p) +
+                                          es * (row_at(a.k, a.from, from[i], fi[i], j[i]) + h * a.k.sh))[c];
+    y[i] = reinterpret_cast<const uint4*>(static_cast<const char*>(a.v.p) +
+                                          es * (row_at(a.v, a.from, from[i], fi[i], j[i]) + h * a.v.sh))[c];
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    if (to[i] < 0) continue;
+    const int r = r0 + per * i;
+    reinterpret_cast<uint4*>(static_cast<char*>(a.k.p) +
+                             es * (row_at(a.k, a.to, to[i], ti[i], r) + h * a.k.sh))[c] = x[i];
+    reinterpret_cast<uint4*>(static_cast<char*>(a.v.p) +
+                             es * (row_at(a.v, a.to, to[i], ti[i], r) + h * a.v.sh))[c] = y[i];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -780,11 +923,11 @@ extern "C" int mtx_kv_append_paged(int dtype, int cache_dtype, int B, int T, int
                counts,
                T,
                H,
-               D,
-               cdiv(T * H * (D / 8), 256)};
+               D * ec / 16,
+               cdiv(T * H * (D * ec / 16), 256)};
   MTX_CHECK_SHAPE((int64_t)B * a.blocks <= INT32_MAX, "append: too many rows in one call");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(B * a.blocks, 2);
+  const dim3 grid(B * a.blocks);
   if (cache_dtype == MTX_F32) hipLaunchKernelGGL((append_kernel<float, float>), grid, dim3(256), 0, st, a);
   else if (dtype == MTX_F32) hipLaunchKernelGGL((append_kernel<float, bf16_t>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((append_kernel<bf16_t, bf16_t>), grid, dim3(256), 0, st, a);
@@ -876,15 +1019,20 @@ extern "C" int mtx_kv_evict_paged(int cache_dtype, int B, int H, int D, int64_t 
               {v_pages, vp_strides[0], vp_strides[1], vp_strides[2]},
               make_table(table, table_ld, max_pages, page, n_pages),
               make_table(to_table, to_ld, to_pages, page, n_pages),
-              lengths, weights, weights_ld, lengths_out, weights_out, slots, B, H, D, cap, keep, recent};
+              lengths, weights, weights_ld, lengths_out, weights_out, slots, B, H, cap, keep, recent,
+              D * ec / 16, ec};
+  const int64_t blocks = cdiv(rows, kRows * (256 / a.C)), fills = std::min(cdiv(std::max(cap, keep), 4096), 64);
+  MTX_CHECK_SHAPE((blocks + fills) * B * H <= INT32_MAX, "evict: too many rows in one call");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(select_kernel, dim3(B * H), dim3(256), 0, st, a);
+  const dim3 grid(B * H);
+  if (cap <= 256 * 4) hipLaunchKernelGGL((select_kernel<256, 4, true>), grid, dim3(256), 0, st, a);
+  else if (cap <= 1024 * 4) hipLaunchKernelGGL((select_kernel<1024, 4, true>), grid, dim3(1024), 0, st, a);
+  else if (cap <= 1024 * 16) hipLaunchKernelGGL((select_kernel<1024, 16, true>), grid, dim3(1024), 0, st, a);
+  else if (cap <= 1024 * 48) hipLaunchKernelGGL((select_kernel<1024, 48, true>), grid, dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL((select_kernel<1024, 16, false>), grid, dim3(1024), 0, st, a);
   MTX_LAUNCHED();
-  const int64_t blocks = ((int64_t)rows * (D / 8) + 255) / 256;
-  MTX_CHECK_SHAPE(blocks * B * H <= INT32_MAX, "evict: too many rows in one call");
-  const dim3 grid((unsigned)(blocks * B * H), 2);
-  if (cache_dtype == MTX_F32) hipLaunchKernelGGL(gather_kernel<float>, grid, dim3(256), 0, st, a, (int)blocks);
-  else hipLaunchKernelGGL(gather_kernel<bf16_t>, grid, dim3(256), 0, st, a, (int)blocks);
+  hipLaunchKernelGGL(gather_kernel, dim3((unsigned)((blocks + fills) * B * H)), dim3(256), 0, st, a, (int)blocks,
+                     (int)fills);
   MTX_LAUNCHED();
   return MTX_OK;
 }
