@@ -11,6 +11,7 @@ is raised.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from pathlib import Path
 
@@ -254,6 +255,12 @@ _STREAM = [None]
 
 def strides(t) -> C.Array:
     s = t.stride()
+    return (C.c_int64 * len(s))(*s)
+
+
+@functools.lru_cache(maxsize=4096)
+def stride_array(s) -> C.Array:
+    """A tuple of element strides as the int64 array the entry points read."""
     return (C.c_int64 * len(s))(*s)
 
 

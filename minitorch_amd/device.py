@@ -40,16 +40,22 @@ def dtype_name(x) -> str:
     if type(x) is DevBuf:
         return x.dtype
     d = x if isinstance(x, (str, type, np.dtype)) else getattr(x, "dtype", x)
-    if isinstance(d, str):
-        name = d
-    else:
-        try:
-            name = np.dtype(d).name
-        except TypeError:
-            name = str(d).rsplit(".", 1)[-1]
-    if name not in ITEMSIZE:
-        raise ValueError(f"unsupported dtype {d!r}")
+    name = _NAMES.get(d)
+    if name is None:
+        if isinstance(d, str):
+            name = d
+        else:
+            try:
+                name = np.dtype(d).name
+            except TypeError:
+                name = str(d).rsplit(".", 1)[-1]
+        if name not in ITEMSIZE:
+            raise ValueError(f"unsupported dtype {d!r}")
+        _NAMES[d] = name
     return name
+
+
+_NAMES: dict = {}  # the names of the dtypes asked for so far
 
 
 _READY = False

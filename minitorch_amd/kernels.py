@@ -164,27 +164,98 @@ def attn_decode(q, k, v, scale: float, out=None, lse=None, lengths=None):
 # keys and values in pages
 # ---------------------------------------------------------------------------
 
+# A decode step makes many small calls, so what a wrapper checks and derives of
+# its operands' shapes, strides and dtypes is kept per combination of them (the
+# cached *_plan functions, which never see an address); a call then only passes
+# pointers.
+
+def _spec(t):
+    """(shape, strides, dtype) of a device array; None for None."""
+    if type(t) is dev.DevBuf:
+        return t.shape, t._strides, t.dtype
+    if t is None:
+        return None
+    _need_cuda(t)
+    return t.shape, t.stride(), t.dtype
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _packed(shape, strides):
+    """Whether strides are C order's (those of dimensions of 1 do not matter)."""
+    acc = 1
+    for n, st in zip(shape[::-1], strides[::-1]):
+        if n != 1 and st != acc:
+            return False
+        acc *= n
+    return True
+
+
+def _vector(name, spec, n, dtype):
+    if spec is not None and (_dt(spec[2]) != dtype or tuple(spec[0]) != (n,) or not _packed(spec[0], spec[1])):
+        raise ValueError(f"{name} must be contiguous {dtype} ({n},)")
+
+
+def _view4(name, spec):
+    """(shape, stride array, dtype) of a 4-d view with a contiguous last axis."""
+    shape, strides, dtype = spec
+    if len(shape) != 4 or strides[3] != 1:
+        raise ValueError(f"{name}: expected a 4-d view with a contiguous last (d) axis, got shape {tuple(shape)}, "
+                         f"strides {tuple(strides)}")
+    return tuple(shape), L.stride_array(tuple(strides)), _dt(dtype)
+
+
 def _paged(k_pages, v_pages, table, lengths):
-    """(n_pages, Hkv, page, D, B) of a paged cache, checked: two
-    (n_pages, Hkv, page, D) views of one dtype, an int32 (B, max_pages) table
-    with contiguous rows and int32 (B,) lengths."""
-    _need_cuda(k_pages, v_pages, table, lengths)
-    if len(k_pages.shape) != 4 or tuple(k_pages.shape) != tuple(v_pages.shape) or _dt(k_pages) != _dt(v_pages):
+    """Checks a paged cache's specs: two (n_pages, Hkv, page, D) views of one
+    dtype, an int32 (B, max_pages) table with contiguous rows and int32 (B,)
+    lengths.  Returns (shape, dtype, the views' strides, B, table row stride,
+    max_pages)."""
+    shape, ks, dtype = _view4("k_pages", k_pages)
+    vshape, vs, vdtype = _view4("v_pages", v_pages)
+    if shape != vshape or dtype != vdtype:
         raise ValueError("k_pages and v_pages must be (n_pages, Hkv, page, D) views of one shape and dtype")
-    if _dt(table) != "int32" or len(table.shape) != 2 or table.stride(1) != 1:
-        raise ValueError("table must be int32 (B, max_pages) with contiguous rows")
-    B = table.shape[0]
-    if _dt(lengths) != "int32" or tuple(lengths.shape) != (B,) or not lengths.is_contiguous():
-        raise ValueError(f"lengths must be contiguous int32 ({B},)")
-    return (*k_pages.shape, B)
+    B, width, ld = _table("table", table)
+    _vector("lengths", lengths, B, "int32")
+    return shape, dtype, ks, vs, B, ld, width
 
 
-def _row_weights(name, w, B, Hkv, cap):
+def _table(name, spec, B=None):
+    shape, strides, dtype = spec
+    if _dt(dtype) != "int32" or len(shape) != 2 or strides[1] != 1 or (B is not None and shape[0] != B):
+        raise ValueError(f"{name} must be int32 ({'B' if B is None else B}, pages) with contiguous rows")
+    return shape[0], shape[1], strides[0]
+
+
+def _row_weights(name, spec, B, Hkv, cap, like=None):
     """Checks weights of cached rows: contiguous fp32 (B, Hkv, >= cap)."""
-    _need_cuda(w)
-    if _dt(w) != "float32" or len(w.shape) != 3 or tuple(w.shape[:2]) != (B, Hkv) or w.shape[2] < cap \
-            or not w.is_contiguous():
-        raise ValueError(f"{name} must be contiguous fp32 ({B}, {Hkv}, >= {cap})")
+    shape, strides, dtype = spec
+    if _dt(dtype) != "float32" or len(shape) != 3 or tuple(shape[:2]) != (B, Hkv) or shape[2] < cap \
+            or not _packed(shape, strides) or (like is not None and shape[2] != like):
+        raise ValueError(f"{name} must be contiguous fp32 ({B}, {Hkv}, {like or f'>= {cap}'})")
+    return shape[2]
+
+
+_CODES = {"float32": L.MTX_F32, "bfloat16": L.MTX_BF16}
+
+
+def _code(dtype):
+    if dtype not in _CODES:
+        raise ValueError(f"unsupported dtype {dtype} (float32 or bfloat16)")
+    return _CODES[dtype]
+
+
+@functools.lru_cache(maxsize=512)
+def _append_plan(k, v, k_pages, v_pages, table, lengths, counts):
+    (n_pages, Hkv, page, D), cache, kps, vps, B, ld, width = _paged(k_pages, v_pages, table, lengths)
+    kshape, ks, kd = _view4("k", k)
+    vshape, vs, vd = _view4("v", v)
+    T = kshape[2]
+    if kshape != (B, Hkv, T, D) or vshape != kshape or kd != vd:
+        raise ValueError(f"k and v must be ({B}, {Hkv}, T, {D}) of one dtype (got {kshape}, {vshape})")
+    _vector("counts", counts, B, "int32")
+    return (_code(kd), _code(cache), B, T, Hkv, D), (ks, vs), (n_pages, page), (kps, vps), (ld, width)
 
 
 def kv_append_paged(k, v, k_pages, v_pages, table, lengths, counts=None):
@@ -192,27 +263,33 @@ def kv_append_paged(k, v, k_pages, v_pages, table, lengths, counts=None):
     (B, Hkv, T, D) views, to the end of its pages (mtx_kv_append_paged).
     lengths (B,) counts them already; counts (int32 (B,)): sequence b appends
     only its first counts[b] rows.  fp32 rows may go to a bf16 pool."""
-    n_pages, Hkv, page, D, B = _paged(k_pages, v_pages, table, lengths)
-    _need_cuda(k, v)
-    _bhtd("k", k)
-    _bhtd("v", v)
-    T = k.shape[2]
-    if tuple(k.shape) != (B, Hkv, T, D) or tuple(v.shape) != (B, Hkv, T, D) or _dt(k) != _dt(v):
-        raise ValueError(f"k and v must be ({B}, {Hkv}, T, {D}) of one dtype (got {tuple(k.shape)}, {tuple(v.shape)})")
-    if counts is not None:
-        _need_cuda(counts)
-        if _dt(counts) != "int32" or tuple(counts.shape) != (B,) or not counts.is_contiguous():
-            raise ValueError(f"counts must be contiguous int32 ({B},)")
-    L.call("mtx_kv_append_paged", L.dtype_code(k), L.dtype_code(k_pages), B, T, Hkv, D, L.ptr(k), L.strides(k),
-           L.ptr(v), L.strides(v), n_pages, page, L.ptr(k_pages), L.strides(k_pages), L.ptr(v_pages),
-           L.strides(v_pages), L.ptr(table), table.stride(0), table.shape[1], L.ptr(lengths),
-           L.ptr(counts) if counts is not None else None, L.stream_handle())
+    sizes, (ks, vs), (n, page), (kps, vps), (ld, width) = _append_plan(
+        _spec(k), _spec(v), _spec(k_pages), _spec(v_pages), _spec(table), _spec(lengths), _spec(counts))
+    L.call("mtx_kv_append_paged", *sizes, k.data_ptr(), ks, v.data_ptr(), vs, n, page, k_pages.data_ptr(), kps,
+           v_pages.data_ptr(), vps, table.data_ptr(), ld, width, lengths.data_ptr(), _ptr(counts), L.stream_handle())
 
 
 @functools.lru_cache(maxsize=512)
-def _decode_paged_workspace_bytes(*sizes):
-    """mtx_attn_decode_paged_workspace_bytes, a function of the sizes alone."""
-    return L.lib().mtx_attn_decode_paged_workspace_bytes(*sizes)
+def _decode_paged_plan(q, k_pages, v_pages, table, lengths, out, lse, weights, weights_in):
+    (n_pages, Hkv, page, D), cache, kps, vps, B, ld, width = _paged(k_pages, v_pages, table, lengths)
+    qshape, qs, qd = _view4("q", q)
+    H = qshape[1]
+    if qshape != (B, H, 1, D):
+        raise ValueError(f"q must be ({B}, H, 1, {D}) (got {qshape})")
+    oshape, os, od = _view4("out", out)
+    if oshape != qshape or od != qd:
+        raise ValueError("out must have q's shape and dtype")
+    if lse is not None and (_dt(lse[2]) != "float32" or tuple(lse[0]) != (B, H) or not _packed(*lse[:2])):
+        raise ValueError("lse must be a contiguous fp32 (B,H) tensor")
+    wld = 0
+    if weights is not None:
+        wld = _row_weights("weights", weights, B, Hkv, width * page)
+        if weights_in is not None:
+            _row_weights("weights_in", weights_in, B, Hkv, width * page, wld)
+    elif weights_in is not None:
+        raise ValueError("weights_in without weights")
+    ws = L.lib().mtx_attn_decode_paged_workspace_bytes(B, H, Hkv, D, page, width, int(weights is not None))
+    return (_code(qd), _code(cache), B, H, Hkv, D), (qs, os), (n_pages, page), (kps, vps), (ld, width), wld, ws
 
 
 def attn_decode_paged(q, k_pages, v_pages, table, lengths, scale: float, out=None, lse=None, weights=None,
@@ -223,42 +300,29 @@ def attn_decode_paged(q, k_pages, v_pages, table, lengths, scale: float, out=Non
     (B, Hkv, >= max_pages * page) fp32: receives weights_in (0 without it; it
     may be weights itself) plus the attention each cached row got.  Returns
     (out like q, lse or None)."""
-    n_pages, Hkv, page, D, B = _paged(k_pages, v_pages, table, lengths)
-    _need_cuda(q)
-    _bhtd("q", q)
-    H = q.shape[1]
-    if tuple(q.shape) != (B, H, 1, D):
-        raise ValueError(f"q must be ({B}, H, 1, {D}) (got {tuple(q.shape)})")
+    qspec = _spec(q)
     if out is None:
-        out = dev.empty_buf((B, H, 1, D), _dt(q))
-    _need_cuda(out)
-    _bhtd("out", out)
-    if tuple(out.shape) != (B, H, 1, D) or _dt(out) != _dt(q):
-        raise ValueError("out must have q's shape and dtype")
-    if lse is not None:
-        _need_cuda(lse)
-        if not lse.is_contiguous() or tuple(lse.shape) != (B, H) or _dt(lse) != "float32":
-            raise ValueError("lse must be a contiguous fp32 (B,H) tensor")
-    width = table.shape[1]
-    wld = 0
-    if weights is not None:
-        _row_weights("weights", weights, B, Hkv, width * page)
-        wld = weights.shape[2]
-        if weights_in is not None:
-            _row_weights("weights_in", weights_in, B, Hkv, width * page)
-            if tuple(weights_in.shape) != tuple(weights.shape):
-                raise ValueError("weights_in must have weights' shape")
-    elif weights_in is not None:
-        raise ValueError("weights_in without weights")
-    ws_bytes = _decode_paged_workspace_bytes(B, H, Hkv, D, page, width, int(weights is not None))
+        out = dev.empty_buf(q.shape, _dt(q))
+    sizes, (qs, os), (n, page), (kps, vps), (ld, width), wld, ws_bytes = _decode_paged_plan(
+        qspec, _spec(k_pages), _spec(v_pages), _spec(table), _spec(lengths), _spec(out), _spec(lse), _spec(weights),
+        _spec(weights_in))
     ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
-    L.call("mtx_attn_decode_paged", L.dtype_code(q), L.dtype_code(k_pages), B, H, Hkv, D, L.ptr(q), L.strides(q),
-           n_pages, page, L.ptr(k_pages), L.strides(k_pages), L.ptr(v_pages), L.strides(v_pages), L.ptr(table),
-           table.stride(0), width, L.ptr(lengths), L.ptr(out), L.strides(out),
-           L.ptr(lse) if lse is not None else None, L.ptr(weights_in) if weights_in is not None else None,
-           L.ptr(weights) if weights is not None else None, wld, L.ptr(ws) if ws is not None else None, ws_bytes,
-           float(scale), L.stream_handle())
+    L.call("mtx_attn_decode_paged", *sizes, q.data_ptr(), qs, n, page, k_pages.data_ptr(), kps, v_pages.data_ptr(),
+           vps, table.data_ptr(), ld, width, lengths.data_ptr(), out.data_ptr(), os, _ptr(lse), _ptr(weights_in),
+           _ptr(weights), wld, _ptr(ws), ws_bytes, float(scale), L.stream_handle())
     return out, lse
+
+
+@functools.lru_cache(maxsize=512)
+def _evict_plan(k_pages, v_pages, table, lengths, weights, to_table, keep, lengths_out, weights_out, slots):
+    (n_pages, Hkv, page, D), cache, kps, vps, B, ld, width = _paged(k_pages, v_pages, table, lengths)
+    wld = _row_weights("weights", weights, B, Hkv, width * page)
+    _, to_pages, to_ld = _table("to_table", to_table, B)
+    _vector("lengths_out", lengths_out, B, "int32")
+    _row_weights("weights_out", weights_out, B, Hkv, width * page, wld)
+    if _dt(slots[2]) != "int32" or tuple(slots[0]) != (B, Hkv, keep) or not _packed(*slots[:2]):
+        raise ValueError(f"slots must be contiguous int32 ({B}, {Hkv}, {keep})")
+    return (_code(cache), B, Hkv, D, n_pages, page), (kps, vps), (ld, width), wld, (to_ld, to_pages)
 
 
 def kv_evict_paged(k_pages, v_pages, table, lengths, weights, to_table, keep: int, recent: int, lengths_out=None,
@@ -269,32 +333,21 @@ def kv_evict_paged(k_pages, v_pages, table, lengths, weights, to_table, keep: in
     that no table of the call reads.  weights as attn_decode_paged accumulates
     them.  Returns (lengths_out (B,), weights_out like weights, slots
     (B, Hkv, keep) int32: the rows kept, then -1)."""
-    n_pages, Hkv, page, D, B = _paged(k_pages, v_pages, table, lengths)
-    width, keep = table.shape[1], int(keep)
-    _row_weights("weights", weights, B, Hkv, width * page)
-    _need_cuda(to_table)
-    if _dt(to_table) != "int32" or len(to_table.shape) != 2 or to_table.shape[0] != B or to_table.stride(1) != 1:
-        raise ValueError(f"to_table must be int32 ({B}, to_pages) with contiguous rows")
+    keep = int(keep)
     if keep < 1:
         raise ValueError("keep must be at least 1")
     if lengths_out is None:
-        lengths_out = dev.empty_buf((B,), "int32")
+        lengths_out = dev.empty_buf(lengths.shape, "int32")
     if weights_out is None:
         weights_out = dev.empty_buf(weights.shape, "float32")
     if slots is None:
-        slots = dev.empty_buf((B, Hkv, keep), "int32")
-    _need_cuda(lengths_out, slots)
-    _row_weights("weights_out", weights_out, B, Hkv, width * page)
-    if tuple(weights_out.shape) != tuple(weights.shape):
-        raise ValueError("weights_out must have weights' shape")
-    if _dt(lengths_out) != "int32" or tuple(lengths_out.shape) != (B,) or not lengths_out.is_contiguous():
-        raise ValueError(f"lengths_out must be contiguous int32 ({B},)")
-    if _dt(slots) != "int32" or tuple(slots.shape) != (B, Hkv, keep) or not slots.is_contiguous():
-        raise ValueError(f"slots must be contiguous int32 ({B}, {Hkv}, {keep})")
-    L.call("mtx_kv_evict_paged", L.dtype_code(k_pages), B, Hkv, D, n_pages, page, L.ptr(k_pages),
-           L.strides(k_pages), L.ptr(v_pages), L.strides(v_pages), L.ptr(table), table.stride(0), width,
-           L.ptr(lengths), L.ptr(weights), weights.shape[2], L.ptr(to_table), to_table.stride(0), to_table.shape[1],
-           keep, int(recent), L.ptr(lengths_out), L.ptr(weights_out), L.ptr(slots), L.stream_handle())
+        slots = dev.empty_buf((table.shape[0], k_pages.shape[1], keep), "int32")
+    sizes, (kps, vps), (ld, width), wld, (to_ld, to_pages) = _evict_plan(
+        _spec(k_pages), _spec(v_pages), _spec(table), _spec(lengths), _spec(weights), _spec(to_table), keep,
+        _spec(lengths_out), _spec(weights_out), _spec(slots))
+    L.call("mtx_kv_evict_paged", *sizes, k_pages.data_ptr(), kps, v_pages.data_ptr(), vps, table.data_ptr(), ld,
+           width, lengths.data_ptr(), weights.data_ptr(), wld, to_table.data_ptr(), to_ld, to_pages, keep,
+           int(recent), lengths_out.data_ptr(), weights_out.data_ptr(), slots.data_ptr(), L.stream_handle())
     return lengths_out, weights_out, slots
 
 
@@ -1083,28 +1136,30 @@ def xent_bwd(logits, labels, lse, gscalar, scale, dlogits, accumulate=False):
 TOP_MAX = 64  # alternatives per row of token_logprobs
 
 
-@functools.lru_cache(maxsize=512)
-def _logprobs_workspace_bytes(rows, V, top):
-    """mtx_token_logprobs_workspace_bytes, a function of the sizes alone."""
-    return L.lib().mtx_token_logprobs_workspace_bytes(rows, V, top)
-
-
 def _logits_rows(logits, tokens, **vectors):
-    """(rows, V, ld) of (rows, V) logits, checked with the int64 (rows,)
-    tokens and fp32 (rows,) vectors (None: not there) that go with them."""
-    _need_cuda(logits, tokens)
-    if len(logits.shape) != 2 or logits.stride(1) != 1:
+    """(dtype code, rows, V, ld) of the spec of (rows, V) logits, checked with
+    those of the int64 (rows,) tokens and fp32 (rows,) vectors (None: not
+    there) that go with them."""
+    shape, strides, dtype = logits
+    if len(shape) != 2 or strides[1] != 1:
         raise ValueError("logits must be (rows, V) with contiguous rows")
-    rows, V = logits.shape
-    if _dt(tokens) != "int64" or tuple(tokens.shape) != (rows,) or not tokens.is_contiguous():
-        raise ValueError(f"tokens must be contiguous int64 ({rows},)")
+    rows, V = shape
+    _vector("tokens", tokens, rows, "int64")
     for name, t in vectors.items():
-        if t is None:
-            continue
-        _need_cuda(t)
-        if _dt(t) != "float32" or tuple(t.shape) != (rows,) or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous fp32 ({rows},)")
-    return rows, V, logits.stride(0)
+        _vector(name, t, rows, "float32")
+    return _code(_dt(dtype)), rows, V, strides[0]
+
+
+@functools.lru_cache(maxsize=512)
+def _logprobs_plan(logits, tokens, top, logprob, entropy, lse, top_ids, top_logprobs):
+    code, rows, V, ld = _logits_rows(logits, tokens, logprob=logprob, entropy=entropy, lse=lse)
+    if not 0 <= top <= min(V, TOP_MAX):
+        raise ValueError(f"top must be between 0 and {min(V, TOP_MAX)} (got {top})")
+    for name, t, dt in (("top_ids", top_ids, "int64"), ("top_logprobs", top_logprobs, "float32")):
+        if _dt(t[2]) != dt or tuple(t[0]) != (rows, top) or (rows and top and not _packed(*t[:2])):
+            raise ValueError(f"{name} must be contiguous {dt} ({rows}, {top})")
+    ws = L.lib().mtx_token_logprobs_workspace_bytes(rows, V, top) if rows else 0
+    return code, rows, V, ld, ws
 
 
 def token_logprobs(logits, tokens, top: int = 0, scale: float = 1.0, logprob=None, entropy=None, lse=None,
@@ -1115,27 +1170,29 @@ def token_logprobs(logits, tokens, top: int = 0, scale: float = 1.0, logprob=Non
     outside [0, V) means the row has none (logprob 0).  Returns (logprob,
     entropy, lse) fp32 (rows,), top_ids int64 and top_logprobs fp32
     (rows, top)."""
-    top = int(top)
-    rows, V, ld = _logits_rows(logits, tokens, logprob=logprob, entropy=entropy, lse=lse)
-    logprob, entropy, lse = (dev.empty_buf((rows,), "float32") if t is None else t for t in (logprob, entropy, lse))
-    if not 0 <= top <= min(V, TOP_MAX):
-        raise ValueError(f"top must be between 0 and {min(V, TOP_MAX)} (got {top})")
+    top, n = int(top), logits.shape[0]
+    logprob, entropy, lse = (dev.empty_buf((n,), "float32") if t is None else t for t in (logprob, entropy, lse))
     if top_ids is None:
-        top_ids = dev.empty_buf((rows, top), "int64")
+        top_ids = dev.empty_buf((n, max(0, top)), "int64")
     if top_logprobs is None:
-        top_logprobs = dev.empty_buf((rows, top), "float32")
-    for name, t, dt in (("top_ids", top_ids, "int64"), ("top_logprobs", top_logprobs, "float32")):
-        _need_cuda(t)
-        if _dt(t) != dt or tuple(t.shape) != (rows, top) or (top and rows and not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {dt} ({rows}, {top})")
+        top_logprobs = dev.empty_buf((n, max(0, top)), "float32")
+    code, rows, V, ld, ws_bytes = _logprobs_plan(_spec(logits), _spec(tokens), top, _spec(logprob), _spec(entropy),
+                                                 _spec(lse), _spec(top_ids), _spec(top_logprobs))
     if rows:
-        ws_bytes = _logprobs_workspace_bytes(rows, V, top)
         ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
-        L.call("mtx_token_logprobs", L.dtype_code(logits), rows, V, L.ptr(logits), ld, L.ptr(tokens), float(scale),
-               L.ptr(logprob), L.ptr(lse), L.ptr(entropy), top, L.ptr(top_ids) if top else None,
-               L.ptr(top_logprobs) if top else None, L.ptr(ws) if ws is not None else None, ws_bytes,
-               L.stream_handle())
+        L.call("mtx_token_logprobs", code, rows, V, logits.data_ptr(), ld, tokens.data_ptr(), float(scale),
+               logprob.data_ptr(), lse.data_ptr(), entropy.data_ptr(), top, top_ids.data_ptr() if top else None,
+               top_logprobs.data_ptr() if top else None, _ptr(ws), ws_bytes, L.stream_handle())
     return logprob, entropy, lse, top_ids, top_logprobs
+
+
+@functools.lru_cache(maxsize=512)
+def _logprobs_bwd_plan(logits, tokens, lse, entropy, g_logprob, g_entropy, dlogits):
+    code, rows, V, ld = _logits_rows(logits, tokens, lse=lse, entropy=entropy, g_logprob=g_logprob,
+                                     g_entropy=g_entropy)
+    if _dt(dlogits[2]) != "float32" or tuple(dlogits[0]) != (rows, V) or dlogits[1][1] != 1:
+        raise ValueError(f"dlogits must be fp32 ({rows}, {V}) with contiguous rows")
+    return code, rows, V, ld, dlogits[1][0]
 
 
 def token_logprobs_bwd(logits, tokens, lse, entropy, g_logprob, g_entropy, scale: float = 1.0, dlogits=None,
@@ -1143,19 +1200,16 @@ def token_logprobs_bwd(logits, tokens, lse, entropy, g_logprob, g_entropy, scale
     """The logits' gradient from those of logprob and entropy (fp32 (rows,),
     None: 0) and the forward's lse and entropy (mtx_token_logprobs_bwd):
     fp32 (rows, V), added to dlogits with accumulate."""
-    rows, V, ld = _logits_rows(logits, tokens, lse=lse, entropy=entropy, g_logprob=g_logprob, g_entropy=g_entropy)
     if dlogits is None:
         if accumulate:
             raise ValueError("accumulate needs dlogits")
-        dlogits = dev.empty_buf((rows, V), "float32")
-    _need_cuda(dlogits)
-    if _dt(dlogits) != "float32" or tuple(dlogits.shape) != (rows, V) or dlogits.stride(1) != 1:
-        raise ValueError(f"dlogits must be fp32 ({rows}, {V}) with contiguous rows")
+        dlogits = dev.empty_buf(logits.shape, "float32")
+    code, rows, V, ld, ldd = _logprobs_bwd_plan(_spec(logits), _spec(tokens), _spec(lse), _spec(entropy),
+                                                _spec(g_logprob), _spec(g_entropy), _spec(dlogits))
     if rows:
-        L.call("mtx_token_logprobs_bwd", L.dtype_code(logits), rows, V, L.ptr(logits), ld, L.ptr(tokens), L.ptr(lse),
-               L.ptr(entropy), L.ptr(g_logprob) if g_logprob is not None else None,
-               L.ptr(g_entropy) if g_entropy is not None else None, float(scale), L.ptr(dlogits), dlogits.stride(0),
-               int(bool(accumulate)), L.stream_handle())
+        L.call("mtx_token_logprobs_bwd", code, rows, V, logits.data_ptr(), ld, tokens.data_ptr(), lse.data_ptr(),
+               entropy.data_ptr(), _ptr(g_logprob), _ptr(g_entropy), float(scale), dlogits.data_ptr(), ldd,
+               1 if accumulate else 0, L.stream_handle())
     return dlogits
 
 
