@@ -59,26 +59,86 @@ __device__ __forceinline__ void load_values(const bf16_t* p, float (&x)[E]) {
 constexpr float kFarBelow = -1e30f;
 __device__ __forceinline__ float below(float d) { return __builtin_elementwise_maximum(d, kFarBelow); }
 
-// 64 values of a wave, largest in lane 0 (bitonic)
-__device__ __forceinline__ float wave_sort(float v, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int m = size >> 1; m >= 1; m >>= 1) {
-      const float o = __shfl_xor(v, m, 64);
-      v = ((lane & size) == 0) == ((lane & m) == 0) ? fmaxf(v, o) : fminf(v, o);
-    }
-  return v;
+// The value of lane `lane ^ M` without the LDS pipe that a shuffle takes (a row of
+// 65 logits needs some 40 of them): DPP within 16 lanes, for 16 and 32 the row
+// swaps, of which pair() gives both partners' values to both, the lower lane's first
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
 }
-// the 64 largest of two sorted waves' values, sorted
-__device__ __forceinline__ float wave_merge(float v, float w, int lane) {
-  v = fmaxf(v, __shfl(w, 63 - lane, 64));
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const float o = __shfl_xor(v, m, 64);
-    v = (lane & m) == 0 ? fmaxf(v, o) : fminf(v, o);
+template <int M>
+__device__ __forceinline__ float lane_xor(float v) {
+  if constexpr (M == 1) return dpp<0xB1>(v);          // quad_perm 1 0 3 2
+  else if constexpr (M == 2) return dpp<0x4E>(v);     // quad_perm 2 3 0 1
+  else if constexpr (M == 4) return dpp<0x1B>(dpp<0x141>(v));  // mirror of 8, then of 4
+  else return dpp<0x128>(v);                          // 8: rotation of 16 by 8
+}
+template <int M>
+__device__ __forceinline__ void pair(float v, float& a, float& b) {
+  const uint32_t u = __float_as_uint(v);
+  if constexpr (M == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+  }
+}
+template <int N, typename F>
+__device__ __forceinline__ float all_lanes(float v, F f) {  // over groups of N >= 16 lanes
+  v = f(v, lane_xor<1>(v));
+  v = f(v, lane_xor<2>(v));
+  v = f(v, lane_xor<4>(v));
+  v = f(v, lane_xor<8>(v));
+  float a, b;
+  if constexpr (N >= 32) {
+    pair<16>(v, a, b);
+    v = f(a, b);
+  }
+  if constexpr (N >= 64) {
+    pair<32>(v, a, b);
+    v = f(a, b);
   }
   return v;
+}
+template <int N = 64>
+__device__ __forceinline__ float all_sum(float v) {
+  return all_lanes<N>(v, [](float a, float b) { return a + b; });
+}
+template <int N = 64>
+__device__ __forceinline__ float all_max(float v) {
+  return all_lanes<N>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+
+// one step of a bitonic network: the larger of lanes l and l ^ M to the lower lane,
+// or, where `up`, to the upper one
+template <int M>
+__device__ __forceinline__ float exchange(float v, int lane, bool up) {
+  float a = v, b;
+  if constexpr (M >= 16) pair<M>(v, a, b);
+  else b = lane_xor<M>(v);
+  return ((lane & M) != 0) == up ? fmaxf(a, b) : fminf(a, b);
+}
+template <int M>
+__device__ __forceinline__ float bitonic(float v, int lane, bool up) {
+  v = exchange<M>(v, lane, up);
+  if constexpr (M > 1) v = bitonic<M / 2>(v, lane, up);
+  return v;
+}
+// N values of N lanes, largest in the first
+template <int N>
+__device__ __forceinline__ float lanes_sort(float v, int lane) {
+  v = bitonic<1>(v, lane, lane & 2);
+  v = bitonic<2>(v, lane, lane & 4);
+  v = bitonic<4>(v, lane, lane & 8);
+  v = bitonic<8>(v, lane, N > 16 && (lane & 16));
+  if constexpr (N >= 32) v = bitonic<16>(v, lane, N > 32 && (lane & 32));
+  if constexpr (N >= 64) v = bitonic<32>(v, lane, false);
+  return v;
+}
+// the 64 largest of two sorted waves' values, sorted; w is read backwards
+__device__ __forceinline__ float wave_merge(float v, float w_backwards, int lane) {
+  return bitonic<32>(fmaxf(v, w_backwards), lane, false);
 }
 
 __device__ __forceinline__ float key_value(uint64_t key) {
@@ -109,21 +169,24 @@ __device__ __forceinline__ void put_top(const LpArgs& a, int64_t r, int rank, ui
 // and rows where too many values reach the bound (ties), take `top` rounds over
 // all values instead.
 
-// ---- rows of up to 64 VPL values: one wave each, the row in registers ----
-constexpr int kSmallCap = 256;
-template <typename T, int VPL>
+// ---- rows of up to LPR VPL values: LPR lanes each, the row in registers, 64 / LPR
+// rows a wave (16384 rows of 65: one row a wave would spend its time on reductions
+// over lanes that hold one value) ----
+constexpr int kSmallCap = 256;  // candidates a row
+template <typename T, int LPR, int VPL>
 __global__ __launch_bounds__(256) void logprobs_small_kernel(const LpArgs a, int64_t rows) {
-  __shared__ uint64_t cands[4][kSmallCap];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t r = (int64_t)blockIdx.x * 4 + wave;
-  if (r >= rows) return;
-  const T* __restrict__ x = static_cast<const T*>(a.x) + r * a.ld;
+  constexpr int RPW = 64 / LPR, CAP = RPW == 1 ? kSmallCap : LPR * VPL;
+  __shared__ uint64_t cands[4 * RPW][CAP];
+  const int lane = threadIdx.x & 63, sub = lane % LPR, row = threadIdx.x / LPR;
+  const int64_t r = (int64_t)blockIdx.x * (4 * RPW) + row;
+  const bool in = r < rows;
+  const T* __restrict__ x = static_cast<const T*>(a.x) + (in ? r : 0) * a.ld;
   float v[VPL], best = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) v[i] = lane + 64 * i < a.V ? Elem<T>::to_f(x[lane + 64 * i]) : -INFINITY;
+  for (int i = 0; i < VPL; ++i) v[i] = sub + LPR * i < a.V ? Elem<T>::to_f(x[sub + LPR * i]) : -INFINITY;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) best = fmaxf(best, v[i]);
-  const float m = fmaxf(wave_max(best), -FLT_MAX), c = a.scale * kLog2e;
+  const float m = fmaxf(all_max<LPR>(best), -FLT_MAX), c = a.scale * kLog2e;
   float l = 0.f, t = 0.f;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
@@ -131,49 +194,51 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const LpArgs a, int
     l += e;
     t = fmaf(e, d, t);
   }
-  l = wave_sum(l);
-  t = wave_sum(t);
-  if (lane == 0) row_result(a, r, x, m, l, t);
+  l = all_sum<LPR>(l);
+  t = all_sum<LPR>(t);
+  if (sub == 0 && in) row_result(a, r, x, m, l, t);
   if (a.top == 0) return;
-  uint64_t* buf = cands[wave];
+  uint64_t* buf = cands[row];
   int n = 0;
-  if (l == l) {
-    const float bound = __shfl(wave_sort(best, lane), a.top - 1, 64);
+  // the top-th largest of the lanes' largest values; all values where there are
+  // fewer lanes than that
+  float bound = -INFINITY;
+  if (a.top <= LPR) bound = __shfl(lanes_sort<LPR>(best, lane), (lane & ~(LPR - 1)) + a.top - 1, 64);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const bool in = v[i] >= bound && lane + 64 * i < a.V;
-      const uint64_t mask = __ballot(in);
-      const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, n));
-      if (in && at < kSmallCap) buf[at] = rank_key(v[i], lane + 64 * i);
-      n += __popcll(mask);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+  for (int i = 0; i < VPL; ++i) {
+    const bool good = v[i] >= bound && sub + LPR * i < a.V;
+    const uint64_t mask = __ballot(good) >> (lane & ~(LPR - 1)) & (LPR == 64 ? ~0ull : (1ull << LPR % 64) - 1);
+    const int at = n + __popcll(mask & ((1ull << sub) - 1));
+    if (good && at < CAP) buf[at] = rank_key(v[i], sub + LPR * i);
+    n += __popcll(mask);
   }
-  if (n >= a.top && n <= kSmallCap) {
-    for (int i = lane; i < n; i += 64) {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const bool slow = l != l || n < a.top || n > CAP;  // alike in a row's lanes
+  if (!slow && in) {
+    for (int i = sub; i < n; i += LPR) {
       const uint64_t mine = buf[i];
       int rank = 0;
       for (int k = 0; k < n; ++k) rank += buf[k] > mine;
       if (rank < a.top) put_top(a, r, rank, mine, key_value(mine), m, l);
     }
-    return;
   }
+  if (!__ballot(slow)) return;
   uint64_t last = ~0ull;
   for (int k = 0; k < a.top; ++k) {
     uint64_t mine = 0;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const uint64_t key = rank_key(v[i], lane + 64 * i);
-      if (lane + 64 * i < a.V && (key < last || k == 0) && key > mine) mine = key;
+      const uint64_t key = rank_key(v[i], sub + LPR * i);
+      if (sub + LPR * i < a.V && (key < last || k == 0) && key > mine) mine = key;
     }
 #pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) {
+    for (int s = LPR / 2; s >= 1; s >>= 1) {
       const uint64_t o = __shfl_xor(mine, s, 64);
       mine = o > mine ? o : mine;
     }
     last = mine;
-    if (lane == 0) put_top(a, r, k, last, Elem<T>::to_f(x[(int)~(uint32_t)last]), m, l);
+    if (sub == 0 && slow && in) put_top(a, r, k, last, Elem<T>::to_f(x[(int)~(uint32_t)last]), m, l);
   }
 }
 
@@ -235,12 +300,12 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
     for (int e = 0; e < E; ++e) add(v[e]);
   }
   const float mine = m;  // the thread's largest value
-  raise(wave_max(m));
-  l = wave_sum(l);
-  t = wave_sum(t);
+  raise(all_max(m));
+  l = all_sum(l);
+  t = all_sum(t);
   if (lane == 0) red[0][wave] = m, red[1][wave] = l, red[2][wave] = t;
   if (a.top) {
-    sorted[wave][lane] = wave_sort(mine, lane);
+    sorted[wave][lane] = lanes_sort<64>(mine, lane);
     if (tid == 0) count = 0;
   }
   __syncthreads();
@@ -260,12 +325,14 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   if (a.top == 0) return;
 #pragma unroll
   for (int s = 1; s < W; s <<= 1) {
-    if (wave % (2 * s) == 0) sorted[wave][lane] = wave_merge(sorted[wave][lane], sorted[wave + s][lane], lane);
+    if (wave % (2 * s) == 0) sorted[wave][lane] = wave_merge(sorted[wave][lane], sorted[wave + s][63 - lane], lane);
     __syncthreads();
   }
   const float bound = sorted[0][a.top - 1];
-  if (l == l && mine >= bound) {
-    for (int i = tid * E; i < a.V; i += STEP) {
+  // a thread's values are read again by its wave, a load each
+  for (uint64_t mask = __ballot(l == l && mine >= bound); mask; mask &= mask - 1) {
+    const int first = (wave * 64 + __ffsll((unsigned long long)mask) - 1) * E;
+    for (int i = first + lane * STEP; i < a.V; i += 64 * STEP) {
       float v[E];
       if (i + E <= a.V) {
         load_values<E>(x + i, v);
@@ -402,14 +469,19 @@ constexpr int kMostTop = 64;
 
 template <typename T>
 int launch_logprobs(const LpArgs& a, int64_t rows, hipStream_t st) {
-  const dim3 four((unsigned)((rows + 3) / 4));
-  if (a.V <= 64) hipLaunchKernelGGL((logprobs_small_kernel<T, 1>), four, dim3(256), 0, st, a, rows);
-  else if (a.V <= 128) hipLaunchKernelGGL((logprobs_small_kernel<T, 2>), four, dim3(256), 0, st, a, rows);
-  else if (a.V <= 256) hipLaunchKernelGGL((logprobs_small_kernel<T, 4>), four, dim3(256), 0, st, a, rows);
-  else if (a.V <= 512) hipLaunchKernelGGL((logprobs_small_kernel<T, 8>), four, dim3(256), 0, st, a, rows);
-  else if (a.V <= 1024) hipLaunchKernelGGL((logprobs_small_kernel<T, 16>), four, dim3(256), 0, st, a, rows);
+#define SMALL(LPR, VPL)                                                                                        \
+  hipLaunchKernelGGL((logprobs_small_kernel<T, LPR, VPL>), dim3((unsigned)((rows * LPR + 255) / 256)), dim3(256), 0, \
+                     st, a, rows)
+  if (a.V <= 16) SMALL(16, 1);
+  else if (a.V <= 48) SMALL(16, 3);
+  else if (a.V <= 80) SMALL(16, 5);
+  else if (a.V <= 128) SMALL(16, 8);
+  else if (a.V <= 256) SMALL(32, 8);
+  else if (a.V <= 512) SMALL(64, 8);
+  else if (a.V <= 1024) SMALL(64, 16);
   else if (a.V <= 8192) hipLaunchKernelGGL((logprobs_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((logprobs_kernel<T, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, a);
+#undef SMALL
   MTX_LAUNCHED();
   return MTX_OK;
 }
