@@ -319,57 +319,56 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
 
   const int split = blockIdx.x % a.S, rest = blockIdx.x / a.S;
   const int ht = rest % a.HT, bh = rest / a.HT, b = bh / a.Hkv, hk = bh % a.Hkv;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, quarter = lane >> 4;
   const int heads = min(16, a.G - 16 * ht), h0 = hk * a.G + 16 * ht;
-  const int n = min(max(a.lengths[b], 0), a.cap);
-  const int c0 = split * a.chunk, c1 = min(n, c0 + a.chunk);
-  if (c0 >= n && !(a.direct && split == 0)) return;  // finish_kernel knows which chunks there are
-
+  const int c0 = split * a.chunk;
+  // the page ids of the whole chunk, whatever the length, so that neither load
+  // waits for the other
+  const int p0 = a.tab.div(c0), np = a.tab.div(min(a.cap, c0 + a.chunk) - 1) - p0 + 1;
+  const int length = a.lengths[b];
+  for (int i = tid; i < np; i += 256) sh.ids[i] = a.tab.id(b, p0 + i);
   Tile tile;
   tile.load_q(col < heads ? static_cast<const TQ*>(a.q) + b * a.qb + (h0 + col) * a.qh : nullptr, quarter);
-  const int p0 = a.tab.div(c0);
-  const int np = c1 > c0 ? a.tab.div(c1 - 1) - p0 + 1 : 0;
-  for (int i = tid; i < np; i += 256) sh.ids[i] = a.tab.id(b, p0 + i);
+  const int n = min(max(length, 0), a.cap), c1 = min(n, c0 + a.chunk);
+  if (c0 >= n && !(a.direct && split == 0)) return;  // finish_kernel knows which chunks there are
   __syncthreads();
 
   const TC* __restrict__ kp = static_cast<const TC*>(a.k.p) + hk * a.k.sh;
   const TC* __restrict__ vp = static_cast<const TC*>(a.v.p) + hk * a.v.sh;
   uint32_t there = 0;  // which of the lane's rows 16 t + 4 quarter + r (bit 4 t + r) are seen
 
-  // row j of the chunk: its offset in a pool, or -1
-  auto look = [&](const Pages& g, int j) -> int64_t {
-    if (j >= c1) return -1;
-    const int pi = a.tab.div(j), id = sh.ids[pi - p0];
-    return id < 0 ? -1 : row_at(g, a.tab, id, pi, j);
+  // offset in a pool of row j, of the pool's first row where j is not there, and
+  // whether it is; without branches, for the waits on the loads in flight
+  auto look = [&](const Pages& g, int j, bool& in) -> int64_t {
+    const int pi = a.tab.div(min(j, c1 - 1)), id = sh.ids[pi - p0];
+    in = j < c1 && id >= 0;
+    return in ? row_at(g, a.tab, id, pi, j) : 0;
   };
   // the same of a row that is one for the whole wave
-  auto look1 = [&](const Pages& g, int j) -> int64_t {
-    if (j >= c1) return -1;
-    const int pi = a.tab.div(j), id = __builtin_amdgcn_readfirstlane(sh.ids[pi - p0]);
-    return id < 0 ? -1 : row_at(g, a.tab, id, pi, j);
+  auto look1 = [&](const Pages& g, int j, bool& in) -> int64_t {
+    const int pi = a.tab.div(min(j, c1 - 1)), id = __builtin_amdgcn_readfirstlane(sh.ids[pi - p0]);
+    in = j < c1 && id >= 0;
+    return in ? row_at(g, a.tab, id, pi, j) : 0;
   };
   auto load_k = [&](int j0) {
+    bool in;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      if constexpr (EVEN) {
-        const int64_t at = look1(a.k, __builtin_amdgcn_readfirstlane(j0 + 16 * t));
-        const TC* base = kp + (at < 0 ? 0 : at);
-        tile.load_k(t, base + col * (int)a.k.sr, quarter);
-      } else {
-        const int64_t at = look(a.k, j0 + 16 * t + col);
-        tile.load_k(t, kp + (at < 0 ? 0 : at), quarter);
-      }
+      if constexpr (EVEN)
+        tile.load_k(t, kp + look1(a.k, j0 + 16 * t, in) + col * (int)a.k.sr, quarter);
+      else
+        tile.load_k(t, kp + look(a.k, j0 + 16 * t + col, in), quarter);
     }
   };
   auto load_v = [&](int j0) {
+    bool in;
     there = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if constexpr (EVEN) {
-        const int j = __builtin_amdgcn_readfirstlane(j0 + 16 * t);
-        const int64_t at = look1(a.v, j);
-        const TC* base = vp + (at < 0 ? 0 : at);
-        const int seen = at < 0 ? 0 : c1 - j;  // rows from j on
+        const TC* base = vp + look1(a.v, j0 + 16 * t, in);
+        const int seen = in ? c1 - j0 - 16 * t : 0;  // rows from j0 + 16 t on
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           tile.load_v(4 * t + r, base + (4 * quarter + r) * (int)a.v.sr + VD * col);
@@ -378,9 +377,8 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int64_t at = look(a.v, j0 + 16 * t + 4 * quarter + r);
-          tile.load_v(4 * t + r, vp + (at < 0 ? 0 : at) + VD * col);
-          there |= (uint32_t)(at >= 0) << (4 * t + r);
+          tile.load_v(4 * t + r, vp + look(a.v, j0 + 16 * t + 4 * quarter + r, in) + VD * col);
+          there |= (uint32_t)in << (4 * t + r);
         }
       }
     }
@@ -404,7 +402,9 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) p[4 * t + r] = s[r] * a.c;
     }
-    if (next < c1) load_k(next);
+    // unconditional, or the wait for V would have to wait for these loads too: behind
+    // the last tile they read the pool's first rows
+    load_k(next);
     if (__ballot(there != (1u << (4 * NT)) - 1)) {  // a hidden row: no weight, and its V is not used
 #pragma unroll
       for (int e = 0; e < 4 * NT; ++e)
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
       l += p[e];
     }
     tile.add_v(p, o);
-    if (next < c1) load_v(next);
+    load_v(next);
   }
 
   // join the waves: head col's values VD (4 quarter + r) + n in o[n][r]
@@ -494,49 +494,58 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
 __device__ __forceinline__ void chunk_total(const float* ml, int chunks, int lane, float& m, float& l) {
   m = -FLT_MAX;
   l = 0.f;
-  for (int i = lane; i < chunks; i += 64) m = fmaxf(m, ml[2 * i]);
-  m = wave_max(m);
-  for (int i = lane; i < chunks; i += 64) l += ml[2 * i + 1] * __builtin_amdgcn_exp2f(ml[2 * i] - m);
-  l = wave_sum(l);
+  for (int i = lane; i < chunks; i += 64) {
+    const f32x2 x = reinterpret_cast<const f32x2*>(ml)[i];
+    const float n = fmaxf(m, x[0]);
+    l = l * __builtin_amdgcn_exp2f(m - n) + x[1] * __builtin_amdgcn_exp2f(x[0] - n);
+    m = n;
+  }
+  const float all = wave_max(m);
+  l = wave_sum(l * __builtin_amdgcn_exp2f(m - all));
+  m = all;
 }
 
-// Joins the chunks of decode_kernel: the first B H workgroups each one head's
-// output, the others kFinishRows rows' weights of one sequence and K/V head
+// Joins the chunks of decode_kernel: the first workgroups each FD values of one
+// head's output, the others kFinishRows rows' weights of one sequence and K/V
+// head.  FD is 16 where there are few heads, whose chunks may be hundreds, and D
+// where there are many
 constexpr int kFinishRows = 1024;
-template <typename TQ, int D>
+template <typename TQ, int D, int FD>
 __global__ __launch_bounds__(256) void finish_kernel(const DecodeArgs a) {
-  constexpr int DL = D / 4, NG = 256 / DL;  // lanes over d, groups of chunks
+  constexpr int DL = FD / 4, NG = 256 / DL, ND = D / FD;  // lanes over d, groups of chunks
   __shared__ union {
-    f32x4 x[NG][DL];
+    f32x4 x[4][DL];
     float lse2[256];
   } sh;
-  const int tid = threadIdx.x, lane = tid & 63;
-  if ((int)blockIdx.x < a.B * a.H) {
-    const int64_t row = blockIdx.x;
-    const int b = blockIdx.x / a.H, h = blockIdx.x % a.H;
+  const int tid = threadIdx.x, lane = tid & 63, outs = a.B * a.H * ND;
+  if ((int)blockIdx.x < outs) {
+    const int64_t row = blockIdx.x / ND;
+    const int b = (int)row / a.H, h = (int)row % a.H;
     const int chunks = (min(max(a.lengths[b], 0), a.cap) + a.chunk - 1) / a.chunk;
     const float* ml = a.part_ml + row * a.S * 2;
     float m, l;
     chunk_total(ml, chunks, lane, m, l);
-    const int d = tid % DL, g = tid / DL;
-    const f32x4* po = reinterpret_cast<const f32x4*>(a.part_o + row * a.S * D) + d;
+    const int d = tid % DL, g = tid / DL, d0 = blockIdx.x % ND * FD;
+    const float* po = a.part_o + row * a.S * D + d0 + 4 * d;
     f32x4 x = zero4();
-    for (int i = g; i < chunks; i += NG) x += po[i * DL] * __builtin_amdgcn_exp2f(ml[2 * i] - m);
-    sh.x[g][d] = x;
+    for (int i = g; i < chunks; i += NG)
+      x += *reinterpret_cast<const f32x4*>(po + (int64_t)i * D) * __builtin_amdgcn_exp2f(ml[2 * i] - m);
+#pragma unroll
+    for (int s = DL; s < 64; s <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], s, 64);
+    if (lane < DL) sh.x[tid >> 6][lane] = x;
     __syncthreads();
     const bool some = l > 0.f || l != l;
-    if (g == 0) {
-      x = sh.x[0][d];
-#pragma unroll
-      for (int i = 1; i < NG; ++i) x += sh.x[i][d];
-      TQ* o = static_cast<TQ*>(a.o) + b * a.ob + h * a.oh + 4 * d;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = Elem<TQ>::from_f(some ? x[e] / l : 0.f);
+    if (tid < FD) {
+      const float* y = reinterpret_cast<const float*>(sh.x) + tid;
+      const float sum = (y[0] + y[FD]) + (y[2 * FD] + y[3 * FD]);
+      static_cast<TQ*>(a.o)[b * a.ob + h * a.oh + d0 + tid] = Elem<TQ>::from_f(some ? sum / l : 0.f);
     }
-    if (tid == 0 && a.lse != nullptr) a.lse[row] = some ? m * kLn2 + logf(l) : -INFINITY;
+    if (tid == 0 && d0 == 0 && a.lse != nullptr) a.lse[row] = some ? m * kLn2 + logf(l) : -INFINITY;
     return;
   }
-  const int i = blockIdx.x - a.B * a.H, blocks = (a.cap + kFinishRows - 1) / kFinishRows;
+  const int i = blockIdx.x - outs, blocks = (a.cap + kFinishRows - 1) / kFinishRows;
   const int bh = i / blocks, b = bh / a.Hkv, hk = bh % a.Hkv;
   const int n = min(max(a.lengths[b], 0), a.cap), j0 = (i % blocks) * kFinishRows, j1 = min(n, j0 + kFinishRows);
   if (j0 >= n) return;
@@ -584,48 +593,64 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // the last kept row (of the cand rows that are not recent, `want` are kept), then
 // the kept rows in order.  The range of keys [lo, hi] is cut into up to 2048 equal
 // bins, counted in LDS; the bin in which the want-th largest key lies is the next
-// range: at most three rounds, fewer where the weights are spread less (equal
-// weights: none).  Rows are held in registers, R a thread (rows 4 (NT i + tid) + e
-// in v[i][e]), where they fit (SINGLE), so that they are read once; otherwise each
-// round reads them again, NT R at a time.
+// range, and once it holds NT / 2 rows or fewer they are ranked among themselves:
+// mostly after one round, three at most.  Rows are held in registers, R a thread,
+// where they fit (SINGLE); otherwise each step reads them again.
 constexpr int kBins = 2048;
 
 template <int NT, int R, bool SINGLE>
 __global__ __launch_bounds__(NT) void select_kernel(const EvictArgs a) {
-  constexpr int W = NT / 64, NI = R / 4, BLOCK = NT * R;
-  __shared__ int bins[kBins], part[W], gts[NI * W], ties[NI * W], total[2];
-  __shared__ uint32_t mins[W], maxs[W], found[3];
-  const int bh = blockIdx.x, b = bh / a.H, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int W = NT / 64;
+  __shared__ int bins[kBins], part[W], gts[W], ties[W];
+  __shared__ uint32_t mins[W], maxs[W], found[4], few[NT / 2];
+  __shared__ int nfew;
+  const int bh = blockIdx.x, b = bh / a.H, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int len = min(max(a.lengths[b], 0), a.cap);
   const float* __restrict__ w = a.w + bh * a.wld;
   int* __restrict__ slots = a.slots + (int64_t)bh * a.keep;
-  float* __restrict__ wo = a.w_out + bh * a.wld;
   if (tid == 0 && bh % a.H == 0) a.lengths_out[b] = min(len, a.keep);
   const int cand = len > a.keep ? len - a.recent : 0;
   int want = a.keep - a.recent;
 
-  uint32_t key[R];  // 0, which no weight has, where there is no candidate
+  // wave w has rows `per` w .. and takes them 64 R at a time: row 64 i + lane of
+  // those in key[i], 0 (which no weight has) behind the last
+  const int per = SINGLE ? 64 * R : (cand + 64 * R * W - 1) / (64 * R * W) * (64 * R);
+  const int first = per * wave, last = min(cand, first + per);
+  uint32_t key[R];
   auto load = [&](int base) {
+    if (!SINGLE && base + 64 * R <= last) {
+      float x[R];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int j = base + 4 * (NT * i + tid);
-      float x[4];
+      for (int i = 0; i < R; ++i) x[i] = w[base + lane + 64 * i];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = j + e < cand ? w[j + e] : 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) key[4 * i + e] = j + e < cand ? weight_key(x[e]) : 0u;
+      for (int i = 0; i < R; ++i) key[i] = weight_key(x[i]);
+      return;
     }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int j = base + lane + 64 * i;
+      key[i] = j < last ? __float_as_uint(w[j]) : 0xffffffffu;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      key[i] = base + lane + 64 * i < last ? weight_key(__uint_as_float(key[i])) : 0u;
   };
-  if (SINGLE) load(0);
+  if (SINGLE) load(first);
   auto each = [&](auto f) {
-    for (int base = 0; base < cand; base += BLOCK) {
-      if (!SINGLE) load(base);
+    if (SINGLE) {
 #pragma unroll
       for (int i = 0; i < R; ++i) f(key[i]);
+    } else {
+      for (int base = first; base < last; base += 64 * R) {
+        load(base);
+#pragma unroll
+        for (int i = 0; i < R; ++i) f(key[i]);
+      }
     }
   };
 
-  uint32_t bound = 0;  // smallest kept key; `want` of the rows that have it are kept
+  uint32_t bound = 0xffffffffu;  // smallest kept key; `want` of the rows that have it are kept
   if (cand > 0 && want > 0) {
     uint32_t lo = 0xffffffffu, hi = 0;
     each([&](uint32_t k) {
@@ -638,24 +663,18 @@ __global__ __launch_bounds__(NT) void select_kernel(const EvictArgs a) {
       hi = max(hi, (uint32_t)__shfl_xor((int)hi, m, 64));
     }
     if (lane == 0) mins[wave] = lo, maxs[wave] = hi;
+    for (int i = tid; i < kBins; i += NT) bins[i] = 0;
     __syncthreads();
     for (int i = 0; i < W; ++i) lo = min(lo, mins[i]), hi = max(hi, maxs[i]);
-    ++lo;
-    while (lo < hi) {
-      const int shift = max(0, 21 - __clz((int)(hi - lo)));  // (hi - lo) >> shift < kBins
-      for (int i = tid; i < kBins; i += NT) bins[i] = 0;
-      __syncthreads();
-      each([&](uint32_t k) {
-        if (k - lo <= hi - lo) atomicAdd(&bins[(k - lo) >> shift], 1);
-      });
-      __syncthreads();
-      // from the top bin down: a thread's bins, its wave's, the waves above
-      constexpr int PB = kBins / NT;
-      const int top = kBins - 1 - PB * tid;
-      int mine = 0;
+    lo = __builtin_amdgcn_readfirstlane(lo + 1), hi = __builtin_amdgcn_readfirstlane(hi);
+    constexpr int PB = kBins / NT;
+    const int top = kBins - 1 - PB * tid;
+    // with the bins counted: this thread's, and those from the top down to them
+    auto scan = [&](int& n, int& upto) {
+      n = 0;
 #pragma unroll
-      for (int i = 0; i < PB; ++i) mine += bins[top - i];
-      int upto = mine;
+      for (int i = 0; i < PB; ++i) n += bins[top - i];
+      upto = n;
 #pragma unroll
       for (int m = 1; m < 64; m <<= 1) {
         const int x = __shfl_up(upto, m, 64);
@@ -664,91 +683,182 @@ __global__ __launch_bounds__(NT) void select_kernel(const EvictArgs a) {
       if (lane == 63) part[wave] = upto;
       __syncthreads();
       for (int i = 0; i < wave; ++i) upto += part[i];
-      if (upto - mine < want && upto >= want) {
-        int above = upto - mine, i = 0;
+    };
+    auto clear = [&] {
+      for (int i = tid; i < kBins; i += NT) bins[i] = 0;
+    };
+    if (NT * 8 < cand && lo < hi) {
+      // 4 NT rows spread over all say between which keys the bound lies (three
+      // deviations of such a sample's median to either side); only the rows between
+      // them, if the count confirms it, go into the rounds below, whose atomics
+      // would else cost most of the time (lanes of a wave meet in few bins)
+      constexpr int S = 4 * NT, MARGIN = 3 * 32;
+      static_assert(S <= 4096, "the margin is three times half the root of 4096");
+      const int shift = max(0, 21 - __clz((int)(hi - lo)));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        atomicAdd(&bins[(weight_key(w[(int64_t)(tid + NT * i) * cand / S]) - lo) >> shift], 1);
+      if (tid == 0) found[0] = lo, found[1] = hi;
+      __syncthreads();
+      int n, upto;
+      scan(n, upto);
+      const int rank = (int)((int64_t)want * S / cand);
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const int x = side ? rank - MARGIN : rank + MARGIN;
+        if (x >= 1 && upto - n < x && upto >= x) {
+          int above = upto - n, i = 0;
+          while (above + bins[top - i] < x) above += bins[top - i++];
+          const uint32_t l = lo + ((uint32_t)(top - i) << shift);
+          found[side] = side ? l + min(hi - l, (1u << shift) - 1) : l;
+        }
+      }
+      __syncthreads();
+      const uint32_t l = __builtin_amdgcn_readfirstlane(found[0]), h = __builtin_amdgcn_readfirstlane(found[1]);
+      clear();
+      int gt = 0, ge = 0;
+      each([&](uint32_t k) {
+        gt += __popcll(__ballot(k > h));
+        ge += __popcll(__ballot(k >= l));
+      });
+      if (lane == 0) gts[wave] = gt, ties[wave] = ge;
+      __syncthreads();
+      gt = ge = 0;
+      for (int i = 0; i < W; ++i) gt += gts[i], ge += ties[i];
+      gt = __builtin_amdgcn_readfirstlane(gt), ge = __builtin_amdgcn_readfirstlane(ge);
+      if (gt < want && want <= ge) lo = l, hi = h, want -= gt;
+    }
+    while (lo < hi) {
+      const int shift = max(0, 21 - __clz((int)(hi - lo)));  // (hi - lo) >> shift < kBins
+      each([&](uint32_t k) {
+        if (k - lo <= hi - lo) atomicAdd(&bins[(k - lo) >> shift], 1);
+      });
+      if (tid == 0) nfew = 0;
+      __syncthreads();
+      // from the top bin down, to that of the want-th largest
+      int n, upto;
+      scan(n, upto);
+      if (upto - n < want && upto >= want) {
+        int above = upto - n, i = 0;
         while (above + bins[top - i] < want) above += bins[top - i++];
         const uint32_t l = lo + ((uint32_t)(top - i) << shift);
         found[0] = l;
         found[1] = l + min(hi - l, (1u << shift) - 1);
         found[2] = (uint32_t)(want - above);
+        found[3] = (uint32_t)bins[top - i];
       }
       __syncthreads();
-      lo = found[0], hi = found[1], want = (int)found[2];
+      lo = __builtin_amdgcn_readfirstlane(found[0]), hi = __builtin_amdgcn_readfirstlane(found[1]);
+      want = __builtin_amdgcn_readfirstlane((int)found[2]);
+      const int in = __builtin_amdgcn_readfirstlane((int)found[3]);
+      if (lo == hi) break;
+      if (in > NT / 2) {
+        clear();
+        __syncthreads();
+        continue;
+      }
+      each([&](uint32_t k) {
+        if (k - lo <= hi - lo) few[atomicAdd(&nfew, 1)] = k;
+      });
+      __syncthreads();
+      if (tid < in) {
+        const uint32_t k = few[tid];
+        int gt = 0, ge = 0;
+        for (int i = 0; i < in; ++i) {
+          const uint32_t o = few[i];
+          gt += o > k;
+          ge += o >= k;
+        }
+        if (gt < want && ge >= want) found[0] = k, found[2] = (uint32_t)(want - gt);
+      }
+      __syncthreads();
+      lo = __builtin_amdgcn_readfirstlane(found[0]);
+      want = __builtin_amdgcn_readfirstlane((int)found[2]);
+      break;
     }
     bound = lo;
   } else {
-    bound = 0xffffffffu;  // no candidate, or none of them
-    want = 0;
+    want = 0;  // no candidate, or none of them
   }
 
-  // positions: rows above the bound and recent ones before a row, and of those
-  // at the bound the first `want`
-  int gat = 0, tat = 0;  // of the blocks before
-  for (int base = 0; base < len; base += BLOCK) {
-    if (!SINGLE) load(base);
-    auto above = [&](int i, int e) {
-      const int j = base + 4 * (NT * i + tid) + e;
-      return key[4 * i + e] > bound || (j >= cand && j < len);
-    };
-    auto equal = [&](int i, int e) { return key[4 * i + e] == bound && want > 0; };
+  // places: how many rows above the bound come before a row, and of those at the
+  // bound the first `want`
+  bound = __builtin_amdgcn_readfirstlane(bound);
+  int g = 0, t = 0;
+  each([&](uint32_t k) {
+    g += __popcll(__ballot(k > bound));
+    t += __popcll(__ballot(k == bound));
+  });
+  if (lane == 0) gts[wave] = g, ties[wave] = t;
+  __syncthreads();
+  g = lane < wave ? gts[lane] : 0, t = lane < wave ? ties[lane] : 0;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      int ng = 0, nt = 0;
+  for (int m = 1; m < W; m <<= 1) g += __shfl_xor(g, m, 64), t += __shfl_xor(t, m, 64);
+  g = __builtin_amdgcn_readfirstlane(g), t = __builtin_amdgcn_readfirstlane(t);
+  asm("" : "+s"(bound));  // the comparisons are made again, not kept (R pairs of masks)
+  int j = first + lane;
+  each([&](uint32_t k) {
+    const bool isg = k > bound, ist = k == bound;
+    const uint64_t bg = __ballot(isg), bt = __ballot(ist);
+    const int ga = __builtin_amdgcn_mbcnt_hi((uint32_t)(bg >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bg, g));
+    const int ta = __builtin_amdgcn_mbcnt_hi((uint32_t)(bt >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bt, t));
+    if (isg | (ist & (ta < want))) slots[ga + min(ta, want)] = j;
+    g += __popcll(bg);
+    t += __popcll(bt);
+    j += 64;
+  });
+  // and the recent ones, or all
+  for (int j = cand + tid; j < len; j += NT) slots[min(len, a.keep) - len + j] = j;
+}
+
+// Selection of up to 64 R rows: one wave each, nothing but ballots.  The last kept
+// key is found bit by bit: the largest with `want` or more rows at or above it
+template <int R>
+__global__ __launch_bounds__(256) void select_small_kernel(const EvictArgs a) {
+  const int bh = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (bh >= a.B * a.H) return;
+  const int b = bh / a.H, len = min(max(a.lengths[b], 0), a.cap);
+  const float* __restrict__ w = a.w + bh * a.wld;
+  if (lane == 0 && bh % a.H == 0) a.lengths_out[b] = min(len, a.keep);
+  const int cand = len > a.keep ? len - a.recent : 0;
+  uint32_t key[R];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        ng += __popcll(__ballot(above(i, e)));
-        nt += __popcll(__ballot(equal(i, e)));
-      }
-      if (lane == 0) gts[i * W + wave] = ng, ties[i * W + wave] = nt;
+  for (int i = 0; i < R; ++i) key[i] = lane + 64 * i < cand ? weight_key(w[lane + 64 * i]) : 0u;
+  int want = cand > 0 ? a.keep - a.recent : 0;
+  uint32_t bound = 0xffffffffu;
+  if (want > 0) {
+    bound = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t t = bound | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= t));
+      if (n >= want) bound = t;
     }
-    __syncthreads();
-    if (wave == 0) {  // exclusive sums in order of rows
-      int g0 = gat, t0 = tat;
-      for (int x0 = 0; x0 < NI * W; x0 += 64) {
-        const int x = x0 + lane;
-        const int g = x < NI * W ? gts[x] : 0, t = x < NI * W ? ties[x] : 0;
-        int gs = g, ts = t;
 #pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-          const int gx = __shfl_up(gs, m, 64), tx = __shfl_up(ts, m, 64);
-          if (lane >= m) gs += gx, ts += tx;
-        }
-        if (x < NI * W) gts[x] = g0 + gs - g, ties[x] = t0 + ts - t;
-        g0 += __shfl(gs, 63, 64);
-        t0 += __shfl(ts, 63, 64);
-      }
-      if (lane == 0) total[0] = g0, total[1] = t0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      // within the wave: lanes below, then this lane's rows in order
-      int ga = gts[i * W + wave], ta = ties[i * W + wave];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint64_t bg = __ballot(above(i, e)), bt = __ballot(equal(i, e));
-        ga = __builtin_amdgcn_mbcnt_hi((uint32_t)(bg >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bg, ga));
-        ta = __builtin_amdgcn_mbcnt_hi((uint32_t)(bt >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bt, ta));
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = base + 4 * (NT * i + tid) + e, pos = ga + min(ta, want);
-        const bool isg = above(i, e), ist = equal(i, e);
-        if ((isg || (ist && ta < want)) && pos < a.keep) {
-          slots[pos] = j;
-          wo[pos] = w[j];
-        }
-        ga += isg;
-        ta += ist;
-      }
-    }
-    gat = total[0], tat = total[1];
-    __syncthreads();
+    for (int i = 0; i < R; ++i) want -= __popcll(__ballot(key[i] > bound));
   }
+  int* __restrict__ slots = a.slots + (int64_t)bh * a.keep;
+  int at = 0, ties = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const bool tie = key[i] == bound;
+    const uint64_t tm = __ballot(tie);
+    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(tm >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)tm, ties));
+    const bool kept = key[i] > bound || (tie && before < want);
+    const uint64_t km = __ballot(kept);
+    const int pos = __builtin_amdgcn_mbcnt_hi((uint32_t)(km >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)km, at));
+    if (kept) slots[pos] = lane + 64 * i;
+    ties += __popcll(tm);
+    at += __popcll(km);
+  }
+  for (int j = cand + lane; j < len; j += 64) slots[min(len, a.keep) - len + j] = j;
 }
 
 // Copies the kept rows, a thread 16 bytes of the keys and the values of kRows
-// rows; the last blocks of a sequence and head clear the weights behind them
+// rows, and their weights; the last blocks of a sequence and head clear the weights
+// behind them
 constexpr int kRows = 4;
 __global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a, int blocks, int fills) {
   const int bh = blockIdx.x / (blocks + fills), block = blockIdx.x % (blocks + fills);
@@ -774,6 +884,11 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a, int bloc
     ti[i] = a.to.div(r0 + per * i);
     from[i] = j[i] < 0 ? -1 : a.from.id(b, fi[i]);
     to[i] = j[i] < 0 ? -1 : a.to.id(b, ti[i]);
+  }
+  if (c == 0) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (j[i] >= 0) a.w_out[bh * a.wld + r0 + per * i] = a.w[bh * a.wld + j[i]];
   }
   uint4 x[kRows], y[kRows];
   const int64_t es = a.es;
@@ -848,9 +963,12 @@ int check_cache(int B, int H, int D, int64_t n_pages, int page, const int* table
   return MTX_OK;
 }
 
-// How a decode call is cut: chunks of rows, a multiple of what four waves take
-// in turn, enough of them for two workgroups a CU where the cache is long, and
-// the workspace [part_o | part_ml | scores].
+// How a decode call is cut, and its workspace [part_o | part_ml | scores].  One
+// chunk a sequence, with no second launch, up to the rows that four waves finish
+// before the second launch would: 512, with more segments to fill the GPU 1024
+// (384 segments of up to 1000 rows: 16.7 us against 15.6 + 4.0) and 2048 (768 of
+// 2048: 147 against 154).  Else chunks of 512 rows, or of up to 1024 where a call
+// may have more than 768 of them (128 segments of 16384: 154 us, 174 with 512)
 struct DecodePlan {
   int chunk, S, HT, direct;
   int64_t n_o, n_ml, n_s, sld;
@@ -859,8 +977,11 @@ struct DecodePlan {
 DecodePlan make_plan(int B, int H, int Hkv, int D, int cap, bool weights) {
   DecodePlan p;
   p.HT = cdiv(H / Hkv, 16);
-  const int64_t want = ((int64_t)cap * B * Hkv * p.HT / 512 + 127) / 128 * 128;
-  p.chunk = (int)std::min<int64_t>(std::max<int64_t>(want, 256), kMaxChunk);
+  const int64_t segments = (int64_t)B * Hkv * p.HT;
+  const int64_t want = (cap * segments / 768 + 127) / 128 * 128;
+  p.chunk = (int)std::min<int64_t>(std::max<int64_t>(want, 512), 1024);
+  if (cap <= 1024 && segments >= 128) p.chunk = 1024;
+  if (cap <= 2048 && segments >= 768) p.chunk = 2048;
   p.S = cdiv(cap, p.chunk);
   p.direct = p.S == 1 && (!weights || p.HT == 1);
   p.sld = ((int64_t)cap + 31) / 32 * 32;
@@ -876,7 +997,11 @@ int launch_decode(bool even, unsigned groups, unsigned finish, const DecodeArgs&
   else hipLaunchKernelGGL((decode_kernel<TQ, TC, D, false>), dim3(groups), dim3(256), 0, st, a);
   MTX_LAUNCHED();
   if (!a.direct) {
-    hipLaunchKernelGGL((finish_kernel<TQ, D>), dim3(finish), dim3(256), 0, st, a);
+    const unsigned heads = (unsigned)(a.B * a.H);
+    if (heads * (D / 16) <= 1024)
+      hipLaunchKernelGGL((finish_kernel<TQ, D, 16>), dim3(heads * (D / 16) + finish), dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((finish_kernel<TQ, D, D>), dim3(heads + finish), dim3(256), 0, st, a);
     MTX_LAUNCHED();
   }
   return MTX_OK;
@@ -972,8 +1097,8 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
   MTX_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need && ((uintptr_t)workspace & 15u) == 0),
                 "workspace: %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
   const int64_t groups = (int64_t)B * Hkv * plan.HT * plan.S;
-  const int64_t finish = (int64_t)B * H + (weights != nullptr ? (int64_t)B * Hkv * cdiv(cap, kFinishRows) : 0);
-  MTX_CHECK_SHAPE(groups <= INT32_MAX && finish <= INT32_MAX, "decode: too many sequences, heads and rows in one call");
+  const int64_t finish = (weights != nullptr ? (int64_t)B * Hkv * cdiv(cap, kFinishRows) : 0);
+  MTX_CHECK_SHAPE(groups <= INT32_MAX && finish <= INT32_MAX / 2, "decode: too many sequences, heads and rows in one call");
   float* ws = static_cast<float*>(workspace);
   DecodeArgs a{q, q_strides[0], q_strides[1],
                {const_cast<void*>(k_pages), kp_strides[0], kp_strides[1], kp_strides[2]},
@@ -1025,11 +1150,16 @@ extern "C" int mtx_kv_evict_paged(int cache_dtype, int B, int H, int D, int64_t 
   MTX_CHECK_SHAPE((blocks + fills) * B * H <= INT32_MAX, "evict: too many rows in one call");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(B * H);
-  if (cap <= 256 * 4) hipLaunchKernelGGL((select_kernel<256, 4, true>), grid, dim3(256), 0, st, a);
-  else if (cap <= 1024 * 4) hipLaunchKernelGGL((select_kernel<1024, 4, true>), grid, dim3(1024), 0, st, a);
-  else if (cap <= 1024 * 16) hipLaunchKernelGGL((select_kernel<1024, 16, true>), grid, dim3(1024), 0, st, a);
-  else if (cap <= 1024 * 48) hipLaunchKernelGGL((select_kernel<1024, 48, true>), grid, dim3(1024), 0, st, a);
-  else hipLaunchKernelGGL((select_kernel<1024, 16, false>), grid, dim3(1024), 0, st, a);
+  const dim3 four(cdiv(B * H, 4));
+#define SELECT(NT, R, SINGLE) hipLaunchKernelGGL((select_kernel<NT, R, SINGLE>), grid, dim3(NT), 0, st, a)
+  if (cap <= 64 * 4) hipLaunchKernelGGL(select_small_kernel<4>, four, dim3(256), 0, st, a);
+  else if (cap <= 256 * 4) SELECT(256, 4, true);
+  else if (cap <= 256 * 16) SELECT(256, 16, true);
+  else if (cap <= 1024 * 16) SELECT(1024, 16, true);
+  else if (cap <= 1024 * 32) SELECT(1024, 32, true);
+  else if (cap <= 1024 * 48) SELECT(1024, 48, true);
+  else SELECT(1024, 16, false);
+#undef SELECT
   MTX_LAUNCHED();
   hipLaunchKernelGGL(gather_kernel, dim3((unsigned)((blocks + fills) * B * H)), dim3(256), 0, st, a, (int)blocks,
                      (int)fills);
