@@ -15,6 +15,7 @@ from .layers import GELU, Dropout, Embedding, LayerNorm, Linear  # noqa: E402
 from .loss import cross_entropy_loss  # noqa: E402
 from .module import Module, Sequential  # noqa: E402
 from .optim import Adam  # noqa: E402
+from .paged import PagedKVCache  # noqa: E402
 from .tensor import Tensor, no_grad  # noqa: E402
 from .transformer import GPT, MultiHeadAttention, TransformerBlock  # noqa: E402
 
@@ -26,5 +27,6 @@ __all__ = [
     "cross_entropy_loss",
     "Adam",
     "CapturedStep",
+    "PagedKVCache",
     "F",
 ]

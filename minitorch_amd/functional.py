@@ -11,6 +11,8 @@ conv.py:66-95):
   mlp_gelu(x, fc1, fc2)        Linear -> GELU -> Linear, GELU in the GEMM epilogues
   causal_attention(q, k, v)    transformer.py:36-44 as one flash kernel
   causal_attention_packed      the same over a packed [q | k | v] tensor
+  token_logprobs(x, tokens)    log probabilities of given tokens, the entropy
+                               and the most likely alternatives, in one pass
 """
 from __future__ import annotations
 
@@ -469,3 +471,46 @@ def cross_entropy(logits, labels):
 
     out = _node(data, (logits,), "cross_entropy", _backward, _track(logits))
     return out
+
+
+def token_logprobs(logits, tokens, top=0, temperature=1.0):
+    """Log probabilities of one token per row of (N, V) logits under
+    softmax(logits / temperature) (log_softmax, functional.py:81-97, at the
+    tokens; the distribution GPT.generate samples from, transformer.py:97-100),
+    and the entropy of each row's distribution: two (N,) Tensors, both
+    differentiable (mtx_token_logprobs and its backward, one pass each).  A
+    negative token means that its row has none (padding): log probability 0, no
+    gradient.  Returns (logprobs, entropy, top_ids, top_logprobs), the latter
+    (N, top) DeviceArrays of the `top` <= 64 most likely tokens, ties to the
+    lowest id, and their log probabilities, without gradients."""
+    N, V = logits.shape
+    if not (np.isfinite(temperature) and temperature > 0):
+        raise ValueError(f"temperature must be finite and > 0 (got {temperature})")
+    if isinstance(tokens, DeviceArray):
+        # device-resident tokens: the kernel takes any outside the vocabulary for none
+        tok = dev.index_array(tokens)
+        if tok.size != N:
+            raise ValueError("one token per row expected")
+        tok = tok.reshape(N).contiguous()
+    else:
+        host = np.asarray(tokens).reshape(-1)
+        if host.size != N:
+            raise ValueError("one token per row expected")
+        if host.size and host.max() >= V:
+            raise IndexError("token out of range")
+        tok = dev.index_array(host.astype(np.int64))
+    xc = logits.data if logits.data.t.stride(1) == 1 else logits.data.contiguous()
+    scale = 1.0 / float(temperature)
+    both = dev.empty((2, N))
+    lp, entropy = both.t[0], both.t[1]
+    _, _, lse, ids, tops = K.token_logprobs(xc.t, tok.t, top=top, scale=scale, logprob=lp, entropy=entropy)
+    out = None
+
+    def _backward():
+        if logits.requires_grad:
+            g = out.grad.contiguous().t
+            target, acc = _grad_target(logits)
+            K.token_logprobs_bwd(xc.t, tok.t, lse, entropy, g[0], g[1], scale=scale, dlogits=target.t, accumulate=acc)
+
+    out = _node(both, (logits,), "token_logprobs", _backward, _track(logits))
+    return out[0], out[1], DeviceArray(ids), DeviceArray(tops)

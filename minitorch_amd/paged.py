@@ -1,0 +1,184 @@
+"""A key-value cache in pages, for generation.
+
+The reference recomputes the whole context for every new token (GPT.generate,
+transformer.py:93-104); GPT.generate_greedy keeps (B, Tmax, C) caches instead,
+sized for the longest sequence.  A ``PagedKVCache`` holds keys and values in
+pages of a fixed number of rows that sequences take as they grow and give back
+when they end, in fp32 or bf16, and can be bounded: with ``keep``, each layer
+and head remembers how much attention every row received, and when a sequence
+has grown past ``keep + slack`` rows it is cut back to its last ``recent`` rows
+and the ``keep - recent`` others that received the most.
+
+All layers and heads of a sequence hold the same number of rows, so they share
+one page table; which tokens' rows they hold differs once rows were evicted
+(attention does not depend on their order).  Lengths and the table live in
+device memory; a step of one token per sequence changes them without a copy
+from the host unless a sequence enters a new page.
+"""
+from __future__ import annotations
+
+import numpy as np
+
+from . import device as dev
+from . import kernels as K
+
+
+class PagedKVCache:
+    """Keys and values of n_layer layers with n_head K/V heads of head_dim for
+    `batch` sequences of up to max_tokens cached rows each.
+
+    page: rows a page; dtype: "float32" or "bfloat16"; pages: pages in the pool
+    (default: enough for every sequence at its longest, and for an eviction).
+    keep, recent, slack bound the cache as the module says (recent defaults to
+    keep // 8, slack to one page); observe: how many of a prompt's last
+    positions count its rows' attention (one-token steps always do)."""
+
+    def __init__(self, n_layer, n_head, head_dim, batch, max_tokens, page=16, dtype="float32", pages=None, keep=None,
+                 recent=None, slack=None, observe=8):
+        if min(n_layer, n_head, head_dim, batch, max_tokens, page) < 1:
+            raise ValueError("sizes must be at least 1")
+        if head_dim not in (16, 32, 64, 128):
+            raise ValueError(f"head_dim {head_dim} not in (16, 32, 64, 128)")
+        if dtype not in ("float32", "bfloat16"):
+            raise ValueError(f"unsupported dtype {dtype!r} (float32 or bfloat16)")
+        self.n_layer, self.n_head, self.head_dim, self.batch = n_layer, n_head, head_dim, batch
+        self.page, self.dtype, self.max_tokens = page, dtype, max_tokens
+        self.width = -(-max_tokens // page)
+        self.keep = keep
+        spare = 0
+        if keep is not None:
+            self.recent = keep // 8 if recent is None else recent
+            self.slack = page if slack is None else slack
+            if not (1 <= keep and 0 <= self.recent <= keep and self.slack >= 0 and observe >= 0):
+                raise ValueError("needs keep >= 1, 0 <= recent <= keep, slack >= 0 and observe >= 0")
+            if keep + self.slack + 1 > max_tokens:
+                raise ValueError(f"keep + slack + 1 = {keep + self.slack + 1} rows exceed max_tokens {max_tokens}")
+            spare = batch * -(-keep // page)
+        elif recent is not None or slack is not None:
+            raise ValueError("recent and slack bound a cache that has keep")
+        self.observed = observe
+        self.n_pages = batch * self.width + spare if pages is None else pages
+        if self.n_pages < 1:
+            raise ValueError("the pool needs at least one page")
+        # stored by heads: a head's rows of a page are adjacent
+        shape = (self.n_pages, n_head, page, head_dim)
+        self.k = [dev.empty_buf(shape, dtype) for _ in range(n_layer)]
+        self.v = [dev.empty_buf(shape, dtype) for _ in range(n_layer)]
+        self.table = dev.full((batch, self.width), -1, "int32").t
+        self.lengths = dev.zeros((batch,), "int32").t
+        self.counts = None  # rows of the append under way, where they differ
+        self.weights = None
+        if keep is not None:
+            w = (batch, n_head, self.width * page)
+            self.weights = [dev.zeros(w).t for _ in range(n_layer)]
+            self._weights_to = dev.empty_buf(w)
+            self._lengths_to = dev.empty_buf((batch,), "int32")
+        # the host's copies
+        self._len = np.zeros(batch, np.int32)
+        self._tab = np.full((batch, self.width), -1, np.int32)
+        self._free = list(range(self.n_pages - 1, -1, -1))
+        self._prompt = False  # the rows being appended are their sequences' first
+
+    # -- what it holds ---------------------------------------------------------
+    def length(self, b: int) -> int:
+        """Cached rows of sequence b."""
+        return int(self._len[b])
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    # -- growing and shrinking ---------------------------------------------------
+    def reserve(self, n=1):
+        """Make room for n new rows in every sequence (an int, or one per
+        sequence; 0 leaves it as it is): the rows that the layers' append then
+        write.  Nothing has changed when it raises."""
+        n = np.broadcast_to(np.asarray(n, np.int32), (self.batch,))
+        if n.min() < 0 or n.max() < 1:
+            raise ValueError("reserve: at least one new row, none negative")
+        grown = self._len + n
+        if grown.max() > self.width * self.page:
+            raise ValueError(f"reserve: {int(grown.max())} rows exceed the {self.width * self.page} a sequence may hold")
+        have, need = -(-self._len // self.page), -(-grown // self.page)
+        if (need - have).sum() > len(self._free):
+            raise RuntimeError(f"reserve: {int((need - have).sum())} pages needed, {len(self._free)} free")
+        for b in np.flatnonzero(need > have):
+            for i in range(have[b], need[b]):
+                self._tab[b, i] = self._free.pop()
+        if (need > have).any():
+            self.table.copy_(self._tab)
+        self._prompt = not self._len.any()
+        if n.min() == n.max() == 1:
+            K.decode_advance(self.lengths)
+            self.counts = None
+        else:
+            self.lengths.copy_(grown)
+            self.counts = None if n.min() == n.max() else dev.from_host(n, np.int32).t
+        self._len = grown
+
+    def release(self, b: int):
+        """Give back a sequence's pages; it is empty afterwards."""
+        self._give_back(b, self._tab[b])
+        self._len[b] = 0
+        self.table.copy_(self._tab)
+        self.lengths.copy_(self._len)
+        if self.weights is not None:
+            for w in self.weights:
+                w[b].fill_(0.0)
+
+    def _give_back(self, b, ids):
+        self._free += [int(i) for i in ids if i >= 0]
+        self._tab[b] = -1
+
+    def trim(self) -> bool:
+        """With keep: if a sequence holds more than keep + slack rows, cut all
+        that hold more than keep back to keep.  Returns whether it did."""
+        if self.keep is None or self._len.max() <= self.keep + self.slack:
+            return False
+        new = np.minimum(self._len, self.keep)
+        need = -(-new // self.page)
+        if need.sum() > len(self._free):
+            raise RuntimeError(f"trim: {int(need.sum())} pages needed, {len(self._free)} free")
+        to = np.full((self.batch, max(1, -(-self.keep // self.page))), -1, np.int32)
+        for b in range(self.batch):
+            to[b, :need[b]] = [self._free.pop() for _ in range(need[b])]
+        to_dev = dev.from_host(to, np.int32).t
+        for i in range(self.n_layer):
+            K.kv_evict_paged(self.k[i], self.v[i], self.table, self.lengths, self.weights[i], to_dev, self.keep,
+                             self.recent, lengths_out=self._lengths_to, weights_out=self._weights_to)
+            self.weights[i], self._weights_to = self._weights_to, self.weights[i]
+        self.lengths, self._lengths_to = self._lengths_to, self.lengths
+        for b in range(self.batch):
+            self._give_back(b, self._tab[b])
+        self._tab[:, :to.shape[1]] = to
+        self.table.copy_(self._tab)
+        self._len = new
+        return True
+
+    # -- a layer's work ----------------------------------------------------------
+    def append(self, layer, k, v):
+        """Write the rows reserved last: k and v (B, n_head, T, head_dim)."""
+        K.kv_append_paged(k, v, self.k[layer], self.v[layer], self.table, self.lengths, counts=self.counts)
+
+    def attend(self, layer, q, scale, out=None):
+        """Attention of one new token per sequence, q (B, H, 1, head_dim) with H
+        a multiple of n_head, over the cached rows, whose weights it counts."""
+        w = None if self.weights is None else self.weights[layer]
+        return K.attn_decode_paged(q, self.k[layer], self.v[layer], self.table, self.lengths, scale, out=out,
+                                   weights=w, weights_in=w)[0]
+
+    def observe(self, layer, q, scale):
+        """Count the attention that a prompt's last positions, q
+        (B, H, T, head_dim), pay its rows (with keep)."""
+        if self.weights is None:
+            return
+        T = q.shape[2]
+        n = min(self.observed, T)
+        if layer == 0:  # the rows that each of those positions sees
+            back = np.arange(n - 1, -1, -1, dtype=np.int32)[:, None]
+            self._seen = dev.from_host(np.maximum(self._len - back, 0), np.int32).t
+        w = self.weights[layer]
+        for i in range(n):
+            t = T - n + i
+            K.attn_decode_paged(q[:, :, t:t + 1], self.k[layer], self.v[layer], self.table, self._seen[i], scale,
+                                weights=w, weights_in=w)

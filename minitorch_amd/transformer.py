@@ -132,15 +132,44 @@ class MultiHeadAttention(Module):
             K.attn_decode(qh, kh, vh, 1.0 / math.sqrt(D), out=out.t.transpose(1, 2))
         else:
             K.attn_fwd(qh, kh, vh, 1.0 / math.sqrt(D), True, out=out.t.transpose(1, 2))
-        o = Tensor(out.reshape(B, T, C))
+        return self._project_residual(Tensor(out.reshape(B, T, C)), residual)
+
+    def _project_residual(self, o, residual):
+        """out_proj(o) (+ residual, added in the epilogue) of attention rows o
+        (B, T, C); inference only."""
+        from . import kernels as K
+
         if residual is None:
             return self.out_proj(o)
+        B, T, C = o.shape
+        rows = B * T
         y = dev.empty((B, T, C))
         K.gemm(o.data.t.reshape(rows, C), self.out_proj.weight.data.t, y.t.view(rows, C),
                bias=self.out_proj.bias.data.t if self.out_proj.bias is not None else None,
                act=K.GEMM_ACT_ADD, aux=residual.data.t.reshape(rows, C))
         return Tensor(y)
 
+    def forward_paged(self, x, cache, layer, residual=None):
+        """Inference-only attention of x (B, T, C) whose keys and values go to
+        the rows that `cache` (a PagedKVCache) reserved last: T = 1 new token per
+        sequence over everything cached, or a whole prompt (the sequences' first
+        rows).  With `residual` the result is residual + attention(x)."""
+        from . import kernels as K
+
+        B, T, C = x.shape
+        H, D = self.n_head, self.head_dim
+        scale = 1.0 / math.sqrt(D)
+        q, k, v = (p(x).data.t.view(B, T, H, D).transpose(1, 2) for p in (self.q_proj, self.k_proj, self.v_proj))
+        cache.append(layer, k, v)
+        out = dev.empty((B, T, H, D))
+        if T == 1:
+            cache.attend(layer, q, scale, out=out.t.transpose(1, 2))
+        else:
+            if not cache._prompt:
+                raise ValueError("forward_paged takes one new token per sequence, or a prompt for empty sequences")
+            K.attn_fwd(q, k, v, scale, True, out=out.t.transpose(1, 2))
+            cache.observe(layer, q, scale)
+        return self._project_residual(Tensor(out.reshape(B, T, C)), residual)
 
     def forward_step(self, x, cache, lengths, residual=None, ln=None):
         """One-token decode step whose positions live in device memory, so a
@@ -253,15 +282,26 @@ class TransformerBlock(Module):
         epilogue (no pre-activation kept), the values of the layer-by-layer
         composition.  fused: the attention's q/k/v projections as one GEMM
         over its fused weight, refreshed by the caller (attn.fuse_qkv)."""
+        return self._forward_inference(
+            x, lambda h, residual=None: self.attn.forward_cached(h, cache, t0, residual=residual, fused=fused))
+
+    def forward_paged(self, x, cache, layer):
+        """forward_cached with the attention's keys and values in the pages of
+        a PagedKVCache (MultiHeadAttention.forward_paged)."""
+        return self._forward_inference(
+            x, lambda h, residual=None: self.attn.forward_paged(h, cache, layer, residual=residual))
+
+    def _forward_inference(self, x, attn):
+        """The block with attn(ln1(x), residual=x) as its attention."""
         from . import kernels as K
 
         fc1, act, fc2, drop = self.mlp.layers
         if not (isinstance(fc1, Linear) and isinstance(act, GELU) and isinstance(fc2, Linear)
                 and fc1.bias is not None and fc2.bias is not None
                 and (not drop._training or drop.p == 0.0)):
-            x = x + self.attn.forward_cached(self.ln1(x), cache, t0, fused=fused)
+            x = x + attn(self.ln1(x))
             return x + self.mlp(self.ln2(x))
-        x = self.attn.forward_cached(self.ln1(x), cache, t0, residual=x, fused=fused)
+        x = attn(self.ln1(x), residual=x)
         B, T, C = x.shape
         rows, Hd = B * T, fc1.weight.shape[1]
         h = dev.empty((rows, Hd))
@@ -654,7 +694,17 @@ class GPT(Module):
         return K.DecodeStep(layers, self.tok_emb.weight.data.t, self.pos_emb.weight.data.t, lnf,
                             self.lm_head.weight.data.t, self.lm_head.bias.data.t, B, Tmax)
 
-    def generate(self, idx, max_new_tokens, temperature=1.0):
+    def paged_cache(self, batch, max_tokens=None, **options):
+        """A PagedKVCache of this model's layers and heads for `batch`
+        sequences of up to max_tokens (default: block_size) cached rows;
+        options as PagedKVCache's."""
+        from .paged import PagedKVCache
+
+        attn = self.blocks[0].attn
+        return PagedKVCache(len(self.blocks), attn.n_head, attn.head_dim, batch,
+                            self.block_size if max_tokens is None else max_tokens, **options)
+
+    def generate(self, idx, max_new_tokens, temperature=1.0, cache=None, return_logprobs=False):
         """Sample tokens as the reference does (transformer.py:93-104): each
         step takes the last position's logits / temperature, a softmax, and
         one np.random.choice per row from NumPy's global RNG, rows in order.
@@ -662,7 +712,11 @@ class GPT(Module):
         block_size; once the reference would crop it (positions shift) they
         come from a full forward over the cropped context.  The softmax runs
         on the device; the host draws.  With active dropout (training mode,
-        p > 0) every step is a full forward, as in the reference."""
+        p > 0) every step is a full forward, as in the reference.  With `cache` (an
+        empty PagedKVCache for this model and batch, paged_cache) the keys and
+        values are kept there, cut back after each step if it is bounded; prompt
+        and new tokens then have to fit block_size.  return_logprobs: returns
+        (ids, log probabilities of the new tokens (B, n))."""
         from . import kernels as K
 
         idx = np.asarray(idx)
@@ -672,12 +726,24 @@ class GPT(Module):
         out = np.empty((B, T0 + n), dtype=np.int64)
         out[:, :T0] = idx
         if n < 1:
-            return out
+            return (out, np.empty((B, 0), np.float32)) if return_logprobs else out
         V = self.lm_head.weight.shape[1]
         C = self.tok_emb.weight.shape[1]
         temp = dev.const(float(temperature))
         mods = [self] + [m for kind, _, m, _ in self._walk() if kind == "module"]
         dropout_on = any(isinstance(m, Dropout) and m._training and m.p > 0.0 for m in mods)
+        if cache is not None:
+            attn = self.blocks[0].attn
+            if (cache.batch, cache.n_layer, cache.n_head, cache.head_dim) != (B, len(self.blocks), attn.n_head,
+                                                                               attn.head_dim):
+                raise ValueError("the cache is for another batch, or another model")
+            if cache._len.any():
+                raise ValueError("the cache is not empty")
+            if T0 + n > blk:
+                raise ValueError(f"prompt + new tokens = {T0 + n} exceeds block_size {blk}")
+            if dropout_on:
+                raise ValueError("a cache does not go with active dropout (use model.eval())")
+        logprobs = []
 
         def sample(logits2d):
             scaled = dev.empty((B, V))
@@ -686,7 +752,10 @@ class GPT(Module):
             K.softmax_fwd(scaled.t, probs.t)
             p = probs.numpy().astype(np.float64)
             p /= p.sum(axis=-1, keepdims=True)
-            return np.array([np.random.choice(V, p=pr) for pr in p])
+            drawn = np.array([np.random.choice(V, p=pr) for pr in p])
+            if return_logprobs:
+                logprobs.append(K.token_logprobs(scaled.t, dev.index_array(drawn.astype(np.int64)).t)[0])
+            return drawn
 
         def last_logits(x):
             x = self.ln_f(Tensor(x.data.t[:, -1:, :]))
@@ -695,12 +764,25 @@ class GPT(Module):
         with no_grad():
             ctx = T0
             caches = None
-            if T0 <= blk and not dropout_on:
+
+            def paged(tokens, t):  # logits after tokens (B, T) at positions t on
+                T = tokens.shape[1]
+                cache.reserve(T)
+                x = self.tok_emb(dev.index_array(tokens)) + self.pos_emb(DeviceArray(pos.t[t:t + T]))
+                for i, block in enumerate(self.blocks):
+                    x = block.forward_paged(x, cache, i)
+                cache.trim()
+                return last_logits(x)
+
+            if cache is not None:
+                pos = self._positions(blk)
+                logits = paged(idx, 0)
+            elif T0 <= blk and not dropout_on:
                 caches = [(dev.empty((B, blk, C)), dev.empty((B, blk, C))) for _ in self.blocks]
                 pos = self._positions(blk)
                 x = self.tok_emb(dev.index_array(idx)) + self.pos_emb(DeviceArray(pos.t[:T0]))
-                for block, cache in zip(self.blocks, caches):
-                    x = block.forward_cached(x, cache, 0)
+                for block, kv in zip(self.blocks, caches):
+                    x = block.forward_cached(x, kv, 0)
                 logits = last_logits(x)
             else:
                 logits = self.forward(out[:, max(0, ctx - blk):ctx]).data.t[:, -1, :]
@@ -709,14 +791,18 @@ class GPT(Module):
                 ctx += 1
                 if i == n - 1:
                     break
-                if caches is not None and ctx <= blk:
+                if cache is not None:
+                    logits = paged(out[:, ctx - 1:ctx], ctx - 1)
+                elif caches is not None and ctx <= blk:
                     # the new token sits at position ctx - 1 of an uncropped context
                     t = ctx - 1
                     x = self.tok_emb(dev.index_array(out[:, t:t + 1])) + self.pos_emb(DeviceArray(pos.t[t:t + 1]))
-                    for block, cache in zip(self.blocks, caches):
-                        x = block.forward_cached(x, cache, t)
+                    for block, kv in zip(self.blocks, caches):
+                        x = block.forward_cached(x, kv, t)
                     logits = last_logits(x)
                 else:
                     caches = None
                     logits = self.forward(out[:, max(0, ctx - blk):ctx]).data.t[:, -1, :]
+        if return_logprobs:
+            return out, np.stack([t.numpy() for t in logprobs], axis=1)
         return out

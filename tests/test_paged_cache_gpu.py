@@ -1,0 +1,275 @@
+"""The paged cache as the framework uses it: PagedKVCache's pages, generation
+through it against generation without, and training on token_logprobs, eagerly
+and as a recorded step.
+
+Tokens drawn with one seed have to be the same whatever cache holds the keys:
+the logits differ by fp32 rounding only (some 1e-6 of their size), far less than
+what moves a draw.  Log probabilities are compared at 1e-4: the logits' own
+1e-5 of values up to 8, as the bars of the GPT tests have it."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def model(seed=0, block=64, n_embd=64, n_head=2, n_layer=2, vocab=50):
+    import minitorch_amd as mt
+
+    m = mt.GPT(vocab, block, n_embd=n_embd, n_head=n_head, n_layer=n_layer)
+    # larger than at the start of training, so that attention is not uniform
+    return m.init_weights(np.random.default_rng(seed), std=0.15)
+
+
+def logprobs_of(m, ids, T0, temperature):
+    """log softmax of the model's full-context logits at the tokens after T0."""
+    import minitorch_amd as mt
+
+    with mt.no_grad():
+        x = m(ids).data.numpy().astype(np.float64)[:, T0 - 1:-1] / temperature
+    x = x - x.max(-1, keepdims=True)
+    x = x - np.log(np.exp(x).sum(-1, keepdims=True))
+    return np.take_along_axis(x, ids[:, T0:, None], -1)[..., 0]
+
+
+@pytest.mark.parametrize("page,T0", [(16, 20), (5, 20), (16, 1)])
+def test_generate_through_pages(dev, page, T0):
+    m = model()
+    rng = np.random.default_rng(1)
+    idx = rng.integers(0, 50, (3, T0))
+    np.random.seed(5)
+    want = m.generate(idx, 30, temperature=0.8)
+    np.random.seed(5)
+    cache = m.paged_cache(3, page=page)
+    got, lp = m.generate(idx, 30, temperature=0.8, cache=cache, return_logprobs=True)
+    assert np.array_equal(got, want)
+    assert np.abs(lp - logprobs_of(m, got, T0, 0.8)).max() <= 1e-4
+    assert [cache.length(b) for b in range(3)] == [T0 + 29] * 3
+    used = 3 * -(-(T0 + 29) // page)
+    assert cache.free_pages == cache.n_pages - used
+    for b in range(3):
+        cache.release(b)
+    assert cache.free_pages == cache.n_pages
+    np.random.seed(5)  # and again, in the pages given back
+    assert np.array_equal(m.generate(idx, 30, temperature=0.8, cache=cache), want)
+
+
+def test_generate_logprobs_without_a_cache(dev):
+    m = model()
+    idx = np.random.default_rng(2).integers(0, 50, (2, 7))
+    np.random.seed(3)
+    got, lp = m.generate(idx, 9, return_logprobs=True)
+    np.random.seed(3)
+    assert np.array_equal(got, m.generate(idx, 9))
+    assert np.abs(lp - logprobs_of(m, got, 7, 1.0)).max() <= 1e-4
+    ids, none = m.generate(idx, 0, return_logprobs=True)
+    assert np.array_equal(ids, idx) and none.shape == (2, 0)
+
+
+def test_generate_with_bf16_pages(dev):
+    """Keys and values rounded to bf16 (half a step 2^-8 each): logits of
+    values up to 8 move by some 2^-8 of that, through two layers."""
+    m = model()
+    idx = np.random.default_rng(4).integers(0, 50, (2, 12))
+    np.random.seed(6)
+    got, lp = m.generate(idx, 20, cache=m.paged_cache(2, dtype="bfloat16"), return_logprobs=True)
+    assert np.abs(lp - logprobs_of(m, got, 12, 1.0)).max() <= 16 * 8 * 2.0 ** -8
+
+
+def test_bounded_cache_that_never_fills_changes_nothing(dev):
+    m = model()
+    idx = np.random.default_rng(7).integers(0, 50, (2, 10))
+    np.random.seed(8)
+    want = m.generate(idx, 20)
+    np.random.seed(8)
+    cache = m.paged_cache(2, max_tokens=48, keep=30, slack=10, page=8)
+    assert np.array_equal(m.generate(idx, 20, cache=cache), want)
+
+
+def test_bounded_cache_stays_bounded(dev):
+    m = model()
+    idx = np.random.default_rng(9).integers(0, 50, (2, 25))
+    cache = m.paged_cache(2, max_tokens=32, keep=16, recent=4, slack=5, page=8)
+    np.random.seed(1)
+    first, lp = m.generate(idx, 35, cache=cache, return_logprobs=True)
+    assert np.isfinite(lp).all() and (lp <= 0).all()
+    assert all(16 <= cache.length(b) <= 21 for b in range(2))
+    assert cache.free_pages == cache.n_pages - sum(-(-cache.length(b) // 8) for b in range(2))
+    assert np.array_equal(cache.lengths.numpy(), [cache.length(b) for b in range(2)])
+    for b in range(2):
+        cache.release(b)
+    np.random.seed(1)
+    again = m.generate(idx, 35, cache=cache)
+    assert np.array_equal(again, first)
+
+
+def test_trim_keeps_what_was_attended_and_the_latest(dev):
+    """After a prompt and one cut, each head's rows are the prompt's, in order,
+    the last `recent` among them and the others those of greatest weight."""
+    import minitorch_amd as mt
+    from minitorch_amd import device
+
+    m = model(n_layer=1)
+    T0, keep, recent = 30, 12, 3
+    idx = np.random.default_rng(11).integers(0, 50, (2, T0))
+    full = m.paged_cache(2, page=8, keep=40, slack=4, max_tokens=60, observe=5)
+    cut = m.paged_cache(2, page=8, keep=keep, recent=recent, slack=0, max_tokens=32, observe=5)
+    pos = m._positions(64)
+    with mt.no_grad():
+        x = m.tok_emb(idx) + m.pos_emb(device.DeviceArray(pos.t[:T0]))
+        for c in (full, cut):
+            c.reserve(T0)
+            m.blocks[0].forward_paged(x, c, 0)
+    w = cut.weights[0].numpy().copy()
+    assert np.array_equal(w[..., :T0], full.weights[0].numpy()[..., :T0])
+    # five positions observed, each with weight 1 a head
+    assert np.abs(w.sum(-1) - 5).max() < 1e-5
+    assert not full.trim() and cut.trim()
+    rows = lambda c, n: [c.k[0].numpy()[c._tab[b]].transpose(1, 0, 2, 3).reshape(2, -1, 32)[:, :n] for b in range(2)]
+    for b, (all_rows, kept) in enumerate(zip(rows(full, T0), rows(cut, keep))):
+        for h in range(2):
+            old = np.sort(np.argsort(-w[b, h, :T0 - recent], kind="stable")[:keep - recent])
+            want = np.concatenate([old, np.arange(T0 - recent, T0)])
+            assert np.array_equal(kept[h], all_rows[h][want])
+            assert np.array_equal(cut.weights[0].numpy()[b, h, :keep], w[b, h, want])
+
+
+def test_cache_refusals(dev):
+    import minitorch_amd as mt
+
+    for bad in (dict(page=0), dict(dtype="int32"), dict(keep=0), dict(keep=8, recent=9), dict(keep=63, slack=4),
+                dict(recent=3), dict(pages=0)):
+        with pytest.raises(ValueError):
+            mt.PagedKVCache(1, 2, 32, 2, 64, **bad)
+    with pytest.raises(ValueError, match="head_dim"):
+        mt.PagedKVCache(1, 2, 48, 2, 64)
+    c = mt.PagedKVCache(1, 2, 32, 2, 64, page=8, pages=5)
+    for n in (0, -1, [1, -1]):
+        with pytest.raises(ValueError):
+            c.reserve(n)
+    with pytest.raises(ValueError, match="exceed"):
+        c.reserve([65, 1])
+    with pytest.raises(RuntimeError, match="pages"):
+        c.reserve([33, 8])
+    assert c.free_pages == 5 and c.length(0) == 0  # nothing changed
+    c.reserve([32, 8])
+    assert c.free_pages == 0
+    m = model()
+    idx = np.zeros((2, 10), np.int64)
+    with pytest.raises(ValueError, match="batch"):
+        m.generate(idx, 3, cache=m.paged_cache(3))
+    with pytest.raises(ValueError, match="block_size"):
+        m.generate(idx, 60, cache=m.paged_cache(2))
+    used = m.paged_cache(2)
+    m.generate(idx, 3, cache=used)
+    with pytest.raises(ValueError, match="empty"):
+        m.generate(idx, 3, cache=used)
+
+
+# ---------------------------------------------------------------------------
+# training on log probabilities
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("N,V", [(7, 33), (40, 1500)])
+def test_token_logprobs_is_cross_entropys_negative(dev, N, V):
+    """mean(-logprob) and its gradient are cross_entropy's."""
+    import minitorch_amd as mt
+
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((N, V)).astype(np.float32) * 3
+    tok = rng.integers(0, V, N)
+    a, b = mt.Tensor(x, requires_grad=True), mt.Tensor(x, requires_grad=True)
+    lp, ent, ids, tops = mt.F.token_logprobs(a, tok, top=3)
+    loss = (-lp).mean()
+    loss.backward()
+    want = mt.F.cross_entropy(b, tok)
+    want.backward()
+    assert abs(float(loss) - float(want)) <= 1e-5 * abs(float(want))
+    # a probability to 1e-4 relative, over N rows
+    g, w = a.grad.numpy(), b.grad.numpy()
+    assert np.all(np.abs(g - w) <= 1e-4 * np.abs(w) + 1e-9)
+    assert ids.shape == (N, 3) and np.array_equal(ids.numpy()[:, 0], x.argmax(1))
+
+
+def test_token_logprobs_gradients_add_up(dev):
+    """A loss of both outputs, twice, with a temperature and rows without a
+    token, against the float64 form; the logits' other consumer adds to it."""
+    import minitorch_amd as mt
+    from oracle import paged as ref
+
+    rng = np.random.default_rng(3)
+    N, V, temperature = 9, 70, 0.5
+    x = rng.standard_normal((N, V)).astype(np.float32)
+    tok = rng.integers(0, V, N)
+    tok[[2, 5]] = -1
+    adv = rng.standard_normal(N).astype(np.float32)
+    t = mt.Tensor(x, requires_grad=True)
+    lp, ent, _, _ = mt.F.token_logprobs(t, tok, temperature=temperature)
+    ((lp * mt.Tensor(adv)).sum() + ent.sum() * 0.25 + t.sum()).backward()
+    want = ref.logprobs_grad(x, tok, adv, np.full(N, 0.25, np.float32), 2.0) + 1
+    got = t.grad.numpy()
+    assert np.all(np.abs(got - want) <= 1e-5 * (1 + np.abs(want)))
+    assert np.all(lp.numpy()[[2, 5]] == 0)
+    # the entropy alone
+    t = mt.Tensor(x, requires_grad=True)
+    mt.F.token_logprobs(t, tok)[1].sum().backward()
+    want = ref.logprobs_grad(x, tok, np.zeros(N, np.float32), np.ones(N, np.float32))
+    assert np.all(np.abs(t.grad.numpy() - want) <= 1e-5)
+    with mt.no_grad():
+        lp, _, _, _ = mt.F.token_logprobs(t, tok)
+    assert not lp.requires_grad
+
+
+def test_token_logprobs_refusals(dev):
+    import minitorch_amd as mt
+
+    x = mt.Tensor(np.zeros((3, 5), np.float32))
+    with pytest.raises(IndexError):
+        mt.F.token_logprobs(x, [0, 1, 5])
+    with pytest.raises(ValueError, match="one token"):
+        mt.F.token_logprobs(x, [0, 1])
+    for bad in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="temperature"):
+            mt.F.token_logprobs(x, [0, 1, 2], temperature=bad)
+    for bad in (-1, 6, 65):
+        with pytest.raises(ValueError, match="top"):
+            mt.F.token_logprobs(x, [0, 1, 2], top=bad)
+
+
+def test_recorded_training_step_on_logprobs(dev):
+    """A policy-gradient step (advantage times log probability, an entropy
+    bonus) recorded and replayed, with an eager graph of the same parameters
+    alive: the eager steps' losses and parameters, bit for bit."""
+    import minitorch_amd as mt
+    from minitorch_amd import device
+
+    rng = np.random.default_rng(13)
+    B, T, V = 4, 16, 50
+    data = [(rng.integers(0, V, (B, T)), rng.integers(0, V, B * T)) for _ in range(7)]
+    adv = rng.standard_normal(B * T).astype(np.float32)
+
+    def run(captured):
+        m = model(seed=2)
+        opt = mt.Adam(m.parameters(), lr=1e-3).capturable()
+        weight = mt.Tensor(adv)
+
+        def step(i, y):
+            opt.zero_grad()
+            logits = m(i).reshape(-1, V)
+            lp, ent, _, _ = mt.F.token_logprobs(logits, y)
+            loss = -(lp * weight).mean() - ent.mean() * 0.01
+            loss.backward()
+            opt.step()
+            return loss
+
+        rec = mt.CapturedStep(step, optimizer=opt) if captured else step
+        losses = []
+        for i, y in data:
+            keep = mt.F.token_logprobs(m(i).reshape(-1, V), y)[0].sum()  # lives over the step
+            losses.append(rec(device.index_array(i), device.index_array(y)).numpy().item())
+            assert np.isfinite(float(keep))
+        return losses, [p.data.numpy() for p in m.parameters()]
+
+    eager, recorded = run(False), run(True)
+    assert eager[0] == recorded[0]
+    assert all(np.array_equal(a, b) for a, b in zip(eager[1], recorded[1]))
