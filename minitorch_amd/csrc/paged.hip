@@ -304,10 +304,10 @@ __device__ __forceinline__ float lane_sum4(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// EVEN: pages of a multiple of 16 rows and row strides that fit 32-bit lane
-// offsets, so 16 rows have one page and one uniform address; otherwise each lane
-// looks up its rows
-template <typename TQ, typename TC, int D, bool EVEN>
+// RUN consecutive rows (aligned to RUN) lie in one page, at row strides that fit
+// 32-bit offsets: 16, a tile's rows have one uniform address; 4, a lane looks up
+// its four V rows at once; 1, each by itself
+template <typename TQ, typename TC, int D, int RUN>
 __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
   using Tile = DecodeTile<TQ, TC, D>;
   constexpr int NT = Tile::NT, VD = Tile::VD, KT = 16 * NT, LD = D + 4;
@@ -317,8 +317,10 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
   } sh;
   __shared__ float lse2[16];
 
-  const int split = blockIdx.x % a.S, rest = blockIdx.x / a.S;
-  const int ht = rest % a.HT, bh = rest / a.HT, b = bh / a.Hkv, hk = bh % a.Hkv;
+  // the HT workgroups that read the same rows are 8 apart: on one XCD, sharing its L2
+  const int eight = blockIdx.x / (8 * a.HT), ht = blockIdx.x / 8 % a.HT, piece = 8 * eight + blockIdx.x % 8;
+  const int split = piece % a.S, bh = piece / a.S, b = bh / a.Hkv, hk = bh % a.Hkv;
+  if (bh >= a.B * a.Hkv) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quarter = lane >> 4;
   const int heads = min(16, a.G - 16 * ht), h0 = hk * a.G + 16 * ht;
@@ -355,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
     bool in;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      if constexpr (EVEN)
+      if constexpr (RUN == 16)
         tile.load_k(t, kp + look1(a.k, j0 + 16 * t, in) + col * (int)a.k.sr, quarter);
       else
         tile.load_k(t, kp + look(a.k, j0 + 16 * t + col, in), quarter);
@@ -366,13 +368,22 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
     there = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      if constexpr (EVEN) {
+      if constexpr (RUN == 16) {
         const TC* base = vp + look1(a.v, j0 + 16 * t, in);
         const int seen = in ? c1 - j0 - 16 * t : 0;  // rows from j0 + 16 t on
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           tile.load_v(4 * t + r, base + (4 * quarter + r) * (int)a.v.sr + VD * col);
           there |= (uint32_t)(4 * quarter + r < seen) << (4 * t + r);
+        }
+      } else if constexpr (RUN == 4) {
+        const int j = j0 + 16 * t + 4 * quarter;
+        const TC* base = vp + look(a.v, j, in) + VD * col;
+        const int seen = in ? c1 - j : 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          tile.load_v(4 * t + r, base + r * (int)a.v.sr);
+          there |= (uint32_t)(r < seen) << (4 * t + r);
         }
       } else {
 #pragma unroll
@@ -992,9 +1003,10 @@ DecodePlan make_plan(int B, int H, int Hkv, int D, int cap, bool weights) {
 }
 
 template <typename TQ, typename TC, int D>
-int launch_decode(bool even, unsigned groups, unsigned finish, const DecodeArgs& a, hipStream_t st) {
-  if (even) hipLaunchKernelGGL((decode_kernel<TQ, TC, D, true>), dim3(groups), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((decode_kernel<TQ, TC, D, false>), dim3(groups), dim3(256), 0, st, a);
+int launch_decode(int run, unsigned groups, unsigned finish, const DecodeArgs& a, hipStream_t st) {
+  if (run == 16) hipLaunchKernelGGL((decode_kernel<TQ, TC, D, 16>), dim3(groups), dim3(256), 0, st, a);
+  else if (run == 4) hipLaunchKernelGGL((decode_kernel<TQ, TC, D, 4>), dim3(groups), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((decode_kernel<TQ, TC, D, 1>), dim3(groups), dim3(256), 0, st, a);
   MTX_LAUNCHED();
   if (!a.direct) {
     const unsigned heads = (unsigned)(a.B * a.H);
@@ -1007,12 +1019,12 @@ int launch_decode(bool even, unsigned groups, unsigned finish, const DecodeArgs&
   return MTX_OK;
 }
 template <typename TQ, typename TC>
-int dispatch_decode(int D, bool even, unsigned groups, unsigned finish, const DecodeArgs& a, hipStream_t st) {
+int dispatch_decode(int D, int run, unsigned groups, unsigned finish, const DecodeArgs& a, hipStream_t st) {
   switch (D) {
-    case 16: return launch_decode<TQ, TC, 16>(even, groups, finish, a, st);
-    case 32: return launch_decode<TQ, TC, 32>(even, groups, finish, a, st);
-    case 64: return launch_decode<TQ, TC, 64>(even, groups, finish, a, st);
-    default: return launch_decode<TQ, TC, 128>(even, groups, finish, a, st);
+    case 16: return launch_decode<TQ, TC, 16>(run, groups, finish, a, st);
+    case 32: return launch_decode<TQ, TC, 32>(run, groups, finish, a, st);
+    case 64: return launch_decode<TQ, TC, 64>(run, groups, finish, a, st);
+    default: return launch_decode<TQ, TC, 128>(run, groups, finish, a, st);
   }
 }
 
@@ -1096,7 +1108,7 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
   const size_t need = plan.bytes();
   MTX_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need && ((uintptr_t)workspace & 15u) == 0),
                 "workspace: %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
-  const int64_t groups = (int64_t)B * Hkv * plan.HT * plan.S;
+  const int64_t groups = ((int64_t)B * Hkv * plan.S + 7) / 8 * 8 * plan.HT;
   const int64_t finish = (weights != nullptr ? (int64_t)B * Hkv * cdiv(cap, kFinishRows) : 0);
   MTX_CHECK_SHAPE(groups <= INT32_MAX && finish <= INT32_MAX / 2, "decode: too many sequences, heads and rows in one call");
   float* ws = static_cast<float*>(workspace);
@@ -1107,12 +1119,12 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
                lengths, o, o_strides[0], o_strides[1], lse, weights_in, weights, weights_ld,
                ws, ws + plan.n_o, ws + plan.n_o + plan.n_ml, plan.sld,
                B, H, Hkv, H / Hkv, plan.S, plan.HT, plan.chunk, cap, plan.direct, scale * kLog2e};
-  // 16 rows at lane offsets of 32 bits from one address
-  const bool even = page % 16 == 0 && std::max(kp_strides[2], vp_strides[2]) < (1 << 24);
+  const bool near = std::max(kp_strides[2], vp_strides[2]) < (1 << 24);
+  const int run = !near || page % 4 ? 1 : page % 16 ? 4 : 16;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache_dtype == MTX_F32) return dispatch_decode<float, float>(D, even, (unsigned)groups, (unsigned)finish, a, st);
-  if (dtype == MTX_F32) return dispatch_decode<float, bf16_t>(D, even, (unsigned)groups, (unsigned)finish, a, st);
-  return dispatch_decode<bf16_t, bf16_t>(D, even, (unsigned)groups, (unsigned)finish, a, st);
+  if (cache_dtype == MTX_F32) return dispatch_decode<float, float>(D, run, (unsigned)groups, (unsigned)finish, a, st);
+  if (dtype == MTX_F32) return dispatch_decode<float, bf16_t>(D, run, (unsigned)groups, (unsigned)finish, a, st);
+  return dispatch_decode<bf16_t, bf16_t>(D, run, (unsigned)groups, (unsigned)finish, a, st);
 }
 
 extern "C" int mtx_kv_evict_paged(int cache_dtype, int B, int H, int D, int64_t n_pages, int page, void* k_pages,
