@@ -55,6 +55,17 @@ __device__ __forceinline__ void load_values(const bf16_t* p, float (&x)[E]) {
   for (int i = 0; i < E; ++i) x[i] = bf2f(u.x[i]);
 }
 
+// the same of the `left` values from p on, -inf behind them
+template <int E, typename T>
+__device__ __forceinline__ void load_left(const T* p, int left, float (&x)[E]) {
+  if (left >= E) {
+    load_values<E>(p, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = i < left ? Elem<T>::to_f(p[i]) : -INFINITY;
+  }
+}
+
 // values of -inf add 0, not 0 * inf; NaN stays
 constexpr float kFarBelow = -1e30f;
 __device__ __forceinline__ float below(float d) { return __builtin_elementwise_maximum(d, kFarBelow); }
@@ -242,10 +253,12 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const LpArgs a, int
   }
 }
 
-// ---- longer rows: a workgroup of NT threads each, one pass with the running
-// maximum and sums, E values (16 bytes) a load and kLoads of them in flight ----
-constexpr int kLoads = 4, kCap = 1024;
-template <typename T, int NT>
+// ---- longer rows: a workgroup of NT threads each, E values (16 bytes) a load, U of
+// them in flight.  WHOLE: the row fits U loads a thread and stays in registers;
+// otherwise one pass with the running maximum and sums, and what is collected for
+// the alternatives is read again ----
+constexpr int kCap = 1024;  // candidates
+template <typename T, int NT, int U, bool WHOLE>
 __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   constexpr int E = Elem<T>::kVec, W = NT / 64, STEP = NT * E;
   __shared__ uint64_t cands[kCap];
@@ -256,70 +269,90 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   const int64_t r = blockIdx.x;
   const T* __restrict__ x = static_cast<const T*>(a.x) + r * a.ld;
   const float c = a.scale * kLog2e;
-  float m = -FLT_MAX, l = 0.f, t = 0.f;
+  float v[U][E], m = -FLT_MAX, l = 0.f, t = 0.f;
   auto raise = [&](float top) {  // the sums relative to a larger maximum
     const float n = fmaxf(m, top), d = fmaxf(m - n, kFarBelow), f = __builtin_amdgcn_exp2f(d * c);
     t = f * fmaf(l, d, t);
     l *= f;
     m = n;
   };
-  auto add = [&](float v) {
-    const float d = below(v - m), e = __builtin_amdgcn_exp2f(d * c);
-    l += e;
-    t = fmaf(e, d, t);
-  };
-  int i = tid * E;
-  for (; i + (kLoads - 1) * STEP + E <= a.V; i += kLoads * STEP) {
-    float v[kLoads][E];
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) load_values<E>(x + i + u * STEP, v[u]);
+  auto largest = [&] {
     float top = v[0][0];
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e) top = fmaxf(top, v[u][e]);
-    raise(top);
+    return top;
+  };
+  auto add = [&] {
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < E; ++e) add(v[u][e]);
-  }
-  for (; i < a.V; i += STEP) {
-    float v[E];
-    if (i + E <= a.V) {
-      load_values<E>(x + i, v);
-    } else {
+      for (int e = 0; e < E; ++e) {
+        const float d = below(v[u][e] - m), p = __builtin_amdgcn_exp2f(d * c);
+        l += p;
+        t = fmaf(p, d, t);
+      }
+  };
+  int i = tid * E;
+  if (!WHOLE) {
+    for (; i + (U - 1) * STEP + E <= a.V; i += U * STEP) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = i + e < a.V ? Elem<T>::to_f(x[i + e]) : -INFINITY;
+      for (int u = 0; u < U; ++u) load_values<E>(x + i + u * STEP, v[u]);
+      raise(largest());
+      add();
     }
-    float top = v[0];
+  }
+  if (WHOLE || i < a.V) {
 #pragma unroll
-    for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);
-    raise(top);
-#pragma unroll
-    for (int e = 0; e < E; ++e) add(v[e]);
+    for (int u = 0; u < U; ++u) load_left<E>(x + i + u * STEP, a.V - i - u * STEP, v[u]);
+    if (WHOLE) {
+      m = fmaxf(m, largest());
+    } else {
+      raise(largest());
+      add();
+    }
   }
   const float mine = m;  // the thread's largest value
-  raise(all_max(m));
+  if (WHOLE) {
+    m = all_max(m);
+    if (W > 1) {
+      if (lane == 0) red[0][wave] = m;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W; ++w) m = fmaxf(m, red[0][w]);
+    }
+    add();
+  } else {
+    raise(all_max(m));
+  }
   l = all_sum(l);
   t = all_sum(t);
-  if (lane == 0) red[0][wave] = m, red[1][wave] = l, red[2][wave] = t;
+  if (lane == 0) {
+    if (!WHOLE) red[0][wave] = m;
+    red[1][wave] = l, red[2][wave] = t;
+  }
   if (a.top) {
     sorted[wave][lane] = lanes_sort<64>(mine, lane);
     if (tid == 0) count = 0;
   }
   __syncthreads();
   // every thread joins the waves' sums in the same order
-  const int w0 = lane % W;
-  m = red[0][w0], l = red[1][w0], t = red[2][w0];
-  float all = red[0][0];
+  if (W > 1) {
+    const int w0 = lane % W;
+    float all = m;
+    if (!WHOLE) {
+      m = red[0][w0], all = red[0][0];
 #pragma unroll
-  for (int w = 1; w < W; ++w) all = fmaxf(all, red[0][w]);
-  raise(all);
+      for (int w = 1; w < W; ++w) all = fmaxf(all, red[0][w]);
+    }
+    l = red[1][w0], t = red[2][w0];
+    if (!WHOLE) raise(all);
 #pragma unroll
-  for (int s = 1; s < W; s <<= 1) {
-    l += __shfl_xor(l, s, 64);
-    t += __shfl_xor(t, s, 64);
+    for (int s = 1; s < W; s <<= 1) {
+      l += __shfl_xor(l, s, 64);
+      t += __shfl_xor(t, s, 64);
+    }
   }
   if (tid == 0) row_result(a, r, x, m, l, t);
   if (a.top == 0) return;
@@ -329,32 +362,38 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
     __syncthreads();
   }
   const float bound = sorted[0][a.top - 1];
-  // a thread's values are read again by its wave, a load each
-  for (uint64_t mask = __ballot(l == l && mine >= bound); mask; mask &= mask - 1) {
-    const int first = (wave * 64 + __ffsll((unsigned long long)mask) - 1) * E;
-    for (int i = first + lane * STEP; i < a.V; i += 64 * STEP) {
-      float v[E];
-      if (i + E <= a.V) {
-        load_values<E>(x + i, v);
-      } else {
+  auto collect = [&](const float (&w)[E], int at) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = i + e < a.V ? Elem<T>::to_f(x[i + e]) : -INFINITY;
+    for (int e = 0; e < E; ++e)
+      if (w[e] >= bound && at + e < a.V) {
+        const int k = atomicAdd(&count, 1);
+        if (k < kCap) cands[k] = rank_key(w[e], at + e);
       }
+  };
+  const bool look = l == l && mine >= bound;
+  if (WHOLE) {
+    if (look) {
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (v[e] >= bound && i + e < a.V) {
-          const int at = atomicAdd(&count, 1);
-          if (at < kCap) cands[at] = rank_key(v[e], i + e);
-        }
+      for (int u = 0; u < U; ++u) collect(v[u], i + u * STEP);
+    }
+  } else {
+    // a thread's values are read again by its wave, a load each
+    for (uint64_t mask = __ballot(look); mask; mask &= mask - 1) {
+      const int first = (wave * 64 + __ffsll((unsigned long long)mask) - 1) * E;
+      for (int j = first + lane * STEP; j < a.V; j += 64 * STEP) {
+        float w[E];
+        load_left<E>(x + j, a.V - j, w);
+        collect(w, j);
+      }
     }
   }
   __syncthreads();
   const int n = count;
   if (n >= a.top && n <= kCap) {
-    for (int i = tid; i < n; i += NT) {
-      const uint64_t key = cands[i];
+    for (int k = tid; k < n; k += NT) {
+      const uint64_t key = cands[k];
       int rank = 0;
-      for (int k = 0; k < n; ++k) rank += cands[k] > key;
+      for (int o = 0; o < n; ++o) rank += cands[o] > key;
       if (rank < a.top) put_top(a, r, rank, key, key_value(key), m, l);
     }
     return;
@@ -362,8 +401,8 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   uint64_t last = ~0ull;
   for (int k = 0; k < a.top; ++k) {
     uint64_t best = 0;
-    for (int i = tid; i < a.V; i += NT) {
-      const uint64_t key = rank_key(Elem<T>::to_f(x[i]), i);
+    for (int j = tid; j < a.V; j += NT) {
+      const uint64_t key = rank_key(Elem<T>::to_f(x[j]), j);
       if ((key < last || k == 0) && key > best) best = key;
     }
 #pragma unroll
@@ -469,6 +508,7 @@ constexpr int kMostTop = 64;
 
 template <typename T>
 int launch_logprobs(const LpArgs& a, int64_t rows, hipStream_t st) {
+  constexpr int E = Elem<T>::kVec;
 #define SMALL(LPR, VPL)                                                                                        \
   hipLaunchKernelGGL((logprobs_small_kernel<T, LPR, VPL>), dim3((unsigned)((rows * LPR + 255) / 256)), dim3(256), 0, \
                      st, a, rows)
@@ -478,9 +518,15 @@ int launch_logprobs(const LpArgs& a, int64_t rows, hipStream_t st) {
   else if (a.V <= 128) SMALL(16, 8);
   else if (a.V <= 256) SMALL(32, 8);
   else if (a.V <= 512) SMALL(64, 8);
-  else if (a.V <= 1024) SMALL(64, 16);
-  else if (a.V <= 8192) hipLaunchKernelGGL((logprobs_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((logprobs_kernel<T, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, a);
+#define ROW(NT, U, WHOLE) \
+  hipLaunchKernelGGL((logprobs_kernel<T, NT, U, WHOLE>), dim3((unsigned)rows), dim3(NT), 0, st, a)
+  else if (a.V <= 64 * E * 2) ROW(64, 2, true);
+  else if (a.V <= 64 * E * 4) ROW(64, 4, true);
+  else if (a.V <= 64 * E * 8) ROW(64, 8, true);
+  else if (a.V <= 256 * E * 4) ROW(256, 4, true);
+  else if (rows >= 256 && a.V * sizeof(T) <= (128 << 10)) ROW(256, 4, false);
+  else ROW(512, 4, false);
+#undef ROW
 #undef SMALL
   MTX_LAUNCHED();
   return MTX_OK;

@@ -165,19 +165,25 @@ def attn_decode(q, k, v, scale: float, out=None, lse=None, lengths=None):
 # ---------------------------------------------------------------------------
 
 # A decode step makes many small calls, so what a wrapper checks and derives of
-# its operands' shapes, strides and dtypes is kept per combination of them (the
-# cached *_plan functions, which never see an address); a call then only passes
-# pointers.
+# its operands' specs -- (shape, strides, dtype) -- is kept per combination of them
+# (the cached *_plan functions, which never see an address); a call then only
+# passes pointers.  The specs of operands that are always there are formed in
+# place: a function call each would cost as much as the rest.
 
 def _spec(t):
-    """(shape, strides, dtype) of a device array; None for None."""
-    if type(t) is dev.DevBuf:
-        return t.shape, t._strides, t.dtype
+    """The spec of a device array; None for None."""
     if t is None:
         return None
-    if not getattr(t, "is_cuda", False):
-        raise ValueError("minitorch_amd kernels take device arrays")
+    if not t.is_cuda:
+        _need_cuda(t)
     return t.shape, t.stride(), t.dtype
+
+
+def _on_device(*ts):
+    """Raises unless every operand is a device array."""
+    for t in ts:
+        if not getattr(t, "is_cuda", False):
+            raise ValueError("minitorch_amd kernels take device arrays")
 
 
 def _ptr(t):
@@ -264,8 +270,12 @@ def kv_append_paged(k, v, k_pages, v_pages, table, lengths, counts=None):
     (B, Hkv, T, D) views, to the end of its pages (mtx_kv_append_paged).
     lengths (B,) counts them already; counts (int32 (B,)): sequence b appends
     only its first counts[b] rows.  fp32 rows may go to a bf16 pool."""
+    if not (k.is_cuda and v.is_cuda and k_pages.is_cuda and v_pages.is_cuda and table.is_cuda and lengths.is_cuda):
+        _on_device(k, v, k_pages, v_pages, table, lengths)
     sizes, (ks, vs), (n, page), (kps, vps), (ld, width) = _append_plan(
-        _spec(k), _spec(v), _spec(k_pages), _spec(v_pages), _spec(table), _spec(lengths), _spec(counts))
+        (k.shape, k.stride(), k.dtype), (v.shape, v.stride(), v.dtype),
+        (k_pages.shape, k_pages.stride(), k_pages.dtype), (v_pages.shape, v_pages.stride(), v_pages.dtype),
+        (table.shape, table.stride(), table.dtype), (lengths.shape, lengths.stride(), lengths.dtype), _spec(counts))
     L.call("mtx_kv_append_paged", *sizes, k.data_ptr(), ks, v.data_ptr(), vs, n, page, k_pages.data_ptr(), kps,
            v_pages.data_ptr(), vps, table.data_ptr(), ld, width, lengths.data_ptr(), _ptr(counts), L.stream_handle())
 
@@ -301,12 +311,14 @@ def attn_decode_paged(q, k_pages, v_pages, table, lengths, scale: float, out=Non
     (B, Hkv, >= max_pages * page) fp32: receives weights_in (0 without it; it
     may be weights itself) plus the attention each cached row got.  Returns
     (out like q, lse or None)."""
-    qspec = _spec(q)
+    if not (q.is_cuda and k_pages.is_cuda and v_pages.is_cuda and table.is_cuda and lengths.is_cuda):
+        _on_device(q, k_pages, v_pages, table, lengths)
     if out is None:
         out = dev.empty_buf(q.shape, _dt(q))
     sizes, (qs, os), (n, page), (kps, vps), (ld, width), wld, ws_bytes = _decode_paged_plan(
-        qspec, _spec(k_pages), _spec(v_pages), _spec(table), _spec(lengths), _spec(out), _spec(lse), _spec(weights),
-        _spec(weights_in))
+        (q.shape, q.stride(), q.dtype), (k_pages.shape, k_pages.stride(), k_pages.dtype),
+        (v_pages.shape, v_pages.stride(), v_pages.dtype), (table.shape, table.stride(), table.dtype),
+        (lengths.shape, lengths.stride(), lengths.dtype), _spec(out), _spec(lse), _spec(weights), _spec(weights_in))
     ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
     L.call("mtx_attn_decode_paged", *sizes, q.data_ptr(), qs, n, page, k_pages.data_ptr(), kps, v_pages.data_ptr(),
            vps, table.data_ptr(), ld, width, lengths.data_ptr(), out.data_ptr(), os, _ptr(lse), _ptr(weights_in),
@@ -1177,8 +1189,14 @@ def token_logprobs(logits, tokens, top: int = 0, scale: float = 1.0, logprob=Non
         top_ids = dev.empty_buf((n, max(0, top)), "int64")
     if top_logprobs is None:
         top_logprobs = dev.empty_buf((n, max(0, top)), "float32")
-    code, rows, V, ld, ws_bytes = _logprobs_plan(_spec(logits), _spec(tokens), top, _spec(logprob), _spec(entropy),
-                                                 _spec(lse), _spec(top_ids), _spec(top_logprobs))
+    if not (logits.is_cuda and tokens.is_cuda and logprob.is_cuda and entropy.is_cuda and lse.is_cuda
+            and top_ids.is_cuda and top_logprobs.is_cuda):
+        _on_device(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs)
+    code, rows, V, ld, ws_bytes = _logprobs_plan(
+        (logits.shape, logits.stride(), logits.dtype), (tokens.shape, tokens.stride(), tokens.dtype), top,
+        (logprob.shape, logprob.stride(), logprob.dtype), (entropy.shape, entropy.stride(), entropy.dtype),
+        (lse.shape, lse.stride(), lse.dtype), (top_ids.shape, top_ids.stride(), top_ids.dtype),
+        (top_logprobs.shape, top_logprobs.stride(), top_logprobs.dtype))
     if rows:
         ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
         L.call("mtx_token_logprobs", code, rows, V, logits.data_ptr(), ld, tokens.data_ptr(), float(scale),
@@ -1205,8 +1223,12 @@ def token_logprobs_bwd(logits, tokens, lse, entropy, g_logprob, g_entropy, scale
         if accumulate:
             raise ValueError("accumulate needs dlogits")
         dlogits = dev.empty_buf(logits.shape, "float32")
-    code, rows, V, ld, ldd = _logprobs_bwd_plan(_spec(logits), _spec(tokens), _spec(lse), _spec(entropy),
-                                                _spec(g_logprob), _spec(g_entropy), _spec(dlogits))
+    if not (logits.is_cuda and tokens.is_cuda and lse.is_cuda and entropy.is_cuda and dlogits.is_cuda):
+        _on_device(logits, tokens, lse, entropy, dlogits)
+    code, rows, V, ld, ldd = _logprobs_bwd_plan(
+        (logits.shape, logits.stride(), logits.dtype), (tokens.shape, tokens.stride(), tokens.dtype),
+        (lse.shape, lse.stride(), lse.dtype), (entropy.shape, entropy.stride(), entropy.dtype), _spec(g_logprob),
+        _spec(g_entropy), (dlogits.shape, dlogits.stride(), dlogits.dtype))
     if rows:
         L.call("mtx_token_logprobs_bwd", code, rows, V, logits.data_ptr(), ld, tokens.data_ptr(), lse.data_ptr(),
                entropy.data_ptr(), _ptr(g_logprob), _ptr(g_entropy), float(scale), dlogits.data_ptr(), ldd,
