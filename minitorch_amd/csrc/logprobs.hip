@@ -495,8 +495,9 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const LpBwdArgs a) {
 
 int check_rows(int dtype, int64_t rows, int V, const void* logits, int64_t ld, const int64_t* tokens, float scale) {
   if (dtype != MTX_F32 && dtype != MTX_BF16) return fail(MTX_ERR_DTYPE, "unsupported dtype %d", dtype);
-  MTX_CHECK_SHAPE(rows >= 1 && rows <= (1 << 30) && V >= 1 && V <= (1 << 27),
-                  "token_logprobs: needs rows >= 1 and 1 <= V <= 2^27 (got %lld, %d)", (long long)rows, V);
+  // a launch's threads, up to 512 a row, are counted in 32 bits
+  MTX_CHECK_SHAPE(rows >= 1 && rows < (1 << 23) && V >= 1 && V <= (1 << 27),
+                  "token_logprobs: needs 1 <= rows < 2^23 and 1 <= V <= 2^27 (got %lld, %d)", (long long)rows, V);
   MTX_CHECK_ARG(logits != nullptr && tokens != nullptr, "logits, tokens: null pointer");
   MTX_CHECK_ARG(((uintptr_t)logits & (dtype == MTX_F32 ? 3u : 1u)) == 0, "logits: pointer must be aligned to its type");
   MTX_CHECK_ARG(ld >= V || (rows == 1 && ld >= 0), "logits: row stride %lld < V=%d", (long long)ld, V);

@@ -870,7 +870,7 @@ __global__ __launch_bounds__(256) void select_small_kernel(const EvictArgs a) {
 // Copies the kept rows, a thread 16 bytes of the keys and the values of kRows
 // rows, and their weights; the last blocks of a sequence and head clear the weights
 // behind them
-constexpr int kRows = 4;
+constexpr int kRows = 2;
 __global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a, int blocks, int fills) {
   const int bh = blockIdx.x / (blocks + fills), block = blockIdx.x % (blocks + fills);
   const int b = bh / a.H, h = bh % a.H;
@@ -933,6 +933,9 @@ int check_dtypes(int dtype, int cache_dtype) {
                 cache_dtype);
   return MTX_OK;
 }
+
+// a launch's threads are counted in 32 bits
+constexpr int64_t kMaxGroups = (1 << 24) - 1;
 
 // the three outer strides of a 4-d view whose d stride is 1
 int check_view(const char* name, const void* p, const int64_t* s, int es) {
@@ -1041,8 +1044,10 @@ extern "C" int mtx_kv_append_paged(int dtype, int cache_dtype, int B, int T, int
   int rc;
   if ((rc = check_dtypes(dtype, cache_dtype))) return rc;
   if ((rc = check_cache(B, H, D, n_pages, page, table, table_ld, max_pages, lengths))) return rc;
-  MTX_CHECK_SHAPE(T >= 1 && (int64_t)T * H * (D / 8) <= (1 << 30), "T=%d new rows of %d heads: at least 1", T, H);
   const int es = dtype == MTX_F32 ? 4 : 2, ec = cache_dtype == MTX_F32 ? 4 : 2;
+  const int64_t chunks = (int64_t)T * H * (D * ec / 16), blocks = (chunks + 255) / 256;
+  MTX_CHECK_SHAPE(T >= 1 && chunks <= (1 << 30) && blocks * B <= kMaxGroups,
+                  "append: %d new rows of %d heads for %d sequences: at least 1, and fewer in one call", T, H, B);
   if ((rc = check_view("k", k, k_strides, es))) return rc;
   if ((rc = check_view("v", v, v_strides, es))) return rc;
   if ((rc = check_view("k_pages", k_pages, kp_strides, ec))) return rc;
@@ -1061,8 +1066,7 @@ extern "C" int mtx_kv_append_paged(int dtype, int cache_dtype, int B, int T, int
                T,
                H,
                D * ec / 16,
-               cdiv(T * H * (D * ec / 16), 256)};
-  MTX_CHECK_SHAPE((int64_t)B * a.blocks <= INT32_MAX, "append: too many rows in one call");
+               (int)blocks};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(B * a.blocks);
   if (cache_dtype == MTX_F32) hipLaunchKernelGGL((append_kernel<float, float>), grid, dim3(256), 0, st, a);
@@ -1110,7 +1114,8 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
                 "workspace: %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
   const int64_t groups = ((int64_t)B * Hkv * plan.S + 7) / 8 * 8 * plan.HT;
   const int64_t finish = (weights != nullptr ? (int64_t)B * Hkv * cdiv(cap, kFinishRows) : 0);
-  MTX_CHECK_SHAPE(groups <= INT32_MAX && finish <= INT32_MAX / 2, "decode: too many sequences, heads and rows in one call");
+  MTX_CHECK_SHAPE(groups <= kMaxGroups && finish + (int64_t)B * H <= kMaxGroups,
+                  "decode: too many sequences, heads and rows in one call");
   float* ws = static_cast<float*>(workspace);
   DecodeArgs a{q, q_strides[0], q_strides[1],
                {const_cast<void*>(k_pages), kp_strides[0], kp_strides[1], kp_strides[2]},
@@ -1159,7 +1164,7 @@ extern "C" int mtx_kv_evict_paged(int cache_dtype, int B, int H, int D, int64_t 
               lengths, weights, weights_ld, lengths_out, weights_out, slots, B, H, cap, keep, recent,
               D * ec / 16, ec};
   const int64_t blocks = cdiv(rows, kRows * (256 / a.C)), fills = std::min(cdiv(std::max(cap, keep), 4096), 64);
-  MTX_CHECK_SHAPE((blocks + fills) * B * H <= INT32_MAX, "evict: too many rows in one call");
+  MTX_CHECK_SHAPE((blocks + fills) * B * H <= kMaxGroups, "evict: too many rows in one call");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(B * H);
   const dim3 four(cdiv(B * H, 4));

@@ -84,7 +84,8 @@ def check(x, tokens, dtype, scale=1.0, top=0, grad=True, ld=0, seed=0):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("V", [1, 2, 3, 63, 64, 65, 255, 256, 1000, 1023, 1025, 4097, 5003])
+@pytest.mark.parametrize("V", [1, 2, 3, 15, 17, 48, 49, 63, 64, 65, 80, 81, 128, 129, 255, 256, 257, 511, 512, 513, 1000,
+                               1023, 1024, 1025, 2047, 2049, 4095, 4097, 5003, 8192, 8193])
 def test_vocabulary_sizes(dev, dtype, V):
     rng = np.random.default_rng(V)
     x, tok = make(rng, 9, V, dtype)
@@ -92,7 +93,7 @@ def test_vocabulary_sizes(dev, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("rows,V", [(1, 50021), (3, 131072), (40, 20000), (300, 8193)])
+@pytest.mark.parametrize("rows,V", [(1, 50021), (3, 131072), (40, 20000), (300, 8193), (257, 32768), (256, 40000)])
 def test_large_vocabularies(dev, dtype, rows, V):
     rng = np.random.default_rng(rows)
     x, tok = make(rng, rows, V, dtype)

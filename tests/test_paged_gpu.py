@@ -147,6 +147,52 @@ def test_decode_lengths(dev, q, cache, lengths, weights):
     check_decode(case, lengths, seed=sum(lengths), with_lse=not weights, in_place=weights)
 
 
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("page", [2, 4, 12, 20, 48])
+def test_decode_page_sizes(dev, q, cache, page):
+    """Pages that hold whole runs of 16 rows, of 4, and neither."""
+    case = dict(q=q, cache=cache, H=3, Hkv=1, D=32, page=page, layout="rows", weights=True)
+    check_decode(case, [1, 3 * page - 1, 130, 0, 257], seed=page)
+
+
+@pytest.mark.parametrize("page", [4, 16])
+def test_decode_rows_far_apart(dev, page):
+    """Row strides that 32-bit offsets from a page do not reach."""
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(page)
+    n, D, far = 3, 16, 1 << 24
+    pools = [rng.standard_normal((n, 1, page, D), dtype=np.float32) for _ in range(2)]
+    base = empty(((page - 1) * far + n * D,), "float32")
+    views = []
+    for i, pool in enumerate(pools):  # page p's rows at p D, one `far` apart; V half a stride on
+        view = base.as_strided((n, 1, page, D), (D, D, far, 1), 0)
+        if i:
+            base = empty(((page - 1) * far + n * D,), "float32")
+            view = base.as_strided((n, 1, page, D), (D, D, far, 1), 0)
+        for r in range(page):
+            view[:, :, r].copy_(dev_array(pool[:, :, r]))
+        views.append(view)
+    table, lens = np.array([[2, 0, 1]], np.int32), np.array([3 * page - 1], np.int32)
+    q = rng.standard_normal((1, 2, 1, D), dtype=np.float32)
+    o, _ = K.attn_decode_paged(dev_array(q), *views, dev_array(table, "int32"), dev_array(lens, "int32"), 0.25)
+    r = ref.decode(q, *pools, table, lens, 0.25)
+    ob, _, _ = decode_bounds(dict(q="float32", cache="float32"), r, 3 * page)
+    assert np.all(np.abs(host(o) - r[0]) <= ob)
+
+
+@pytest.mark.parametrize("B,H,Hkv,D,lengths", [
+    (1, 2, 1, 16, (512, 513)), (130, 1, 1, 16, (1000, 1024, 700)), (100, 8, 8, 16, (2000, 60, 1100)),
+    (1, 20, 1, 32, (1500,)), (2, 34, 2, 16, (3000, 1)), (9, 17, 1, 16, (1300, 5))])
+@pytest.mark.parametrize("weights", [False, True])
+def test_decode_one_chunk_and_many(dev, B, H, Hkv, D, lengths, weights):
+    """Around the sizes where a sequence takes one workgroup, or several that
+    a second launch joins, with more than 16 heads a K/V head too."""
+    for n in ([lengths] if B > 1 else [(x,) for x in lengths]):
+        case = dict(q="bfloat16", cache="bfloat16", H=H, Hkv=Hkv, D=D, page=16, weights=weights)
+        check_decode(case, [n[i % len(n)] for i in range(B)], seed=B + n[0])
+
+
 @pytest.mark.parametrize("page,D", [(32, 128), (37, 64)])
 def test_decode_long_cache(dev, page, D):
     case = dict(q="bfloat16", cache="bfloat16", H=4, Hkv=1, D=D, page=page, weights=True)
@@ -440,6 +486,34 @@ def test_evict_long(dev):
         return w
 
     check_evict([70001, 66000], 20000, 500, Hkv=1, D=16, page=64, cache="bfloat16", seed=12, weights=weights)
+
+
+@pytest.mark.parametrize("n", [256, 257, 1024, 1025, 4096, 4097, 16384, 16385, 32768, 32769, 49152, 49153])
+def test_evict_around_the_selections_sizes(dev, n):
+    check_evict([n], n // 3, n // 50, Hkv=1, D=16, page=128, cache="bfloat16", seed=n)
+
+
+@pytest.mark.parametrize("kind", ["sampled_large", "sampled_small", "two_halves", "one_value_but_few"])
+@pytest.mark.parametrize("n,keep", [(20000, 5000), (20000, 300), (60000, 59000)])
+def test_evict_where_a_sample_misleads(dev, kind, n, keep):
+    """Rows that a selection samples say nothing, or the wrong thing, of the
+    others; half the rows below the other half; nearly all of one weight."""
+    def weights(rng, shape):
+        w = rng.random(shape, dtype=np.float32)
+        at = (np.arange(4096) * (n - 7)) // 4096
+        if kind == "sampled_large":
+            w[..., at] += 10
+        elif kind == "sampled_small":
+            w[..., at] -= 10
+        elif kind == "two_halves":
+            w[..., n // 2:] += 100
+        else:
+            w[:] = 0.5
+            w[..., rng.integers(0, n, 50)] = 0.25
+            w[..., rng.integers(0, n, 50)] = 0.75
+        return w
+
+    check_evict([n], keep, 7, Hkv=1, D=16, page=128, cache="bfloat16", seed=keep, weights=weights)
 
 
 def test_evict_pages_that_are_not_there(dev):
