@@ -795,6 +795,7 @@ __global__ __launch_bounds__(NT) void select_kernel(const EvictArgs a) {
   // places: how many rows above the bound come before a row, and of those at the
   // bound the first `want`
   bound = __builtin_amdgcn_readfirstlane(bound);
+  __syncthreads();  // gts and ties may still be read, for the sample
   int g = 0, t = 0;
   each([&](uint32_t k) {
     g += __popcll(__ballot(k > bound));
