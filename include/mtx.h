@@ -352,7 +352,9 @@ int mtx_kv_append_paged(int dtype, int cache_dtype, int B, int T, int Hkv, int D
  * h / (H / Hkv).  s_j = scale * q.k_j, lse = log sum_j exp(s_j) (fp32 (B, H)
  * contiguous, may be NULL), o = sum_j exp(s_j - lse) v_j over the rows
  * j < lengths[b] that are there; a sequence without any gets o = 0 and
- * lse = -inf.  Rows that are not seen may hold anything, NaN included.
+ * lse = -inf.  Rows that are not seen may hold anything, NaN included; a value
+ * that is not finite in a row that is seen, or in q, makes that head's results NaN
+ * where fp32 arithmetic might give an infinity.
  * weights (may be NULL): fp32 (B, Hkv, weights_ld) contiguous, weights_ld >=
  * max_pages * page; for j < lengths[b]
  *   weights[b][hk][j] = weights_in[b][hk][j] + sum over hk's query heads of

@@ -190,6 +190,15 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _ints(*xs):
+    """ints as the C ints of an argument list, converted once."""
+    return tuple(ctypes.c_int(x) for x in xs)
+
+
+def _longs(*xs):
+    return tuple(ctypes.c_int64(x) for x in xs)
+
+
 def _packed(shape, strides):
     """Whether strides are C order's (those of dimensions of 1 do not matter)."""
     acc = 1
@@ -300,7 +309,8 @@ def _decode_paged_plan(q, k_pages, v_pages, table, lengths, out, lse, weights, w
     elif weights_in is not None:
         raise ValueError("weights_in without weights")
     ws = L.lib().mtx_attn_decode_paged_workspace_bytes(B, H, Hkv, D, page, width, int(weights is not None))
-    return (_code(qd), _code(cache), B, H, Hkv, D), (qs, os), (n_pages, page), (kps, vps), (ld, width), wld, ws
+    return (_ints(_code(qd), _code(cache), B, H, Hkv, D), (qs, os), (*_longs(n_pages), *_ints(page)), (kps, vps),
+            (*_longs(ld), *_ints(width)), *_longs(wld), ws)
 
 
 def attn_decode_paged(q, k_pages, v_pages, table, lengths, scale: float, out=None, lse=None, weights=None,
