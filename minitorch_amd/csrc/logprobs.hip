@@ -379,10 +379,17 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
       for (int u = 0; u < U; ++u) collect(v[u], i + u * STEP);
     }
   } else {
-    // a thread's values are read again by its wave, a load each
-    for (uint64_t mask = __ballot(look); mask; mask &= mask - 1) {
-      const int first = (wave * 64 + __ffsll((unsigned long long)mask) - 1) * E;
-      for (int j = first + lane * STEP; j < a.V; j += 64 * STEP) {
+    // a thread's values are read again by lanes of its wave, a load each, and where
+    // they are few those of several threads at once (8 x 20000 bf16 7.6 us, one thread
+    // at a time 9.3)
+    int per = 64;
+    while (per > 8 && (per / 2) * STEP >= a.V) per /= 2;
+    for (uint64_t mask = __ballot(look); mask;) {
+      int from = -1;
+      for (int k = 0; k < 64 && mask; k += per, mask &= mask - 1)
+        if (lane >= k && lane < k + per) from = __ffsll((unsigned long long)mask) - 1;
+      if (from < 0) continue;
+      for (int j = (wave * 64 + from) * E + (lane & (per - 1)) * STEP; j < a.V; j += per * STEP) {
         float w[E];
         load_left<E>(x + j, a.V - j, w);
         collect(w, j);
@@ -520,7 +527,7 @@ int launch_logprobs(const LpArgs& a, int64_t rows, hipStream_t st) {
   // row, 12.3 by 64; 16384 x 1500 fp32 28 whole in a wave, 43 in one pass, 60 by 256
   // threads; 8192 x 3000 fp32 30 whole in 256 threads, 35 in one pass; 4096 x 9000 33
   // by 256 threads, 39 by 512, 64 by 1024; 2048 x 50021 fp32 88 by 256, 79 by 512;
-  // 8 x 50021 bf16 11.8 by 256, 10.1 by 512, 12.3 by 1024
+  // 8 x 50021 bf16 11.4 by 256, 9.1 by 512, 10.6 by 1024
 #define SMALL(LPR, VPL)                                                                                        \
   hipLaunchKernelGGL((logprobs_small_kernel<T, LPR, VPL>), dim3((unsigned)((rows * LPR + 255) / 256)), dim3(256), 0, \
                      st, a, rows)
