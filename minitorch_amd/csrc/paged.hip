@@ -830,58 +830,130 @@ __global__ __launch_bounds__(NT) void select_kernel(const EvictArgs a) {
   for (int j = cand + tid; j < len; j += NT) slots[min(len, a.keep) - len + j] = j;
 }
 
-// Selection of up to 64 R rows: one wave each, nothing but ballots.  The last kept
-// key is found bit by bit: the largest with `want` or more rows at or above it
-template <int R>
-__global__ __launch_bounds__(256) void select_small_kernel(const EvictArgs a) {
-  const int bh = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (bh >= a.B * a.H) return;
-  const int b = bh / a.H, len = min(max(a.lengths[b], 0), a.cap);
-  const float* __restrict__ w = a.w + bh * a.wld;
-  if (lane == 0 && bh % a.H == 0) a.lengths_out[b] = min(len, a.keep);
-  const int cand = len > a.keep ? len - a.recent : 0;
-  uint32_t key[R];
+// Copying the kept rows: a thread takes 16 bytes (number c) of the keys and the
+// values of the rows r0 + per i, i < kRows, which are the old rows j[i] (-1: none),
+// and the first of a row's threads its weight
+constexpr int kRows = 2;
+struct RowCopy {
+  int c, per, r0, j[kRows], from[kRows], to[kRows], ti[kRows];
+
+  __device__ __forceinline__ RowCopy(const EvictArgs& a, int block) {
+    c = threadIdx.x & (a.C - 1);
+    per = 256 / a.C;
+    r0 = block * per * kRows + threadIdx.x / a.C;
+  }
+  __device__ __forceinline__ void copy(const EvictArgs& a, int bh, int h) const {
+    if (c == 0) {
 #pragma unroll
-  for (int i = 0; i < R; ++i) key[i] = lane + 64 * i < cand ? weight_key(w[lane + 64 * i]) : 0u;
-  int want = cand > 0 ? a.keep - a.recent : 0;
-  uint32_t bound = 0xffffffffu;
-  if (want > 0) {
-    bound = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t t = bound | (1u << bit);
-      int n = 0;
+      for (int i = 0; i < kRows; ++i)
+        if (j[i] >= 0) a.w_out[bh * a.wld + r0 + per * i] = a.w[bh * a.wld + j[i]];
+    }
+    uint4 x[kRows], y[kRows];
+    const int64_t es = a.es;
 #pragma unroll
-      for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= t));
-      if (n >= want) bound = t;
+    for (int i = 0; i < kRows; ++i) {
+      x[i] = y[i] = make_uint4(0, 0, 0, 0);
+      if (from[i] < 0) continue;
+      const int fi = a.from.div(j[i]);
+      x[i] = reinterpret_cast<const uint4*>(static_cast<const char*>(a.k.p) +
+                                            es * (row_at(a.k, a.from, from[i], fi, j[i]) + h * a.k.sh))[c];
+      y[i] = reinterpret_cast<const uint4*>(static_cast<const char*>(a.v.p) +
+                                            es * (row_at(a.v, a.from, from[i], fi, j[i]) + h * a.v.sh))[c];
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) want -= __popcll(__ballot(key[i] > bound));
+    for (int i = 0; i < kRows; ++i) {
+      if (to[i] < 0) continue;
+      const int r = r0 + per * i;
+      reinterpret_cast<uint4*>(static_cast<char*>(a.k.p) +
+                               es * (row_at(a.k, a.to, to[i], ti[i], r) + h * a.k.sh))[c] = x[i];
+      reinterpret_cast<uint4*>(static_cast<char*>(a.v.p) +
+                               es * (row_at(a.v, a.to, to[i], ti[i], r) + h * a.v.sh))[c] = y[i];
+    }
   }
-  int* __restrict__ slots = a.slots + (int64_t)bh * a.keep;
-  int at = 0, ties = 0;
+};
+
+// Selection and copy of caches of up to 64 R rows in one launch: each of a
+// sequence and head's `blocks` workgroups selects, by its first wave with nothing
+// but ballots, and copies its share of the rows.  The last kept key is found bit by
+// bit: the largest with `want` or more rows at or above it
+template <int R>
+__global__ __launch_bounds__(256) void evict_small_kernel(const EvictArgs a, int blocks) {
+  __shared__ int rows[64 * R], ids[64 * R];
+  const int bh = blockIdx.x / blocks, block = blockIdx.x % blocks, b = bh / a.H, tid = threadIdx.x;
+  const int length = a.lengths[b];
+  RowCopy copy(a, block);
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const bool tie = key[i] == bound;
-    const uint64_t tm = __ballot(tie);
-    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(tm >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)tm, ties));
-    const bool kept = key[i] > bound || (tie && before < want);
-    const uint64_t km = __ballot(kept);
-    const int pos = __builtin_amdgcn_mbcnt_hi((uint32_t)(km >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)km, at));
-    if (kept) slots[pos] = lane + 64 * i;
-    ties += __popcll(tm);
-    at += __popcll(km);
+  for (int i = 0; i < kRows; ++i) {
+    const int r = copy.r0 + copy.per * i;
+    copy.ti[i] = a.to.div(r);
+    copy.to[i] = r < min(a.keep, a.cap) ? a.to.id(b, copy.ti[i]) : -1;
   }
-  for (int j = cand + lane; j < len; j += 64) slots[min(len, a.keep) - len + j] = j;
+  const int len = min(max(length, 0), a.cap), new_len = min(len, a.keep);
+  const int cand = len > a.keep ? len - a.recent : 0;
+  if (tid < 64) {
+    const float* __restrict__ w = a.w + bh * a.wld;
+    uint32_t key[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) key[i] = tid + 64 * i < a.cap ? weight_key(w[tid + 64 * i]) : 0u;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (tid + 64 * i >= cand) key[i] = 0u;
+    int want = cand > 0 ? a.keep - a.recent : 0;
+    uint32_t bound = 0xffffffffu;
+    if (want > 0) {
+      bound = 0;
+#pragma unroll 1
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t t = bound | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= t));
+        if (n >= want) bound = t;
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) want -= __popcll(__ballot(key[i] > bound));
+    }
+    int at = 0, ties = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const bool tie = key[i] == bound;
+      const uint64_t tm = __ballot(tie);
+      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(tm >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)tm, ties));
+      const bool kept = key[i] > bound || (tie && before < want);
+      const uint64_t km = __ballot(kept);
+      const int pos = __builtin_amdgcn_mbcnt_hi((uint32_t)(km >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)km, at));
+      if (kept) rows[pos] = tid + 64 * i;
+      ties += __popcll(tm);
+      at += __popcll(km);
+    }
+    for (int j = cand + tid; j < len; j += 64) rows[new_len - len + j] = j;
+  } else {
+    for (int i = tid - 64; i < a.from.width; i += 192) ids[i] = a.from.id(b, i);
+  }
+  __syncthreads();
+  int* slots = a.slots + (int64_t)bh * a.keep;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int r = copy.r0 + copy.per * i;
+    copy.j[i] = r < new_len ? rows[r] : -1;
+    copy.from[i] = r < new_len ? ids[a.from.div(copy.j[i])] : -1;
+    if (r >= new_len) copy.to[i] = -1;
+    else if (copy.c == 0) slots[r] = copy.j[i];
+  }
+  copy.copy(a, bh, bh % a.H);
+  if (block) return;
+  if (tid == 0 && bh % a.H == 0) a.lengths_out[b] = new_len;
+  for (int j = new_len + tid; j < max(a.cap, a.keep); j += 256) {
+    if (j < a.cap) a.w_out[bh * a.wld + j] = 0.f;
+    if (j < a.keep) slots[j] = -1;
+  }
 }
 
-// Copies the kept rows, a thread 16 bytes of the keys and the values of kRows
-// rows, and their weights; the last blocks of a sequence and head clear the weights
-// behind them
-constexpr int kRows = 2;
+// The copy behind select_kernel; the last blocks of a sequence and head clear the
+// weights behind its rows
 __global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a, int blocks, int fills) {
   const int bh = blockIdx.x / (blocks + fills), block = blockIdx.x % (blocks + fills);
-  const int b = bh / a.H, h = bh % a.H;
+  const int b = bh / a.H;
   const int new_len = min(min(max(a.lengths[b], 0), a.cap), a.keep);
   if (block >= blocks) {
     float* wo = a.w_out + bh * a.wld;
@@ -892,43 +964,20 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a, int bloc
     }
     return;
   }
-  const int c = threadIdx.x & (a.C - 1), per = 256 / a.C, r0 = block * per * kRows + threadIdx.x / a.C;
   const int* __restrict__ slots = a.slots + (int64_t)bh * a.keep;
-  int j[kRows], fi[kRows], from[kRows], to[kRows], ti[kRows];
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) j[i] = r0 + per * i < new_len ? slots[r0 + per * i] : -1;
+  RowCopy copy(a, block);
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    fi[i] = a.from.div(max(j[i], 0));
-    ti[i] = a.to.div(r0 + per * i);
-    from[i] = j[i] < 0 ? -1 : a.from.id(b, fi[i]);
-    to[i] = j[i] < 0 ? -1 : a.to.id(b, ti[i]);
-  }
-  if (c == 0) {
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-      if (j[i] >= 0) a.w_out[bh * a.wld + r0 + per * i] = a.w[bh * a.wld + j[i]];
-  }
-  uint4 x[kRows], y[kRows];
-  const int64_t es = a.es;
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    x[i] = y[i] = make_uint4(0, 0, 0, 0);
-    if (from[i] < 0) continue;
-    x[i] = reinterpret_cast<const uint4*>(static_cast<const char*>(a.k.p) +
-                                          es * (row_at(a.k, a.from, from[i], fi[i], j[i]) + h * a.k.sh))[c];
-    y[i] = reinterpret_cast<const uint4*>(static_cast<const char*>(a.v.p) +
-                                          es * (row_at(a.v, a.from, from[i], fi[i], j[i]) + h * a.v.sh))[c];
+    const int r = copy.r0 + copy.per * i;
+    copy.j[i] = r < new_len ? slots[r] : -1;
   }
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    if (to[i] < 0) continue;
-    const int r = r0 + per * i;
-    reinterpret_cast<uint4*>(static_cast<char*>(a.k.p) +
-                             es * (row_at(a.k, a.to, to[i], ti[i], r) + h * a.k.sh))[c] = x[i];
-    reinterpret_cast<uint4*>(static_cast<char*>(a.v.p) +
-                             es * (row_at(a.v, a.to, to[i], ti[i], r) + h * a.v.sh))[c] = y[i];
+    copy.ti[i] = a.to.div(copy.r0 + copy.per * i);
+    copy.from[i] = copy.j[i] < 0 ? -1 : a.from.id(b, a.from.div(copy.j[i]));
+    copy.to[i] = copy.j[i] < 0 ? -1 : a.to.id(b, copy.ti[i]);
   }
+  copy.copy(a, bh, bh % a.H);
 }
 
 // ---------------------------------------------------------------------------
@@ -1175,14 +1224,18 @@ extern "C" int mtx_kv_evict_paged(int cache_dtype, int B, int H, int D, int64_t 
   MTX_CHECK_SHAPE((blocks + fills) * B * H <= kMaxGroups, "evict: too many rows in one call");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(B * H);
-  const dim3 four(cdiv(B * H, 4));
+  constexpr int kSmall = 4;
+  if (cap <= 64 * kSmall) {
+    hipLaunchKernelGGL(evict_small_kernel<kSmall>, dim3((unsigned)(blocks * B * H)), dim3(256), 0, st, a, (int)blocks);
+    MTX_LAUNCHED();
+    return MTX_OK;
+  }
   // measured for 64 sequences and heads (192 for 256 rows), us: 256 rows 5.6 by a
   // wave, 8.6 by a workgroup; 1000 rows 12.7 by a wave, 5.8; 4000 rows 11.2 by 1024
   // threads, 9.2 by 256; 32768 rows 19.6 held in registers, 35 read again each step;
   // 49152 rows 27.6 and 40; with 64 rows a thread registers spill: 48
 #define SELECT(NT, R, SINGLE) hipLaunchKernelGGL((select_kernel<NT, R, SINGLE>), grid, dim3(NT), 0, st, a)
-  if (cap <= 64 * 4) hipLaunchKernelGGL(select_small_kernel<4>, four, dim3(256), 0, st, a);
-  else if (cap <= 256 * 4) SELECT(256, 4, true);
+  if (cap <= 256 * 4) SELECT(256, 4, true);
   else if (cap <= 256 * 16) SELECT(256, 16, true);
   else if (cap <= 1024 * 16) SELECT(1024, 16, true);
   else if (cap <= 1024 * 32) SELECT(1024, 32, true);
