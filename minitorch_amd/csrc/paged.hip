@@ -617,17 +617,13 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 constexpr int kBins = 2048;
 
 template <int NT, int R, bool SINGLE>
-__global__ __launch_bounds__(NT) void select_kernel(const EvictArgs a) {
+__device__ __forceinline__ void select_rows(const EvictArgs& a, int bh, int len, int* slots) {
   constexpr int W = NT / 64;
   __shared__ int bins[kBins], part[W], gts[W], ties[W];
   __shared__ uint32_t mins[W], maxs[W], found[4], few[NT / 2];
   __shared__ int nfew;
-  const int bh = blockIdx.x, b = bh / a.H, tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int len = min(max(a.lengths[b], 0), a.cap);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float* __restrict__ w = a.w + bh * a.wld;
-  int* __restrict__ slots = a.slots + (int64_t)bh * a.keep;
-  if (tid == 0 && bh % a.H == 0) a.lengths_out[b] = min(len, a.keep);
   const int cand = len > a.keep ? len - a.recent : 0;
   int want = a.keep - a.recent;
 
@@ -830,6 +826,56 @@ __global__ __launch_bounds__(NT) void select_kernel(const EvictArgs a) {
   for (int j = cand + tid; j < len; j += NT) slots[min(len, a.keep) - len + j] = j;
 }
 
+template <int NT, int R, bool SINGLE>
+__global__ __launch_bounds__(NT) void select_kernel(const EvictArgs a) {
+  const int bh = blockIdx.x, b = bh / a.H, len = min(max(a.lengths[b], 0), a.cap);
+  if (threadIdx.x == 0 && bh % a.H == 0) a.lengths_out[b] = min(len, a.keep);
+  select_rows<NT, R, SINGLE>(a, bh, len, a.slots + (int64_t)bh * a.keep);
+}
+
+// The same of up to 64 R rows by one wave, with nothing but ballots.  The last kept
+// key is found bit by bit: the largest with `want` or more rows at or above it
+template <int R>
+__device__ __forceinline__ void select_few(const EvictArgs& a, int bh, int len, int* slots) {
+  const int lane = threadIdx.x & 63, cand = len > a.keep ? len - a.recent : 0;
+  const float* __restrict__ w = a.w + bh * a.wld;
+  uint32_t key[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) key[i] = lane + 64 * i < a.cap ? weight_key(w[lane + 64 * i]) : 0u;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (lane + 64 * i >= cand) key[i] = 0u;
+  int want = cand > 0 ? a.keep - a.recent : 0;
+  uint32_t bound = 0xffffffffu;
+  if (want > 0) {
+    bound = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t t = bound | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= t));
+      if (n >= want) bound = t;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) want -= __popcll(__ballot(key[i] > bound));
+  }
+  int at = 0, ties = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const bool tie = key[i] == bound;
+    const uint64_t tm = __ballot(tie);
+    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(tm >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)tm, ties));
+    const bool kept = key[i] > bound || (tie && before < want);
+    const uint64_t km = __ballot(kept);
+    const int pos = __builtin_amdgcn_mbcnt_hi((uint32_t)(km >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)km, at));
+    if (kept) slots[pos] = lane + 64 * i;
+    ties += __popcll(tm);
+    at += __popcll(km);
+  }
+  for (int j = cand + lane; j < len; j += 64) slots[min(len, a.keep) - len + j] = j;
+}
+
 // Copying the kept rows: a thread takes 16 bytes (number c) of the keys and the
 // values of the rows r0 + per i, i < kRows, which are the old rows j[i] (-1: none),
 // and the first of a row's threads its weight
@@ -872,13 +918,11 @@ struct RowCopy {
   }
 };
 
-// Selection and copy of caches of up to 64 R rows in one launch: each of a
-// sequence and head's `blocks` workgroups selects, by its first wave with nothing
-// but ballots, and copies its share of the rows.  The last kept key is found bit by
-// bit: the largest with `want` or more rows at or above it
-template <int R>
-__global__ __launch_bounds__(256) void evict_small_kernel(const EvictArgs a, int blocks) {
-  __shared__ int rows[64 * R], ids[64 * R];
+// Selection and copy in one launch, of caches of up to N rows: each of a sequence
+// and head's `blocks` workgroups selects the rows, into LDS, and copies its share
+template <int N>
+__global__ __launch_bounds__(256) void evict_kernel(const EvictArgs a, int blocks) {
+  __shared__ int rows[N], ids[N];
   const int bh = blockIdx.x / blocks, block = blockIdx.x % blocks, b = bh / a.H, tid = threadIdx.x;
   const int length = a.lengths[b];
   RowCopy copy(a, block);
@@ -889,46 +933,13 @@ __global__ __launch_bounds__(256) void evict_small_kernel(const EvictArgs a, int
     copy.to[i] = r < min(a.keep, a.cap) ? a.to.id(b, copy.ti[i]) : -1;
   }
   const int len = min(max(length, 0), a.cap), new_len = min(len, a.keep);
-  const int cand = len > a.keep ? len - a.recent : 0;
-  if (tid < 64) {
-    const float* __restrict__ w = a.w + bh * a.wld;
-    uint32_t key[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) key[i] = tid + 64 * i < a.cap ? weight_key(w[tid + 64 * i]) : 0u;
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (tid + 64 * i >= cand) key[i] = 0u;
-    int want = cand > 0 ? a.keep - a.recent : 0;
-    uint32_t bound = 0xffffffffu;
-    if (want > 0) {
-      bound = 0;
-#pragma unroll 1
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t t = bound | (1u << bit);
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= t));
-        if (n >= want) bound = t;
-      }
-#pragma unroll
-      for (int i = 0; i < R; ++i) want -= __popcll(__ballot(key[i] > bound));
-    }
-    int at = 0, ties = 0;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const bool tie = key[i] == bound;
-      const uint64_t tm = __ballot(tie);
-      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(tm >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)tm, ties));
-      const bool kept = key[i] > bound || (tie && before < want);
-      const uint64_t km = __ballot(kept);
-      const int pos = __builtin_amdgcn_mbcnt_hi((uint32_t)(km >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)km, at));
-      if (kept) rows[pos] = tid + 64 * i;
-      ties += __popcll(tm);
-      at += __popcll(km);
-    }
-    for (int j = cand + tid; j < len; j += 64) rows[new_len - len + j] = j;
+  constexpr bool few = N <= 256;  // by the first wave alone, the others read the page ids
+  if (!few || tid >= 64)
+    for (int i = few ? tid - 64 : tid; i < a.from.width; i += few ? 192 : 256) ids[i] = a.from.id(b, i);
+  if constexpr (few) {
+    if (tid < 64) select_few<N / 64>(a, bh, len, rows);
   } else {
-    for (int i = tid - 64; i < a.from.width; i += 192) ids[i] = a.from.id(b, i);
+    select_rows<256, N / 256, true>(a, bh, len, rows);
   }
   __syncthreads();
   int* slots = a.slots + (int64_t)bh * a.keep;
@@ -1224,16 +1235,21 @@ extern "C" int mtx_kv_evict_paged(int cache_dtype, int B, int H, int D, int64_t 
   MTX_CHECK_SHAPE((blocks + fills) * B * H <= kMaxGroups, "evict: too many rows in one call");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(B * H);
-  constexpr int kSmall = 4;
-  if (cap <= 64 * kSmall) {
-    hipLaunchKernelGGL(evict_small_kernel<kSmall>, dim3((unsigned)(blocks * B * H)), dim3(256), 0, st, a, (int)blocks);
+  // in one launch, us, against two: 192 sequences and heads of 256 rows 11.5, 15.9; 768
+  // of 37.5, 37.0; 1000 rows by 1024 workgroups 12.1, 14.9, by 2048 20.4, 19.8 (each
+  // selects for itself); 4000 rows by 448 14.3, 14.6, by 832 23.7, 16.9
+#define FUSED(N) hipLaunchKernelGGL(evict_kernel<N>, dim3((unsigned)(blocks * B * H)), dim3(256), 0, st, a, (int)blocks)
+  if (cap <= 256 || (cap <= 4096 && blocks * B * H <= (cap <= 1024 ? 1536 : 512))) {
+    if (cap <= 256) FUSED(256);
+    else if (cap <= 1024) FUSED(1024);
+    else FUSED(4096);
     MTX_LAUNCHED();
     return MTX_OK;
   }
-  // measured for 64 sequences and heads (192 for 256 rows), us: 256 rows 5.6 by a
-  // wave, 8.6 by a workgroup; 1000 rows 12.7 by a wave, 5.8; 4000 rows 11.2 by 1024
-  // threads, 9.2 by 256; 32768 rows 19.6 held in registers, 35 read again each step;
-  // 49152 rows 27.6 and 40; with 64 rows a thread registers spill: 48
+#undef FUSED
+  // else measured for 64 sequences and heads, us: 4000 rows 11.2 by 1024 threads, 9.2
+  // by 256; 32768 rows 19.6 held in registers, 35 read again each step; 49152 rows
+  // 27.6 and 40; with 64 rows a thread registers spill: 48
 #define SELECT(NT, R, SINGLE) hipLaunchKernelGGL((select_kernel<NT, R, SINGLE>), grid, dim3(NT), 0, st, a)
   if (cap <= 256 * 4) SELECT(256, 4, true);
   else if (cap <= 256 * 16) SELECT(256, 16, true);

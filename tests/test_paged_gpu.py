@@ -516,6 +516,17 @@ def test_evict_where_a_sample_misleads(dev, kind, n, keep):
     check_evict([n], keep, 7, Hkv=1, D=16, page=128, cache="bfloat16", seed=keep, weights=weights)
 
 
+@pytest.mark.parametrize("B, Hkv, D, n, keep", [
+    (6, 8, 128, 700, 500),   # 1536 workgroups: one launch
+    (6, 8, 128, 700, 513),   # 1584: two
+    (2, 8, 128, 2000, 512),  # 512
+    (2, 8, 128, 2000, 520),  # 528
+    (3, 8, 128, 250, 249),
+])
+def test_evict_many_heads(dev, B, Hkv, D, n, keep):
+    check_evict([n - 13 * b for b in range(B)], keep, keep // 5, Hkv=Hkv, D=D, page=20, seed=n + keep)
+
+
 def test_evict_pages_that_are_not_there(dev):
     """Kept rows of pages outside the pool become zeros; rows whose new page
     is outside it are dropped."""
