@@ -59,12 +59,13 @@ _NAMES: dict = {}  # the names of the dtypes asked for so far
 
 
 _READY = False
+SEVERAL = False  # whether tensors can lie on other GPUs than the library's
 
 
 def device() -> int:
     """Initialise the library on GPU 0 (once) and return its index.  Raises
     when no GPU is visible: there is no CPU fallback."""
-    global _READY
+    global _READY, SEVERAL
     if not _READY:
         n = C.c_int(0)
         L.call("mtx_device_count", C.byref(n))
@@ -72,6 +73,7 @@ def device() -> int:
             raise RuntimeError("minitorch_amd needs a GPU (MI355X); none is visible and there is "
                                "no CPU fallback")
         L.call("mtx_device_init", 0)
+        SEVERAL = n.value > 1
         _READY = True
     return 0
 

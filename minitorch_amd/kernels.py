@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import sys
 
 import numpy as np
 
@@ -186,6 +187,17 @@ def _on_device(*ts):
             raise ValueError("minitorch_amd kernels take device arrays")
 
 
+def _on_gpu0(*ts):
+    """Where there are several GPUs: raises unless every operand (None: not
+    there) lies on the library's and the thread's launches go there."""
+    for t in ts:
+        if getattr(t, "get_device", int)() != 0:
+            raise ValueError("minitorch_amd kernels take arrays of GPU 0")
+    torch = sys.modules.get("torch")
+    if torch is not None and torch.cuda.is_initialized() and torch.cuda.current_device() != 0:
+        raise ValueError("minitorch_amd kernels run on GPU 0, which is not the current device")
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -271,6 +283,7 @@ def _append_plan(k, v, k_pages, v_pages, table, lengths, counts):
     if kshape != (B, Hkv, T, D) or vshape != kshape or kd != vd:
         raise ValueError(f"k and v must be ({B}, {Hkv}, T, {D}) of one dtype (got {kshape}, {vshape})")
     _vector("counts", counts, B, "int32")
+    dev.device()
     return (_code(kd), _code(cache), B, T, Hkv, D), (ks, vs), (n_pages, page), (kps, vps), (ld, width)
 
 
@@ -285,6 +298,8 @@ def kv_append_paged(k, v, k_pages, v_pages, table, lengths, counts=None):
         (k.shape, k.stride(), k.dtype), (v.shape, v.stride(), v.dtype),
         (k_pages.shape, k_pages.stride(), k_pages.dtype), (v_pages.shape, v_pages.stride(), v_pages.dtype),
         (table.shape, table.stride(), table.dtype), (lengths.shape, lengths.stride(), lengths.dtype), _spec(counts))
+    if dev.SEVERAL:
+        _on_gpu0(k, v, k_pages, v_pages, table, lengths, counts)
     L.call("mtx_kv_append_paged", *sizes, k.data_ptr(), ks, v.data_ptr(), vs, n, page, k_pages.data_ptr(), kps,
            v_pages.data_ptr(), vps, table.data_ptr(), ld, width, lengths.data_ptr(), _ptr(counts), L.stream_handle())
 
@@ -309,6 +324,7 @@ def _decode_paged_plan(q, k_pages, v_pages, table, lengths, out, lse, weights, w
     elif weights_in is not None:
         raise ValueError("weights_in without weights")
     ws = L.lib().mtx_attn_decode_paged_workspace_bytes(B, H, Hkv, D, page, width, int(weights is not None))
+    dev.device()
     return (_ints(_code(qd), _code(cache), B, H, Hkv, D), (qs, os), (*_longs(n_pages), *_ints(page)), (kps, vps),
             (*_longs(ld), *_ints(width)), *_longs(wld), ws)
 
@@ -329,6 +345,8 @@ def attn_decode_paged(q, k_pages, v_pages, table, lengths, scale: float, out=Non
         (q.shape, q.stride(), q.dtype), (k_pages.shape, k_pages.stride(), k_pages.dtype),
         (v_pages.shape, v_pages.stride(), v_pages.dtype), (table.shape, table.stride(), table.dtype),
         (lengths.shape, lengths.stride(), lengths.dtype), _spec(out), _spec(lse), _spec(weights), _spec(weights_in))
+    if dev.SEVERAL:
+        _on_gpu0(q, k_pages, v_pages, table, lengths, out, lse, weights, weights_in)
     ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
     L.call("mtx_attn_decode_paged", *sizes, q.data_ptr(), qs, n, page, k_pages.data_ptr(), kps, v_pages.data_ptr(),
            vps, table.data_ptr(), ld, width, lengths.data_ptr(), out.data_ptr(), os, _ptr(lse), _ptr(weights_in),
@@ -345,6 +363,7 @@ def _evict_plan(k_pages, v_pages, table, lengths, weights, to_table, keep, lengt
     _row_weights("weights_out", weights_out, B, Hkv, width * page, wld)
     if _dt(slots[2]) != "int32" or tuple(slots[0]) != (B, Hkv, keep) or not _packed(*slots[:2]):
         raise ValueError(f"slots must be contiguous int32 ({B}, {Hkv}, {keep})")
+    dev.device()
     return (_code(cache), B, Hkv, D, n_pages, page), (kps, vps), (ld, width), wld, (to_ld, to_pages)
 
 
@@ -368,6 +387,8 @@ def kv_evict_paged(k_pages, v_pages, table, lengths, weights, to_table, keep: in
     sizes, (kps, vps), (ld, width), wld, (to_ld, to_pages) = _evict_plan(
         _spec(k_pages), _spec(v_pages), _spec(table), _spec(lengths), _spec(weights), _spec(to_table), keep,
         _spec(lengths_out), _spec(weights_out), _spec(slots))
+    if dev.SEVERAL:
+        _on_gpu0(k_pages, v_pages, table, lengths, weights, to_table, lengths_out, weights_out, slots)
     L.call("mtx_kv_evict_paged", *sizes, k_pages.data_ptr(), kps, v_pages.data_ptr(), vps, table.data_ptr(), ld,
            width, lengths.data_ptr(), weights.data_ptr(), wld, to_table.data_ptr(), to_ld, to_pages, keep,
            int(recent), lengths_out.data_ptr(), weights_out.data_ptr(), slots.data_ptr(), L.stream_handle())
@@ -1182,6 +1203,7 @@ def _logprobs_plan(logits, tokens, top, logprob, entropy, lse, top_ids, top_logp
         if _dt(t[2]) != dt or tuple(t[0]) != (rows, top) or (rows and top and not _packed(*t[:2])):
             raise ValueError(f"{name} must be contiguous {dt} ({rows}, {top})")
     ws = L.lib().mtx_token_logprobs_workspace_bytes(rows, V, top) if rows else 0
+    dev.device()
     return code, rows, V, ld, ws
 
 
@@ -1207,6 +1229,8 @@ def token_logprobs(logits, tokens, top: int = 0, scale: float = 1.0, logprob=Non
         (logprob.shape, logprob.stride(), logprob.dtype), (entropy.shape, entropy.stride(), entropy.dtype),
         (lse.shape, lse.stride(), lse.dtype), (top_ids.shape, top_ids.stride(), top_ids.dtype),
         (top_logprobs.shape, top_logprobs.stride(), top_logprobs.dtype))
+    if dev.SEVERAL:
+        _on_gpu0(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs)
     if rows:
         ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
         L.call("mtx_token_logprobs", code, rows, V, logits.data_ptr(), ld, tokens.data_ptr(), float(scale),
@@ -1221,6 +1245,7 @@ def _logprobs_bwd_plan(logits, tokens, lse, entropy, g_logprob, g_entropy, dlogi
                                      g_entropy=g_entropy)
     if _dt(dlogits[2]) != "float32" or tuple(dlogits[0]) != (rows, V) or dlogits[1][1] != 1:
         raise ValueError(f"dlogits must be fp32 ({rows}, {V}) with contiguous rows")
+    dev.device()
     return code, rows, V, ld, dlogits[1][0]
 
 
@@ -1239,6 +1264,8 @@ def token_logprobs_bwd(logits, tokens, lse, entropy, g_logprob, g_entropy, scale
         (logits.shape, logits.stride(), logits.dtype), (tokens.shape, tokens.stride(), tokens.dtype),
         (lse.shape, lse.stride(), lse.dtype), (entropy.shape, entropy.stride(), entropy.dtype), _spec(g_logprob),
         _spec(g_entropy), (dlogits.shape, dlogits.stride(), dlogits.dtype))
+    if dev.SEVERAL:
+        _on_gpu0(logits, tokens, lse, entropy, g_logprob, g_entropy, dlogits)
     if rows:
         L.call("mtx_token_logprobs_bwd", code, rows, V, logits.data_ptr(), ld, tokens.data_ptr(), lse.data_ptr(),
                entropy.data_ptr(), _ptr(g_logprob), _ptr(g_entropy), float(scale), dlogits.data_ptr(), ldd,

@@ -184,3 +184,66 @@ def test_logprobs_forward_checks(over, code, frag):
 def test_logprobs_backward_checks(over, frag):
     rc, msg = backward(over)
     assert rc == L.MTX_ERR_ARG and frag in msg
+
+
+class OnGpu:
+    """What the wrappers look at of a tensor on GPU `index`."""
+
+    is_cuda = True
+
+    def __init__(self, shape, dtype="float32", index=0):
+        self.shape, self.dtype, self.index = shape, dtype, index
+
+    def stride(self, d=None):
+        s = [1]
+        for n in self.shape[:0:-1]:
+            s.insert(0, s[0] * n)
+        return tuple(s) if d is None else s[d]
+
+    def get_device(self):
+        return self.index
+
+    def data_ptr(self):
+        raise AssertionError("launched")
+
+
+@pytest.mark.parametrize("elsewhere", range(7))
+def test_arrays_of_another_gpu_are_refused(monkeypatch, elsewhere):
+    from minitorch_amd import kernels as K
+
+    monkeypatch.setattr(K.dev, "device", lambda: 0)
+    monkeypatch.setattr(K.dev, "SEVERAL", True)
+    monkeypatch.setattr(K.dev, "empty_buf", lambda shape, dtype="float32": OnGpu(tuple(shape), dtype))
+    gpu = [int(i == elsewhere) for i in range(9)]
+    pool, head = (10, 4, 8, 64), (2, 4, 1, 64)
+    kp, vp = OnGpu(pool, index=gpu[0]), OnGpu(pool, index=gpu[1])
+    table, lengths = OnGpu((2, 5), "int32", gpu[2]), OnGpu((2,), "int32", gpu[3])
+    rows = [OnGpu(head, index=gpu[4]), OnGpu(head, index=gpu[5])]
+    counts = OnGpu((2,), "int32", gpu[6])
+    with pytest.raises(ValueError, match="GPU 0"):
+        K.kv_append_paged(*rows, kp, vp, table, lengths, counts)
+    w = OnGpu((2, 4, 40), index=gpu[6])
+    with pytest.raises(ValueError, match="GPU 0"):
+        K.attn_decode_paged(rows[0], kp, vp, table, lengths, 0.125, out=rows[1], weights=w)
+    to, w_out = OnGpu((2, 2), "int32", gpu[4]), OnGpu((2, 4, 40), index=gpu[5])
+    with pytest.raises(ValueError, match="GPU 0"):
+        K.kv_evict_paged(kp, vp, table, lengths, w, to, 16, 4, weights_out=w_out)
+    x, tok = OnGpu((6, 50), index=gpu[0]), OnGpu((6,), "int64", gpu[1])
+    lp, h, lse = (OnGpu((6,), index=gpu[i]) for i in (2, 3, 4))
+    ids, tops = OnGpu((6, 3), "int64", gpu[5]), OnGpu((6, 3), index=gpu[6])
+    with pytest.raises(ValueError, match="GPU 0"):
+        K.token_logprobs(x, tok, 3, 1.0, lp, h, lse, ids, tops)
+    g = [OnGpu((6,), index=gpu[i]) for i in (2, 5)]
+    with pytest.raises(ValueError, match="GPU 0"):
+        K.token_logprobs_bwd(x, tok, lse, h, *g, dlogits=OnGpu((6, 50), index=gpu[6]))
+
+
+def test_arrays_of_the_librarys_gpu_are_not(monkeypatch):
+    from minitorch_amd import kernels as K
+
+    monkeypatch.setattr(K.dev, "device", lambda: 0)
+    monkeypatch.setattr(K.dev, "SEVERAL", True)
+    x, tok = OnGpu((6, 50)), OnGpu((6,), "int64")
+    v = [OnGpu((6,)) for _ in range(3)]
+    with pytest.raises(AssertionError, match="launched"):
+        K.token_logprobs(x, tok, 0, 1.0, *v, OnGpu((6, 0), "int64"), OnGpu((6, 0)))
