@@ -11,6 +11,9 @@ Modules
                backward closures the reference's autograd runs for it.
   gpt       -- the GPT training step and greedy generation (transformer.py,
                layers.py, functional.py, loss.py, optim.py).
+  paged     -- a cache in pages, attention over it, its eviction and token log
+               probabilities, in float64 from their formulas (the reference has
+               none of them).
 
 How each function is pinned (checked against something other than itself) is
 stated in its docstring; see also tests/test_oracle.py.
