@@ -363,7 +363,8 @@ int mtx_kv_append_paged(int dtype, int cache_dtype, int B, int T, int Hkv, int D
  * may be `weights` itself, which then accumulates over calls (what
  * mtx_kv_evict_paged goes by).  A workspace of
  * mtx_attn_decode_paged_workspace_bytes() bytes, 16-byte aligned, is written by
- * the call and free after it; calls that overlap need their own.  Deterministic.
+ * the call and free after it; calls that overlap need their own.  Deterministic; a
+ * long sequence is cut by the lengths of all, and so are the last bits of its sums.
  */
 size_t mtx_attn_decode_paged_workspace_bytes(int B, int H, int Hkv, int D, int page, int max_pages,
                                              int with_weights);

@@ -26,17 +26,32 @@ struct Pages {  // (n_pages, heads, page, D) view: element strides, d stride 1
   int64_t sp, sh, sr;
 };
 
+// Division by a number that the host knows: j / d = (mulhi(j, mul) + j) >> shift for
+// j < 2^31, the smallest shift with 2^shift >= d, and mul = 2^32 (2^shift - d) / d + 1
+// (Granlund and Montgomery's division by an invariant integer)
+struct Divisor32 {
+  uint32_t mul;
+  int shift;
+  __device__ __forceinline__ int quotient(int j) const {
+    return (int)((__umulhi((uint32_t)j, mul) + (uint32_t)j) >> shift);
+  }
+};
+Divisor32 divisor32(int d) {
+  int shift = 0;
+  while (((int64_t)1 << shift) < d) ++shift;
+  return Divisor32{(uint32_t)(((((uint64_t)1 << shift) - d) << 32) / d + 1), shift};
+}
+
 struct Table {
   const int* ids;
   int64_t ld;
   int width;        // pages per sequence
   int page;         // rows per page
   int64_t n_pages;  // pages in the pool
-  uint32_t mul;     // j / page = (mulhi(j, mul) + j) >> shift for j < 2^31
-  int shift;
+  Divisor32 by;     // page
 
   // the index of the page that holds row j
-  __device__ __forceinline__ int div(int j) const { return (int)((__umulhi((uint32_t)j, mul) + (uint32_t)j) >> shift); }
+  __device__ __forceinline__ int div(int j) const { return by.quotient(j); }
   // the id at index i of sequence b's pages, or -1
   __device__ __forceinline__ int id(int b, int i) const {
     const int x = ids[b * ld + i];
@@ -44,14 +59,8 @@ struct Table {
   }
 };
 
-// rows of `page` a page: the smallest shift with 2^shift >= page, and
-// 2^32 (2^shift - page) / page + 1 (Granlund and Montgomery's division by an
-// invariant integer)
 Table make_table(const int* ids, int64_t ld, int width, int page, int64_t n_pages) {
-  int shift = 0;
-  while ((1 << shift) < page) ++shift;
-  const uint32_t mul = (uint32_t)((((uint64_t)(1u << shift) - page) << 32) / page + 1);
-  return Table{ids, ld, width, page, n_pages, mul, shift};
+  return Table{ids, ld, width, page, n_pages, divisor32(page)};
 }
 
 // offset of row j, whose page's index is i and id is `id`
@@ -127,14 +136,13 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
 // and q and the weights as three (24 bits) for fp32 rows.
 //
 // Measured, 16 sequences of 8000 to 16384 rows, 8 K/V heads of 128 in bf16 (797
-// MB), 32 query heads: 153 us, 5.2 TB/s (a plain read of the same pages: 136 us;
-// the loads of this kernel without its products: 145 us); one of 131071 rows (67
-// MB): 17.2 us, of which 11 at the memory's rate.
+// MB), 32 query heads: 139 us, 5.7 TB/s (a plain read of the same pages: 136 us); one of
+// 131071 rows (67 MB): 17.5 us, of which 11 at the memory's rate.
 //
-// A workgroup takes `chunk` rows of one sequence and K/V head, its four waves in
-// turn tiles of 16 NT rows, and joins them in LDS; several chunks of a sequence
-// are joined by finish_kernel.
-constexpr int kMaxChunk = 2048;
+// A workgroup takes some rows of one sequence and K/V head (make_plan), its four
+// waves in turn tiles of 16 NT of them, and joins them in LDS; several workgroups'
+// results for a sequence are joined by finish_kernel.
+constexpr int kMaxIds = 4096;  // page ids of a chunk, in LDS
 constexpr float kRaise = 8.f;
 
 struct DecodeArgs {
@@ -149,13 +157,16 @@ struct DecodeArgs {
   const float* win;
   float* w;
   int64_t wld;
-  float* part_o;  // [B H][S][D] sums, relative to part_ml's maximum
-  float* part_ml; // [B H][S][2] maximum (log2 units) and sum
+  float* part_o;  // [B H][S][D] or [P][H][D] sums, relative to part_ml's maximum
+  float* part_ml; // [B H][S][2] or [P][H][2] maximum (log2 units) and sum
   float* s;       // [B H][sld] scores (log2 units), with weights
   int64_t sld;
+  int* cuts;      // [B][2] with P: first piece of a sequence, how many
   int B, H, Hkv, G, S, HT, chunk, cap;
+  int P, most;    // pieces the sequences are cut into, by their lengths, of at most 64 `most` rows (0: S chunks each)
   int direct;     // the workgroup's result is final: no finish_kernel
   float c;        // scale * log2(e)
+  Divisor32 by_ht, by_hkv, by_s;
 };
 
 template <typename TQ, typename TC, int D> struct DecodeTile;
@@ -309,6 +320,77 @@ __device__ __forceinline__ float lane_sum4(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
+// Cutting up to 128 sequences into at most P pieces, by their lengths: the size (a
+// multiple of 64 rows, 256 or more) that needs no more than P, from 64 sizes tried at
+// once, a lane each.  Every wave of every workgroup comes to the same: false if there is
+// no piece q, otherwise its sequence, its number in it, its rows [c0, c1), the sequence's
+// length n and how many pieces it has.  It costs 1 to 1.5 us before the first load of a
+// page id
+struct Cut {
+  int b, split, count, c0, c1, n;
+};
+// u > 0 units in pieces of m, exact for u < 2^21: u - 1/2 is half a piece's unit away
+// from where the result changes, which is more than the product's rounding
+__device__ __forceinline__ int pieces(int u, float inv) { return u ? (int)(((float)u - 0.5f) * inv) + 1 : 0; }
+// f over the lanes up to each, in the wave's last lane over all of them
+template <typename F>
+__device__ __forceinline__ int wave_scan(int x, F f) {
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast 15, 31
+  return f(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+}
+__device__ __forceinline__ bool cut_rows(const DecodeArgs& a, int q, int lane, Cut& x) {
+  if (a.B == 1) {  // no trying: 0.7 us less
+    x.n = min(max(a.lengths[0], 0), a.cap);
+    const int size = min(max((x.n + a.P - 1) / a.P + 63 & ~63, 256), 64 * a.most);
+    x.b = 0;
+    x.split = q;
+    x.count = (x.n + size - 1) / size;
+    x.c0 = q * size;
+    x.c1 = min(x.n, x.c0 + size);
+    return q < x.count;
+  }
+  int len[2], u[2], sum = 0, top = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    len[i] = 2 * lane + i < a.B ? a.lengths[2 * lane + i] : 0;
+    len[i] = min(max(len[i], 0), a.cap);
+    u[i] = (len[i] + 63) >> 6;
+    sum += u[i];
+    top = max(top, u[i]);
+  }
+  const auto add = [](int x, int y) { return x + y; };
+  sum = __builtin_amdgcn_readlane(wave_scan(sum, add), 63);
+  top = __builtin_amdgcn_readlane(wave_scan(top, [](int x, int y) { return max(x, y); }), 63);
+  const float hi = (float)min(max(top, 4), a.most), lo = fminf(fmaxf(ceilf((float)sum / (float)a.P), 4.f), hi);
+  const float f = __builtin_amdgcn_exp2f(__builtin_amdgcn_logf(hi / lo) * ((float)lane * (1.f / 63.f)));
+  const float m = lane == 0 ? lo : lane == 63 ? hi : fminf(ceilf(lo * f), hi), inv = 1.f / m;
+  int need = 0;
+  for (int s = 0; 2 * s < a.B; ++s)
+    need += pieces(__builtin_amdgcn_readlane(u[0], s), inv) + pieces(__builtin_amdgcn_readlane(u[1], s), inv);
+  const uint64_t fits = __ballot(need <= a.P);
+  const int pick = fits ? __ffsll((unsigned long long)fits) - 1 : 63;
+  const int size = 64 * (int)__uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(m), pick));
+  const float by = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(inv), pick));
+  const int c0 = pieces(u[0], by), mine = c0 + pieces(u[1], by), upto = wave_scan(mine, add);
+  const uint64_t in = __ballot(q < upto && q >= upto - mine);
+  if (!in) return false;
+  const int at = __ffsll((unsigned long long)in) - 1;
+  const int first = __builtin_amdgcn_readlane(c0, at);
+  x.split = q - __builtin_amdgcn_readlane(upto - mine, at);
+  const int i = x.split >= first;
+  x.b = 2 * at + i;
+  x.split -= i ? first : 0;
+  x.count = i ? __builtin_amdgcn_readlane(mine, at) - first : first;
+  x.n = __builtin_amdgcn_readlane(i ? len[1] : len[0], at);
+  x.c0 = x.split * size;
+  x.c1 = min(x.n, x.c0 + size);
+  return true;
+}
+
 // RUN consecutive rows (aligned to RUN) lie in one page, at row strides that fit
 // 32-bit offsets: 16, a tile's rows have one uniform address; 4, a lane looks up
 // its four V rows at once (64 sequences in pages of 20: 13.8 us a call, 15.8 with
@@ -318,28 +400,49 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
   using Tile = DecodeTile<TQ, TC, D>;
   constexpr int NT = Tile::NT, VD = Tile::VD, KT = 16 * NT, LD = D + 4;
   __shared__ union {
-    int ids[kMaxChunk + 2];
+    int ids[kMaxIds];
     struct { float o[4][16][LD], m[4][16], l[4][16]; } j;
   } sh;
   __shared__ float lse2[16];
 
   // the HT workgroups that read the same rows are 8 apart: on one XCD, sharing its L2
-  const int eight = blockIdx.x / (8 * a.HT), ht = blockIdx.x / 8 % a.HT, piece = 8 * eight + blockIdx.x % 8;
-  const int split = piece % a.S, bh = piece / a.S, b = bh / a.Hkv, hk = bh % a.Hkv;
-  if (bh >= a.B * a.Hkv) return;
+  const int group = blockIdx.x / 8, eight = a.by_ht.quotient(group), ht = group - eight * a.HT;
+  const int piece = 8 * eight + blockIdx.x % 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quarter = lane >> 4;
+  Cut x;
+  int hk, slot = 0;
+  if (__builtin_expect(a.P != 0, 0)) {
+    // the pieces that there are come first, so that the GPU's compute units get one each,
+    // and a piece's heads on another XCD each time (an XCD's L2 has its channels by
+    // address: one head's rows of a pool stored by rows lie in few of them)
+    slot = a.by_hkv.quotient(piece);
+    hk = piece + slot;
+    hk -= a.by_hkv.quotient(hk) * a.Hkv;
+    if (slot >= a.P || !cut_rows(a, slot, lane, x)) return;
+    if (x.split == 0 && hk == 0 && ht == 0 && tid == 0) a.cuts[2 * x.b] = slot, a.cuts[2 * x.b + 1] = x.count;
+  } else {
+    const int bh = a.by_s.quotient(piece);
+    x.b = a.by_hkv.quotient(bh);
+    if (x.b >= a.B) return;
+    hk = bh - x.b * a.Hkv;
+    // (piece + bh) mod S: the first chunks, which most sequences have, lie on all XCDs in
+    // turn, also where S is a multiple of 8
+    x.split = piece + bh - a.by_s.quotient(piece + bh) * a.S;
+    x.c0 = x.split * a.chunk;
+    x.c1 = min(a.cap, x.c0 + a.chunk);
+  }
+  const int b = x.b, c0 = x.c0, bh = b * a.Hkv + hk;
   const int heads = min(16, a.G - 16 * ht), h0 = hk * a.G + 16 * ht;
-  const int c0 = split * a.chunk;
-  // the page ids of the whole chunk, whatever the length, so that neither load
-  // waits for the other
-  const int p0 = a.tab.div(c0), np = a.tab.div(min(a.cap, c0 + a.chunk) - 1) - p0 + 1;
-  const int length = a.lengths[b];
+  // the page ids of the whole chunk, without P whatever the length, so that neither
+  // load waits for the other
+  const int p0 = a.tab.div(c0), np = a.tab.div(x.c1 - 1) - p0 + 1;
+  if (!a.P) x.n = a.lengths[b];
   for (int i = tid; i < np; i += 256) sh.ids[i] = a.tab.id(b, p0 + i);
   Tile tile;
   tile.load_q(col < heads ? static_cast<const TQ*>(a.q) + b * a.qb + (h0 + col) * a.qh : nullptr, quarter);
-  const int n = min(max(length, 0), a.cap), c1 = min(n, c0 + a.chunk);
-  if (c0 >= n && !(a.direct && split == 0)) return;  // finish_kernel knows which chunks there are
+  const int n = min(max(x.n, 0), a.cap), c1 = min(n, x.c1);
+  if (c0 >= n && !(a.direct && c0 == 0)) return;  // finish_kernel knows which chunks there are
   __syncthreads();
 
   const TC* __restrict__ kp = static_cast<const TC*>(a.k.p) + hk * a.k.sh;
@@ -472,26 +575,27 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
   for (int i = tid; i < heads * D; i += 256) {
     const int h = i / D, d = i % D;
     const float m = fmaxf(fmaxf(sh.j.m[0][h], sh.j.m[1][h]), fmaxf(sh.j.m[2][h], sh.j.m[3][h]));
-    float x = 0.f, sum = 0.f;
+    float value = 0.f, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float f = __builtin_amdgcn_exp2f(sh.j.m[w][h] - m);
-      x += f * sh.j.o[w][h][d];
+      value += f * sh.j.o[w][h][d];
       sum += f * sh.j.l[w][h];
     }
     const int64_t row = (int64_t)b * a.H + h0 + h;
     if (a.direct) {
       const bool some = sum > 0.f || sum != sum;
-      static_cast<TQ*>(a.o)[b * a.ob + (h0 + h) * a.oh + d] = Elem<TQ>::from_f(some ? x / sum : 0.f);
+      static_cast<TQ*>(a.o)[b * a.ob + (h0 + h) * a.oh + d] = Elem<TQ>::from_f(some ? value / sum : 0.f);
       if (d == 0) {
         if (a.lse != nullptr) a.lse[row] = some ? m * kLn2 + logf(sum) : -INFINITY;
         lse2[h] = some ? m + log2f(sum) : 0.f;
       }
     } else {
-      a.part_o[(row * a.S + split) * D + d] = x;
+      const int64_t at = a.P ? (int64_t)slot * a.H + h0 + h : row * a.S + x.split;
+      a.part_o[at * D + d] = value;
       if (d == 0) {
-        a.part_ml[(row * a.S + split) * 2] = m;
-        a.part_ml[(row * a.S + split) * 2 + 1] = sum;
+        a.part_ml[at * 2] = m;
+        a.part_ml[at * 2 + 1] = sum;
       }
     }
   }
@@ -507,12 +611,29 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
   }
 }
 
+// a sequence's chunks: how many of `n` rows, the place of head h's first in part_o
+// and part_ml, and how far apart they are
+struct Chunks {
+  int count, step;
+  int64_t first;
+  __device__ __forceinline__ Chunks(const DecodeArgs& a, int b, int h, int n) {
+    if (a.P) {
+      count = n ? a.cuts[2 * b + 1] : 0;
+      step = a.H;
+      first = n ? (int64_t)a.cuts[2 * b] * a.H + h : 0;
+    } else {
+      count = (n + a.chunk - 1) / a.chunk;
+      step = 1;
+      first = ((int64_t)b * a.H + h) * a.S;
+    }
+  }
+};
 // maximum and sum of one head over its chunks, by one wave
-__device__ __forceinline__ void chunk_total(const float* ml, int chunks, int lane, float& m, float& l) {
+__device__ __forceinline__ void chunk_total(const float* ml, const Chunks& c, int lane, float& m, float& l) {
   m = -FLT_MAX;
   l = 0.f;
-  for (int i = lane; i < chunks; i += 64) {
-    const f32x2 x = reinterpret_cast<const f32x2*>(ml)[i];
+  for (int i = lane; i < c.count; i += 64) {
+    const f32x2 x = reinterpret_cast<const f32x2*>(ml)[(int64_t)i * c.step];
     const float n = fmaxf(m, x[0]);
     l = l * __builtin_amdgcn_exp2f(m - n) + x[1] * __builtin_amdgcn_exp2f(x[0] - n);
     m = n;
@@ -539,15 +660,17 @@ __global__ __launch_bounds__(256) void finish_kernel(const DecodeArgs a) {
   if ((int)blockIdx.x < outs) {
     const int64_t row = blockIdx.x / ND;
     const int b = (int)row / a.H, h = (int)row % a.H;
-    const int chunks = (min(max(a.lengths[b], 0), a.cap) + a.chunk - 1) / a.chunk;
-    const float* ml = a.part_ml + row * a.S * 2;
+    const Chunks chunks(a, b, h, min(max(a.lengths[b], 0), a.cap));
+    const float* ml = a.part_ml + chunks.first * 2;
     float m, l;
     chunk_total(ml, chunks, lane, m, l);
     const int d = tid % DL, g = tid / DL, d0 = blockIdx.x % ND * FD;
-    const float* po = a.part_o + row * a.S * D + d0 + 4 * d;
+    const float* po = a.part_o + chunks.first * D + d0 + 4 * d;
     f32x4 x = zero4();
-    for (int i = g; i < chunks; i += NG)
-      x += *reinterpret_cast<const f32x4*>(po + (int64_t)i * D) * __builtin_amdgcn_exp2f(ml[2 * i] - m);
+    for (int i = g; i < chunks.count; i += NG) {
+      const int64_t at = (int64_t)i * chunks.step;
+      x += *reinterpret_cast<const f32x4*>(po + at * D) * __builtin_amdgcn_exp2f(ml[2 * at] - m);
+    }
 #pragma unroll
     for (int s = DL; s < 64; s <<= 1)
 #pragma unroll
@@ -567,11 +690,11 @@ __global__ __launch_bounds__(256) void finish_kernel(const DecodeArgs a) {
   const int bh = i / blocks, b = bh / a.Hkv, hk = bh % a.Hkv;
   const int n = min(max(a.lengths[b], 0), a.cap), j0 = (i % blocks) * kFinishRows, j1 = min(n, j0 + kFinishRows);
   if (j0 >= n) return;
-  const int chunks = (n + a.chunk - 1) / a.chunk;
   const int64_t row = (int64_t)b * a.H + hk * a.G;
   for (int g = tid >> 6; g < a.G; g += 4) {
+    const Chunks chunks(a, b, hk * a.G + g, n);
     float m, l;
-    chunk_total(a.part_ml + (row + g) * a.S * 2, chunks, lane, m, l);
+    chunk_total(a.part_ml + chunks.first * 2, chunks, lane, m, l);
     if (lane == 0) sh.lse2[g] = l > 0.f || l != l ? m + log2f(l) : 0.f;
   }
   __syncthreads();
@@ -1045,31 +1168,50 @@ int check_cache(int B, int H, int D, int64_t n_pages, int page, const int* table
   return MTX_OK;
 }
 
-// How a decode call is cut, and its workspace [part_o | part_ml | scores].  One
-// chunk a sequence, with no second launch, up to the rows that four waves finish
-// before the second launch would: 512, with more segments to fill the GPU 1024
-// (384 segments of up to 1000 rows: 16.7 us against 15.6 + 4.0) and 2048 (768 of
-// 2048: 147 against 154).  Else chunks of 512 rows, or of up to 1024 where a call
-// may have more than 768 of them (128 segments of 16384: 154 us, 174 with 512)
+// How a decode call is cut, and its workspace [part_o | part_ml | scores | cuts].
+//
+// Whole sequences, with no second launch, where the rows are few (1280 rows of 64
+// values, 640 of 128: 8.6 us in one workgroup, 12.5 in several) or the workgroups
+// enough for the GPU (B = 32, 4 K/V heads of 128, 1500 rows: 21 us, 23 to 25 in chunks;
+// 64 sequences of 100 to 3000 rows, 8 of 128: 85, 97).
+//
+// Else up to 128 sequences and heads: P pieces by the lengths (cut_rows), one for each
+// compute unit.  16 sequences of 8000 to 16384 rows, 8 heads: 143 us, in chunks of 1024
+// rows 157; one of 16384 and 15 of 300: 25, 57; 7 sequences of 9000, 2 heads, 21.7, 20.1.
+//
+// Else chunks alike, 512 to 1024 rows each, some 768 or more: they come to the compute
+// units as those get free, which P pieces of unequal size would not (20 sequences of
+// 10000 rows, 8 heads of 64: 80 us, 89 by pieces)
 struct DecodePlan {
-  int chunk, S, HT, direct;
-  int64_t n_o, n_ml, n_s, sld;
-  size_t bytes() const { return (size_t)(n_o + n_ml + n_s) * sizeof(float); }
+  int chunk, S, HT, P, most, direct;
+  int64_t n_o, n_ml, n_s, n_cuts, sld;
+  size_t bytes() const { return (size_t)(n_o + n_ml + n_s + n_cuts) * sizeof(float); }
 };
-DecodePlan make_plan(int B, int H, int Hkv, int D, int cap, bool weights) {
-  DecodePlan p;
+DecodePlan make_plan(int B, int H, int Hkv, int D, int page, int max_pages, bool weights) {
+  const int cap = page * max_pages;
+  DecodePlan p{};
   p.HT = cdiv(H / Hkv, 16);
-  const int64_t segments = (int64_t)B * Hkv * p.HT;
-  const int64_t want = (cap * segments / 768 + 127) / 128 * 128;
-  p.chunk = (int)std::min<int64_t>(std::max<int64_t>(want, 512), 1024);
-  if (cap <= 1024 && segments >= 128) p.chunk = 1024;
-  if (cap <= 2048 && segments >= 768) p.chunk = 2048;
+  const int64_t share = (int64_t)Hkv * p.HT, segments = B * share;
+  p.most = (int)(std::min<int64_t>((int64_t)(kMaxIds - 2) * page, 1 << 27) / 64);
+  const int one = (segments >= 384 ? 4096 : 2048) / (D >= 64 ? 1 : 2);
+  if (cap <= one && (segments >= 128 || cap * std::max(D, 64) <= 81920)) {
+    p.chunk = cap;
+  } else if (segments <= 128 && cap <= (1 << 27)) {
+    p.P = (int)std::max<int64_t>(std::min<int64_t>(256 / share, (int64_t)B * cdiv(cap, 256)),
+                                 (int64_t)B * cdiv(cap, 64 * p.most));
+    p.chunk = cap;
+  } else {
+    const int64_t want = std::min<int64_t>(std::max<int64_t>(cap * segments / 768, 512), 1024);
+    p.chunk = (cdiv(cap, cdiv(cap, (int)want)) + 63) / 64 * 64;
+  }
   p.S = cdiv(cap, p.chunk);
-  p.direct = p.S == 1 && (!weights || p.HT == 1);
+  p.direct = !p.P && p.S == 1 && (!weights || p.HT == 1);
   p.sld = ((int64_t)cap + 31) / 32 * 32;
-  p.n_o = p.direct ? 0 : (int64_t)B * H * p.S * D;
-  p.n_ml = p.direct ? 0 : ((int64_t)B * H * p.S * 2 + 3) / 4 * 4;
+  const int64_t parts = p.direct ? 0 : p.P ? (int64_t)p.P * H : (int64_t)B * H * p.S;
+  p.n_o = parts * D;
+  p.n_ml = (parts * 2 + 3) / 4 * 4;
   p.n_s = weights ? (int64_t)B * H * p.sld : 0;
+  p.n_cuts = p.P ? (2 * B + 3) / 4 * 4 : 0;
   return p;
 }
 
@@ -1149,7 +1291,7 @@ extern "C" size_t mtx_attn_decode_paged_workspace_bytes(int B, int H, int Hkv, i
   if (B < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || page < 1 || max_pages < 1 ||
       (int64_t)page * max_pages > (1 << 28))
     return 0;
-  return make_plan(B, H, Hkv, D, page * max_pages, with_weights != 0).bytes();
+  return make_plan(B, H, Hkv, D, page, max_pages, with_weights != 0).bytes();
 }
 
 extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, int Hkv, int D, const void* q,
@@ -1176,11 +1318,11 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
   MTX_CHECK_ARG(weights != nullptr || weights_in == nullptr, "weights_in without weights");
   MTX_CHECK_ARG(weights == nullptr || weights_ld >= cap, "weights: rows of %lld values for %d cached rows",
                 (long long)weights_ld, cap);
-  const DecodePlan plan = make_plan(B, H, Hkv, D, cap, weights != nullptr);
+  const DecodePlan plan = make_plan(B, H, Hkv, D, page, max_pages, weights != nullptr);
   const size_t need = plan.bytes();
   MTX_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need && ((uintptr_t)workspace & 15u) == 0),
                 "workspace: %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
-  const int64_t groups = ((int64_t)B * Hkv * plan.S + 7) / 8 * 8 * plan.HT;
+  const int64_t groups = (Hkv * (plan.P ? plan.P : (int64_t)B * plan.S) + 7) / 8 * 8 * plan.HT;
   const int64_t finish = (weights != nullptr ? (int64_t)B * Hkv * cdiv(cap, kFinishRows) : 0);
   MTX_CHECK_SHAPE(groups <= kMaxGroups && finish + (int64_t)B * H <= kMaxGroups,
                   "decode: too many sequences, heads and rows in one call");
@@ -1191,7 +1333,9 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
                make_table(table, table_ld, max_pages, page, n_pages),
                lengths, o, o_strides[0], o_strides[1], lse, weights_in, weights, weights_ld,
                ws, ws + plan.n_o, ws + plan.n_o + plan.n_ml, plan.sld,
-               B, H, Hkv, H / Hkv, plan.S, plan.HT, plan.chunk, cap, plan.direct, scale * kLog2e};
+               reinterpret_cast<int*>(ws + plan.n_o + plan.n_ml + plan.n_s),
+               B, H, Hkv, H / Hkv, plan.S, plan.HT, plan.chunk, cap, plan.P, plan.most, plan.direct, scale * kLog2e,
+               divisor32(plan.HT), divisor32(Hkv), divisor32(plan.S)};
   const bool near = std::max(kp_strides[2], vp_strides[2]) < (1 << 24);
   const int run = !near || page % 4 ? 1 : page % 16 ? 4 : 16;
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -199,6 +199,39 @@ def test_decode_long_cache(dev, page, D):
     check_decode(case, [40001], seed=3)
 
 
+@pytest.mark.parametrize("H,Hkv,D,page,lengths", [
+    (4, 2, 128, 64, [20000, 300, 1, 300, 300]),
+    (2, 1, 64, 16, [0, 5000, 0, 0, 63, 64, 65, 8001, 256, 0]),
+    (8, 4, 64, 16, [2304] * 4),
+    (8, 4, 64, 16, [2304, 4608]),
+    (1, 1, 16, 8, [1 + 37 * i % 4000 for i in range(128)]),
+    (1, 1, 16, 16, [4000] + [0] * 126 + [1]),
+    (2, 1, 16, 1, [9000, 100, 4033, 4032]),
+    (64, 2, 32, 20, [3000, 1000, 2999]),
+    (2048, 8, 16, 16, [2500]),
+    (12, 12, 16, 32, [6000, 700]),
+    (1, 1, 16, 16, [1 + 41 * i % 2500 for i in range(130)]),
+    (9, 9, 16, 16, [8100 - 517 * i for i in range(15)]),
+    (3, 3, 16, 16, [4096 - 30 * i for i in range(128)])],
+    ids=["skewed", "empty_between", "equal", "twice", "128_sequences", "first_and_last", "pages_of_one", "head_tiles",
+         "many_head_tiles", "more_heads", "130_sequences", "chunks_of_8", "whole_of_4096"])
+@pytest.mark.parametrize("weights", [False, True])
+def test_decode_cuts(dev, H, Hkv, D, page, lengths, weights):
+    """How sequences are shared out among workgroups: by the lengths of all, in
+    chunks alike, and whole."""
+    case = dict(q="bfloat16", cache="bfloat16", H=H, Hkv=Hkv, D=D, page=page, weights=weights)
+    check_decode(case, lengths, seed=len(lengths) + H)
+
+
+def test_decode_nothing_cached(dev):
+    """A wide table and no rows at all: zeros and -inf, weights as they were."""
+    def edit(a, rng):
+        a["lengths"] = np.array([0, 0, -1], np.int32)
+
+    case = dict(q="float32", cache="float32", H=4, Hkv=2, D=64, page=16, weights=True)
+    check_decode(case, [3000, 20, 700], seed=2, edit=edit)
+
+
 def test_decode_lengths_behind_the_table_and_negative(dev):
     def edit(a, rng):
         a["lengths"] = np.array([10 ** 9, -4, 20], np.int32)
