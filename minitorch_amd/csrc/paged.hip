@@ -164,6 +164,7 @@ struct DecodeArgs {
   int* cuts;      // [B][2] with P: first piece of a sequence, how many
   int B, H, Hkv, G, S, HT, chunk, cap;
   int P, most;    // pieces the sequences are cut into, by their lengths, of at most 64 `most` rows (0: S chunks each)
+  int lines;      // heads' rows share 128-byte lines
   int direct;     // the workgroup's result is final: no finish_kernel
   float c;        // scale * log2(e)
   Divisor32 by_ht, by_hkv, by_s;
@@ -410,25 +411,38 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(const DecodeArgs a) {
   const int piece = 8 * eight + blockIdx.x % 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quarter = lane >> 4;
+  // piece `slot` of all heads' rows (with P of cut_rows, else chunk r = slot mod S of
+  // sequence slot / S) and K/V head hk of it
   Cut x;
-  int hk, slot = 0;
-  if (__builtin_expect(a.P != 0, 0)) {
+  int hk, slot;
+  if (__builtin_expect(a.lines != 0, 0)) {
+    // a piece's heads 8 workgroups apart too
+    const int e = a.by_hkv.quotient(eight);
+    hk = eight - e * a.Hkv;
+    slot = 8 * e + blockIdx.x % 8;
+    if (!a.P) x.b = a.by_s.quotient(slot);
+  } else if (__builtin_expect(a.P != 0, 0)) {
     // the pieces that there are come first, so that the GPU's compute units get one each,
     // and a piece's heads on another XCD each time (an XCD's L2 has its channels by
     // address: one head's rows of a pool stored by rows lie in few of them)
     slot = a.by_hkv.quotient(piece);
     hk = piece + slot;
     hk -= a.by_hkv.quotient(hk) * a.Hkv;
-    if (slot >= a.P || !cut_rows(a, slot, lane, x)) return;
-    if (x.split == 0 && hk == 0 && ht == 0 && tid == 0) a.cuts[2 * x.b] = slot, a.cuts[2 * x.b + 1] = x.count;
   } else {
     const int bh = a.by_s.quotient(piece);
     x.b = a.by_hkv.quotient(bh);
-    if (x.b >= a.B) return;
     hk = bh - x.b * a.Hkv;
-    // (piece + bh) mod S: the first chunks, which most sequences have, lie on all XCDs in
-    // turn, also where S is a multiple of 8
-    x.split = piece + bh - a.by_s.quotient(piece + bh) * a.S;
+    slot = piece - (bh - x.b) * a.S;
+  }
+  if (__builtin_expect(a.P != 0, 0)) {
+    if (slot >= a.P || !cut_rows(a, slot, lane, x)) return;
+    if (x.split == 0 && hk == 0 && ht == 0 && tid == 0) a.cuts[2 * x.b] = slot, a.cuts[2 * x.b + 1] = x.count;
+  } else {
+    if (x.b >= a.B) return;
+    // the first chunks, which most sequences have, lie on all XCDs in turn, also where S
+    // is a multiple of 8
+    const int t = slot + (a.lines ? x.b : x.b * a.Hkv + hk);
+    x.split = t - a.by_s.quotient(t) * a.S;
     x.c0 = x.split * a.chunk;
     x.c1 = min(a.cap, x.c0 + a.chunk);
   }
@@ -1322,7 +1336,13 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
   const size_t need = plan.bytes();
   MTX_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need && ((uintptr_t)workspace & 15u) == 0),
                 "workspace: %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
-  const int64_t groups = (Hkv * (plan.P ? plan.P : (int64_t)B * plan.S) + 7) / 8 * 8 * plan.HT;
+  // one XCD reads the lines that heads share, where its pieces are about as many as
+  // another's (64 sequences of 1000 to 3000 rows, 8 heads of 16 bf16 stored by rows:
+  // 25 us, else 47)
+  const int64_t slots = plan.P ? plan.P : (int64_t)B * plan.S;
+  const int lines = Hkv > 1 && std::max(kp_strides[1], vp_strides[1]) * (cache_dtype == MTX_F32 ? 4 : 2) < 128 &&
+                    (slots % 8 == 0 || slots >= 64);
+  const int64_t groups = (lines ? (slots + 7) / 8 * 8 * Hkv : (slots * Hkv + 7) / 8 * 8) * plan.HT;
   const int64_t finish = (weights != nullptr ? (int64_t)B * Hkv * cdiv(cap, kFinishRows) : 0);
   MTX_CHECK_SHAPE(groups <= kMaxGroups && finish + (int64_t)B * H <= kMaxGroups,
                   "decode: too many sequences, heads and rows in one call");
@@ -1334,7 +1354,7 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
                lengths, o, o_strides[0], o_strides[1], lse, weights_in, weights, weights_ld,
                ws, ws + plan.n_o, ws + plan.n_o + plan.n_ml, plan.sld,
                reinterpret_cast<int*>(ws + plan.n_o + plan.n_ml + plan.n_s),
-               B, H, Hkv, H / Hkv, plan.S, plan.HT, plan.chunk, cap, plan.P, plan.most, plan.direct, scale * kLog2e,
+               B, H, Hkv, H / Hkv, plan.S, plan.HT, plan.chunk, cap, plan.P, plan.most, lines, plan.direct, scale * kLog2e,
                divisor32(plan.HT), divisor32(Hkv), divisor32(plan.S)};
   const bool near = std::max(kp_strides[2], vp_strides[2]) < (1 << 24);
   const int run = !near || page % 4 ? 1 : page % 16 ? 4 : 16;

@@ -223,6 +223,19 @@ def test_decode_cuts(dev, H, Hkv, D, page, lengths, weights):
     check_decode(case, lengths, seed=len(lengths) + H)
 
 
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("H,Hkv,D,lengths", [
+    (8, 4, 16, [1 + 11 * i % 700 for i in range(70)]),
+    (34, 2, 16, [1 + 11 * i % 300 for i in range(64)]),
+    (4, 4, 16, [3000, 100, 0, 5000]),
+    (40, 2, 32, [2900, 1400]),
+    (4, 4, 16, [2500 - 60 * i for i in range(40)]),
+    (5, 5, 32, [9000, 1])])
+def test_decode_heads_that_share_lines(dev, q, cache, H, Hkv, D, lengths):
+    case = dict(q=q, cache=cache, H=H, Hkv=Hkv, D=D, page=16, layout="rows", weights=H == 8)
+    check_decode(case, lengths, seed=H + D)
+
+
 def test_decode_nothing_cached(dev):
     """A wide table and no rows at all: zeros and -inf, weights as they were."""
     def edit(a, rng):
