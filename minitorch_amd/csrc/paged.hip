@@ -749,15 +749,18 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // the kept rows in order.  The range of keys [lo, hi] is cut into up to 2048 equal
 // bins, counted in LDS; the bin in which the want-th largest key lies is the next
 // range, and once it holds NT / 2 rows or fewer they are ranked among themselves:
-// mostly after one round, three at most.  Rows are held in registers, R a thread,
-// where they fit (SINGLE); otherwise each step reads them again.
+// mostly after one round, three at most.  A sample of long sequences says first where
+// the key lies, mostly in a list of some thousand.  Rows are held in registers, R a
+// thread, where they fit (SINGLE); otherwise each step reads them again.  Bound by its
+// vector instructions, some 30 a row, on as many compute units as there are sequences
+// and heads (64 of 30000 to 40000 rows: 24 us).
 constexpr int kBins = 2048;
 
 template <int NT, int R, bool SINGLE>
 __device__ __forceinline__ void select_rows(const EvictArgs& a, int bh, int len, int* slots) {
   constexpr int W = NT / 64;
   __shared__ int bins[kBins], part[W], gts[W], ties[W];
-  __shared__ uint32_t mins[W], maxs[W], found[4], few[NT / 2];
+  __shared__ uint32_t mins[W], maxs[W], found[4], few[NT / 2], list[4 * NT];
   __shared__ int nfew;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float* __restrict__ w = a.w + bh * a.wld;
@@ -804,20 +807,19 @@ __device__ __forceinline__ void select_rows(const EvictArgs& a, int bh, int len,
   uint32_t bound = 0xffffffffu;  // smallest kept key; `want` of the rows that have it are kept
   if (cand > 0 && want > 0) {
     uint32_t lo = 0xffffffffu, hi = 0;
-    each([&](uint32_t k) {
-      lo = min(lo, k - 1u);
-      hi = max(hi, k);
-    });
+    // the least and largest of the workgroup's keys, of which a thread has lo + 1 and hi
+    auto range = [&] {
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-      lo = min(lo, (uint32_t)__shfl_xor((int)lo, m, 64));
-      hi = max(hi, (uint32_t)__shfl_xor((int)hi, m, 64));
-    }
-    if (lane == 0) mins[wave] = lo, maxs[wave] = hi;
-    for (int i = tid; i < kBins; i += NT) bins[i] = 0;
-    __syncthreads();
-    for (int i = 0; i < W; ++i) lo = min(lo, mins[i]), hi = max(hi, maxs[i]);
-    lo = __builtin_amdgcn_readfirstlane(lo + 1), hi = __builtin_amdgcn_readfirstlane(hi);
+      for (int m = 32; m >= 1; m >>= 1) {
+        lo = min(lo, (uint32_t)__shfl_xor((int)lo, m, 64));
+        hi = max(hi, (uint32_t)__shfl_xor((int)hi, m, 64));
+      }
+      if (lane == 0) mins[wave] = lo, maxs[wave] = hi;
+      for (int i = tid; i < kBins; i += NT) bins[i] = 0;
+      __syncthreads();
+      for (int i = 0; i < W; ++i) lo = min(lo, mins[i]), hi = max(hi, maxs[i]);
+      lo = __builtin_amdgcn_readfirstlane(lo + 1), hi = __builtin_amdgcn_readfirstlane(hi);
+    };
     constexpr int PB = kBins / NT;
     const int top = kBins - 1 - PB * tid;
     // with the bins counted: this thread's, and those from the top down to them
@@ -838,18 +840,24 @@ __device__ __forceinline__ void select_rows(const EvictArgs& a, int bh, int len,
     auto clear = [&] {
       for (int i = tid; i < kBins; i += NT) bins[i] = 0;
     };
-    if (NT * 8 < cand && lo < hi) {
+    bool known = false;  // lo and hi hold the bound between them
+    int listed = -1;     // the keys between them are in the list, if not negative
+    if (NT * 8 < cand) {
       // 4 NT rows spread over all say between which keys the bound lies (three
-      // deviations of such a sample's median to either side); only the rows between
-      // them, if the count confirms it, go into the rounds below, whose atomics
-      // would else cost most of the time (lanes of a wave meet in few bins)
+      // deviations of such a sample's median to either side); if the count confirms it
+      // only the rows between them are looked at below, in a list where they fit
       constexpr int S = 4 * NT, MARGIN = 3 * 32;
       static_assert(S <= 4096, "the margin is three times half the root of 4096");
+      uint32_t some[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) some[i] = weight_key(w[(int64_t)(tid + NT * i) * cand / S]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lo = min(lo, some[i] - 1u), hi = max(hi, some[i]);
+      range();
       const int shift = max(0, 21 - __clz((int)(hi - lo)));
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        atomicAdd(&bins[(weight_key(w[(int64_t)(tid + NT * i) * cand / S]) - lo) >> shift], 1);
-      if (tid == 0) found[0] = lo, found[1] = hi;
+      for (int i = 0; i < 4; ++i) atomicAdd(&bins[(some[i] - lo) >> shift], 1);
+      if (tid == 0) found[0] = 1, found[1] = 0xffffffffu;
       __syncthreads();
       int n, upto;
       scan(n, upto);
@@ -867,21 +875,55 @@ __device__ __forceinline__ void select_rows(const EvictArgs& a, int bh, int len,
       __syncthreads();
       const uint32_t l = __builtin_amdgcn_readfirstlane(found[0]), h = __builtin_amdgcn_readfirstlane(found[1]);
       clear();
-      int gt = 0, ge = 0;
+      int gt = 0, in = 0;  // of the lane
       each([&](uint32_t k) {
-        gt += __popcll(__ballot(k > h));
-        ge += __popcll(__ballot(k >= l));
+        gt += k > h;
+        in += k - l <= h - l;
       });
-      if (lane == 0) gts[wave] = gt, ties[wave] = ge;
+      int upin = wave_scan(in, [](int x, int y) { return x + y; }), upgt = wave_scan(gt, [](int x, int y) { return x + y; });
+      if (lane == 63) gts[wave] = upgt, ties[wave] = upin;
       __syncthreads();
-      gt = ge = 0;
-      for (int i = 0; i < W; ++i) gt += gts[i], ge += ties[i];
-      gt = __builtin_amdgcn_readfirstlane(gt), ge = __builtin_amdgcn_readfirstlane(ge);
-      if (gt < want && want <= ge) lo = l, hi = h, want -= gt;
+      int all = 0, before = upin - in;
+      gt = 0;
+      for (int i = 0; i < W; ++i) {
+        gt += gts[i];
+        if (i == wave) before += all;
+        all += ties[i];
+      }
+      gt = __builtin_amdgcn_readfirstlane(gt), all = __builtin_amdgcn_readfirstlane(all);
+      if (gt < want && want <= gt + all) {
+        known = true;
+        lo = l, hi = h, want -= gt;
+        if (lo < hi && all <= 4 * NT) {
+          listed = all;
+          asm("" : "+s"(lo));  // compared again, as below
+          each([&](uint32_t k) {
+            if (k - lo <= h - lo) list[before++] = k;
+          });
+          __syncthreads();
+        }
+      } else {
+        lo = 0xffffffffu, hi = 0;
+        __syncthreads();  // mins and maxs may still be read
+      }
     }
+    if (!known) {
+      each([&](uint32_t k) {
+        lo = min(lo, k - 1u);
+        hi = max(hi, k);
+      });
+      range();
+    }
+    auto between = [&](auto f) {
+      if (listed >= 0) {
+        for (int i = tid; i < listed; i += NT) f(list[i]);
+      } else {
+        each(f);
+      }
+    };
     while (lo < hi) {
       const int shift = max(0, 21 - __clz((int)(hi - lo)));  // (hi - lo) >> shift < kBins
-      each([&](uint32_t k) {
+      between([&](uint32_t k) {
         if (k - lo <= hi - lo) atomicAdd(&bins[(k - lo) >> shift], 1);
       });
       if (tid == 0) nfew = 0;
@@ -908,7 +950,7 @@ __device__ __forceinline__ void select_rows(const EvictArgs& a, int bh, int len,
         __syncthreads();
         continue;
       }
-      each([&](uint32_t k) {
+      between([&](uint32_t k) {
         if (k - lo <= hi - lo) few[atomicAdd(&nfew, 1)] = k;
       });
       __syncthreads();
@@ -952,11 +994,17 @@ __device__ __forceinline__ void select_rows(const EvictArgs& a, int bh, int len,
   each([&](uint32_t k) {
     const bool isg = k > bound, ist = k == bound;
     const uint64_t bg = __ballot(isg), bt = __ballot(ist);
-    const int ga = __builtin_amdgcn_mbcnt_hi((uint32_t)(bg >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bg, g));
-    const int ta = __builtin_amdgcn_mbcnt_hi((uint32_t)(bt >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bt, t));
-    if (isg | (ist & (ta < want))) slots[ga + min(ta, want)] = j;
+    if (bt == 0) {  // mostly
+      const int at = g + min(t, want);
+      const int pos = __builtin_amdgcn_mbcnt_hi((uint32_t)(bg >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bg, at));
+      if (isg) slots[pos] = j;
+    } else {
+      const int ga = __builtin_amdgcn_mbcnt_hi((uint32_t)(bg >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bg, g));
+      const int ta = __builtin_amdgcn_mbcnt_hi((uint32_t)(bt >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bt, t));
+      if (isg | (ist & (ta < want))) slots[ga + min(ta, want)] = j;
+      t += __popcll(bt);
+    }
     g += __popcll(bg);
-    t += __popcll(bt);
     j += 64;
   });
   // and the recent ones, or all
@@ -1412,8 +1460,8 @@ extern "C" int mtx_kv_evict_paged(int cache_dtype, int B, int H, int D, int64_t 
   }
 #undef FUSED
   // else measured for 64 sequences and heads, us: 4000 rows 11.2 by 1024 threads, 9.2
-  // by 256; 32768 rows 19.6 held in registers, 35 read again each step; 49152 rows
-  // 27.6 and 40; with 64 rows a thread registers spill: 48
+  // by 256; 32768 rows 18 held in registers, 35 read again each step; 49152 rows
+  // 24 and 40; with 64 rows a thread registers spill: 48
 #define SELECT(NT, R, SINGLE) hipLaunchKernelGGL((select_kernel<NT, R, SINGLE>), grid, dim3(NT), 0, st, a)
   if (cap <= 256 * 4) SELECT(256, 4, true);
   else if (cap <= 256 * 16) SELECT(256, 16, true);

@@ -562,6 +562,10 @@ def test_evict_where_a_sample_misleads(dev, kind, n, keep):
     check_evict([n], keep, 7, Hkv=1, D=16, page=128, cache="bfloat16", seed=keep, weights=weights)
 
 
+def test_evict_more_rows_between_than_are_listed(dev):
+    check_evict([150000, 8000], 50000, 100, Hkv=1, D=16, page=64, cache="bfloat16", seed=15)
+
+
 @pytest.mark.parametrize("B, Hkv, D, n, keep", [
     (6, 8, 128, 700, 500),   # 1536 workgroups: one launch
     (6, 8, 128, 700, 513),   # 1584: two
