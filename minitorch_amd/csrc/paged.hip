@@ -1237,8 +1237,9 @@ int check_cache(int B, int H, int D, int64_t n_pages, int page, const int* table
 // enough for the GPU (B = 32, 4 K/V heads of 128, 1500 rows: 21 us, 23 to 25 in chunks;
 // 64 sequences of 100 to 3000 rows, 8 of 128: 85, 97).
 //
-// Else up to 128 sequences and heads: P pieces by the lengths (cut_rows), one for each
-// compute unit.  16 sequences of 8000 to 16384 rows, 8 heads: 143 us, in chunks of 1024
+// Else up to 128 sequences and K/V heads: P pieces by the lengths (cut_rows), one for each
+// compute unit, or for each HT workgroups' where there are many (30 sequences of 1000 to
+// 9000 rows, 3 K/V heads of 128, 96 query heads: 78 us, in chunks 101).  16 sequences of 8000 to 16384 rows, 8 heads: 143 us, in chunks of 1024
 // rows 157; one of 16384 and 15 of 300: 25, 57; 7 sequences of 9000, 2 heads, 21.7, 20.1.
 //
 // Else chunks alike, 512 to 1024 rows each, some 768 or more: they come to the compute
@@ -1253,13 +1254,15 @@ DecodePlan make_plan(int B, int H, int Hkv, int D, int page, int max_pages, bool
   const int cap = page * max_pages;
   DecodePlan p{};
   p.HT = cdiv(H / Hkv, 16);
-  const int64_t share = (int64_t)Hkv * p.HT, segments = B * share;
+  const int64_t segments = (int64_t)B * Hkv * p.HT;
   p.most = (int)(std::min<int64_t>((int64_t)(kMaxIds - 2) * page, 1 << 27) / 64);
   const int one = (segments >= 384 ? 4096 : 2048) / (D >= 64 ? 1 : 2);
   if (cap <= one && (segments >= 128 || cap * std::max(D, 64) <= 81920)) {
     p.chunk = cap;
-  } else if (segments <= 128 && cap <= (1 << 27)) {
-    p.P = (int)std::max<int64_t>(std::min<int64_t>(256 / share, (int64_t)B * cdiv(cap, 256)),
+  } else if (B * Hkv <= 128 && cap <= (1 << 27)) {
+    // the HT workgroups of a piece lie on one XCD: each of the 8 has place for 32 / HT
+    const int n = (segments <= 128 ? 8 * (32 / p.HT) : 256) / Hkv;
+    p.P = (int)std::max<int64_t>(std::min<int64_t>(n, (int64_t)B * cdiv(cap, 256)),
                                  (int64_t)B * cdiv(cap, 64 * p.most));
     p.chunk = cap;
   } else {

@@ -210,11 +210,13 @@ def test_decode_long_cache(dev, page, D):
     (64, 2, 32, 20, [3000, 1000, 2999]),
     (2048, 8, 16, 16, [2500]),
     (12, 12, 16, 32, [6000, 700]),
+    (48, 1, 64, 64, [9000, 3000]),
+    (96, 2, 16, 16, [2200 + 9 * i for i in range(40)]),
     (1, 1, 16, 16, [1 + 41 * i % 2500 for i in range(130)]),
     (9, 9, 16, 16, [8100 - 517 * i for i in range(15)]),
     (3, 3, 16, 16, [4096 - 30 * i for i in range(128)])],
     ids=["skewed", "empty_between", "equal", "twice", "128_sequences", "first_and_last", "pages_of_one", "head_tiles",
-         "many_head_tiles", "more_heads", "130_sequences", "chunks_of_8", "whole_of_4096"])
+         "many_head_tiles", "more_heads", "three_head_tiles", "80_of_three", "130_sequences", "chunks_of_8", "whole_of_4096"])
 @pytest.mark.parametrize("weights", [False, True])
 def test_decode_cuts(dev, H, Hkv, D, page, lengths, weights):
     """How sequences are shared out among workgroups: by the lengths of all, in
