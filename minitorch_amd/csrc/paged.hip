@@ -1260,8 +1260,10 @@ DecodePlan make_plan(int B, int H, int Hkv, int D, int page, int max_pages, bool
   if (cap <= one && (segments >= 128 || cap * std::max(D, 64) <= 81920)) {
     p.chunk = cap;
   } else if (B * Hkv <= 128 && cap <= (1 << 27)) {
-    // the HT workgroups of a piece lie on one XCD: each of the 8 has place for 32 / HT
-    const int n = (segments <= 128 ? 8 * (32 / p.HT) : 256) / Hkv;
+    // two a compute unit where a tile is small (32 sequences of 30000 rows, 4 heads of 32:
+    // 97 us, 124 with one; 5 of 43000, 8 heads of 16: 30, 43); the HT workgroups of a piece
+    // lie on one XCD: each of the 8 has place for 32 / HT
+    const int n = 8 * (D < 64 ? 2 : 1) * (segments <= 128 ? 32 / p.HT : 32) / Hkv;
     p.P = (int)std::max<int64_t>(std::min<int64_t>(n, (int64_t)B * cdiv(cap, 256)),
                                  (int64_t)B * cdiv(cap, 64 * p.most));
     p.chunk = cap;
