@@ -77,7 +77,10 @@ class PagedKVCache:
         self._len = np.zeros(batch, np.int32)
         self._tab = np.full((batch, self.width), -1, np.int32)
         self._free = list(range(self.n_pages - 1, -1, -1))
-        self._prompt = False  # the rows being appended are their sequences' first
+        # of the rows being appended
+        self._rows = 0  # how many, of the sequence that gets most
+        self._prompt = False  # whether they are their sequences' first
+        self._active = None  # the lengths, 0 where none is new, if that is anywhere
 
     # -- what it holds ---------------------------------------------------------
     def length(self, b: int) -> int:
@@ -91,8 +94,8 @@ class PagedKVCache:
     # -- growing and shrinking ---------------------------------------------------
     def reserve(self, n=1):
         """Make room for n new rows in every sequence (an int, or one per
-        sequence; 0 leaves it as it is): the rows that the layers' append then
-        write.  Nothing has changed when it raises."""
+        sequence; 0 leaves it as it is, its queries see nothing): the rows that
+        the layers' append then write.  Nothing has changed when it raises."""
         n = np.broadcast_to(np.asarray(n, np.int32), (self.batch,))
         if n.min() < 0 or n.max() < 1:
             raise ValueError("reserve: at least one new row, none negative")
@@ -114,12 +117,15 @@ class PagedKVCache:
         else:
             self.lengths.copy_(grown)
             self.counts = None if n.min() == n.max() else dev.from_host(n, np.int32).t
+        self._rows = int(n.max())
+        self._active = None if n.min() else dev.from_host(np.where(n > 0, grown, 0), np.int32).t
         self._len = grown
 
     def release(self, b: int):
         """Give back a sequence's pages; it is empty afterwards."""
         self._give_back(b, self._tab[b])
         self._len[b] = 0
+        self._active = None
         self.table.copy_(self._tab)
         self.lengths.copy_(self._len)
         if self.weights is not None:
@@ -151,20 +157,25 @@ class PagedKVCache:
         for b in range(self.batch):
             self._give_back(b, self._tab[b])
         self._tab[:, :to.shape[1]] = to
+        self._active = None
         self.table.copy_(self._tab)
         self._len = new
         return True
 
     # -- a layer's work ----------------------------------------------------------
     def append(self, layer, k, v):
-        """Write the rows reserved last: k and v (B, n_head, T, head_dim)."""
+        """Write the rows reserved last: k and v (B, n_head, T, head_dim), T the
+        most that a sequence gets."""
+        if k.shape[2] != self._rows:
+            raise ValueError(f"append: {k.shape[2]} rows, {self._rows} reserved")
         K.kv_append_paged(k, v, self.k[layer], self.v[layer], self.table, self.lengths, counts=self.counts)
 
     def attend(self, layer, q, scale, out=None):
         """Attention of one new token per sequence, q (B, H, 1, head_dim) with H
         a multiple of n_head, over the cached rows, whose weights it counts."""
         w = None if self.weights is None else self.weights[layer]
-        return K.attn_decode_paged(q, self.k[layer], self.v[layer], self.table, self.lengths, scale, out=out,
+        lengths = self.lengths if self._active is None else self._active
+        return K.attn_decode_paged(q, self.k[layer], self.v[layer], self.table, lengths, scale, out=out,
                                    weights=w, weights_in=w)[0]
 
     def observe(self, layer, q, scale):
@@ -172,6 +183,8 @@ class PagedKVCache:
         (B, H, T, head_dim), pay its rows (with keep)."""
         if self.weights is None:
             return
+        if self.counts is not None:
+            raise ValueError("observe: prompts of one length")
         T = q.shape[2]
         n = min(self.observed, T)
         if layer == 0:  # the rows that each of those positions sees

@@ -159,14 +159,16 @@ class MultiHeadAttention(Module):
         B, T, C = x.shape
         H, D = self.n_head, self.head_dim
         scale = 1.0 / math.sqrt(D)
+        if T > 1 and not cache._prompt:
+            raise ValueError("forward_paged takes one new token per sequence, or a prompt for empty sequences")
+        if T > 1 and cache.keep is not None and cache.counts is not None:
+            raise ValueError("forward_paged: a bounded cache takes prompts of one length")
         q, k, v = (p(x).data.t.view(B, T, H, D).transpose(1, 2) for p in (self.q_proj, self.k_proj, self.v_proj))
         cache.append(layer, k, v)
         out = dev.empty((B, T, H, D))
         if T == 1:
             cache.attend(layer, q, scale, out=out.t.transpose(1, 2))
         else:
-            if not cache._prompt:
-                raise ValueError("forward_paged takes one new token per sequence, or a prompt for empty sequences")
             K.attn_fwd(q, k, v, scale, True, out=out.t.transpose(1, 2))
             cache.observe(layer, q, scale)
         return self._project_residual(Tensor(out.reshape(B, T, C)), residual)

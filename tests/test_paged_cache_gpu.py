@@ -165,6 +165,58 @@ def test_cache_refusals(dev):
         m.generate(idx, 3, cache=used)
 
 
+def test_sequences_that_get_no_row_are_left_as_they_are(dev):
+    """A step of some sequences: the others' rows, weights and lengths stay, and
+    their queries see nothing."""
+    import minitorch_amd as mt
+    from minitorch_amd import device
+
+    rng = np.random.default_rng(21)
+    c = mt.PagedKVCache(1, 2, 32, 3, 64, page=8, keep=40, slack=4)
+
+    def rows(T):
+        return device.from_host(rng.standard_normal((3, 2, T, 32)), np.float32).t
+
+    c.reserve([3, 12, 0])
+    c.append(0, rows(12), rows(12))
+    first = c.attend(0, rows(1), 0.2).numpy()  # of the prompts: counts weights
+    assert np.abs(first[:2]).min() > 0 and not first[2].any()
+    weights = c.weights[0].numpy()
+    before = [p.numpy().view(np.uint32) for p in (c.k[0], c.v[0])]
+    c.reserve([1, 0, 1])
+    c.append(0, rows(1), rows(1))
+    out = c.attend(0, rows(1), 0.2).numpy()
+    assert not out[1].any() and np.abs(out[[0, 2]]).min() > 0
+    now = c.weights[0].numpy()
+    assert np.array_equal(now[1], weights[1]) and np.array_equal(c.lengths.numpy(), [4, 12, 1])
+    assert np.abs(now.sum((1, 2)) - weights.sum((1, 2)) - [2, 0, 2]).max() < 1e-5
+    for p, was in zip((c.k[0], c.v[0]), before):
+        assert (p.numpy().view(np.uint32) != was).any((2, 3)).sum() == 4  # a page and head each of two sequences
+    c.reserve(1)  # and all again
+    c.append(0, rows(1), rows(1))
+    assert np.abs(c.attend(0, rows(1), 0.2).numpy()).min() > 0
+
+
+def test_append_refuses_other_rows_than_reserved(dev):
+    import minitorch_amd as mt
+
+    c = mt.PagedKVCache(1, 2, 32, 2, 64, page=8)
+    k = mt.Tensor(np.zeros((2, 2, 3, 32), np.float32)).data.t
+    c.reserve([2, 1])
+    with pytest.raises(ValueError, match="reserved"):
+        c.append(0, k, k)
+    m = model(n_layer=1)
+    bounded = m.paged_cache(2, max_tokens=40, keep=20)
+    bounded.reserve([5, 4])
+    with mt.no_grad(), pytest.raises(ValueError, match="one length"):
+        m.blocks[0].forward_paged(mt.Tensor(np.zeros((2, 5, 64), np.float32)), bounded, 0)
+    c = m.paged_cache(2)
+    for _ in range(2):
+        c.reserve(3)
+    with mt.no_grad(), pytest.raises(ValueError, match="empty sequences"):
+        m.blocks[0].forward_paged(mt.Tensor(np.zeros((2, 3, 64), np.float32)), c, 0)
+
+
 # ---------------------------------------------------------------------------
 # training on log probabilities
 # ---------------------------------------------------------------------------
