@@ -259,10 +259,11 @@ __global__ __launch_bounds__(256) void logprobs_small_kernel(const LpArgs a, int
 // them in flight.  WHOLE: the row fits U loads a thread and stays in registers;
 // otherwise one pass with the running maximum and sums, and what is collected for
 // the alternatives is read again ----
-constexpr int kCap = 1024;  // candidates
 template <typename T, int NT, int U, bool WHOLE>
 __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
-  constexpr int E = Elem<T>::kVec, W = NT / 64, STEP = NT * E;
+  // kCap candidates: with 1024 LDS would leave half the place for single waves (16384 x
+  // 700 bf16 20.3 us, 24.7)
+  constexpr int E = Elem<T>::kVec, W = NT / 64, STEP = NT * E, kCap = NT == 64 ? 256 : 1024;
   __shared__ uint64_t cands[kCap];
   __shared__ float sorted[W][64], red[3][W];
   __shared__ int count;
@@ -278,22 +279,29 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
     l *= f;
     m = n;
   };
+  // whether the wave has values in round u of a whole row
+  const int first = __builtin_amdgcn_readfirstlane(wave) * 64 * E;
+  auto some = [&](int u) { return !WHOLE || first + u * STEP < a.V; };
   auto largest = [&] {
-    float top = v[0][0];
+    float top = WHOLE ? -INFINITY : v[0][0];
 #pragma unroll
     for (int u = 0; u < U; ++u)
+      if (some(u)) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) top = fmaxf(top, v[u][e]);
+        for (int e = 0; e < E; ++e) top = fmaxf(top, v[u][e]);
+      }
     return top;
   };
   auto add = [&] {
 #pragma unroll
     for (int u = 0; u < U; ++u)
+      if (some(u)) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float d = below(v[u][e] - m), p = __builtin_amdgcn_exp2f(d * c);
-        l += p;
-        t = fmaf(p, d, t);
+        for (int e = 0; e < E; ++e) {
+          const float d = below(v[u][e] - m), p = __builtin_amdgcn_exp2f(d * c);
+          l += p;
+          t = fmaf(p, d, t);
+        }
       }
   };
   int i = tid * E;
@@ -307,7 +315,8 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   }
   if (WHOLE || i < a.V) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_left<E>(x + i + u * STEP, a.V - i - u * STEP, v[u]);
+    for (int u = 0; u < U; ++u)
+      if (some(u)) load_left<E>(x + i + u * STEP, a.V - i - u * STEP, v[u]);
     if (WHOLE) {
       m = fmaxf(m, largest());
     } else {
@@ -376,7 +385,8 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   if (WHOLE) {
     if (look) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) collect(v[u], i + u * STEP);
+      for (int u = 0; u < U; ++u)
+        if (some(u)) collect(v[u], i + u * STEP);
     }
   } else {
     // a thread's values are read again by lanes of its wave, a load each, and where
@@ -524,8 +534,8 @@ template <typename T>
 int launch_logprobs(const LpArgs& a, int64_t rows, hipStream_t st) {
   constexpr int E = Elem<T>::kVec;
   // measured with 10 alternatives, us: 16384 x 65 (5 alternatives) 5.5 by 16 lanes a
-  // row, 12.3 by 64; 16384 x 1500 fp32 28 whole in a wave, 43 in one pass, 60 by 256
-  // threads; 8192 x 3000 fp32 30 whole in 256 threads, 35 in one pass; 4096 x 9000 33
+  // row, 12.3 by 64; 16384 x 1500 fp32 26 whole in a wave, 43 in one pass, 60 by 256
+  // threads; 8192 x 3000 fp32 29 whole in 256 threads, 35 in one pass; 4096 x 9000 32
   // by 256 threads, 39 by 512, 64 by 1024; 2048 x 50021 fp32 88 by 256, 79 by 512;
   // 8 x 50021 bf16 11.4 by 256, 9.1 by 512, 10.6 by 1024
 #define SMALL(LPR, VPL)                                                                                        \
