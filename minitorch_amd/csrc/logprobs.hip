@@ -270,7 +270,12 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   __shared__ uint64_t bests[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
-  const T* __restrict__ x = static_cast<const T*>(a.x) + r * a.ld;
+  const T* __restrict__ row = static_cast<const T*>(a.x) + r * a.ld;
+  // loads at odd bf16 addresses are slower than at even ones (2048 x 50021: 54 us, 47): the
+  // first value of such a row is thread 0's
+  const int odd = !WHOLE && sizeof(T) == 2 ? (int)((uintptr_t)row >> 1 & 1) : 0, V = a.V - odd;
+  const T* __restrict__ x = row + odd;
+  const float head = odd && tid == 0 ? Elem<T>::to_f(*row) : -INFINITY;
   const float c = a.scale * kLog2e;
   float v[U][E], m = -FLT_MAX, l = 0.f, t = 0.f;
   auto raise = [&](float top) {  // the sums relative to a larger maximum
@@ -281,7 +286,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   };
   // whether the wave has values in round u of a whole row
   const int first = __builtin_amdgcn_readfirstlane(wave) * 64 * E;
-  auto some = [&](int u) { return !WHOLE || first + u * STEP < a.V; };
+  auto some = [&](int u) { return !WHOLE || first + u * STEP < V; };
   auto largest = [&] {
     float top = WHOLE ? -INFINITY : v[0][0];
 #pragma unroll
@@ -306,23 +311,29 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   };
   int i = tid * E;
   if (!WHOLE) {
-    for (; i + (U - 1) * STEP + E <= a.V; i += U * STEP) {
+    for (; i + (U - 1) * STEP + E <= V; i += U * STEP) {
 #pragma unroll
       for (int u = 0; u < U; ++u) load_values<E>(x + i + u * STEP, v[u]);
       raise(largest());
       add();
     }
   }
-  if (WHOLE || i < a.V) {
+  if (WHOLE || i < V) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (some(u)) load_left<E>(x + i + u * STEP, a.V - i - u * STEP, v[u]);
+      if (some(u)) load_left<E>(x + i + u * STEP, V - i - u * STEP, v[u]);
     if (WHOLE) {
       m = fmaxf(m, largest());
     } else {
       raise(largest());
       add();
     }
+  }
+  if (odd && tid == 0) {
+    raise(head);
+    const float d = below(head - m), p = __builtin_amdgcn_exp2f(d * c);
+    l += p;
+    t = fmaf(p, d, t);
   }
   const float mine = m;  // the thread's largest value
   if (WHOLE) {
@@ -365,7 +376,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
       t += __shfl_xor(t, s, 64);
     }
   }
-  if (tid == 0) row_result(a, r, x, m, l, t);
+  if (tid == 0) row_result(a, r, row, m, l, t);
   if (a.top == 0) return;
 #pragma unroll
   for (int s = 1; s < W; s <<= 1) {
@@ -376,9 +387,9 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   auto collect = [&](const float (&w)[E], int at) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (w[e] >= bound && at + e < a.V) {
+      if (w[e] >= bound && at + e < V) {
         const int k = atomicAdd(&count, 1);
-        if (k < kCap) cands[k] = rank_key(w[e], at + e);
+        if (k < kCap) cands[k] = rank_key(w[e], at + e + odd);
       }
   };
   const bool look = l == l && mine >= bound;
@@ -393,17 +404,21 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
     // they are few those of several threads at once (8 x 20000 bf16 7.6 us, one thread
     // at a time 9.3)
     int per = 64;
-    while (per > 8 && (per / 2) * STEP >= a.V) per /= 2;
+    while (per > 8 && (per / 2) * STEP >= V) per /= 2;
     for (uint64_t mask = __ballot(look); mask;) {
       int from = -1;
       for (int k = 0; k < 64 && mask; k += per, mask &= mask - 1)
         if (lane >= k && lane < k + per) from = __ffsll((unsigned long long)mask) - 1;
       if (from < 0) continue;
-      for (int j = (wave * 64 + from) * E + (lane & (per - 1)) * STEP; j < a.V; j += per * STEP) {
+      for (int j = (wave * 64 + from) * E + (lane & (per - 1)) * STEP; j < V; j += per * STEP) {
         float w[E];
-        load_left<E>(x + j, a.V - j, w);
+        load_left<E>(x + j, V - j, w);
         collect(w, j);
       }
+    }
+    if (odd && tid == 0 && look && head >= bound) {
+      const int k = atomicAdd(&count, 1);
+      if (k < kCap) cands[k] = rank_key(head, 0);
     }
   }
   __syncthreads();
@@ -421,7 +436,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
   for (int k = 0; k < a.top; ++k) {
     uint64_t best = 0;
     for (int j = tid; j < a.V; j += NT) {
-      const uint64_t key = rank_key(Elem<T>::to_f(x[j]), j);
+      const uint64_t key = rank_key(Elem<T>::to_f(row[j]), j);
       if ((key < last || k == 0) && key > best) best = key;
     }
 #pragma unroll
@@ -435,7 +450,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
     last = bests[0];
 #pragma unroll
     for (int w = 1; w < W; ++w) last = bests[w] > last ? bests[w] : last;
-    if (tid == 0) put_top(a, r, k, last, Elem<T>::to_f(x[(int)~(uint32_t)last]), m, l);
+    if (tid == 0) put_top(a, r, k, last, Elem<T>::to_f(row[(int)~(uint32_t)last]), m, l);
   }
 }
 
