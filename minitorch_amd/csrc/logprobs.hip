@@ -5,9 +5,10 @@
 // entropy = -sum p log p.  With e = exp(x - max), l = sum e it is computed as
 // log l + (sum e (max - x)) / l: both terms are >= 0, so nothing cancels where
 // the distribution is nearly certain.  All sums are fp32.  Long rows are bound by
-// the memory (fp32) or by some eleven instructions a value (bf16: 3.7 to 4.7 TB/s),
-// short ones by the reductions and the ranking of a row's candidates.  The reference has log_softmax
-// (functional.py:81-97) and samples from softmax (transformer.py:93-104).
+// the memory (fp32: 5.2 to 6 TB/s; bf16, with ten instructions a value beside the
+// loads, 4.2 to 4.7), short ones by the reductions and the ranking of a row's
+// candidates.  The reference has log_softmax (functional.py:81-97)
+// and samples from softmax (transformer.py:93-104).
 #include "mtx_common.h"
 
 #include <algorithm>
