@@ -131,9 +131,8 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
 // exponent (probabilities stay below 2^8, the sums in fp32), which in practice
 // happens in a wave's first tile.
 //
-// fp32 pools use fp32 matrix instructions.  Over bf16 pools the weights enter the
-// products as two bf16 pieces (16 bits; the output is rounded to 8) for bf16 rows,
-// and q and the weights as three (24 bits) for fp32 rows.
+// fp32 pools use fp32 matrix instructions.  Over bf16 pools the weights, and fp32 rows'
+// q, enter the products as three bf16 pieces (24 bits, as fp32 has).
 //
 // Measured, 16 sequences of 8000 to 16384 rows, 8 K/V heads of 128 in bf16 (797
 // MB), 32 query heads: 139 us, 5.7 TB/s (a plain read of the same pages: 136 us); one of
@@ -176,7 +175,7 @@ template <typename TQ, typename TC, int D> struct DecodeTile;
 template <typename TQ, int D>
 struct DecodeTile<TQ, bf16_t, D> {
   static constexpr int NT = 2, VD = D / 16, NC = D >= 32 ? D / 32 : 1, VW = VD >= 2 ? VD / 2 : 1;
-  static constexpr int QP = sizeof(TQ) == 4 ? 3 : 1, PP = sizeof(TQ) == 4 ? 3 : 2;
+  static constexpr int QP = sizeof(TQ) == 4 ? 3 : 1, PP = 3;
   bf16x8 q[QP][NC];
   uint4 k[NT][NC];
   uint32_t v[4 * NT][VW];

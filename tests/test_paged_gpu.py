@@ -690,3 +690,40 @@ def test_recorded_step_follows_device_state(dev):
             relw = rel.reshape(B, -1, G).max(-1)[..., None]
             assert np.all(np.abs(got - r[2]) <= relw * r[2] + (G + 3) * U * (before + r[2])), i
             assert np.array_equal(host_pool(s["dk"]), s["kp"])
+
+
+@pytest.mark.parametrize("q", ["float32", "bfloat16"])
+@pytest.mark.parametrize("B,width", [(64, 1), (3, 300)])
+def test_decode_weights_keep_fp32s_bits(dev, q, B, width):
+    """Values that cancel show the weights' own precision behind bf16 outputs:
+    three rows, the first of score 0 and value 0, the others' scores 2^-12 apart
+    and their values each other's negatives, so that o is some 2^-12 of sum p|v|.
+    The scores are exact in fp32.  A weight is then off by 3 u |s| (the scale's
+    two roundings and the product's; |s| <= 1.5), 2 u (the exponential) and u (its
+    pieces), the sums and the quotient by 8 u: below 16 u, or 2^-20, of sum p|v|
+    in all, and a bf16 output by half a step 2^-8 of itself besides.  Two bf16
+    pieces of a weight would be off by up to 2^-16 of it."""
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(B)
+    H, D, page = 16, 16, 16
+    a = bf16_round(rng.uniform(0.5, 1, (B, H)).astype(np.float32))
+    b = bf16_round(rng.uniform(0.25, 1.5, B).astype(np.float32))
+    v = bf16_round(rng.uniform(1, 2, (B, D)).astype(np.float32))
+    qs = np.zeros((B, H, 1, D), np.float32)
+    qs[:, :, 0, 0], qs[:, :, 0, 1] = a, 2.0 ** -6
+    kp, vp = (np.zeros((B, 1, page, D), np.float32) for _ in range(2))
+    kp[:, 0, 1:3, 0] = -b[:, None]
+    kp[:, 0, 2, 1] = -2.0 ** -6
+    vp[:, 0, 1], vp[:, 0, 2] = v, -v
+    table = np.full((B, width), -1, np.int32)
+    table[:, 0] = rng.permutation(B)
+    kp[table[:, 0]], vp[table[:, 0]] = kp.copy(), vp.copy()
+    lens = np.full(B, 3, np.int32)
+    o, _ = K.attn_decode_paged(dev_array(qs, q), dev_array(kp, "bfloat16"), dev_array(vp, "bfloat16"),
+                               dev_array(table, "int32"), dev_array(lens, "int32"), 1.0)
+    want, _, _, _, pv = ref.decode(qs, kp, vp, table[:, :1], lens, 1.0)
+    assert np.abs(want).max() < 2.0 ** -10 * pv.max()
+    bound = 2.0 ** -20 * pv + (2.0 ** -8 if q == "bfloat16" else 0) * np.abs(want)
+    off = np.abs(host(o) - want) / bound
+    assert off.max() <= 1, float(off.max())
