@@ -81,6 +81,8 @@ class PagedKVCache:
         self._rows = 0  # how many, of the sequence that gets most
         self._prompt = False  # whether they are their sequences' first
         self._active = None  # the lengths, 0 where none is new, if that is anywhere
+        self._new = np.zeros(batch, np.int32)  # how many of each sequence undo can take back
+        self._written = set()  # the layers that have them
 
     # -- what it holds ---------------------------------------------------------
     def length(self, b: int) -> int:
@@ -95,7 +97,10 @@ class PagedKVCache:
     def reserve(self, n=1):
         """Make room for n new rows in every sequence (an int, or one per
         sequence; 0 leaves it as it is, its queries see nothing): the rows that
-        the layers' append then write.  Nothing has changed when it raises."""
+        the layers' append then write.  Nothing has changed when it raises.  The
+        sequences count the rows from here on: a step that is not carried out
+        takes them back with undo; append and forward_paged do so before they
+        raise, unless all layers have the rows."""
         n = np.broadcast_to(np.asarray(n, np.int32), (self.batch,))
         if n.min() < 0 or n.max() < 1:
             raise ValueError("reserve: at least one new row, none negative")
@@ -119,12 +124,42 @@ class PagedKVCache:
             self.counts = None if n.min() == n.max() else dev.from_host(n, np.int32).t
         self._rows = int(n.max())
         self._active = None if n.min() else dev.from_host(np.where(n > 0, grown, 0), np.int32).t
-        self._len = grown
+        self._len, self._new = grown, n.copy()
+        self._written.clear()
+
+    def undo(self):
+        """Take back the rows reserved last, in all layers: lengths, table and
+        free pages are what they were, the rows' weights 0.  (What a layer's
+        attend has added to other rows' weights stays.)  Nothing happens if there
+        are none, or trim has cut the sequences since."""
+        if not self._new.any():
+            return
+        grown, self._len = self._len, self._len - self._new
+        for b in np.flatnonzero(self._new)[::-1]:
+            for i in range(-(-grown[b] // self.page) - 1, -(-self._len[b] // self.page) - 1, -1):
+                self._free.append(int(self._tab[b, i]))
+                self._tab[b, i] = -1
+            for w in self.weights or ():
+                w[b, :, int(self._len[b]):int(grown[b])].fill_(0.0)
+        self._settle()
+        self._rows, self._prompt, self.counts = 0, False, None
+        self.table.copy_(self._tab)
+        self.lengths.copy_(self._len)
+
+    def _abandon(self):
+        """What a layer does before it raises: a step that has not come through
+        all layers leaves no rows."""
+        if len(self._written) < self.n_layer:
+            self.undo()
+
+    def _settle(self):
+        self._active = None
+        self._new = np.zeros(self.batch, np.int32)
 
     def release(self, b: int):
         """Give back a sequence's pages; it is empty afterwards."""
         self._give_back(b, self._tab[b])
-        self._len[b] = 0
+        self._len[b] = self._new[b] = 0
         self._active = None
         self.table.copy_(self._tab)
         self.lengths.copy_(self._len)
@@ -157,7 +192,7 @@ class PagedKVCache:
         for b in range(self.batch):
             self._give_back(b, self._tab[b])
         self._tab[:, :to.shape[1]] = to
-        self._active = None
+        self._settle()
         self.table.copy_(self._tab)
         self._len = new
         return True
@@ -166,9 +201,14 @@ class PagedKVCache:
     def append(self, layer, k, v):
         """Write the rows reserved last: k and v (B, n_head, T, head_dim), T the
         most that a sequence gets."""
-        if k.shape[2] != self._rows:
-            raise ValueError(f"append: {k.shape[2]} rows, {self._rows} reserved")
-        K.kv_append_paged(k, v, self.k[layer], self.v[layer], self.table, self.lengths, counts=self.counts)
+        try:
+            if k.shape[2] != self._rows:
+                raise ValueError(f"append: {k.shape[2]} rows, {self._rows} reserved")
+            K.kv_append_paged(k, v, self.k[layer], self.v[layer], self.table, self.lengths, counts=self.counts)
+        except BaseException:
+            self._abandon()
+            raise
+        self._written.add(layer)
 
     def attend(self, layer, q, scale, out=None):
         """Attention of one new token per sequence, q (B, H, 1, head_dim) with H

@@ -153,7 +153,15 @@ class MultiHeadAttention(Module):
         """Inference-only attention of x (B, T, C) whose keys and values go to
         the rows that `cache` (a PagedKVCache) reserved last: T = 1 new token per
         sequence over everything cached, or a whole prompt (the sequences' first
-        rows).  With `residual` the result is residual + attention(x)."""
+        rows).  With `residual` the result is residual + attention(x).  If it
+        raises, the rows are taken back (PagedKVCache.reserve)."""
+        try:
+            return self._forward_paged(x, cache, layer, residual)
+        except BaseException:
+            cache._abandon()
+            raise
+
+    def _forward_paged(self, x, cache, layer, residual):
         from . import kernels as K
 
         B, T, C = x.shape
@@ -770,9 +778,13 @@ class GPT(Module):
             def paged(tokens, t):  # logits after tokens (B, T) at positions t on
                 T = tokens.shape[1]
                 cache.reserve(T)
-                x = self.tok_emb(dev.index_array(tokens)) + self.pos_emb(DeviceArray(pos.t[t:t + T]))
-                for i, block in enumerate(self.blocks):
-                    x = block.forward_paged(x, cache, i)
+                try:
+                    x = self.tok_emb(dev.index_array(tokens)) + self.pos_emb(DeviceArray(pos.t[t:t + T]))
+                    for i, block in enumerate(self.blocks):
+                        x = block.forward_paged(x, cache, i)
+                except BaseException:
+                    cache.undo()
+                    raise
                 cache.trim()
                 return last_logits(x)
 

@@ -325,3 +325,149 @@ def test_recorded_training_step_on_logprobs(dev):
     eager, recorded = run(False), run(True)
     assert eager[0] == recorded[0]
     assert all(np.array_equal(a, b) for a, b in zip(eager[1], recorded[1]))
+
+
+# ---------------------------------------------------------------------------
+# steps that are refused or fail, and pools that are just large enough
+# ---------------------------------------------------------------------------
+
+
+def run_paged(m, cache, tokens, first):
+    """Logits (B, T, V) of tokens (B, T) at positions first[b] on, whose rows
+    the cache has reserved."""
+    import minitorch_amd as mt
+    from minitorch_amd import device
+
+    tokens = np.asarray(tokens)
+    pos = np.asarray(first)[:, None] + np.arange(tokens.shape[1])
+    with mt.no_grad():
+        x = m.tok_emb(device.index_array(tokens)) + m.pos_emb(device.index_array(pos))
+        for i, block in enumerate(m.blocks):
+            x = block.forward_paged(x, cache, i)
+        return m.lm_head(m.ln_f(x)).data.numpy()
+
+
+def state(c):
+    """What a cache holds, as far as its calls can tell."""
+    return dict(lengths=c.lengths.numpy().tolist(), host=[c.length(b) for b in range(c.batch)],
+                table=c.table.numpy().tolist(), pages=c._tab.tolist(), free=list(c._free))
+
+
+@pytest.mark.parametrize("keep", [None, 20])
+def test_rows_of_a_refused_step_are_taken_back(dev, keep):
+    """A step that is refused after its rows were reserved leaves the cache as
+    it was before; the next step's logits are those of a cache that never saw it,
+    bit for bit."""
+    import minitorch_amd as mt
+
+    m = model()
+    rng = np.random.default_rng(31)
+    prompt, step = rng.integers(0, 50, (2, 7)), rng.integers(0, 50, (2, 1))
+    caches = [m.paged_cache(2, page=4, max_tokens=40, keep=keep) for _ in range(2)]
+    for c in caches:
+        c.reserve(7)
+        run_paged(m, c, prompt, [0, 0])
+    c = caches[0]
+    before = state(c)
+
+    def refused(n, T, match):
+        c.reserve(n)
+        assert state(c) != before
+        with pytest.raises(ValueError, match=match):
+            run_paged(m, c, rng.integers(0, 50, (2, T)), [7, 7])
+        assert state(c) == before
+
+    refused(3, 3, "empty sequences")
+    refused([2, 0], 2, "empty sequences")
+    refused(1, 3, "one new token|reserved")
+    refused([1, 3], 1, "reserved")
+    c.reserve([0, 6])  # rows of a wrong head size, refused by the kernel's wrapper
+    k = mt.Tensor(np.zeros((2, 2, 6, 16), np.float32)).data.t
+    with pytest.raises(ValueError):
+        c.append(0, k, k)
+    assert state(c) == before
+    c.reserve([5, 1])
+    c.undo()
+    c.undo()  # there is nothing more to take back
+    assert state(c) == before
+    out = []
+    for c in caches:
+        c.reserve(1)
+        out.append(run_paged(m, c, step, [7, 7]))
+    assert np.array_equal(*out) and np.isfinite(out[0]).all()
+    if keep:
+        for i in range(2):
+            assert np.array_equal(caches[0].weights[i].numpy(), caches[1].weights[i].numpy())
+    # a call that reserved nothing takes nothing of the step before it
+    before = state(c)
+    for T in (2, 3):
+        with pytest.raises(ValueError, match="one new token"):
+            run_paged(m, c, rng.integers(0, 50, (2, T)), [8, 8])
+    with pytest.raises(ValueError, match="reserved"):
+        c.append(1, k, k)
+    assert state(c) == before and c.length(0) == 8
+
+
+def test_a_refused_prompt_leaves_an_empty_cache(dev):
+    m = model()
+    c = m.paged_cache(2, max_tokens=40, keep=20)
+    before = state(c)
+    c.reserve([5, 4])
+    with pytest.raises(ValueError, match="one length"):
+        run_paged(m, c, np.zeros((2, 5), np.int64), [0, 0])
+    assert state(c) == before
+    idx = np.random.default_rng(32).integers(0, 50, (2, 6))
+    np.random.seed(2)
+    want = m.generate(idx, 8)
+    np.random.seed(2)
+    assert np.array_equal(m.generate(idx, 8, cache=c), want)
+
+
+def test_undo_clears_the_rows_weights(dev):
+    """Weights that a step counted for rows that are then taken back."""
+    import minitorch_amd as mt
+    from minitorch_amd import device
+
+    rng = np.random.default_rng(33)
+    rows = lambda T: device.from_host(rng.standard_normal((2, 2, T, 32)), np.float32).t
+    c = mt.PagedKVCache(2, 2, 32, 2, 64, page=8, keep=40, slack=4)
+    c.reserve([3, 12])
+    for i in range(2):
+        c.append(i, rows(12), rows(12))
+        c.attend(i, rows(1), 0.2)
+    c.reserve([2, 1])
+    for i in range(2):
+        c.append(i, rows(2), rows(2))
+        c.attend(i, rows(1), 0.2)
+        assert (c.weights[i].numpy()[0, :, 3:5] > 0).all() and (c.weights[i].numpy()[1, :, 12] > 0).all()
+    c.undo()
+    assert [c.length(b) for b in range(2)] == [3, 12]
+    for i in range(2):
+        w = c.weights[i].numpy()
+        assert not w[0, :, 3:].any() and not w[1, :, 12:].any()
+        assert (w[0, :, :3] > 0).all() and (w[1, :, :12] > 0).all()
+    c.reserve(1)
+    c.release(0)  # gives its row back by itself
+    c.undo()
+    assert [c.length(b) for b in range(2)] == [0, 12] and c.lengths.numpy().tolist() == [0, 12]
+    assert sorted(c._free + [i for i in c._tab.ravel() if i >= 0]) == list(range(c.n_pages))
+
+
+def test_a_generation_that_fails_leaves_written_rows_alone(dev, monkeypatch):
+    """A failure in a layer of the fourth step: its rows are taken back."""
+    m = model()
+    c = m.paged_cache(2, page=4)
+    idx = np.random.default_rng(44).integers(0, 50, (2, 6))
+    work, calls = m.blocks[1].forward_paged, []
+
+    def fails(x, cache, layer):
+        calls.append(1)
+        if len(calls) == 4:
+            raise MemoryError("planted")
+        return work(x, cache, layer)
+
+    monkeypatch.setattr(m.blocks[1], "forward_paged", fails)
+    with pytest.raises(MemoryError):
+        m.generate(idx, 10, cache=c)
+    assert [c.length(b) for b in range(2)] == [8, 8] and c.lengths.numpy().tolist() == [8, 8]
+    assert c.free_pages == c.n_pages - 4
