@@ -101,12 +101,14 @@ class PagedKVCache:
         sequences count the rows from here on: a step that is not carried out
         takes them back with undo; append and forward_paged do so before they
         raise, unless all layers have the rows."""
-        n = np.broadcast_to(np.asarray(n, np.int32), (self.batch,))
+        n, most = np.broadcast_to(np.asarray(n, np.int64), (self.batch,)), self.width * self.page
         if n.min() < 0 or n.max() < 1:
             raise ValueError("reserve: at least one new row, none negative")
+        if (n > most - self._len).any():
+            rows = max(int(x) + int(y) for x, y in zip(self._len, n))
+            raise ValueError(f"reserve: {rows} rows exceed the {most} a sequence may hold")
+        n = n.astype(np.int32)
         grown = self._len + n
-        if grown.max() > self.width * self.page:
-            raise ValueError(f"reserve: {int(grown.max())} rows exceed the {self.width * self.page} a sequence may hold")
         have, need = -(-self._len // self.page), -(-grown // self.page)
         if (need - have).sum() > len(self._free):
             raise RuntimeError(f"reserve: {int((need - have).sum())} pages needed, {len(self._free)} free")
@@ -124,7 +126,7 @@ class PagedKVCache:
             self.counts = None if n.min() == n.max() else dev.from_host(n, np.int32).t
         self._rows = int(n.max())
         self._active = None if n.min() else dev.from_host(np.where(n > 0, grown, 0), np.int32).t
-        self._len, self._new = grown, n.copy()
+        self._len, self._new = grown, n
         self._written.clear()
 
     def undo(self):

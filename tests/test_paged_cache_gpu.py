@@ -471,3 +471,16 @@ def test_a_generation_that_fails_leaves_written_rows_alone(dev, monkeypatch):
         m.generate(idx, 10, cache=c)
     assert [c.length(b) for b in range(2)] == [8, 8] and c.lengths.numpy().tolist() == [8, 8]
     assert c.free_pages == c.n_pages - 4
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 62, 2 ** 63 - 1])
+def test_reserve_refuses_more_rows_than_an_int_holds(dev, n):
+    import minitorch_amd as mt
+
+    c = mt.PagedKVCache(1, 2, 32, 2, 64, page=8)
+    c.reserve([3, 5])
+    before = state(c)
+    for rows in (n, [n, 1], [1, n], np.array([n, n])):
+        with pytest.raises(ValueError, match="exceed"):
+            c.reserve(rows)
+        assert state(c) == before
