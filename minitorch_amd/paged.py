@@ -80,6 +80,7 @@ class PagedKVCache:
         # of the rows being appended
         self._rows = 0  # how many, of the sequence that gets most
         self._prompt = False  # whether they are their sequences' first
+        self._ragged = False  # whether sequences that get some get different numbers
         self._active = None  # the lengths, 0 where none is new, if that is anywhere
         self._new = np.zeros(batch, np.int32)  # how many of each sequence undo can take back
         self._written = set()  # the layers that have them
@@ -117,7 +118,8 @@ class PagedKVCache:
                 self._tab[b, i] = self._free.pop()
         if (need > have).any():
             self.table.copy_(self._tab)
-        self._prompt = not self._len.any()
+        self._prompt = not self._len[n > 0].any()
+        self._ragged = n[n > 0].min() != n.max()
         if n.min() == n.max() == 1:
             K.decode_advance(self.lengths)
             self.counts = None
@@ -222,16 +224,18 @@ class PagedKVCache:
 
     def observe(self, layer, q, scale):
         """Count the attention that a prompt's last positions, q
-        (B, H, T, head_dim), pay its rows (with keep)."""
+        (B, H, T, head_dim), pay its rows (with keep), in the sequences that got
+        rows last."""
         if self.weights is None:
             return
-        if self.counts is not None:
+        if self._ragged:
             raise ValueError("observe: prompts of one length")
         T = q.shape[2]
         n = min(self.observed, T)
         if layer == 0:  # the rows that each of those positions sees
             back = np.arange(n - 1, -1, -1, dtype=np.int32)[:, None]
-            self._seen = dev.from_host(np.maximum(self._len - back, 0), np.int32).t
+            lengths = np.where(self._new > 0, self._len, 0)
+            self._seen = dev.from_host(np.maximum(lengths - back, 0), np.int32).t
         w = self.weights[layer]
         for i in range(n):
             t = T - n + i

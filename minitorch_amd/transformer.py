@@ -152,9 +152,10 @@ class MultiHeadAttention(Module):
     def forward_paged(self, x, cache, layer, residual=None):
         """Inference-only attention of x (B, T, C) whose keys and values go to
         the rows that `cache` (a PagedKVCache) reserved last: T = 1 new token per
-        sequence over everything cached, or a whole prompt (the sequences' first
-        rows).  With `residual` the result is residual + attention(x).  If it
-        raises, the rows are taken back (PagedKVCache.reserve)."""
+        sequence over everything cached, or whole prompts, the first rows of the
+        sequences that get any (what comes out for the others means nothing).
+        With `residual` the result is residual + attention(x).  If it raises, the
+        rows are taken back (PagedKVCache.reserve)."""
         try:
             return self._forward_paged(x, cache, layer, residual)
         except BaseException:
@@ -169,7 +170,7 @@ class MultiHeadAttention(Module):
         scale = 1.0 / math.sqrt(D)
         if T > 1 and not cache._prompt:
             raise ValueError("forward_paged takes one new token per sequence, or a prompt for empty sequences")
-        if T > 1 and cache.keep is not None and cache.counts is not None:
+        if T > 1 and cache.keep is not None and cache._ragged:
             raise ValueError("forward_paged: a bounded cache takes prompts of one length")
         q, k, v = (p(x).data.t.view(B, T, H, D).transpose(1, 2) for p in (self.q_proj, self.k_proj, self.v_proj))
         cache.append(layer, k, v)

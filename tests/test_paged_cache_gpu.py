@@ -484,3 +484,52 @@ def test_reserve_refuses_more_rows_than_an_int_holds(dev, n):
         with pytest.raises(ValueError, match="exceed"):
             c.reserve(rows)
         assert state(c) == before
+
+
+@pytest.mark.parametrize("keep", [None, 30])
+def test_prompt_into_a_released_slot(dev, keep):
+    """A sequence that ended gives its slot to a new prompt while the others
+    hold theirs: its logits, and theirs from then on, against the whole model's
+    over each sequence."""
+    m = model()
+    rng = np.random.default_rng(34)
+    c = m.paged_cache(3, page=4, max_tokens=48, keep=keep, observe=4)
+    held = [list(rng.integers(0, 50, 9)) for _ in range(3)]
+    c.reserve(9)
+    run_paged(m, c, held, [0, 0, 0])
+
+    def steps(n):
+        for _ in range(n):
+            new = rng.integers(0, 50, (3, 1))
+            at = [len(x) for x in held]
+            for x, t in zip(held, new[:, 0]):
+                x.append(t)
+            c.reserve(1)
+            got = run_paged(m, c, new, at)
+            for b, x in enumerate(held):
+                want = m(np.array([x])).data.numpy()[0, -1]
+                assert np.abs(got[b, 0] - want).max() <= 1e-4, b
+
+    steps(2)
+    c.release(1)
+    held[1] = list(rng.integers(0, 50, 6))
+    if keep:
+        weights = [w.numpy() for w in c.weights]
+    c.reserve([0, 6, 0])
+    tokens = rng.integers(0, 50, (3, 6))  # the others' rows are nobody's
+    tokens[1] = held[1]
+    got = run_paged(m, c, tokens, [0, 0, 0])[1]
+    assert np.abs(got - m(np.array([held[1]])).data.numpy()[0]).max() <= 1e-4
+    assert [c.length(b) for b in range(3)] == [11, 6, 11]
+    if keep:  # four positions observed, of weight 1 a head each
+        for w, was in zip((w.numpy() for w in c.weights), weights):
+            assert np.array_equal(w[[0, 2]], was[[0, 2]])
+            assert np.abs(w[1].sum(-1) - 4).max() < 1e-5 and not w[1, :, 6:].any()
+    steps(3)
+    # a slot's first rows beside another's further ones are no prompt
+    c.release(1)
+    before = state(c)
+    c.reserve([1, 3, 1])
+    with pytest.raises(ValueError, match="empty sequences"):
+        run_paged(m, c, np.zeros((3, 3), np.int64), [0, 0, 0])
+    assert state(c) == before
