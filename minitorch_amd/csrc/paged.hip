@@ -1062,7 +1062,7 @@ __device__ __forceinline__ void select_few(const EvictArgs& a, int bh, int len, 
 
 // Copying the kept rows: a thread takes 16 bytes (number c) of the keys and the
 // values of the rows r0 + per i, i < kRows, which are the old rows j[i] (-1: none),
-// and the first of a row's threads its weight
+// and the first of a row's threads its weight.  A row without a new page is not read
 constexpr int kRows = 2;
 struct RowCopy {
   int c, per, r0, j[kRows], from[kRows], to[kRows], ti[kRows];
@@ -1131,9 +1131,9 @@ __global__ __launch_bounds__(256) void evict_kernel(const EvictArgs a, int block
   for (int i = 0; i < kRows; ++i) {
     const int r = copy.r0 + copy.per * i;
     copy.j[i] = r < new_len ? rows[r] : -1;
-    copy.from[i] = r < new_len ? ids[a.from.div(copy.j[i])] : -1;
     if (r >= new_len) copy.to[i] = -1;
     else if (copy.c == 0) slots[r] = copy.j[i];
+    copy.from[i] = copy.to[i] < 0 ? -1 : ids[a.from.div(copy.j[i])];
   }
   copy.copy(a, bh, bh % a.H);
   if (block) return;
@@ -1171,6 +1171,7 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictArgs a, int bloc
     copy.ti[i] = a.to.div(copy.r0 + copy.per * i);
     copy.from[i] = copy.j[i] < 0 ? -1 : a.from.id(b, a.from.div(copy.j[i]));
     copy.to[i] = copy.j[i] < 0 ? -1 : a.to.id(b, copy.ti[i]);
+    if (copy.to[i] < 0) copy.from[i] = -1;
   }
   copy.copy(a, bh, bh % a.H);
 }

@@ -177,29 +177,44 @@ class PagedKVCache:
 
     def trim(self) -> bool:
         """With keep: if a sequence holds more than keep + slack rows, cut all
-        that hold more than keep back to keep.  Returns whether it did."""
+        that hold more than keep back to keep, as many at a time as there are
+        free pages for; the others stay where they are.  Returns whether it did;
+        nothing has changed when there is not room for one."""
         if self.keep is None or self._len.max() <= self.keep + self.slack:
             return False
-        new = np.minimum(self._len, self.keep)
-        need = -(-new // self.page)
-        if need.sum() > len(self._free):
-            raise RuntimeError(f"trim: {int(need.sum())} pages needed, {len(self._free)} free")
-        to = np.full((self.batch, max(1, -(-self.keep // self.page))), -1, np.int32)
-        for b in range(self.batch):
-            to[b, :need[b]] = [self._free.pop() for _ in range(need[b])]
-        to_dev = dev.from_host(to, np.int32).t
-        for i in range(self.n_layer):
-            K.kv_evict_paged(self.k[i], self.v[i], self.table, self.lengths, self.weights[i], to_dev, self.keep,
-                             self.recent, lengths_out=self._lengths_to, weights_out=self._weights_to)
-            self.weights[i], self._weights_to = self._weights_to, self.weights[i]
+        cut, need = np.flatnonzero(self._len > self.keep), -(-self.keep // self.page)
+        if need > len(self._free):
+            raise RuntimeError(f"trim: {need} pages needed, {len(self._free)} free")
+        first = 0
+        while len(cut):  # a sequence that is cut gives back as many pages as it takes, or more
+            n = min(len(cut), len(self._free) // need)
+            end = int(cut[n]) if n < len(cut) else self.batch
+            self._cut(cut[:n], first, end, need)
+            first, cut = end, cut[n:]
         self.lengths, self._lengths_to = self._lengths_to, self.lengths
-        for b in range(self.batch):
-            self._give_back(b, self._tab[b])
-        self._tab[:, :to.shape[1]] = to
         self._settle()
         self.table.copy_(self._tab)
-        self._len = new
         return True
+
+    def _cut(self, cut, first, end, need):
+        """Cut the sequences `cut` of [first, end), `need` new pages each."""
+        to = np.full((end - first, need), -1, np.int32)  # a sequence that has no new pages is not copied
+        for b in cut:
+            to[b - first] = [self._free.pop() for _ in range(need)]
+        to_dev = dev.from_host(to, np.int32).t
+        part = slice(first, end)
+        for i in range(self.n_layer):
+            K.kv_evict_paged(self.k[i], self.v[i], self.table[part], self.lengths[part], self.weights[i][part], to_dev,
+                             self.keep, self.recent, lengths_out=self._lengths_to[part],
+                             weights_out=self._weights_to[part])
+            if end - first == self.batch:
+                self.weights[i], self._weights_to = self._weights_to, self.weights[i]
+            else:
+                self.weights[i][part].copy_(self._weights_to[part])
+        for b in cut:
+            self._give_back(b, self._tab[b])
+            self._tab[b, :need] = to[b - first]
+            self._len[b] = self.keep
 
     # -- a layer's work ----------------------------------------------------------
     def append(self, layer, k, v):

@@ -533,3 +533,139 @@ def test_prompt_into_a_released_slot(dev, keep):
     with pytest.raises(ValueError, match="empty sequences"):
         run_paged(m, c, np.zeros((3, 3), np.int64), [0, 0, 0])
     assert state(c) == before
+
+
+class Shadow:
+    """What a PagedKVCache should hold, in host arrays: each layer and
+    sequence's rows (heads, n, D) of keys, values and their weights."""
+
+    def __init__(self, c, rng):
+        self.c, self.rng = c, rng
+        empty = lambda: np.zeros((c.n_head, 0, c.head_dim), np.float32)
+        self.k, self.v = ([[empty() for _ in range(c.batch)] for _ in range(c.n_layer)] for _ in range(2))
+
+    def step(self, n, H):
+        """Reserve, append and attend once in every layer; the attention and
+        its weights against oracle.paged's on the rows held here."""
+        from minitorch_amd import device
+        from oracle import paged as ref
+
+        c, n = self.c, np.broadcast_to(n, self.c.batch)
+        c.reserve(n)
+        for i in range(c.n_layer):
+            k, v = (self.rng.standard_normal((c.batch, c.n_head, n.max(), c.head_dim), dtype=np.float32)
+                    for _ in range(2))
+            q = (2 * self.rng.standard_normal((c.batch, H, 1, c.head_dim))).astype(np.float32)
+            c.append(i, *(device.from_host(x, np.float32).t for x in (k, v)))
+            was = None if c.weights is None else c.weights[i].numpy().astype(np.float64)
+            got = c.attend(i, device.from_host(q, np.float32).t, 0.2).numpy()
+            for b in range(c.batch):
+                if not n[b]:
+                    assert not got[b].any()
+                    continue
+                for rows, new in ((self.k, k), (self.v, v)):
+                    rows[i][b] = np.concatenate([rows[i][b], new[b, :, :n[b]]], 1)
+                L = self.k[i][b].shape[1]
+                o, _, w, _, pv = ref.decode(q[b:b + 1], self.k[i][b][None], self.v[i][b][None],
+                                            np.zeros((1, 1), np.int32), np.array([L]), 0.2)
+                # a score is off by (D + 8) u of scale sum|q k|, some 12: 3e-5, and what
+                # comes of it by twice that
+                assert np.abs(got[b] - o[0]).max() <= 1e-4 * (1 + pv.max())
+                if was is not None:
+                    now = c.weights[i].numpy()[b]
+                    assert np.abs(now[:, :L] - was[b, :, :L] - w[0]).max() <= 1e-4 * H
+                    assert not now[:, L:].any()
+
+    def cut(self, keep, recent):
+        """The rows that a cut should keep, by the weights the cache holds."""
+        self.w = [w.numpy() for w in self.c.weights]
+        for i in range(self.c.n_layer):
+            for b in range(self.c.batch):
+                n = self.k[i][b].shape[1]
+                kept = []
+                for h in range(self.c.n_head):
+                    at = np.arange(n)
+                    if n > keep:
+                        old = np.argsort(-self.w[i][b, h, :n - recent], kind="stable")[:keep - recent]
+                        at = np.concatenate([np.sort(old), np.arange(n - recent, n)])
+                    kept.append(at)
+                    w = self.w[i][b, h, at]
+                    self.w[i][b, h] = 0
+                    self.w[i][b, h, :len(at)] = w
+                for rows in (self.k, self.v):
+                    rows[i][b] = np.stack([rows[i][b][h, at] for h, at in enumerate(kept)])
+
+    def check(self):
+        c = self.c
+        assert [c.length(b) for b in range(c.batch)] == [x.shape[1] for x in self.k[0]]
+        assert c.lengths.numpy().tolist() == [x.shape[1] for x in self.k[0]]
+        assert np.array_equal(c.table.numpy(), c._tab)
+        assert sorted(c._free + [int(i) for i in c._tab.ravel() if i >= 0]) == list(range(c.n_pages))
+        for i in range(c.n_layer):
+            assert np.array_equal(c.weights[i].numpy(), self.w[i])
+            for pool, rows in ((c.k[i].numpy(), self.k[i]), (c.v[i].numpy(), self.v[i])):
+                for b, x in enumerate(rows):
+                    n = x.shape[1]
+                    ids = c._tab[b, :-(-n // c.page)]
+                    assert (ids >= 0).all()
+                    held = pool[ids].transpose(1, 0, 2, 3).reshape(c.n_head, -1, c.head_dim)
+                    assert np.array_equal(held[:, :n], x)
+
+
+@pytest.mark.parametrize("pages,groups", [(None, 1), (20, 2), (17, 3)])
+def test_trim_cuts_the_long_sequences_alone(dev, pages, groups):
+    """Ragged lengths, three layers, three cuts after one another, in pools with
+    room for all sequences at once, for two and for one: every layer's rows,
+    weights and attention against the plain forms; sequences of `keep` rows or
+    fewer stay in their pages."""
+    import minitorch_amd as mt
+    from minitorch_amd import kernels as K
+
+    keep, recent, page, H = 12, 4, 4, 4
+    c = mt.PagedKVCache(3, 2, 32, 4, 24, page=page, keep=keep, recent=recent, slack=3, pages=pages)
+    s = Shadow(c, np.random.default_rng(41))
+    s.step([14, 5, 12, 13], H)
+    s.step(1, H)
+    assert not c.trim()  # 15 rows at most
+    for i in range(3):
+        s.step([1, 0, 0, 1], H)
+        if i:
+            assert not c.trim()
+            s.step([2, 0, 2, 2], H)
+        long, pages_before = c._len > keep, c._tab.copy()
+        calls, evict = [], K.kv_evict_paged
+        try:
+            K.kv_evict_paged = lambda *a, **kw: calls.append(1) or evict(*a, **kw)
+            s.cut(keep, recent)
+            assert c.trim() and not c.trim()
+        finally:
+            K.kv_evict_paged = evict
+        assert long.any() and not long.all()
+        if i == 0:
+            assert len(calls) == 3 * groups
+        s.check()
+        assert np.array_equal(c._tab[~long], pages_before[~long])
+        s.step(1, H)
+
+
+def test_trim_in_a_pool_that_cannot_hold_all_cuts_at_once(dev):
+    """Two sequences of 22 rows in 6 of 8 pages: their cuts take 2 pages each,
+    and the first one's frees 3."""
+    import minitorch_amd as mt
+
+    c = mt.PagedKVCache(2, 2, 32, 2, 32, page=8, keep=16, recent=4, slack=5, pages=8)
+    s = Shadow(c, np.random.default_rng(42))
+    s.step(22, 2)
+    s.cut(16, 4)
+    assert c.trim()
+    s.check()
+    s.step(1, 2)
+    # and where there is no room for a single one nothing has changed
+    c = mt.PagedKVCache(1, 2, 32, 2, 32, page=8, keep=16, recent=4, slack=5, pages=7)
+    c.reserve(22)
+    before = state(c)
+    with pytest.raises(RuntimeError, match="2 pages needed, 1 free"):
+        c.trim()
+    assert state(c) == before
+    c.release(1)
+    assert c.trim() and c.length(0) == 16
