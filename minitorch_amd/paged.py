@@ -94,6 +94,19 @@ class PagedKVCache:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _check_room(self, prompt, steps):
+        """Raises, as reserve or trim would on the way, unless prompts of that
+        many rows in every sequence, and steps of one row after them, each followed
+        by trim, fit the empty cache."""
+        rows, spare = prompt + steps, 0
+        if self.keep is not None and rows > self.keep + self.slack:
+            rows, spare = max(prompt, self.keep + self.slack + 1), -(-self.keep // self.page)
+        if rows > self.width * self.page:
+            raise ValueError(f"{rows} rows exceed the {self.width * self.page} a sequence may hold")
+        need = self.batch * -(-rows // self.page) + spare
+        if need > len(self._free):
+            raise RuntimeError(f"{need} pages needed, {len(self._free)} free")
+
     # -- growing and shrinking ---------------------------------------------------
     def reserve(self, n=1):
         """Make room for n new rows in every sequence (an int, or one per

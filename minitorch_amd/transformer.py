@@ -726,8 +726,8 @@ class GPT(Module):
         p > 0) every step is a full forward, as in the reference.  With `cache` (an
         empty PagedKVCache for this model and batch, paged_cache) the keys and
         values are kept there, cut back after each step if it is bounded; prompt
-        and new tokens then have to fit block_size.  return_logprobs: returns
-        (ids, log probabilities of the new tokens (B, n))."""
+        and new tokens then have to fit block_size, and their rows the cache.
+        return_logprobs: returns (ids, log probabilities of the new tokens (B, n))."""
         from . import kernels as K
 
         idx = np.asarray(idx)
@@ -754,6 +754,7 @@ class GPT(Module):
                 raise ValueError(f"prompt + new tokens = {T0 + n} exceeds block_size {blk}")
             if dropout_on:
                 raise ValueError("a cache does not go with active dropout (use model.eval())")
+            cache._check_room(T0, n - 1)
         logprobs = []
 
         def sample(logits2d):

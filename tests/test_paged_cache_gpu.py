@@ -669,3 +669,30 @@ def test_trim_in_a_pool_that_cannot_hold_all_cuts_at_once(dev):
     assert state(c) == before
     c.release(1)
     assert c.trim() and c.length(0) == 16
+
+
+def test_generate_refuses_what_a_cache_cannot_hold_before_any_work(dev):
+    m = model()
+    idx = np.random.default_rng(43).integers(0, 50, (2, 10))
+
+    def refused(error, match, n, **options):
+        c = m.paged_cache(2, page=8, **options)
+        before = state(c)
+        with pytest.raises(error, match=match):
+            m.generate(idx, n, cache=c)
+        assert state(c) == before
+        return c
+
+    refused(ValueError, "exceed", 16, max_tokens=24)  # 25 rows at the end
+    c = refused(RuntimeError, "pages", 24, pages=8)  # 33 rows, in 5 pages each
+    np.random.seed(4)
+    want = m.generate(idx, 23)
+    np.random.seed(4)
+    assert np.array_equal(m.generate(idx, 23, cache=c), want)  # 32, in 4
+    # at most 17 rows a sequence in 3 pages each, and 2 for a cut
+    options = dict(max_tokens=24, keep=12, slack=4)
+    refused(RuntimeError, "pages", 30, pages=7, **options)
+    np.random.seed(4)
+    want = m.generate(idx, 30, cache=m.paged_cache(2, page=8, **options))
+    np.random.seed(4)
+    assert np.array_equal(m.generate(idx, 30, cache=m.paged_cache(2, page=8, pages=8, **options)), want)
