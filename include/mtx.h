@@ -386,7 +386,8 @@ int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, int Hkv, int
  * and may be shared.  The order of cached rows does not matter to attention, and
  * a head's row i need not be another head's token.  Written besides:
  *   lengths_out[b] = min(lengths[b], keep);
- *   weights_out (laid out as weights): the kept rows' weights, then 0;
+ *   weights_out (laid out as weights): the kept rows' weights, then 0, up to
+ *   max_pages * page; what lies behind that in a wider row is left as it was;
  *   slots (B, Hkv, keep): the rows they came from, ascending, then -1.
  * lengths_out, weights_out and to_table are other memory than lengths, weights
  * and table.  A kept row that is not there becomes zeros; one whose new page is

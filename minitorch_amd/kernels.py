@@ -374,13 +374,15 @@ def kv_evict_paged(k_pages, v_pages, table, lengths, weights, to_table, keep: in
     to_table (mtx_kv_evict_paged): int32 (B, to_pages), pages of the same pool
     that no table of the call reads.  weights as attn_decode_paged accumulates
     them.  Returns (lengths_out (B,), weights_out like weights, slots
-    (B, Hkv, keep) int32: the rows kept, then -1)."""
+    (B, Hkv, keep) int32: the rows kept, then -1).  Columns of weights_out behind
+    the table's rows are 0 if it is not given, else left as they were."""
     keep = int(keep)
     if keep < 1:
         raise ValueError("keep must be at least 1")
     if lengths_out is None:
         lengths_out = dev.empty_buf(lengths.shape, "int32")
-    if weights_out is None:
+    made = weights_out is None
+    if made:
         weights_out = dev.empty_buf(weights.shape, "float32")
     if slots is None:
         slots = dev.empty_buf((table.shape[0], k_pages.shape[1], keep), "int32")
@@ -389,6 +391,8 @@ def kv_evict_paged(k_pages, v_pages, table, lengths, weights, to_table, keep: in
         _spec(lengths_out), _spec(weights_out), _spec(slots))
     if dev.SEVERAL:
         _on_gpu0(k_pages, v_pages, table, lengths, weights, to_table, lengths_out, weights_out, slots)
+    if made and wld > width * k_pages.shape[2]:
+        weights_out.fill_(0.0)
     L.call("mtx_kv_evict_paged", *sizes, k_pages.data_ptr(), kps, v_pages.data_ptr(), vps, table.data_ptr(), ld,
            width, lengths.data_ptr(), weights.data_ptr(), wld, to_table.data_ptr(), to_ld, to_pages, keep,
            int(recent), lengths_out.data_ptr(), weights_out.data_ptr(), slots.data_ptr(), L.stream_handle())

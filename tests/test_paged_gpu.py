@@ -727,3 +727,34 @@ def test_decode_weights_keep_fp32s_bits(dev, q, B, width):
     bound = 2.0 ** -20 * pv + (2.0 ** -8 if q == "bfloat16" else 0) * np.abs(want)
     off = np.abs(host(o) - want) / bound
     assert off.max() <= 1, float(off.max())
+
+
+def test_evict_weights_wider_than_the_table(dev):
+    """Columns behind the table's rows: 0 where the call makes the new weights
+    itself, left as they were in a caller's; a wider table then counts from there."""
+    from minitorch_amd import device, kernels as K
+
+    rng = np.random.default_rng(17)
+    B, Hkv, D, page, keep = 2, 2, 16, 4, 6
+    kp, vp = (make_pool(rng, 12, Hkv, page, D, "float32") for _ in range(2))
+    dk, dv = dev_array(kp), dev_array(vp)
+    table, to = np.array([[0, 1], [2, 3]], np.int32), np.array([[4, 5, 6, -1], [7, 8, 9, -1]], np.int32)
+    lens = np.array([8, 5], np.int32)
+    w = rng.random((B, Hkv, 16), dtype=np.float32)
+    args = (dk, dv, dev_array(table, "int32"), dev_array(lens, "int32"), dev_array(w), dev_array(to, "int32"), keep, 2)
+    device.empty_cache()
+    junk = [full(w.shape, 7.0) for _ in range(4)]  # what freed memory holds
+    del junk
+    n, w_out, _ = K.kv_evict_paged(*args)
+    got = host(w_out)
+    assert not got[..., 8:].any()
+    n = host(n)
+    assert n.tolist() == [6, 5]
+    assert np.all(host(K.kv_evict_paged(*args, weights_out=full(w.shape, 3.0))[1])[..., 8:] == 3.0)
+    # two rows more each, in the wider table
+    lens = (n + 5).astype(np.int32)
+    q = rng.standard_normal((B, Hkv, 1, D), dtype=np.float32)
+    K.attn_decode_paged(dev_array(q), dk, dv, dev_array(to, "int32"), dev_array(lens, "int32"), 0.2, weights=w_out,
+                        weights_in=w_out)
+    r = ref.decode(q, host_pool(dk), host_pool(dv), to, lens, 0.2)
+    assert np.abs(host(w_out) - got - r[2]).max() <= 1e-5
