@@ -808,7 +808,8 @@ int mtx_xent_bwd_f32(const float* logits, int64_t ld, const int64_t* labels, con
  * Log probabilities of given tokens (log_softmax, functional.py:81-97, at the
  * tokens; generation samples from softmax(logits / temperature),
  * transformer.py:97-100, scale = 1 / temperature).  With x = scale * logits[r]
- * (rows x V, row stride ld, fp32 or bf16; rows < 2^23, V <= 2^27):
+ * (rows x V, row stride ld, fp32 or bf16; rows < 2^23, V <= 2^27; scale from 1e-27
+ * to 1e38):
  *   lse = log sum exp x;  logprob = x[token] - lse;  entropy = -sum p log p;
  *   top_ids, top_logprobs (rows, top): the `top` <= 64 largest logits, largest
  *   first, ties to the lowest id (NaN counts above every number), and their log

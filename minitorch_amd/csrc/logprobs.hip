@@ -69,8 +69,9 @@ __device__ __forceinline__ void load_left(const T* p, int left, float (&x)[E]) {
   }
 }
 
-// values of -inf add 0, not 0 * inf; NaN stays
-constexpr float kFarBelow = -1e30f;
+// values of -inf add 0, not 0 * inf; NaN stays.  exp(kFarBelow * scale) is 0 for every
+// scale that is taken, from kLeastScale on
+constexpr float kFarBelow = -1e30f, kLeastScale = 1e-27f, kMostScale = 1e38f;
 __device__ __forceinline__ float below(float d) { return __builtin_elementwise_maximum(d, kFarBelow); }
 
 // The value of lane `lane ^ M` without the LDS pipe that a shuffle takes (a row of
@@ -540,7 +541,7 @@ int check_rows(int dtype, int64_t rows, int V, const void* logits, int64_t ld, c
   MTX_CHECK_ARG(logits != nullptr && tokens != nullptr, "logits, tokens: null pointer");
   MTX_CHECK_ARG(((uintptr_t)logits & (dtype == MTX_F32 ? 3u : 1u)) == 0, "logits: pointer must be aligned to its type");
   MTX_CHECK_ARG(ld >= V || (rows == 1 && ld >= 0), "logits: row stride %lld < V=%d", (long long)ld, V);
-  MTX_CHECK_ARG(std::isfinite(scale) && scale > 0.f, "scale must be finite and > 0");
+  MTX_CHECK_ARG(scale >= kLeastScale && scale <= kMostScale, "scale=%g must be between 1e-27 and 1e38", scale);
   return MTX_OK;
 }
 

@@ -484,8 +484,8 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
     (N, top) DeviceArrays of the `top` <= 64 most likely tokens, ties to the
     lowest id, and their log probabilities, without gradients."""
     N, V = logits.shape
-    if not (np.isfinite(temperature) and temperature > 0):
-        raise ValueError(f"temperature must be finite and > 0 (got {temperature})")
+    if not 1e-38 <= temperature <= 1e27:
+        raise ValueError(f"temperature must be between 1e-38 and 1e27 (got {temperature})")
     if isinstance(tokens, DeviceArray):
         # device-resident tokens: the kernel takes any outside the vocabulary for none
         tok = dev.index_array(tokens)

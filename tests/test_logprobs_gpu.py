@@ -260,3 +260,38 @@ def test_recorded_calls(dev):
             want = [host(t) for t in s["call"]()]
             s["graph"].replay()
             assert all(np.array_equal(host(a), b) for a, b in zip(s["out"], want))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("V", [7, 65, 300, 700, 5003, 50021])
+@pytest.mark.parametrize("scale", [2.0 ** -89, 1e-20, 1e20, 1e37])
+def test_scales_at_the_ends(dev, dtype, V, scale):
+    """Scales near the ends of what is taken, with hidden logits: a nearly
+    even distribution over the others, or one value."""
+    rng = np.random.default_rng(V)
+    x, tok = make(rng, 6, V, dtype)
+    x[1, ::2] = -np.inf
+    x[2, 1:] = -np.inf
+    x[3, 1::2] = np.finfo(np.float32).min if dtype == "float32" else -3e38
+    tok[1:4] = 0
+    x *= np.float32(0.1) if scale > 1 else np.float32(1)
+    if dtype == "bfloat16":
+        x = bf16_round(x)
+    from minitorch_amd import kernels as K
+
+    lp, ent, lse, _, _ = (host(t) for t in K.token_logprobs(dev_array(x, dtype), dev_array(tok, "int64"), scale=scale))
+    xd = x.astype(np.float64) * scale
+    d = xd - xd.max(1, keepdims=True)
+    logl = np.log(np.exp(d).sum(1))
+    p = np.exp(d - logl[:, None])
+    want = np.take_along_axis(d, tok[:, None], 1)[:, 0] - logl
+    e = U * (V / 64 + 80)
+    # differences are formed before the scale: 3 u of them
+    with np.errstate(invalid="ignore"):
+        assert np.all((lp == want) | (np.abs(lp - want) <= e + 4 * U * (np.abs(want) + logl)))
+    ld = np.log(np.where(p > 0, p, 1))
+    terms = (p * (1 + np.abs(ld))).sum(1)
+    # an exponent d scale is off by 3 u of itself, so is what its term adds
+    assert np.all(np.abs(ent + (p * ld).sum(1)) <= 3 * e * terms + 8 * U * (1 + logl) + 4 * U * (p * ld ** 2).sum(1))
+    if scale <= 1:
+        assert np.all(np.abs(lse - (xd.max(1) + logl)) <= e + 4 * U * (logl + np.abs(xd.max(1))))

@@ -696,3 +696,20 @@ def test_generate_refuses_what_a_cache_cannot_hold_before_any_work(dev):
     want = m.generate(idx, 30, cache=m.paged_cache(2, page=8, **options))
     np.random.seed(4)
     assert np.array_equal(m.generate(idx, 30, cache=m.paged_cache(2, page=8, pages=8, **options)), want)
+
+
+def test_token_logprobs_temperatures(dev):
+    """Hidden tokens have probability 0 up to the largest temperature; beyond
+    it, where the others' 1 / temperature is no longer large beside that of
+    -inf's stand-in, and where it overflows, the call is refused."""
+    import minitorch_amd as mt
+
+    x = np.array([[1.0, -np.inf, 2.0, -np.inf, 0.5]], np.float32)
+    lp, ent, _, tops = mt.F.token_logprobs(mt.Tensor(x), [0], top=5, temperature=1e27)
+    assert abs(float(lp.numpy()[0]) + np.log(3)) < 1e-6 and abs(float(ent.numpy()[0]) - np.log(3)) < 1e-6
+    assert np.isneginf(tops.numpy()[0, 3:]).all()
+    lp, ent, _, _ = mt.F.token_logprobs(mt.Tensor(x), [2], temperature=1e-38)
+    assert float(lp.numpy()[0]) == 0 and float(ent.numpy()[0]) == 0
+    for bad in (1e28, 1e30, 1e300, 0.9e-38, 5e-324):
+        with pytest.raises(ValueError, match="temperature"):
+            mt.F.token_logprobs(mt.Tensor(x), [0], temperature=bad)

@@ -247,3 +247,12 @@ def test_arrays_of_the_librarys_gpu_are_not(monkeypatch):
     v = [OnGpu((6,)) for _ in range(3)]
     with pytest.raises(AssertionError, match="launched"):
         K.token_logprobs(x, tok, 0, 1.0, *v, OnGpu((6, 0), "int64"), OnGpu((6, 0)))
+
+
+@pytest.mark.parametrize("fn", [forward, backward])
+@pytest.mark.parametrize("scale", [1e-28, 1e-40, 1.01e38, 3e38])
+def test_scales_that_hidden_logits_or_fp32_do_not_stand(fn, scale):
+    """Logits far below the maximum are taken for 1e30 below it, which has to
+    have probability 0; the scale times log2 e has to be finite."""
+    rc, msg = fn(dict(scale=scale))
+    assert rc == L.MTX_ERR_ARG and "scale" in msg
