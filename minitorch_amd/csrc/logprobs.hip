@@ -476,8 +476,11 @@ struct LpBwdArgs {
 };
 
 // dx = p (A + B log p) with A = -scale (g + gh H), B = -scale gh, and scale g at
-// the token: one pass, 4 values a load and store, up to kUnroll of them a thread
+// the token: one pass, 4 values a load and store, up to kUnroll of them a thread.
+// log p is taken for kLeastLog at least, whose p is 0 already, so that B log p does
+// not overflow where p is 0 (0 * inf)
 constexpr int kUnroll = 4;
+constexpr float kLeastLog = -128.f;
 template <typename T>
 __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const LpBwdArgs a) {
   const int64_t r = (int64_t)blockIdx.x * (256 / a.per) + threadIdx.x / a.per;
@@ -511,7 +514,8 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const LpBwdArgs a) {
     float d[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float lp = below(fmaf(v[u][e], a.scale, -off)), p = __builtin_amdgcn_exp2f(lp * kLog2e);
+      const float lp = __builtin_elementwise_maximum(fmaf(v[u][e], a.scale, -off), kLeastLog);
+      const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
       d[e] = p * fmaf(Bf, lp, A);
       if (i + e == tok) d[e] += own;
     }

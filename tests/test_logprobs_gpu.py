@@ -295,3 +295,28 @@ def test_scales_at_the_ends(dev, dtype, V, scale):
     assert np.all(np.abs(ent + (p * ld).sum(1)) <= 3 * e * terms + 8 * U * (1 + logl) + 4 * U * (p * ld ** 2).sum(1))
     if scale <= 1:
         assert np.all(np.abs(lse - (xd.max(1) + logl)) <= e + 4 * U * (logl + np.abs(xd.max(1))))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("gradient", [1e9, -1e12, 1e30])
+def test_gradient_of_large_upstream_gradients_at_hidden_logits(dev, dtype, gradient):
+    """-inf, the type's lowest value and logits far below the others get 0
+    whatever comes from upstream; the others the formula's."""
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(5)
+    x, tok = make(rng, 4, 130, dtype)
+    low = np.float32(np.finfo(np.float32).min) if dtype == "float32" else np.float32(-3.3e38)
+    x[:, 3], x[:, 50], x[:, 70] = -np.inf, low, -500.0
+    if dtype == "bfloat16":
+        x = bf16_round(x)
+    tok[:] = 1
+    dx, dt = dev_array(x, dtype), dev_array(tok, "int64")
+    _, ent, lse, _, _ = K.token_logprobs(dx, dt)
+    g = np.full(4, gradient, np.float32)
+    d = host(K.token_logprobs_bwd(dx, dt, lse, ent, None, dev_array(g)))
+    assert not d[:, [3, 50, 70]].any()
+    seen, none = [i for i in range(130) if i not in (3, 50, 70)], np.zeros(4, np.float32)
+    x, d = x[:, seen], d[:, seen]
+    want = ref.logprobs_grad(x, tok, none, g)
+    assert np.all(np.abs(d - want) <= grad_bound(x, tok, 1.0, ref.logprobs(x, tok), none, g, want))
