@@ -40,18 +40,25 @@ def dtype_name(x) -> str:
     if type(x) is DevBuf:
         return x.dtype
     d = x if isinstance(x, (str, type, np.dtype)) else getattr(x, "dtype", x)
-    name = _NAMES.get(d)
+    try:
+        name = _NAMES.get(d)
+    except TypeError:  # it cannot be hashed
+        return _find_name(d)
     if name is None:
-        if isinstance(d, str):
-            name = d
-        else:
-            try:
-                name = np.dtype(d).name
-            except TypeError:
-                name = str(d).rsplit(".", 1)[-1]
-        if name not in ITEMSIZE:
-            raise ValueError(f"unsupported dtype {d!r}")
-        _NAMES[d] = name
+        name = _NAMES[d] = _find_name(d)
+    return name
+
+
+def _find_name(d) -> str:
+    if isinstance(d, str):
+        name = d
+    else:
+        try:
+            name = np.dtype(d).name
+        except TypeError:
+            name = str(d).rsplit(".", 1)[-1]
+    if name not in ITEMSIZE:
+        raise ValueError(f"unsupported dtype {d!r}")
     return name
 
 

@@ -130,3 +130,21 @@ def test_noalloc_rejects_oversize_before_any_hip_call():
     rc = L.lib().mtx_attn_bwd_noalloc(L.MTX_F32, 1, 1, Tq, Tq, 64, p, s, p, s, p, s, p, s, p, s, p,
                                       p, s, p, s, p, s, 0.125, 1, 0, None)
     assert rc == L.MTX_ERR_SHAPE and "scratch" in L.lib().mtx_last_error().decode()
+
+
+@pytest.mark.parametrize("bad", [[], {}, set(), bytearray(b"float32"), np.zeros(2, "float64"), "float16", 3])
+def test_dtype_names_that_are_none(bad):
+    """Whatever has no name of a supported dtype is a ValueError, also what
+    cannot be hashed."""
+    with pytest.raises(ValueError, match="unsupported dtype"):
+        dev.dtype_name(bad)
+
+
+def test_dtype_name_of_an_object_that_cannot_be_hashed():
+    class Odd:
+        __hash__ = None
+
+        def __str__(self):
+            return "somewhere.float32"
+
+    assert dev.dtype_name(Odd()) == "float32"
