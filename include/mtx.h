@@ -816,11 +816,9 @@ int mtx_xent_bwd_f32(const float* logits, int64_t ld, const int64_t* labels, con
  *   probabilities.  top may be 0.
  * A logit of -inf has probability 0 and adds nothing to the entropy; a row of
  * nothing else gets lse, log probabilities -inf and entropy 0.  A row whose token
- * is outside [0, V) has no token: logprob 0.  Workspace:
- * mtx_token_logprobs_workspace_bytes() bytes, 16-byte aligned, free after the
- * call; calls that overlap need their own.  Deterministic.
+ * is outside [0, V) has no token: logprob 0.  No workspace is needed: workspace and
+ * workspace_bytes are not looked at (NULL, 0).  Deterministic.
  */
-size_t mtx_token_logprobs_workspace_bytes(int64_t rows, int V, int top);
 int mtx_token_logprobs(int dtype, int64_t rows, int V, const void* logits, int64_t ld, const int64_t* tokens,
                        float scale, float* logprob, float* lse, float* entropy, int top, int64_t* top_ids,
                        float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);

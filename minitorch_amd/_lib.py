@@ -153,7 +153,6 @@ SIGNATURES = {
     "mtx_gelu_bwd_f32": (_I, [_P, _P, _P, _I64, _I, _P]),
     "mtx_xent_fwd_f32": (_I, [_P, _I64, _P, _P, _P, _I64, _I, _P]),
     "mtx_xent_bwd_f32": (_I, [_P, _I64, _P, _P, _P, _F, _P, _I64, _I64, _I, _I, _P]),
-    "mtx_token_logprobs_workspace_bytes": (_SZ, [_I64, _I, _I]),
     "mtx_token_logprobs": (_I, [_I, _I64, _I, _P, _I64, _P, _F, _P, _P, _P, _I, _P, _P, _P, _SZ, _P]),
     "mtx_token_logprobs_bwd": (_I, [_I, _I64, _I, _P, _I64, _P, _P, _P, _P, _P, _F, _P, _I64, _I, _P]),
     "mtx_embedding_fwd_f32": (_I, [_P, _I64, _I64, _P, _I64, _P, _I64, _I, _P]),

@@ -570,7 +570,7 @@ int launch_logprobs(const LpArgs& a, int64_t rows, hipStream_t st) {
   else if (a.V <= 512) SMALL(64, 8);
 #define ROW(NT, U, WHOLE) \
   hipLaunchKernelGGL((logprobs_kernel<T, NT, U, WHOLE>), dim3((unsigned)rows), dim3(NT), 0, st, a)
-  else if (a.V <= 64 * E * 2) ROW(64, 2, true);
+  else if (sizeof(T) == 2 && a.V <= 64 * E * 2) ROW(64, sizeof(T) == 2 ? 2 : 4, true);
   else if (a.V <= 64 * E * 4) ROW(64, 4, true);
   else if (a.V <= 64 * E * 8) ROW(64, 8, true);
   else if (a.V <= 256 * E * 4) ROW(256, 4, true);
@@ -587,12 +587,9 @@ int launch_logprobs(const LpArgs& a, int64_t rows, hipStream_t st) {
 
 using namespace mtx;
 
-extern "C" size_t mtx_token_logprobs_workspace_bytes(int64_t rows, int V, int top) { return 0; }
-
 extern "C" int mtx_token_logprobs(int dtype, int64_t rows, int V, const void* logits, int64_t ld,
                                   const int64_t* tokens, float scale, float* logprob, float* lse, float* entropy,
-                                  int top, int64_t* top_ids, float* top_logprobs, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
+                                  int top, int64_t* top_ids, float* top_logprobs, void*, size_t, void* stream) {
   int rc;
   if ((rc = check_rows(dtype, rows, V, logits, ld, tokens, scale))) return rc;
   MTX_CHECK_ARG(logprob && lse && entropy, "logprob, lse, entropy: null pointer");

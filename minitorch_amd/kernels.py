@@ -1206,9 +1206,8 @@ def _logprobs_plan(logits, tokens, top, logprob, entropy, lse, top_ids, top_logp
     for name, t, dt in (("top_ids", top_ids, "int64"), ("top_logprobs", top_logprobs, "float32")):
         if _dt(t[2]) != dt or tuple(t[0]) != (rows, top) or (rows and top and not _packed(*t[:2])):
             raise ValueError(f"{name} must be contiguous {dt} ({rows}, {top})")
-    ws = L.lib().mtx_token_logprobs_workspace_bytes(rows, V, top) if rows else 0
     dev.device()
-    return code, rows, V, ld, ws
+    return code, rows, V, ld
 
 
 def token_logprobs(logits, tokens, top: int = 0, scale: float = 1.0, logprob=None, entropy=None, lse=None,
@@ -1228,7 +1227,7 @@ def token_logprobs(logits, tokens, top: int = 0, scale: float = 1.0, logprob=Non
     if not (logits.is_cuda and tokens.is_cuda and logprob.is_cuda and entropy.is_cuda and lse.is_cuda
             and top_ids.is_cuda and top_logprobs.is_cuda):
         _on_device(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs)
-    code, rows, V, ld, ws_bytes = _logprobs_plan(
+    code, rows, V, ld = _logprobs_plan(
         (logits.shape, logits.stride(), logits.dtype), (tokens.shape, tokens.stride(), tokens.dtype), top,
         (logprob.shape, logprob.stride(), logprob.dtype), (entropy.shape, entropy.stride(), entropy.dtype),
         (lse.shape, lse.stride(), lse.dtype), (top_ids.shape, top_ids.stride(), top_ids.dtype),
@@ -1236,10 +1235,9 @@ def token_logprobs(logits, tokens, top: int = 0, scale: float = 1.0, logprob=Non
     if dev.SEVERAL:
         _on_gpu0(logits, tokens, logprob, entropy, lse, top_ids, top_logprobs)
     if rows:
-        ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
         L.call("mtx_token_logprobs", code, rows, V, logits.data_ptr(), ld, tokens.data_ptr(), float(scale),
                logprob.data_ptr(), lse.data_ptr(), entropy.data_ptr(), top, top_ids.data_ptr() if top else None,
-               top_logprobs.data_ptr() if top else None, _ptr(ws), ws_bytes, L.stream_handle())
+               top_logprobs.data_ptr() if top else None, None, 0, L.stream_handle())
     return logprob, entropy, lse, top_ids, top_logprobs
 
 
