@@ -713,3 +713,37 @@ def test_token_logprobs_temperatures(dev):
     for bad in (1e28, 1e30, 1e300, 0.9e-38, 5e-324):
         with pytest.raises(ValueError, match="temperature"):
             mt.F.token_logprobs(mt.Tensor(x), [0], temperature=bad)
+
+
+def test_generate_with_bf16_pages_is_the_rounded_caches_model(dev):
+    """The log probabilities of a generation through bf16 pages against the
+    model's layers around an attention in 64 bits, whose steps see keys and values
+    rounded to bf16 (a prompt's own positions see them in fp32)."""
+    import minitorch_amd as mt
+    from oracle.attention import bf16_round
+
+    m = model()
+    T0, n = 12, 20
+    idx = np.random.default_rng(4).integers(0, 50, (2, T0))
+    np.random.seed(6)
+    ids, lp = m.generate(idx, n, cache=m.paged_cache(2, page=8, dtype="bfloat16"), return_logprobs=True)
+    T, H, D = T0 + n - 1, 2, 32
+    with mt.no_grad():
+        x = m.tok_emb(ids[:, :T]) + m.pos_emb(np.arange(T))
+        for block in m.blocks:
+            h, a = block.ln1(x), block.attn
+            q, k, v = (p(h).data.numpy().astype(np.float64).reshape(2, T, H, D).transpose(0, 2, 1, 3)
+                       for p in (a.q_proj, a.k_proj, a.v_proj))
+            o = np.zeros((2, H, T, D))
+            for t in range(T):
+                ks, vs = (y[:, :, :t + 1] if t < T0 else bf16_round(y[:, :, :t + 1].astype(np.float32)).astype(float)
+                          for y in (k, v))
+                s = np.matmul(ks, q[:, :, t, :, None])[..., 0] / np.sqrt(D)
+                p = np.exp(s - s.max(-1, keepdims=True))
+                o[:, :, t] = np.matmul((p / p.sum(-1, keepdims=True))[:, :, None], vs)[:, :, 0]
+            x = x + a.out_proj(mt.Tensor(o.transpose(0, 2, 1, 3).reshape(2, T, H * D).astype(np.float32)))
+            x = x + block.mlp(block.ln2(x))
+        y = m.lm_head(m.ln_f(x)).data.numpy().astype(np.float64)[:, T0 - 1:]
+    y = y - y.max(-1, keepdims=True)
+    y = y - np.log(np.exp(y).sum(-1, keepdims=True))
+    assert np.abs(lp - np.take_along_axis(y, ids[:, T0:, None], -1)[..., 0]).max() <= 1e-4

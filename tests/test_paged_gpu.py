@@ -758,3 +758,48 @@ def test_evict_weights_wider_than_the_table(dev):
                         weights_in=w_out)
     r = ref.decode(q, host_pool(dk), host_pool(dv), to, lens, 0.2)
     assert np.abs(host(w_out) - got - r[2]).max() <= 1e-5
+
+
+def test_calls_on_another_stream(dev):
+    """Append, attention, eviction and log probabilities launched on a stream
+    of their own: the null stream's bits."""
+    import ctypes
+
+    from minitorch_amd import _lib as L, device, kernels as K
+
+    rng = np.random.default_rng(51)
+    B, H, Hkv, D, page = 3, 4, 2, 64, 16
+    lens = [3000, 17, 700]
+    table, total, free = make_table(rng, lens, page, spare=3 * 16)
+    kp, vp = (make_pool(rng, total, Hkv, page, D, "bfloat16") for _ in range(2))
+    new = rng.standard_normal((2, B, Hkv, 1, D), dtype=np.float32)
+    q = dev_array(rng.standard_normal((B, H, 1, D), dtype=np.float32))
+    dk, dv = dev_array(new[0]), dev_array(new[1])
+    dt, dl = dev_array(table, "int32"), dev_array(np.array(lens, np.int32), "int32")
+    to = dev_array(free[:48].reshape(3, 16).copy(), "int32")
+    x = dev_array(rng.standard_normal((9, 5000), dtype=np.float32))
+    tok, g = dev_array(rng.integers(0, 5000, 9), "int64"), dev_array(rng.standard_normal(9).astype(np.float32))
+
+    def work():
+        a, b = dev_array(kp, "bfloat16"), dev_array(vp, "bfloat16")
+        w = full((B, Hkv, table.shape[1] * page), 0.0)
+        K.kv_append_paged(dk, dv, a, b, dt, dl)
+        lse = empty((B, H))
+        o, _ = K.attn_decode_paged(q, a, b, dt, dl, 0.125, lse=lse, weights=w)
+        out = [a, b, o, lse, w, *K.kv_evict_paged(a, b, dt, dl, w, to, 256, 32)]
+        lp = K.token_logprobs(x, tok, top=7)
+        return out + [*lp, K.token_logprobs_bwd(x, tok, lp[2], lp[1], g, g)]
+
+    want = [host(t) for t in work()]
+    device.synchronize()
+    stream = ctypes.c_void_p()
+    L.call("mtx_stream_create", ctypes.byref(stream))
+    try:
+        L._STREAM[0] = stream
+        out = work()
+        L.call("mtx_stream_sync", stream)
+    finally:
+        L._STREAM[0] = None
+        L.call("mtx_stream_destroy", stream)
+    for a, b in zip(out, want):
+        assert np.array_equal(host(a), b, equal_nan=True)
