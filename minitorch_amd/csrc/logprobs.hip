@@ -458,7 +458,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LpArgs a) {
 
 // The gradient reads the logits once more and writes as many fp32 values: bound by
 // the memory, 4096 x 50021 fp32 in 313 us (5.2 TB/s; a large copy reaches 5.2).  The
-// forward's pass over the same logits takes 136 us (6.0 TB/s) by itself, 174 behind
+// forward's pass over the same logits takes 137 us (6.0 TB/s) by itself, 179 behind
 // the gradient's, whose last writes are then still on their way.
 struct LpBwdArgs {
   const void* x;

@@ -135,8 +135,10 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
 // q, enter the products as three bf16 pieces (24 bits, as fp32 has).
 //
 // Measured, 16 sequences of 8000 to 16384 rows, 8 K/V heads of 128 in bf16 (797
-// MB), 32 query heads: 139 us, 5.7 TB/s (a plain read of the same pages: 136 us); one of
-// 131071 rows (67 MB): 17.5 us, of which 11 at the memory's rate.
+// MB), 32 query heads: 140 us, 5.7 TB/s (a plain read of the same pages: 136 us); one of
+// 131071 rows (67 MB): 18 us, of which 11 at the memory's rate.  The third piece of the
+// weights costs no time there and more the smaller the heads are (64 sequences of 1000 to
+// 3000 rows, 8 K/V heads of 16, 32 query heads: 28.1 us, 24.5 with two).
 //
 // A workgroup takes some rows of one sequence and K/V head (make_plan), its four
 // waves in turn tiles of 16 NT of them, and joins them in LDS; several workgroups'
@@ -1239,12 +1241,13 @@ int check_cache(int B, int H, int D, int64_t n_pages, int page, const int* table
 //
 // Else up to 128 sequences and K/V heads: P pieces by the lengths (cut_rows), one for each
 // compute unit, or for each HT workgroups' where there are many (30 sequences of 1000 to
-// 9000 rows, 3 K/V heads of 128, 96 query heads: 78 us, in chunks 101).  16 sequences of 8000 to 16384 rows, 8 heads: 143 us, in chunks of 1024
-// rows 157; one of 16384 and 15 of 300: 25, 57; 7 sequences of 9000, 2 heads, 21.7, 20.1.
+// 9000 rows, 3 K/V heads of 128, 96 query heads: 77 us, in chunks 102).  16 sequences of
+// 8000 to 16384 rows, 8 heads: 144 us, in chunks of 1024 rows 156; one of 16384 and 15 of
+// 300: 25, 38; 7 sequences of 9000, 2 heads, 21.0, 20.0.
 //
 // Else chunks alike, 512 to 1024 rows each, some 768 or more: they come to the compute
 // units as those get free, which P pieces of unequal size would not (20 sequences of
-// 10000 rows, 8 heads of 64: 80 us, 89 by pieces)
+// 10000 rows, 8 heads of 64: 83 us, 90 by pieces)
 struct DecodePlan {
   int chunk, S, HT, P, most, direct;
   int64_t n_o, n_ml, n_s, n_cuts, sld;
@@ -1261,7 +1264,7 @@ DecodePlan make_plan(int B, int H, int Hkv, int D, int page, int max_pages, bool
     p.chunk = cap;
   } else if (B * Hkv <= 128 && cap <= (1 << 27)) {
     // two a compute unit where a tile is small (32 sequences of 30000 rows, 4 heads of 32:
-    // 97 us, 124 with one; 5 of 43000, 8 heads of 16: 30, 43); the HT workgroups of a piece
+    // 96 us, 121 with one; 5 of 43000, 8 heads of 16: 36, 54); the HT workgroups of a piece
     // lie on one XCD: each of the 8 has place for 32 / HT
     const int n = 8 * (D < 64 ? 2 : 1) * (segments <= 128 ? 32 / p.HT : 32) / Hkv;
     p.P = (int)std::max<int64_t>(std::min<int64_t>(n, (int64_t)B * cdiv(cap, 256)),
@@ -1391,7 +1394,7 @@ extern "C" int mtx_attn_decode_paged(int dtype, int cache_dtype, int B, int H, i
                 "workspace: %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
   // one XCD reads the lines that heads share, where its pieces are about as many as
   // another's (64 sequences of 1000 to 3000 rows, 8 heads of 16 bf16 stored by rows:
-  // 25 us, else 47)
+  // 27 us, else 50)
   const int64_t slots = plan.P ? plan.P : (int64_t)B * plan.S;
   const int lines = Hkv > 1 && std::max(kp_strides[1], vp_strides[1]) * (cache_dtype == MTX_F32 ? 4 : 2) < 128 &&
                     (slots % 8 == 0 || slots >= 64);
