@@ -82,6 +82,7 @@ class PagedKVCache:
         self._prompt = False  # whether they are their sequences' first
         self._ragged = False  # whether sequences that get some get different numbers
         self._active = None  # the lengths, 0 where none is new, if that is anywhere
+        self._got = np.zeros(batch, bool)  # which sequences get some
         self._new = np.zeros(batch, np.int32)  # how many of each sequence undo can take back
         self._written = set()  # the layers that have them
 
@@ -141,14 +142,16 @@ class PagedKVCache:
             self.counts = None if n.min() == n.max() else dev.from_host(n, np.int32).t
         self._rows = int(n.max())
         self._active = None if n.min() else dev.from_host(np.where(n > 0, grown, 0), np.int32).t
-        self._len, self._new = grown, n
+        # rows reserved before that no layer has yet go with these
+        self._len, self._new, self._got = grown, n if self._written else n + self._new, n > 0
         self._written.clear()
 
     def undo(self):
-        """Take back the rows reserved last, in all layers: lengths, table and
-        free pages are what they were, the rows' weights 0.  (What a layer's
-        attend has added to other rows' weights stays.)  Nothing happens if there
-        are none, or trim has cut the sequences since."""
+        """Take back the rows reserved last, in all layers (and those reserved
+        before them if no layer had written any): lengths, table and free pages
+        are what they were, the rows' weights 0.  (What a layer's attend has added
+        to other rows' weights stays.)  Nothing happens if there are none, or trim
+        has cut the sequences since."""
         if not self._new.any():
             return
         grown, self._len = self._len, self._len - self._new
@@ -262,7 +265,7 @@ class PagedKVCache:
         n = min(self.observed, T)
         if layer == 0:  # the rows that each of those positions sees
             back = np.arange(n - 1, -1, -1, dtype=np.int32)[:, None]
-            lengths = np.where(self._new > 0, self._len, 0)
+            lengths = np.where(self._got, self._len, 0)
             self._seen = dev.from_host(np.maximum(lengths - back, 0), np.int32).t
         w = self.weights[layer]
         for i in range(n):

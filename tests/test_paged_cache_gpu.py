@@ -350,7 +350,7 @@ def run_paged(m, cache, tokens, first):
 def state(c):
     """What a cache holds, as far as its calls can tell."""
     return dict(lengths=c.lengths.numpy().tolist(), host=[c.length(b) for b in range(c.batch)],
-                table=c.table.numpy().tolist(), pages=c._tab.tolist(), free=list(c._free))
+                table=c.table.numpy().tolist(), pages=c._tab.tolist(), free=sorted(c._free))
 
 
 @pytest.mark.parametrize("keep", [None, 20])
@@ -747,3 +747,28 @@ def test_generate_with_bf16_pages_is_the_rounded_caches_model(dev):
     y = y - y.max(-1, keepdims=True)
     y = y - np.log(np.exp(y).sum(-1, keepdims=True))
     assert np.abs(lp - np.take_along_axis(y, ids[:, T0:, None], -1)[..., 0]).max() <= 1e-4
+
+
+def test_rows_reserved_twice_and_never_written_are_all_taken_back(dev):
+    """A refusal after two calls of reserve without a layer's append between
+    leaves neither's rows; once layers have written, only the last ones'."""
+    m = model()
+    rng = np.random.default_rng(35)
+    c = m.paged_cache(2, page=4)
+    before = state(c)
+    for n in (3, [2, 4]):
+        c.reserve(n)
+    with pytest.raises(ValueError, match="empty sequences"):
+        run_paged(m, c, rng.integers(0, 50, (2, 4)), [0, 0])
+    assert state(c) == before
+    c.reserve(5)
+    run_paged(m, c, rng.integers(0, 50, (2, 5)), [0, 0])
+    before = state(c)
+    for n in (1, 1, [0, 7]):
+        c.reserve(n)
+    c.undo()
+    assert state(c) == before and c.length(0) == 5
+    c.reserve(1)
+    run_paged(m, c, rng.integers(0, 50, (2, 1)), [5, 5])
+    c.undo()
+    assert state(c) == before
