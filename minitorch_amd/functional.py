@@ -475,9 +475,9 @@ def cross_entropy(logits, labels):
 
 def token_logprobs(logits, tokens, top=0, temperature=1.0):
     """Log probabilities of one token per row of (N, V) logits under
-    softmax(logits / temperature) (log_softmax, functional.py:81-97, at the
-    tokens; the distribution GPT.generate samples from, transformer.py:97-100),
-    and the entropy of each row's distribution: two (N,) Tensors, both
+    softmax(logits / temperature), temperature from 1e-38 to 1e27 (log_softmax,
+    functional.py:81-97, at the tokens; the distribution GPT.generate samples
+    from, transformer.py:97-100), and the entropy of each row's distribution: two (N,) Tensors, both
     differentiable (mtx_token_logprobs and its backward, one pass each).  A
     negative token means that its row has none (padding): log probability 0, no
     gradient.  Returns (logprobs, entropy, top_ids, top_logprobs), the latter

@@ -1213,7 +1213,7 @@ def _logprobs_plan(logits, tokens, top, logprob, entropy, lse, top_ids, top_logp
 def token_logprobs(logits, tokens, top: int = 0, scale: float = 1.0, logprob=None, entropy=None, lse=None,
                    top_ids=None, top_logprobs=None):
     """Log probabilities of one token per row of logits (rows, V), fp32 or
-    bf16, at scale * logits, the entropy, and the `top` (<= 64) most likely
+    bf16, at scale * logits (1e-27 to 1e38), the entropy, and the `top` (<= 64) most likely
     tokens with theirs, ties to the lowest id (mtx_token_logprobs).  A token
     outside [0, V) means the row has none (logprob 0).  Returns (logprob,
     entropy, lse) fp32 (rows,), top_ids int64 and top_logprobs fp32
