@@ -248,6 +248,21 @@ int mtx_dropout_keep_philox(uint8_t* keep, int64_t rows, int cols, int64_t ld, f
                             uint64_t seed, uint64_t offset, void* stream);
 
 /*
+ * Dropout whose mask is never stored (Dropout.forward, layers.py:113-126):
+ *   y = residual + (keep ? x * scale : 0)          (residual may be NULL)
+ * over rows x cols values of fp32 or bf16, row strides ldx, ldr, ldy; x, residual
+ * and y may be one array.  keep is mtx_dropout_keep_philox's: element e has word
+ * e % 4 of counter offset + base[0] + e/4 (base, device memory: NULL counts as 0)
+ * with `subsequence` as the counter's third word.  The gradient is the same call on the
+ * upstream gradient; with residual = y it is added.  A recorded call draws other
+ * numbers in every replay if base[0] changes in between.  0 <= p < 1.  At most 2^33
+ * values.
+ */
+int mtx_dropout(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y, int64_t ldy,
+                int64_t rows, int cols, float p, float scale, uint64_t seed, uint64_t offset, uint32_t subsequence,
+                const uint64_t* base, void* stream);
+
+/*
  * Packed q/k/v projection support.  MultiHeadAttention's q_proj, k_proj and
  * v_proj (transformer.py:32-34, three Linear(C, C) on the same input) run as
  * one GEMM over the concatenated (C_in, 3C) weight; the reference has no
@@ -834,6 +849,33 @@ int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void* logits, i
                            const float* lse, const float* entropy, const float* g_logprob, const float* g_entropy,
                            float scale, float* dlogits, int64_t ldd, int accumulate, void* stream);
 
+/*
+ * The vocabulary projection and the softmax cross-entropy (transformer.py:91,
+ * layers.py:31-37, loss.py:17-27) with their gradients, without the logits in
+ * memory as a whole.  x (n x C, row stride ldx) and w (C x V, strides swc, swv, one
+ * of them 1: a Linear's weight, or a (V, C) table transposed) are fp32 or bf16,
+ * bias fp32 (V) or NULL.  With z = x w + bias:
+ *   lse[r] = log sum exp z[r];  row_loss[r] = lse[r] - z[r][labels[r]];
+ *   loss[0] = the mean of row_loss over the rows that have a label.
+ * A label outside [0, V) is none: row_loss 0, no gradient; loss is 0 if no row has
+ * one.  dx (n x C), dw (C x V, strides sdc, sdv, one of them 1) and db (V) receive
+ * the gradients of loss; those that are NULL are not worked out.  dx and dw are
+ * fp32, or bf16 with bf16 inputs (grad_dtype; not looked at without gradients);
+ * db is fp32.  A logit of -inf has probability 0; a row of nothing else has
+ * lse -inf, row_loss +inf and, as gradient, its label's own term alone.  Infinities
+ * and NaN in x or w give NaN (fp32: in every logit that they meet).
+ * The rows are worked through in blocks whose logits (fp32) fill at most logits_bytes
+ * (one row at least); fewer, larger blocks are faster.  bf16 gradients are products of the logits' gradient rounded to bf16,
+ * fp32 ones of all its 24 bits; either way sums are fp32, rounded once.
+ * n < 2^31, C <= 2^20, V <= 2^27.  Deterministic.
+ */
+size_t mtx_linear_xent_workspace_bytes(int dtype, int grad_dtype, int64_t n, int C, int V, int bias,
+                                       int64_t logits_bytes);
+int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int V, const void* x, int64_t ldx, const void* w,
+                    int64_t swc, int64_t swv, const float* bias, const int64_t* labels, float* loss,
+                    float* row_loss, float* lse, void* dx, int64_t lddx, void* dw, int64_t sdc, int64_t sdv,
+                    float* db, int64_t logits_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------ */
 /* Embedding and optimizer                                                  */
 /* ------------------------------------------------------------------------ */
@@ -843,6 +885,24 @@ int mtx_embedding_fwd_f32(const float* weight, int64_t ldw, int64_t V, const int
 /* dweight[v, :] (+)= sum_{i: idx[i]==v} grad[i, :]  (np.add.at, tensor.py:382); deterministic */
 int mtx_embedding_bwd_f32(const int64_t* idx, int64_t n, const float* grad, int64_t ldg, float* dweight,
                           int64_t lddw, int64_t V, int C, int accumulate, void* stream);
+
+/*
+ * Scaled lookup: out[i, :] = scale * weight[ids[i], :] (layers.py:102-104), zeros
+ * where ids[i] is outside [0, V): no token, padding.  Table and output are fp32 or
+ * bf16 each, the product is rounded once.  n, V < 2^31.
+ */
+int mtx_embedding_lookup(int dtype, int out_dtype, const void* weight, int64_t ldw, int64_t V, const int64_t* ids,
+                         int64_t n, int C, float scale, void* out, int64_t ldo, void* stream);
+/*
+ * Its gradient by sorted tokens: dweight[v, :] (+)= scale * the sum of the rows
+ * grad[i, :] (fp32 or bf16) with ids[i] = v (np.add.at, tensor.py:382), in fp32 and
+ * in token order.  Tokens outside [0, V) add to nothing.  Without accumulate every row of dweight
+ * is written, with it only those that have tokens.  Deterministic.
+ */
+size_t mtx_embedding_grad_workspace_bytes(int64_t n, int64_t V, int C);
+int mtx_embedding_grad(int dtype, const int64_t* ids, int64_t n, const void* grad, int64_t ldg, float scale,
+                       float* dweight, int64_t lddw, int64_t V, int C, int accumulate, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /*
  * One-hot rows: out[i, v] = (idx[i] == v) as float32, (n, V) row-major.  With

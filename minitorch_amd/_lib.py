@@ -88,6 +88,8 @@ SIGNATURES = {
                                   _P, _I64P, _P, _I64P, _P, _I64P,
                                   _P, _SZ, _F, _I, _I, _P, _I64, _F, _P]),
     "mtx_dropout_keep_philox": (_I, [_P, _I64, _I, _I64, _F, C.c_uint64, C.c_uint64, _P]),
+    "mtx_dropout": (_I, [_I, _P, _I64, _P, _I64, _P, _I64, _I64, _I, _F, _F, C.c_uint64, C.c_uint64, C.c_uint32, _P,
+                         _P]),
     "mtx_pack3_f32": (_I, [_P, _P, _P, _I64, _I64, _P, _P]),
     "mtx_unpack3_f32": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P]),
     "mtx_attn_decode": (_I, [_I, _I, _I, _I, _I,
@@ -155,6 +157,12 @@ SIGNATURES = {
     "mtx_xent_bwd_f32": (_I, [_P, _I64, _P, _P, _P, _F, _P, _I64, _I64, _I, _I, _P]),
     "mtx_token_logprobs": (_I, [_I, _I64, _I, _P, _I64, _P, _F, _P, _P, _P, _I, _P, _P, _P, _SZ, _P]),
     "mtx_token_logprobs_bwd": (_I, [_I, _I64, _I, _P, _I64, _P, _P, _P, _P, _P, _F, _P, _I64, _I, _P]),
+    "mtx_linear_xent_workspace_bytes": (_SZ, [_I, _I, _I64, _I, _I, _I, _I64]),
+    "mtx_linear_xent": (_I, [_I, _I, _I64, _I, _I, _P, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _P, _I64,
+                             _I64, _P, _I64, _P, _SZ, _P]),
+    "mtx_embedding_lookup": (_I, [_I, _I, _P, _I64, _I64, _P, _I64, _I, _F, _P, _I64, _P]),
+    "mtx_embedding_grad_workspace_bytes": (_SZ, [_I64, _I64, _I]),
+    "mtx_embedding_grad": (_I, [_I, _P, _I64, _P, _I64, _F, _P, _I64, _I64, _I, _I, _P, _SZ, _P]),
     "mtx_embedding_fwd_f32": (_I, [_P, _I64, _I64, _P, _I64, _P, _I64, _I, _P]),
     "mtx_embedding_bwd_f32": (_I, [_P, _I64, _P, _I64, _P, _I64, _I64, _I, _I, _P]),
     "mtx_adam_blocks": (_I, [_I64P, _I, _I64P, _I64P]),
@@ -250,6 +258,7 @@ def call(fn_name: str, *args) -> None:
 # The stream every launch goes to: None = the null stream (eager work);
 # graphs.capture() points it at its capture stream while recording.
 _STREAM = [None]
+_GRAPH = [None]  # the graphs.Graph that is being recorded
 
 
 def strides(t) -> C.Array:

@@ -13,6 +13,12 @@ conv.py:66-95):
   causal_attention_packed      the same over a packed [q | k | v] tensor
   token_logprobs(x, tokens)    log probabilities of given tokens, the entropy
                                and the most likely alternatives, in one pass
+  embedding(weight, idx)       scaled table rows; the gradient by sorted tokens
+  dropout(x, p)                dropout (and a residual) whose mask is drawn on
+                               the device where it is used and never stored
+  linear_cross_entropy(x, W, b, labels)
+                               a projection and its cross entropy, with the
+                               gradients, without keeping the logits
 """
 from __future__ import annotations
 
@@ -514,3 +520,136 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
 
     out = _node(both, (logits,), "token_logprobs", _backward, _track(logits))
     return out[0], out[1], DeviceArray(ids), DeviceArray(tops)
+
+
+def embedding(weight, idx, scale=1.0):
+    """scale * weight[idx] for a (V, C) table (Embedding.forward, layers.py:102-104,
+    times a constant), (*idx.shape, C).  A negative id has no row: zeros, and no
+    gradient (padding); device-resident ids outside the table count as that too.
+    The gradient adds the rows up by token, in token order, from the tokens sorted
+    on the device (mtx_embedding_lookup, mtx_embedding_grad)."""
+    V, C = weight.shape
+    if not isinstance(idx, DeviceArray):
+        idx = np.asarray(idx)
+        if idx.size and idx.max() >= V:
+            raise IndexError(f"token out of range for a table of {V} rows")
+    ids = dev.index_array(idx)
+    shape = tuple(ids.shape) + (C,)
+    ids = ids.reshape(-1).contiguous().t
+    data = dev.empty(shape)
+    K.embedding_lookup(weight.data.t, ids, scale=scale, out=data.t.view(-1, C))
+    out = None
+
+    def _backward():
+        if weight.requires_grad:
+            target, acc = _grad_target(weight)
+            K.embedding_grad(ids, out.grad.contiguous().t.reshape(-1, C), target.t, scale=scale, accumulate=acc)
+
+    out = _node(data, (weight,), "embedding", _backward, _track(weight))
+    return out
+
+
+# Where F.dropout's generator stands: Philox4x32-10 keyed by the seed.  Eager calls
+# draw from its subsequence 1, one after another; every recorded graph has a
+# subsequence of its own (graphs.Graph); attention_keep_mask's masks are in
+# subsequence 0.
+_LAYER_RNG = {"seed": 0, "offset": 0}
+
+
+def set_dropout_seed(seed: int) -> None:
+    """Restart F.dropout's generator (a graph recorded before keeps its own)."""
+    _LAYER_RNG.update(seed=int(seed), offset=0)
+
+
+def dropout(x, p=0.5, residual=None):
+    """Inverted dropout of x (Dropout.forward, layers.py:113-126), plus `residual`
+    (shaped like x) if given -- the block's x + drop(mlp(...)) (transformer.py:65) --
+    in one pass each way.  The mask comes from the device generator and is drawn
+    again, not read, in the backward (mtx_dropout); set_dropout_seed restarts it.
+    In a recorded step every replay draws other masks."""
+    from . import _lib
+
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"dropout probability must be in [0, 1) (got {p})")
+    if residual is not None and tuple(residual.shape) != tuple(x.shape):
+        raise AssertionError(f"dropout: residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+    if p == 0.0:
+        return x if residual is None else residual + x
+    flat = lambda a: a.contiguous().t.reshape(1, -1)  # noqa: E731
+    calls = (x.data.size + 3) // 4
+    graph = _lib._GRAPH[0]
+    if graph is not None:
+        at = dict(seed=_LAYER_RNG["seed"], offset=graph.draws, subsequence=graph.subsequence, base=graph.base)
+        graph.draws += calls
+    else:
+        at = dict(seed=_LAYER_RNG["seed"], offset=_LAYER_RNG["offset"], subsequence=1)
+        _LAYER_RNG["offset"] += calls
+    data = DeviceArray(_empty(x.shape, x.data.t.dtype))
+    K.dropout(flat(x.data), p, residual=None if residual is None else flat(residual.data), out=flat(data), **at)
+    prev = (x,) if residual is None else (x, residual)
+    out = None
+
+    def _backward():
+        if residual is not None and residual.requires_grad:
+            _accum_grad(residual, out.grad)
+        if x.requires_grad:
+            g = flat(out.grad)
+            target, acc = _grad_target(x)
+            t = flat(target)
+            K.dropout(g, p, residual=t if acc else None, out=t, **at)
+
+    out = _node(data, prev, "dropout", _backward, _track(*prev))
+    return out
+
+
+def linear_cross_entropy(x, weight, bias, labels, logits_bytes=1 << 31):
+    """Mean softmax cross-entropy of the logits x @ weight + bias against integer
+    labels (cross_entropy of linear: transformer.py:91, loss.py:17-27) over the rows
+    that have one: a negative label has none (padding), nor has a device-resident
+    one outside the vocabulary.  x (..., C), weight (C, V) (a table's transpose
+    too), bias (V,) or None.  Where gradients are wanted they are worked out here,
+    while a block of rows' logits is there (mtx_linear_xent), and the backward
+    scales them by its upstream gradient."""
+    C, V = weight.shape
+    if x.shape[-1] != C:
+        raise AssertionError(f"Linear expects last dim {C}, got {x.shape[-1]}")
+    n = int(np.prod(x.shape[:-1]))
+    if isinstance(labels, DeviceArray):
+        lab = dev.index_array(labels)
+        if lab.size != n:
+            raise ValueError("one label per row expected")
+        lab = lab.reshape(n).contiguous()
+    else:
+        host = np.asarray(labels).reshape(-1)
+        if host.size != n:
+            raise ValueError("one label per row expected")
+        if host.size and host.max() >= V:
+            raise IndexError("label out of range")
+        lab = dev.index_array(host.astype(np.int64))
+    x2 = x.data.t.reshape(n, C)
+    if x2.stride(1) != 1 and C > 1:
+        x2 = x2.contiguous()
+    prev = (x, weight) if bias is None else (x, weight, bias)
+    track = _track(*prev)
+    want = [track and t.requires_grad for t in prev]
+    dx = dev.empty((n, C)).t if want[0] else None
+    dw = _empty_like(weight.data.t) if want[1] else None
+    db = dev.empty((V,)).t if want[-1] and bias is not None else None
+    loss, _, _ = K.linear_xent(x2, weight.data.t, lab.t, bias=None if bias is None else bias.data.t, dx=dx, dw=dw, db=db,
+                               logits_bytes=logits_bytes)
+    out = None
+
+    def _backward():
+        for t, g in zip(prev, (dx, dw, db)):
+            if not t.requires_grad or g is None:
+                continue
+            g = g.view(*t.shape) if t is x else g
+            if t.grad is None:
+                scaled = _empty_like(g)  # a transposed table's gradient keeps its layout
+                K.ewise("MUL", scaled, g, out.grad.t)
+                _accum_grad(t, DeviceArray(scaled), owned=True)
+            else:
+                K.ewise("MUL", _grad_target(t)[0].t, g, out.grad.t, accumulate=True)
+
+    out = _node(DeviceArray(loss.view()), prev, "linear_cross_entropy", _backward, track)
+    return out

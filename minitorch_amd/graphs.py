@@ -8,6 +8,8 @@ reused, so the step must read no host state that changes between calls:
 
 * inputs are device arrays; each call copies its arguments into static
   buffers the recorded step reads (device-to-device, outside the graph);
+* F.dropout reads where its numbers start from device memory, which replay()
+  moves on, so every replay draws others;
 * the optimizer runs in capturable mode (optim.Adam.capturable: persistent
   gradient buffers, step count in device memory), and its host-side
   bookkeeping (the step count, the bias-correction table) is advanced around
@@ -46,8 +48,12 @@ class Graph:
     """One recorded HIP graph.  ``with g.capture(): ...`` records every launch
     the block issues (none of them runs); ``g.replay()`` runs them all."""
 
+    _recorded = 0  # graphs recorded by this process
+
     def __init__(self):
         self._h = None
+        self.draws = 0  # calls of F.dropout's generator in one replay
+        self.replays = 0
 
     @contextmanager
     def capture(self):
@@ -55,16 +61,22 @@ class Graph:
             raise RuntimeError("this graph is already recorded")
         if L.capturing():
             raise RuntimeError("a capture is already in progress")
+        # F.dropout's numbers: a recorded call's lie at `base` plus what the step drew
+        # before it, in a subsequence of this graph's own; replay() moves base on
+        self.base, self.draws, self.replays = dev.zeros((1,), "int64").t, 0, 0
+        Graph._recorded += 1
+        self.subsequence = 1 + Graph._recorded
         dev.synchronize()
         s = _capture_stream()
         L.call("mtx_graph_begin", s)
         L._STREAM[0] = s
+        L._GRAPH[0] = self
         ok = False
         try:
             yield self
             ok = True
         finally:
-            L._STREAM[0] = None
+            L._STREAM[0] = L._GRAPH[0] = None
             h = C.c_void_p()
             rc = L.lib().mtx_graph_end(s, C.byref(h))
             if ok:
@@ -79,6 +91,9 @@ class Graph:
     def replay(self):
         if self._h is None:
             raise RuntimeError("nothing recorded")
+        if self.draws and self.replays:
+            L.call("mtx_fill", self.base.data_ptr(), 1, self.replays * self.draws, 8, None)
+        self.replays += 1
         L.call("mtx_graph_launch", self._h, None)
 
     def __del__(self):

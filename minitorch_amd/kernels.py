@@ -1299,6 +1299,212 @@ def embedding_bwd(idx, grad, dweight, accumulate=False):
     return dweight
 
 
+# ---------------------------------------------------------------------------
+# training with a large vocabulary
+# ---------------------------------------------------------------------------
+
+def _matrix(name, spec, shape=None):
+    """(shape, row stride, dtype) of a (rows, cols) view with contiguous rows."""
+    got, strides, dtype = spec
+    if len(got) != 2 or (shape is not None and tuple(got) != shape):
+        want = "(rows, cols)" if shape is None else shape
+        raise ValueError(f"{name} must be {want}, got shape {tuple(got)}")
+    rows, cols = got
+    if strides[1] != 1 and cols != 1:
+        raise ValueError(f"{name} must have contiguous rows")
+    ld = strides[0] if rows > 1 else cols
+    if ld < cols:
+        raise ValueError(f"{name}: its rows overlap")
+    return (rows, cols), ld, _dt(dtype)
+
+
+@functools.lru_cache(maxsize=512)
+def _lookup_plan(weight, ids, out):
+    (V, C), ldw, dtype = _matrix("weight", weight)
+    n = ids[0][0] if len(ids[0]) == 1 else -1
+    _vector("ids", ids, n, "int64")
+    _, ldo, odt = _matrix("out", out, (n, C))
+    if not V or not C:
+        raise ValueError(f"weight of shape {(V, C)} has no rows")
+    dev.device()
+    return (_code(dtype), _code(odt)), (ldw, V), (n, C), ldo
+
+
+def embedding_lookup(weight, ids, scale: float = 1.0, out=None):
+    """out[i] = scale * weight[ids[i]] for a (V, C) table, fp32 or bf16, and int64
+    (n,) ids (mtx_embedding_lookup); zeros for an id outside [0, V): padding.
+    out: (n, C), fp32 or bf16 (default: like the table)."""
+    if out is None:
+        out = dev.empty_buf((ids.shape[0], weight.shape[1]), _dt(weight))
+    if not (weight.is_cuda and ids.is_cuda and out.is_cuda):
+        _on_device(weight, ids, out)
+    codes, table, (n, C), ldo = _lookup_plan((weight.shape, weight.stride(), weight.dtype),
+                                             (ids.shape, ids.stride(), ids.dtype), (out.shape, out.stride(), out.dtype))
+    if dev.SEVERAL:
+        _on_gpu0(weight, ids, out)
+    if n:
+        L.call("mtx_embedding_lookup", *codes, weight.data_ptr(), *table, ids.data_ptr(), n, C, float(scale),
+               out.data_ptr(), ldo, L.stream_handle())
+    return out
+
+
+@functools.lru_cache(maxsize=512)
+def _grad_plan(ids, grad, dweight):
+    (V, C), lddw, wdt = _matrix("dweight", dweight)
+    if wdt != "float32":
+        raise ValueError("dweight must be fp32")
+    if not V or not C:
+        raise ValueError(f"dweight of shape {(V, C)} has no rows")
+    n = ids[0][0] if len(ids[0]) == 1 else -1
+    _vector("ids", ids, n, "int64")
+    _, ldg, dtype = _matrix("grad", grad, (n, C))
+    dev.device()
+    return _code(dtype), n, ldg, (lddw, V, C), L.lib().mtx_embedding_grad_workspace_bytes(n, V, C)
+
+
+def embedding_grad(ids, grad, dweight, scale: float = 1.0, accumulate: bool = False):
+    """dweight (V, C) fp32 = (with accumulate: +=) scale * the rows of grad (n, C),
+    fp32 or bf16, added up by their int64 (n,) ids in token order
+    (mtx_embedding_grad).  Rows whose id is outside [0, V) add to nothing."""
+    if not (ids.is_cuda and grad.is_cuda and dweight.is_cuda):
+        _on_device(ids, grad, dweight)
+    code, n, ldg, table, ws_bytes = _grad_plan((ids.shape, ids.stride(), ids.dtype),
+                                               (grad.shape, grad.stride(), grad.dtype),
+                                               (dweight.shape, dweight.stride(), dweight.dtype))
+    if dev.SEVERAL:
+        _on_gpu0(ids, grad, dweight)
+    ws = dev.empty_buf((ws_bytes,), "uint8") if ws_bytes else None
+    L.call("mtx_embedding_grad", code, ids.data_ptr() if n else None, n, grad.data_ptr() if n else None, ldg,
+           float(scale), dweight.data_ptr(), *table, 1 if accumulate else 0, _ptr(ws), ws_bytes, L.stream_handle())
+    return dweight
+
+
+@functools.lru_cache(maxsize=512)
+def _dropout_plan(x, residual, out):
+    (rows, cols), ldx, dtype = _matrix("x", x)
+    lds = [ldx]
+    for name, spec in (("residual", residual), ("out", out)):
+        if spec is None:
+            lds.append(cols)
+            continue
+        _, ld, dt = _matrix(name, spec, (rows, cols))
+        if dt != dtype:
+            raise ValueError(f"{name} must be {dtype} like x (got {dt})")
+        lds.append(ld)
+    dev.device()
+    return _code(dtype), rows, cols, lds
+
+
+def dropout(x, p: float, seed: int, offset: int = 0, residual=None, out=None, subsequence: int = 0, base=None):
+    """(residual +) x * keep / (1 - p) over a (rows, cols) view, fp32 or bf16, the
+    keep-mask drawn where it is used (mtx_dropout): dropout_keep_philox's at
+    (seed, offset), with the generator's `subsequence`.  The gradient is the same
+    call on the upstream gradient; out may be x or residual.  base: a device int64
+    (1,) array that is added to offset when the kernel runs.  Returns out."""
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"dropout probability must be in [0, 1) (got {p})")
+    if out is None:
+        out = dev.empty_buf(x.shape, _dt(x))
+    if not (x.is_cuda and out.is_cuda):
+        _on_device(x, out)
+    code, rows, cols, (ldx, ldr, ldo) = _dropout_plan((x.shape, x.stride(), x.dtype), _spec(residual),
+                                                      (out.shape, out.stride(), out.dtype))
+    if base is not None:
+        _on_device(base)
+        _vector("base", _spec(base), 1, "int64")
+    if dev.SEVERAL:
+        _on_gpu0(*(t for t in (x, residual, out, base) if t is not None))
+    if rows and cols:
+        L.call("mtx_dropout", code, x.data_ptr(), ldx, _ptr(residual), ldr, out.data_ptr(), ldo, rows, cols, p,
+               1.0 / (1.0 - p), int(seed) & (2**64 - 1), int(offset) & (2**64 - 1), int(subsequence) & (2**32 - 1),
+               _ptr(base), L.stream_handle())
+    return out
+
+
+def dropout_calls(x) -> int:
+    """How far a dropout of x moves its generator's offset on."""
+    return (x.numel() + 3) // 4
+
+
+def _either_order(name, spec, shape):
+    """(row stride, column stride, dtype) of a matrix that is contiguous along
+    its rows or its columns."""
+    got, strides, dtype = spec
+    if len(got) != 2 or (shape is not None and tuple(got) != shape):
+        raise ValueError(f"{name} must be {'(C, V)' if shape is None else shape}, got shape {tuple(got)}")
+    (rows, cols), (sr, sc) = got, strides
+    # strides of an axis of one element mean nothing
+    if cols == 1:
+        sc = 1 if sr != 1 or rows == 1 else rows
+    if rows == 1 and sc == 1:
+        sr = cols
+    if not ((sc == 1 and sr >= cols) or (sr == 1 and sc >= rows)):
+        raise ValueError(f"{name}: its rows or its columns must be contiguous and not overlap (strides "
+                         f"{tuple(strides)})")
+    return sr, sc, _dt(dtype)
+
+
+@functools.lru_cache(maxsize=512)
+def _xent_plan(x, w, labels, bias, loss, row_loss, lse, dx, dw, db, logits_bytes):
+    (n, C), ldx, dtype = _matrix("x", x)
+    code = _code(dtype)
+    swc, swv, wdt = _either_order("w", w, None)
+    V = w[0][1]
+    if w[0][0] != C or wdt != dtype or not C or not V:
+        raise ValueError(f"w must be ({C}, V) {dtype} like x, got {tuple(w[0])} {wdt}")
+    _vector("labels", labels, n, "int64")
+    for name, t, size in (("bias", bias, V), ("loss", loss, 1), ("row_loss", row_loss, n), ("lse", lse, n),
+                          ("db", db, V)):
+        _vector(name, t, size, "float32")
+    if db is not None and bias is None:
+        raise ValueError("db without a bias")
+    gdt, lddx, sdc, sdv = None, C, V, 1
+    if dx is not None:
+        _, lddx, gdt = _matrix("dx", dx, (n, C))
+    if dw is not None:
+        sdc, sdv, other = _either_order("dw", dw, (C, V))
+        if gdt not in (None, other):
+            raise ValueError(f"dx and dw must share a dtype (got {gdt}, {other})")
+        gdt = other
+    if gdt is None and db is not None:
+        gdt = "float32"
+    if gdt is not None and gdt not in ("float32", dtype):
+        raise ValueError(f"gradients of {dtype} inputs must be float32 or {dtype} (got {gdt})")
+    dev.device()
+    gcode = -1 if gdt is None else _code(gdt)
+    ws = L.lib().mtx_linear_xent_workspace_bytes(code, gcode, n, C, V, 0 if db is None else 1, logits_bytes)
+    return (code, gcode, n, C, V), ldx, (swc, swv), lddx, (sdc, sdv), ws
+
+
+def linear_xent(x, w, labels, bias=None, loss=None, row_loss=None, lse=None, dx=None, dw=None, db=None,
+                logits_bytes: int = 1 << 31):
+    """Softmax cross-entropy of the logits x @ w + bias, and its gradients, without
+    the logits in memory (mtx_linear_xent).  x (n, C) and w (C, V), contiguous along
+    either axis (a (V, C) table's .t()), fp32 or bf16; labels int64 (n,), one outside
+    [0, V): none; bias fp32 (V,).  Returns (loss (1,): the mean over the rows that
+    have a label, row_loss (n,), lse (n,)), fp32.  dx (n, C), dw (C, V) and db (V,),
+    where given, receive the gradients of loss: fp32, dx and dw also bf16 with bf16
+    inputs.  The logits of as many rows as fill logits_bytes are kept at a time."""
+    if logits_bytes < 1:
+        raise ValueError(f"logits_bytes must be positive (got {logits_bytes})")
+    n = x.shape[0]
+    loss = dev.empty_buf((1,), "float32") if loss is None else loss
+    row_loss, lse = (dev.empty_buf((n,), "float32") if t is None else t for t in (row_loss, lse))
+    if not (x.is_cuda and w.is_cuda and labels.is_cuda and loss.is_cuda and row_loss.is_cuda and lse.is_cuda):
+        _on_device(x, w, labels, loss, row_loss, lse)
+    sizes, ldx, sw, lddx, sd, ws_bytes = _xent_plan(
+        (x.shape, x.stride(), x.dtype), (w.shape, w.stride(), w.dtype), (labels.shape, labels.stride(), labels.dtype),
+        _spec(bias), (loss.shape, loss.stride(), loss.dtype), (row_loss.shape, row_loss.stride(), row_loss.dtype),
+        (lse.shape, lse.stride(), lse.dtype), _spec(dx), _spec(dw), _spec(db), int(logits_bytes))
+    if dev.SEVERAL:
+        _on_gpu0(*(t for t in (x, w, labels, bias, loss, row_loss, lse, dx, dw, db) if t is not None))
+    ws = dev.empty_buf((ws_bytes,), "uint8")
+    L.call("mtx_linear_xent", *sizes, x.data_ptr(), ldx, w.data_ptr(), *sw, _ptr(bias), labels.data_ptr(),
+           loss.data_ptr(), row_loss.data_ptr(), lse.data_ptr(), _ptr(dx), lddx, _ptr(dw), *sd, _ptr(db), int(logits_bytes),
+           ws.data_ptr(), ws_bytes, L.stream_handle())
+    return loss, row_loss, lse
+
+
 class AdamTable:
     """Device table for the one-launch multi-tensor Adam (layout of the C
     struct AdamEntry: p, g, m, v, n, block0 -- six 64-bit words)."""

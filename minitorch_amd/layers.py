@@ -97,15 +97,20 @@ class LayerNorm(Module):
 
 class Embedding(Module):
     """Lookup table (layers.py:92-104): weight[idx] gathers rows; the backward
-    scatters with repeated ids adding up (np.add.at)."""
+    scatters with repeated ids adding up (np.add.at).  With `scale` the rows come
+    out times that constant, negative ids are padding, and the gradient goes by
+    sorted tokens (F.embedding)."""
 
-    def __init__(self, num_embeddings, embed_dim):
+    def __init__(self, num_embeddings, embed_dim, scale=None):
         super().__init__()
         assert num_embeddings > 0 and embed_dim > 0, "sizes must be positive"
         self.weight = Tensor((np.random.randn(num_embeddings, embed_dim) * 0.02).astype(np.float32),
                              requires_grad=True)
+        self.scale = scale
 
     def forward(self, idx):
+        if self.scale is not None:
+            return F.embedding(self.weight, idx, self.scale)
         if isinstance(idx, DeviceArray):
             return self.weight[idx]
         return self.weight[np.asarray(idx)]
@@ -114,15 +119,21 @@ class Embedding(Module):
 class Dropout(Module):
     """Inverted dropout (layers.py:107-131).  Identity in eval mode or with
     p == 0 (the same Tensor is returned).  The keep-mask is drawn on the host
-    from NumPy's global RNG, as the reference draws it."""
+    from NumPy's global RNG, as the reference draws it, or, with rng="device",
+    on the device where it is used (F.dropout)."""
 
-    def __init__(self, p=0.5):
+    def __init__(self, p=0.5, rng="host"):
         super().__init__()
         assert 0.0 <= p < 1.0, "dropout probability must be in [0, 1)"
+        if rng not in ("host", "device"):
+            raise ValueError(f"unknown dropout RNG {rng!r}")
         self.p = p
+        self.rng = rng
 
     def forward(self, x):
         if not self._training or self.p == 0.0:
             return x
+        if self.rng == "device":
+            return F.dropout(x, self.p)
         mask = (np.random.rand(*x.shape) > self.p).astype(np.float32) * np.float32(1.0 / (1.0 - self.p))
         return x * Tensor(mask)

@@ -256,9 +256,10 @@ class MultiHeadAttention(Module):
 
 
 class TransformerBlock(Module):
-    """Pre-norm block: x + attn(ln1(x)), then x + mlp(ln2(x))."""
+    """Pre-norm block: x + attn(ln1(x)), then x + mlp(ln2(x)).  dropout_rng: where
+    the MLP's dropout draws (Dropout)."""
 
-    def __init__(self, n_embd, n_head, dropout=0.0):
+    def __init__(self, n_embd, n_head, dropout=0.0, dropout_rng="host"):
         super().__init__()
         self.ln1 = LayerNorm(n_embd)
         self.attn = MultiHeadAttention(n_embd, n_head, dropout)
@@ -267,7 +268,7 @@ class TransformerBlock(Module):
             Linear(n_embd, 4 * n_embd),
             GELU(),
             Linear(4 * n_embd, n_embd),
-            Dropout(dropout),
+            Dropout(dropout, dropout_rng),
         )
 
     def forward(self, x):
@@ -280,6 +281,8 @@ class TransformerBlock(Module):
             # Linear -> GELU -> Linear as one node (GELU in the GEMM epilogues)
             if isinstance(drop, Dropout) and (not drop._training or drop.p == 0.0):
                 x = F.mlp_gelu(self.ln2(x), fc1, fc2, residual=x)
+            elif isinstance(drop, Dropout) and drop.rng == "device":
+                x = F.dropout(F.mlp_gelu(self.ln2(x), fc1, fc2), drop.p, residual=x)
             else:
                 x = x + drop(F.mlp_gelu(self.ln2(x), fc1, fc2))
         else:
@@ -400,13 +403,13 @@ class TransformerBlock(Module):
 
 
 class GPT(Module):
-    def __init__(self, vocab_size, block_size, n_embd=64, n_head=4, n_layer=2, dropout=0.0):
+    def __init__(self, vocab_size, block_size, n_embd=64, n_head=4, n_layer=2, dropout=0.0, dropout_rng="host"):
         super().__init__()
         self.block_size = block_size
         self.tok_emb = Embedding(vocab_size, n_embd)
         self.pos_emb = Embedding(block_size, n_embd)
-        self.drop = Dropout(dropout)
-        self.blocks = [TransformerBlock(n_embd, n_head, dropout) for _ in range(n_layer)]
+        self.drop = Dropout(dropout, dropout_rng)
+        self.blocks = [TransformerBlock(n_embd, n_head, dropout, dropout_rng) for _ in range(n_layer)]
         self.ln_f = LayerNorm(n_embd)
         self.lm_head = Linear(n_embd, vocab_size)
 
@@ -438,13 +441,29 @@ class GPT(Module):
             idx = np.asarray(idx)
         B, T = idx.shape
         assert T <= self.block_size, f"sequence length {T} exceeds block_size {self.block_size}"
-        tok = self.tok_emb(idx)
+        return self.lm_head(self._trunk(self.tok_emb(idx), T))
+
+    def _trunk(self, tok, T):
+        """The blocks and the last LayerNorm over token embeddings (B, T, C)."""
         pos = self.pos_emb(self._positions(T))
         x = self.drop(tok + pos)
         for block in self.blocks:
             x = block(x)
-        x = self.ln_f(x)
-        return self.lm_head(x)
+        return self.ln_f(x)
+
+    def loss(self, idx, targets):
+        """Mean cross-entropy of the logits after idx (B, T) against targets (B, T)
+        -- cross_entropy_loss(model(idx), targets), char_transformer.py:70-77 -- for
+        vocabularies of any size: the logits are never kept (F.linear_cross_entropy)
+        and the token table's gradient goes by sorted tokens (F.embedding).
+        Negative ids are padding: such a token is embedded as zeros, such a target
+        counts nowhere."""
+        if not isinstance(idx, DeviceArray):
+            idx = np.asarray(idx)
+        B, T = idx.shape
+        assert T <= self.block_size, f"sequence length {T} exceeds block_size {self.block_size}"
+        tok = F.embedding(self.tok_emb.weight, idx, 1.0 if self.tok_emb.scale is None else self.tok_emb.scale)
+        return F.linear_cross_entropy(self._trunk(tok, T), self.lm_head.weight, self.lm_head.bias, targets)
 
     def generate_greedy(self, idx, max_new_tokens, return_margins=False, graph=True):
         """Greedy decoding: argmax (first maximum, as np.argmax) of the last
@@ -476,6 +495,8 @@ class GPT(Module):
         Tmax = T0 + n
         if Tmax > self.block_size:
             raise ValueError(f"prompt + new tokens = {Tmax} exceeds block_size {self.block_size}")
+        if any(e.scale not in (None, 1.0) for e in (self.tok_emb, self.pos_emb)):
+            raise NotImplementedError("greedy decode steps read embedding tables without a scale (use generate())")
         if n < 1:
             return (idx.copy(), np.empty((B, 0))) if return_margins else idx.copy()
         C = self.tok_emb.weight.shape[1]
