@@ -899,7 +899,7 @@ int mtx_embedding_lookup(int dtype, int out_dtype, const void* weight, int64_t l
  * in token order.  Tokens outside [0, V) add to nothing.  Without accumulate every row of dweight
  * is written, with it only those that have tokens.  Deterministic.
  */
-size_t mtx_embedding_grad_workspace_bytes(int64_t n, int64_t V, int C);
+size_t mtx_embedding_grad_workspace_bytes(int dtype, int64_t n, int64_t V, int C);
 int mtx_embedding_grad(int dtype, const int64_t* ids, int64_t n, const void* grad, int64_t ldg, float scale,
                        float* dweight, int64_t lddw, int64_t V, int C, int accumulate, void* workspace,
                        size_t workspace_bytes, void* stream);

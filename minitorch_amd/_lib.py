@@ -161,7 +161,7 @@ SIGNATURES = {
     "mtx_linear_xent": (_I, [_I, _I, _I64, _I, _I, _P, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _P, _I64,
                              _I64, _P, _I64, _P, _SZ, _P]),
     "mtx_embedding_lookup": (_I, [_I, _I, _P, _I64, _I64, _P, _I64, _I, _F, _P, _I64, _P]),
-    "mtx_embedding_grad_workspace_bytes": (_SZ, [_I64, _I64, _I]),
+    "mtx_embedding_grad_workspace_bytes": (_SZ, [_I, _I64, _I64, _I]),
     "mtx_embedding_grad": (_I, [_I, _P, _I64, _P, _I64, _F, _P, _I64, _I64, _I, _I, _P, _SZ, _P]),
     "mtx_embedding_fwd_f32": (_I, [_P, _I64, _I64, _P, _I64, _P, _I64, _I, _P]),
     "mtx_embedding_bwd_f32": (_I, [_P, _I64, _P, _I64, _P, _I64, _I64, _I, _I, _P]),

@@ -1359,7 +1359,7 @@ def _grad_plan(ids, grad, dweight):
     _vector("ids", ids, n, "int64")
     _, ldg, dtype = _matrix("grad", grad, (n, C))
     dev.device()
-    return _code(dtype), n, ldg, (lddw, V, C), L.lib().mtx_embedding_grad_workspace_bytes(n, V, C)
+    return _code(dtype), n, ldg, (lddw, V, C), L.lib().mtx_embedding_grad_workspace_bytes(_code(dtype), n, V, C)
 
 
 def embedding_grad(ids, grad, dweight, scale: float = 1.0, accumulate: bool = False):
