@@ -867,7 +867,8 @@ int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void* logits, i
  * The rows are worked through in blocks whose logits (fp32) fill at most logits_bytes
  * (one row at least); fewer, larger blocks are faster.  bf16 gradients are products of the logits' gradient rounded to bf16,
  * fp32 ones of all its 24 bits; either way sums are fp32, rounded once.
- * n < 2^31, C <= 2^20, V <= 2^27.  Deterministic.
+ * n < 2^31, C <= 2^20, V <= 2^27; bf16: V < 2^22, and rows of dx and dw less than 2^26
+ * values apart.  Deterministic.
  */
 size_t mtx_linear_xent_workspace_bytes(int dtype, int grad_dtype, int64_t n, int C, int V, int bias,
                                        int64_t logits_bytes);

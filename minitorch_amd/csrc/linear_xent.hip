@@ -47,6 +47,15 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ ro
   }
 }
 
+// rows x cols values of `size` bytes = 0
+__global__ __launch_bounds__(256) void zero_kernel(void* p, int size, int64_t sr, int64_t sc, int rows, int cols) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows * cols; i += (int64_t)gridDim.x * 256) {
+    const int64_t at = i / cols * sr + i % cols * sc;
+    if (size == 4) static_cast<float*>(p)[at] = 0.f;
+    else static_cast<bf16_t*>(p)[at] = 0;
+  }
+}
+
 // pieces: 0 no gradient, -1 dz in place of z (fp32), 1 or 3 bf16 pieces of dz.
 struct RowArgs {
   float* z;
@@ -128,13 +137,22 @@ constexpr int kRowWgs = 1024;
 struct Plan {
   int64_t ldz;
   int rows, wgs, pieces;
-  size_t z, dz, db, dw, gemm, bytes;  // offsets, and the whole
+  bool pack_x, pack_w;
+  size_t z, dz, db, dw, x, w, gemm, bytes;  // offsets, and the whole
 };
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// The rows whose logits are kept at a time are as many as have logits_bytes of them
-Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logits_bytes) {
+// Whether rows of `cols` bf16 values at p, ld values apart, are whole 16-byte vectors
+// that the products can take as they are.
+bool whole(const void* p, int64_t ld, int cols) {
+  return cols % 8 == 0 && ld % 8 == 0 && ld < kGemmBf16MaxLd && ((uintptr_t)p & 15) == 0;
+}
+
+// The rows whose logits are kept at a time are as many as have logits_bytes of them.
+// The query for the workspace's size does not know where the operands lie and counts
+// their copies (pack_x, pack_w) in.
+Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logits_bytes, bool pack_x, bool pack_w) {
   Plan p{};
   p.ldz = (V + 7) / 8 * 8;
   const int64_t fit = std::max<int64_t>(logits_bytes / (4 * p.ldz), 1);
@@ -150,15 +168,33 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   if (p.pieces && bias) at += up((size_t)p.wgs * p.ldz * 4);
   p.dw = at;  // a bf16 gradient of the weights is summed over blocks of rows in fp32
   if (p.pieces == 1 && p.rows < n) at += up((size_t)C * V * 4);
+  p.pack_x = dtype == MTX_BF16 && pack_x;
+  p.pack_w = dtype == MTX_BF16 && pack_w;
+  const int64_t c8 = (C + 7) / 8 * 8, longer = std::max<int64_t>(C * p.ldz, V * c8);
+  p.x = at;
+  if (p.pack_x) at += up((size_t)p.rows * c8 * 2);
+  p.w = at;
+  if (p.pack_w) at += up((size_t)longer * 2);
   p.gemm = at;
   size_t most = 0;
-  if (dtype == MTX_F32)
-    for (int r : {p.rows, (int)(n % p.rows)}) {
-      if (!r) continue;
-      most = std::max(most, mtx_gemm_workspace_bytes(r, V, C, 1));
-      if (p.pieces) most = std::max({most, mtx_gemm_workspace_bytes(r, C, V, 1), mtx_gemm_workspace_bytes(C, V, r, 1),
-                                     mtx_gemm_workspace_bytes(V, C, r, 1)});
+  for (int r : {p.rows, (int)(n % p.rows)}) {
+    if (!r) continue;
+    auto bytes = [&](int M, int N, int K) {
+      most = std::max(most, dtype == MTX_F32 ? mtx_gemm_workspace_bytes(M, N, K, 1)
+                                             : gemm_bf16_workspace_bytes(M, N, K, N == V && M == r ? 1 : p.pieces));
+    };
+    bytes(r, V, C);
+    if (!p.pieces) continue;
+    if (dtype == MTX_F32) {
+      bytes(r, C, V);
+      bytes(C, V, r);
+      bytes(V, C, r);
+    } else {
+      most = std::max({most, gemm_bf16_workspace_bytes(r, C, (int)p.ldz, p.pieces),
+                       gemm_bf16_workspace_bytes(C, V, r, p.pieces), gemm_bf16_workspace_bytes(V, C, r, p.pieces),
+                       gemm_bf16_workspace_bytes(r, C, V, p.pieces)});
     }
+  }
   p.bytes = at + up(most);
   return p;
 }
@@ -173,7 +209,7 @@ using namespace mtx;
 extern "C" size_t mtx_linear_xent_workspace_bytes(int dtype, int grad_dtype, int64_t n, int C, int V, int bias,
                                                   int64_t logits_bytes) {
   if (n < 0 || C < 1 || V < 1 || n >= (1LL << 31)) return 0;
-  return plan(dtype, grad_dtype, std::max<int64_t>(n, 1), C, V, bias != 0, logits_bytes).bytes;
+  return plan(dtype, grad_dtype, std::max<int64_t>(n, 1), C, V, bias != 0, logits_bytes, true, true).bytes;
 }
 
 extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int V, const void* x, int64_t ldx,
@@ -195,7 +231,14 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   MTX_CHECK_ARG(!dx || lddx >= C, "linear_xent: rows of dx overlap");
   MTX_CHECK_ARG(!dw || (sdv == 1 && sdc >= V) || (sdc == 1 && sdv >= C),
                 "linear_xent: dw needs a unit stride and rows that do not overlap");
-  const Plan p = plan(dtype, grad ? grad_dtype : -1, std::max<int64_t>(n, 1), C, V, db != nullptr, logits_bytes);
+  MTX_CHECK_ARG(dtype == MTX_F32 || (V < kGemmBf16MaxLd && (!dx || lddx < kGemmBf16MaxLdc) &&
+                                     (!dw || std::max(sdc, sdv) < kGemmBf16MaxLdc)),
+                "linear_xent: bf16 needs V below 2^22 and gradients' rows less than 2^26 values apart");
+  // W's rows in memory: of V values, or of C
+  const bool wv = swv == 1 && swc >= V;
+  const int64_t ldw = wv ? swc : swv;
+  const Plan p = plan(dtype, grad ? grad_dtype : -1, std::max<int64_t>(n, 1), C, V, db != nullptr, logits_bytes,
+                      !whole(x, ldx, C), !whole(w, ldw, wv ? V : C));
   MTX_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
                 "linear_xent: workspace of %zu bytes, need %zu aligned to 256", workspace_bytes, p.bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -205,39 +248,91 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   bf16_t* dz = reinterpret_cast<bf16_t*>(ws + p.dz);
   float* part = reinterpret_cast<float*>(ws + p.db);
   float* sum = reinterpret_cast<float*>(ws + p.dw);
+  bf16_t* xp = reinterpret_cast<bf16_t*>(ws + p.x);
+  bf16_t* wp = reinterpret_cast<bf16_t*>(ws + p.w);
   void* gws = ws + p.gemm;
   const size_t gbytes = workspace_bytes - p.gemm;
   const int64_t piece = (int64_t)p.rows * p.ldz;
+  const int c8 = (C + 7) / 8 * 8;
 
   hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, st, labels, n, V, inv);
   MTX_LAUNCHED();
-  for (int64_t r0 = 0; r0 < n || r0 == 0; r0 += p.rows) {
+  if (n == 0) {
+    if (dw) {
+      hipLaunchKernelGGL(zero_kernel, dim3((unsigned)std::min<int64_t>(((int64_t)C * V + 255) / 256, 16384)), dim3(256), 0,
+                         st, dw, grad_dtype == MTX_F32 ? 4 : 2, sdc, sdv, C, V);
+      MTX_LAUNCHED();
+    }
+  }
+  // the weights as the bf16 products take them
+  const bf16_t* wb = static_cast<const bf16_t*>(w);
+  int64_t ldwb = ldw;
+  if (p.pack_w && n) {
+    ldwb = wv ? p.ldz : c8;
+    if (int rc = pack_bf16(wb, ldw, wv ? C : V, wv ? V : C, wp, ldwb, st)) return rc;
+    wb = wp;
+  }
+  for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
     const int r = (int)std::min<int64_t>(p.rows, n - r0);
     const bool first = r0 == 0, last = r0 + r == n;
     const float* xf = static_cast<const float*>(x) + r0 * ldx;
     const bf16_t* xb = static_cast<const bf16_t*>(x) + r0 * ldx;
+    int64_t ldxb = ldx;
     int rc;
-    if (dtype == MTX_F32)
+    if (p.pack_x) {
+      ldxb = c8;
+      if ((rc = pack_bf16(xb, ldx, r, C, xp, ldxb, st))) return rc;
+      xb = xp;
+    }
+    if (dtype == MTX_F32) {
       rc = mtx_gemm_f32(r, V, C, 1, 1.f, xf, ldx, 1, 0, static_cast<const float*>(w), swc, swv, 0, 0.f, z, p.ldz, 1, 0,
                         bias, gws, gbytes, stream);
-    else
-      rc = gemm_bf16(GemmBf16{xb, ldx, 1, 0, static_cast<const bf16_t*>(w), swc, swv, 0, 1, z, p.ldz, 1, false, nullptr,
-                              0, 0, bias, r, V, C}, st);
-    if (rc) return rc;
-    if (r > 0) {
-      const RowArgs a{z, p.ldz, labels + r0, inv, row_loss + r0, lse + r0, dz, p.ldz, piece, db ? part : nullptr, r, V,
-                      p.pieces, first};
-      hipLaunchKernelGGL(row_kernel, dim3(first ? p.wgs : std::min(r, p.wgs)), dim3(256), 0, st, a);
-      MTX_LAUNCHED();
+    } else {
+      GemmBf16 g{};
+      g.a = xb;
+      g.lda = ldxb;
+      g.a_k = true;
+      g.b = wb;
+      g.ldb = ldwb;
+      g.b_k = !wv;
+      g.pieces = 1;
+      g.c = z;
+      g.ldc = p.ldz;
+      g.bias = bias;
+      g.M = r;
+      g.N = V;
+      g.K = c8;  // behind C: zeros in x
+      g.kb = wv ? C : 0;
+      rc = gemm_bf16(g, gws, st);
     }
-    if (dx && r > 0) {
-      if (dtype == MTX_F32)
+    if (rc) return rc;
+    const RowArgs a{z, p.ldz, labels + r0, inv, row_loss + r0, lse + r0, dz, p.ldz, piece, db ? part : nullptr, r, V,
+                    p.pieces, first};
+    hipLaunchKernelGGL(row_kernel, dim3(first ? p.wgs : std::min(r, p.wgs)), dim3(256), 0, st, a);
+    MTX_LAUNCHED();
+    if (dx) {
+      if (dtype == MTX_F32) {
         rc = mtx_gemm_f32(r, C, V, 1, 1.f, z, p.ldz, 1, 0, static_cast<const float*>(w), swv, swc, 0, 0.f,
                           static_cast<float*>(dx) + r0 * lddx, lddx, 1, 0, nullptr, gws, gbytes, stream);
-      else
-        rc = gemm_bf16(GemmBf16{dz, p.ldz, 1, piece, static_cast<const bf16_t*>(w), swv, swc, 0, p.pieces,
-                                static_cast<char*>(dx) + r0 * lddx * (grad_dtype == MTX_F32 ? 4 : 2), lddx, 1,
-                                grad_dtype == MTX_BF16, nullptr, 0, 0, nullptr, r, C, V}, st);
+      } else {
+        GemmBf16 g{};
+        g.a = dz;
+        g.lda = p.ldz;
+        g.pa = piece;
+        g.a_k = true;
+        g.b = wb;
+        g.ldb = ldwb;
+        g.b_k = wv;
+        g.pieces = p.pieces;
+        g.c = static_cast<char*>(dx) + r0 * lddx * (grad_dtype == MTX_F32 ? 4 : 2);
+        g.ldc = lddx;
+        g.c_bf16 = grad_dtype == MTX_BF16;
+        g.M = r;
+        g.N = C;
+        g.K = (int)p.ldz;  // behind V: zeros in dz, and zeros or nothing in W
+        g.kb = wv ? 0 : V;
+        rc = gemm_bf16(g, gws, st);
+      }
       if (rc) return rc;
     }
     if (dw) {
@@ -254,12 +349,10 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       } else {
         GemmBf16 g{};
         g.a = rows ? xb : dz;
-        g.sam = 1;
-        g.sak = rows ? ldx : p.ldz;
+        g.lda = rows ? ldxb : p.ldz;
         g.pa = rows ? 0 : piece;
         g.b = rows ? dz : xb;
-        g.sbk = rows ? p.ldz : ldx;
-        g.sbn = 1;
+        g.ldb = rows ? p.ldz : ldxb;
         g.pb = rows ? piece : 0;
         g.pieces = p.pieces;
         g.M = M;
@@ -269,18 +362,15 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
         const bool narrow = grad_dtype == MTX_BF16;
         g.c_bf16 = narrow && last;
         g.c = narrow && !last ? static_cast<void*>(sum) : dw;
-        g.scm = narrow && !last ? N : ld;
-        g.scn = 1;
+        g.ldc = narrow && !last ? N : ld;
         if (!first) {
           g.add = narrow ? sum : static_cast<const float*>(dw);
-          g.sdm = narrow ? N : ld;
-          g.sdn = 1;
+          g.ldadd = narrow ? N : ld;
         }
-        rc = gemm_bf16(g, st);
+        rc = gemm_bf16(g, gws, st);
       }
       if (rc) return rc;
     }
-    if (r == 0) break;
   }
   if (db) {
     hipLaunchKernelGGL(bias_kernel, dim3(cdiv(V, 256)), dim3(256), 0, st, part, p.ldz, n ? p.wgs : 0, V, db);

@@ -101,6 +101,9 @@ def xent(over):
     (xent, dict(loss=None), L.MTX_ERR_ARG, "null"),
     (xent, dict(row=None), L.MTX_ERR_ARG, "null"),
     (xent, dict(lse=None), L.MTX_ERR_ARG, "null"),
+    (xent, dict(V=1 << 22, swc=1 << 22, sdc=1 << 22), L.MTX_ERR_ARG, "2^22"),
+    (xent, dict(lddx=1 << 26), L.MTX_ERR_ARG, "2^26"),
+    (xent, dict(sdc=1 << 26), L.MTX_ERR_ARG, "2^26"),
     (xent, dict(logits=0), L.MTX_ERR_ARG, "logits_bytes"),
     (xent, dict(ws=None), L.MTX_ERR_ARG, "workspace"),
     (xent, dict(ws=p(128)), L.MTX_ERR_ARG, "workspace"),
