@@ -10,8 +10,8 @@
 // impose, by permuting which 16 bytes of global memory a lane asks for:
 //   contiguous along k: [row][32 k], chunk c (8 k) of row r at c ^ (r / 4 & 3), read
 //     with ds_read_b128: 16 rows cover the 16 bank groups once;
-//   contiguous along rows: [k][rows], chunk c (8 rows) of row k at c ^ 4 (k & 3),
-//     read with the transposing ds_read_b64_tr_b16: four k cover them.
+//   contiguous along rows: [32 rows][k][row], read with the transposing
+//     ds_read_b64_tr_b16: four k of a panel cover them.
 #include "gemm_bf16.h"
 
 #include <algorithm>
@@ -43,17 +43,17 @@ struct Tile {
   uint32_t off[PW];
   int ck;  // KC: the lane's first k in a stage
 
-  __device__ __forceinline__ void init(int64_t ld, int wid, int lane) {
+  __device__ __forceinline__ void init(const Bf16Matrix& m, int wid, int lane) {
 #pragma unroll
     for (int j = 0; j < PW; ++j) {
       const int at = (wid * PW + j) * 64 + lane;
       if constexpr (KC) {
         const int row = at / 4, c = (at & 3) ^ ((row >> 2) & 3);
-        off[j] = (uint32_t)row * (uint32_t)(ld * 2) + c * 16;
+        off[j] = (uint32_t)row * (uint32_t)(m.row * 2) + c * 16;
         ck = c * 8;  // (row / 4 & 3 is the same for all j)
       } else {
-        const int k = at / (R / 8), c = (at % (R / 8)) ^ ((k & 3) << 2);
-        off[j] = (uint32_t)k * (uint32_t)(ld * 2) + c * 16;
+        const int panel = at / 128, k = at / 4 % 32, c = at & 3;
+        off[j] = (uint32_t)panel * (uint32_t)(m.panel * 2) + (uint32_t)k * (uint32_t)(m.row * 2) + c * 16;
       }
     }
   }
@@ -75,8 +75,9 @@ struct Tile {
   // Where a lane reads MFMA operands, in bytes from the tile's begin: of rows rb + 32 x
   // .. and k = 16 kk .., lane l needs row l % 32 and k = 8 (l / 32) + 0..7.
   // KC: at[kk] + 2048 x.  Else the lane of a group of 16 addresses four rows of k row
-  // j / 4 and receives one row's four k: at[x], + 32 R kk, + 8 R for the second four.
-  static constexpr int NA = KC ? 2 : R / 64;
+  // j / 4 and receives one row's four k: at[0] + 2048 x + 1024 kk, + 256 for the second
+  // four.
+  static constexpr int NA = KC ? 2 : 1;
   __device__ __forceinline__ static void places(uint32_t (&at)[NA], int rb, int lane) {
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
@@ -85,8 +86,7 @@ struct Tile {
         at[i] = row * BK * 2 + ((c ^ ((row >> 2) & 3)) * 16);
       } else {
         const int G = lane >> 4, j = lane & 15, k = 8 * (G >> 1) + (j >> 2);
-        const int row = rb + 32 * i + 16 * (G & 1) + 4 * (j & 3);
-        at[i] = k * R * 2 + (((row >> 3) ^ ((j >> 2) << 2)) * 16) + (row & 7) * 2;
+        at[i] = rb * BK * 2 + k * 64 + (16 * (G & 1) + 4 * (j & 3)) * 2;
       }
     }
   }
@@ -108,9 +108,8 @@ struct Half {
 template <int MI, bool AK, bool BKC, int KK>
 __device__ __forceinline__ void frags(const uint32_t* pa, const uint32_t* pb, uint32_t la, uint32_t lb, bf16x8 (&fa)[MI],
                                       bf16x8 (&fb)[2]) {
-  constexpr int RA = 64 * MI, RB = 128;
+  const uint32_t a = la + pa[AK ? KK : 0], b = lb + pb[BKC ? KK : 0];
   if constexpr (AK && BKC) {
-    const uint32_t a = la + pa[KK], b = lb + pb[KK];
     if constexpr (MI == 4)
       asm volatile(MTX_RK("%4", "%7", "0") MTX_RK("%0", "%6", "0") MTX_RK("%5", "%7", "2048") MTX_RK("%1", "%6", "2048")
                        MTX_RK("%2", "%6", "4096") MTX_RK("%3", "%6", "6144") MTX_DONE
@@ -124,49 +123,44 @@ __device__ __forceinline__ void frags(const uint32_t* pa, const uint32_t* pb, ui
                    : "v"(a), "v"(b)
                    : "memory");
   } else {
+    constexpr int k = 1024 * KK;
     Half ha[MI], hb[2];
-    const uint32_t b0 = lb + pb[0], b1 = lb + pb[1];
     if constexpr (AK) {
-      const uint32_t a = la + pa[KK];
       if constexpr (MI == 4)
-        asm volatile(MTX_RR("%4", "%9", "%c11") MTX_RR("%5", "%9", "%c12") MTX_RK("%0", "%8", "0")
-                         MTX_RR("%6", "%10", "%c11") MTX_RR("%7", "%10", "%c12") MTX_RK("%1", "%8", "2048")
+        asm volatile(MTX_RR("%4", "%9", "%c10") MTX_RR("%5", "%9", "%c11") MTX_RK("%0", "%8", "0")
+                         MTX_RR("%6", "%9", "%c12") MTX_RR("%7", "%9", "%c13") MTX_RK("%1", "%8", "2048")
                              MTX_RK("%2", "%8", "4096") MTX_RK("%3", "%8", "6144") MTX_DONE
                      : "=&v"(fa[0]), "=&v"(fa[1]), "=&v"(fa[2]), "=&v"(fa[3]), "=&v"(hb[0].lo), "=&v"(hb[0].hi),
                        "=&v"(hb[1].lo), "=&v"(hb[1].hi)
-                     : "v"(a), "v"(b0), "v"(b1), "n"(32 * RB * KK), "n"(32 * RB * KK + 8 * RB)
+                     : "v"(a), "v"(b), "n"(k), "n"(k + 256), "n"(k + 2048), "n"(k + 2304)
                      : "memory");
       else
-        asm volatile(MTX_RR("%2", "%7", "%c9") MTX_RR("%3", "%7", "%c10") MTX_RK("%0", "%6", "0")
-                         MTX_RR("%4", "%8", "%c9") MTX_RR("%5", "%8", "%c10") MTX_RK("%1", "%6", "2048") MTX_DONE
+        asm volatile(MTX_RR("%2", "%7", "%c8") MTX_RR("%3", "%7", "%c9") MTX_RK("%0", "%6", "0")
+                         MTX_RR("%4", "%7", "%c10") MTX_RR("%5", "%7", "%c11") MTX_RK("%1", "%6", "2048") MTX_DONE
                      : "=&v"(fa[0]), "=&v"(fa[1]), "=&v"(hb[0].lo), "=&v"(hb[0].hi), "=&v"(hb[1].lo), "=&v"(hb[1].hi)
-                     : "v"(a), "v"(b0), "v"(b1), "n"(32 * RB * KK), "n"(32 * RB * KK + 8 * RB)
+                     : "v"(a), "v"(b), "n"(k), "n"(k + 256), "n"(k + 2048), "n"(k + 2304)
                      : "memory");
     } else {
-      const uint32_t a0 = la + pa[0], a1 = la + pa[1];
-      if constexpr (MI == 4) {
-        const uint32_t a2 = la + pa[2], a3 = la + pa[3];
-        asm volatile(MTX_RR("%8", "%16", "%c20") MTX_RR("%9", "%16", "%c21") MTX_RR("%0", "%12", "%c18")
-                         MTX_RR("%1", "%12", "%c19") MTX_RR("%10", "%17", "%c20") MTX_RR("%11", "%17", "%c21")
-                             MTX_RR("%2", "%13", "%c18") MTX_RR("%3", "%13", "%c19") MTX_RR("%4", "%14", "%c18")
-                                 MTX_RR("%5", "%14", "%c19") MTX_RR("%6", "%15", "%c18") MTX_RR("%7", "%15", "%c19")
+      if constexpr (MI == 4)
+        asm volatile(MTX_RR("%8", "%13", "%c14") MTX_RR("%9", "%13", "%c15") MTX_RR("%0", "%12", "%c14")
+                         MTX_RR("%1", "%12", "%c15") MTX_RR("%10", "%13", "%c16") MTX_RR("%11", "%13", "%c17")
+                             MTX_RR("%2", "%12", "%c16") MTX_RR("%3", "%12", "%c17") MTX_RR("%4", "%12", "%c18")
+                                 MTX_RR("%5", "%12", "%c19") MTX_RR("%6", "%12", "%c20") MTX_RR("%7", "%12", "%c21")
                                      MTX_DONE
                      : "=&v"(ha[0].lo), "=&v"(ha[0].hi), "=&v"(ha[1].lo), "=&v"(ha[1].hi), "=&v"(ha[2].lo),
                        "=&v"(ha[2].hi), "=&v"(ha[3].lo), "=&v"(ha[3].hi), "=&v"(hb[0].lo), "=&v"(hb[0].hi),
                        "=&v"(hb[1].lo), "=&v"(hb[1].hi)
-                     : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "v"(b0), "v"(b1), "n"(32 * RA * KK),
-                       "n"(32 * RA * KK + 8 * RA), "n"(32 * RB * KK), "n"(32 * RB * KK + 8 * RB)
+                     : "v"(a), "v"(b), "n"(k), "n"(k + 256), "n"(k + 2048), "n"(k + 2304), "n"(k + 4096), "n"(k + 4352),
+                       "n"(k + 6144), "n"(k + 6400)
                      : "memory");
-      } else {
-        asm volatile(MTX_RR("%4", "%10", "%c14") MTX_RR("%5", "%10", "%c15") MTX_RR("%0", "%8", "%c12")
-                         MTX_RR("%1", "%8", "%c13") MTX_RR("%6", "%11", "%c14") MTX_RR("%7", "%11", "%c15")
-                             MTX_RR("%2", "%9", "%c12") MTX_RR("%3", "%9", "%c13") MTX_DONE
+      else
+        asm volatile(MTX_RR("%4", "%9", "%c10") MTX_RR("%5", "%9", "%c11") MTX_RR("%0", "%8", "%c10")
+                         MTX_RR("%1", "%8", "%c11") MTX_RR("%6", "%9", "%c12") MTX_RR("%7", "%9", "%c13")
+                             MTX_RR("%2", "%8", "%c12") MTX_RR("%3", "%8", "%c13") MTX_DONE
                      : "=&v"(ha[0].lo), "=&v"(ha[0].hi), "=&v"(ha[1].lo), "=&v"(ha[1].hi), "=&v"(hb[0].lo),
                        "=&v"(hb[0].hi), "=&v"(hb[1].lo), "=&v"(hb[1].hi)
-                     : "v"(a0), "v"(a1), "v"(b0), "v"(b1), "n"(32 * RA * KK), "n"(32 * RA * KK + 8 * RA),
-                       "n"(32 * RB * KK), "n"(32 * RB * KK + 8 * RB)
+                     : "v"(a), "v"(b), "n"(k), "n"(k + 256), "n"(k + 2048), "n"(k + 2304)
                      : "memory");
-      }
 #pragma unroll
       for (int x = 0; x < MI; ++x) fa[x] = ha[x].both();
     }
@@ -196,8 +190,8 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
   const int wm = (wid >> 1) * 32 * MI, wn = (wid & 1) * 32 * NI;
   TA ta;
   TB tb;
-  ta.init(g.lda, wid, lane);
-  tb.init(g.ldb, wid, lane);
+  ta.init(g.a, wid, lane);
+  tb.init(g.b, wid, lane);
   uint32_t pa[TA::NA], pb[TB::NA];
   TA::places(pa, wm, lane);
   TB::places(pb, wn, lane);
@@ -244,14 +238,15 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
     r.left = q.s1 - q.s0;
     const int p = q.s0 / kpiece;
     r.k0 = (q.s0 - p * kpiece) * BK;
-    r.a = reinterpret_cast<const char*>(g.a + p * g.pa + (AK ? (int64_t)q.m0 * g.lda + r.k0 : (int64_t)r.k0 * g.lda + q.m0));
-    r.b = reinterpret_cast<const char*>(g.b + p * g.pb + (BKC ? (int64_t)q.n0 * g.ldb + r.k0 : (int64_t)r.k0 * g.ldb + q.n0));
-    // (to whole 16 bytes: a last one that is cut would read as zeros)
-    const int m8 = (g.M + 7) & ~7, n8 = (g.N + 7) & ~7, kb = g.kb ? g.kb : g.K;
-    r.la = 2 * (AK ? (int64_t)(g.M - 1 - q.m0) * g.lda + g.K - r.k0 : (int64_t)(g.K - 1 - r.k0) * g.lda + m8 - q.m0);
-    r.lb = 2 * (BKC ? (int64_t)(g.N - 1 - q.n0) * g.ldb + g.K - r.k0 : (int64_t)(kb - 1 - r.k0) * g.ldb + n8 - q.n0);
+    const int64_t fa = AK ? q.m0 * g.a.row + r.k0 / 32 * g.a.panel : r.k0 * g.a.row + q.m0 / 32 * g.a.panel;
+    const int64_t fb = BKC ? q.n0 * g.b.row + r.k0 / 32 * g.b.panel : r.k0 * g.b.row + q.n0 / 32 * g.b.panel;
+    r.a = reinterpret_cast<const char*>(g.a.p + p * g.a.piece + fa);
+    r.b = reinterpret_cast<const char*>(g.b.p + p * g.b.piece + fb);
+    r.la = 2 * (g.a.size - fa);
+    r.lb = 2 * (g.b.size - fb);
   };
-  const int64_t sa = AK ? 2 * BK : 2 * BK * g.lda, sb = BKC ? 2 * BK : 2 * BK * g.ldb;  // a stage's bytes along k
+  // a stage's bytes along k
+  const int64_t sa = 2 * (AK ? g.a.panel : BK * g.a.row), sb = 2 * (BKC ? g.b.panel : BK * g.b.row);
   int rbuf = 0;
   bool more = true;
   auto request = [&] {
@@ -271,8 +266,8 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
     r.la -= sa;
     r.lb -= sb;
     if (r.k0 >= g.K) {  // the next piece begins
-      r.a += 2 * g.pa - kpiece * sa;
-      r.b += 2 * g.pb - kpiece * sb;
+      r.a += 2 * g.a.piece - kpiece * sa;
+      r.b += 2 * g.b.piece - kpiece * sb;
       r.la += kpiece * sa;
       r.lb += kpiece * sb;
       r.k0 = 0;
@@ -336,6 +331,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
     constexpr int kSize = OUT >= 2 ? 2 : 4;
     uint32_t oo[NI], ao[NI];
     float bias[NI];
+    const float scale = g.scale ? *g.scale : 1.f;
 #pragma unroll
     for (int y = 0; y < NI; ++y) {
       const int n = 32 * y + lr;
@@ -361,7 +357,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
           const auto ra = rows(g.add, g.ldadd, 4, mw + 32 * x + 2 * e + i);
 #pragma unroll
           for (int y = 0; y < NI; ++y) {
-            v[i][y] = acc[x][y][e + i] + bias[y];
+            v[i][y] = scale * acc[x][y][e + i] + bias[y];
             if constexpr (OUT & 1) v[i][y] += __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ra, (int)ao[y], 0, 0));
           }
         }
@@ -379,12 +375,17 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
   }
 }
 
+struct __attribute__((aligned(16))) Pack8 {
+  bf16_t v[8];
+};
+
 // The tiles that were taken in ranges of k: the ranges' sums in order, then the
 // epilogue.
 template <int BM, int BN>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   const GemmBf16& g = a.g;
   const int t = blockIdx.x, tiles = gridDim.x;
+  const float scale = g.scale ? *g.scale : 1.f;
   const int tile = a.whole + t;
   const int panel = 8 * a.gx, first = tile / panel * 8, high = min(8, a.gy - first), in = tile % panel;
   const int m0 = (first + in % high) * BM, n0 = in / high * BN;
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (n + j >= g.N) break;
-      float x = v[j] + (g.bias ? g.bias[n + j] : 0.f);
+      float x = scale * v[j] + (g.bias ? g.bias[n + j] : 0.f);
       if (g.add) x += g.add[(int64_t)m * g.ldadd + n + j];
       if (g.c_bf16) static_cast<bf16_t*>(g.c)[(int64_t)m * g.ldc + n + j] = f2bf(x);
       else static_cast<float*>(g.c)[(int64_t)m * g.ldc + n + j] = x;
@@ -405,13 +406,28 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   }
 }
 
+// A thread a row's eight columns: whole 16 bytes of the panel.
 __global__ __launch_bounds__(256) void pack_kernel(const bf16_t* __restrict__ from, int64_t ldf, int64_t rows, int cols,
-                                                   bf16_t* __restrict__ to, int64_t ld) {
-  const int64_t total = rows * ld;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / ld;
-    const int c = (int)(i - r * ld);
-    to[i] = c < cols ? from[r * ldf + c] : 0;
+                                                   bf16_t* __restrict__ to, int64_t rows32, int panels, int vec) {
+  // 64 rows x 32 columns a workgroup and step
+  const int64_t blocks = (rows32 + 63) / 64 * panels;
+  for (int64_t i = blockIdx.x; i < blocks; i += gridDim.x) {
+    const int panel = (int)(i % panels);
+    const int64_t r = i / panels * 64 + threadIdx.x / 4;
+    const int c = panel * 32 + threadIdx.x % 4 * 8;
+    if (r >= rows32) continue;
+    Pack8 q{};
+    if (r < rows) {
+      const bf16_t* p = from + r * ldf + c;
+      if (vec && c + 8 <= cols) {
+        q = *reinterpret_cast<const Pack8*>(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j < cols) q.v[j] = p[j];
+      }
+    }
+    *reinterpret_cast<Pack8*>(to + (panel * rows32 + r) * 32 + threadIdx.x % 4 * 8) = q;
   }
 }
 
@@ -475,8 +491,11 @@ size_t gemm_bf16_workspace_bytes(int M, int N, int K, int pieces) {
 int gemm_bf16(const GemmBf16& g, void* workspace, hipStream_t st) {
   if (g.M == 0 || g.N == 0) return MTX_OK;
   const Plan p = plan(g.M, g.N, g.K, g.pieces);
-  MTX_CHECK_ARG(g.K > 0 && (g.a_k || !g.b_k) && g.lda < kGemmBf16MaxLd && g.ldb < kGemmBf16MaxLd &&
-                    (g.lda | g.ldb | g.pa | g.pb) % 8 == 0 && (!g.a_k || g.K % 8 == 0) &&
+  auto bad = [](const Bf16Matrix& m) {
+    return ((uintptr_t)m.p & 15) || (m.row | m.panel | m.piece | m.size) % 8 || m.row >= kGemmBf16MaxLd ||
+           m.panel >= kGemmBf16MaxPanel;
+  };
+  MTX_CHECK_ARG(g.K > 0 && (g.a_k || !g.b_k) && (!g.a_k || g.K % 8 == 0) && !bad(g.a) && !bad(g.b) &&
                     g.ldc < kGemmBf16MaxLdc && g.ldadd < kGemmBf16MaxLdc,
                 "bf16 product: operand layout");
   const Args a{g, p.gx, p.gy, p.whole, p.split, p.units, p.ksteps, p.per, static_cast<float*>(workspace)};
@@ -494,9 +513,12 @@ int gemm_bf16(const GemmBf16& g, void* workspace, hipStream_t st) {
   return MTX_OK;
 }
 
-int pack_bf16(const bf16_t* from, int64_t ldf, int64_t rows, int cols, bf16_t* to, int64_t ld, hipStream_t st) {
-  const int blocks = (int)std::min<int64_t>((rows * ld + 255) / 256, 16384);
-  hipLaunchKernelGGL(pack_kernel, dim3(blocks), dim3(256), 0, st, from, ldf, rows, cols, to, ld);
+int pack_bf16(const bf16_t* from, int64_t ldf, int64_t rows, int cols, bf16_t* to, int64_t rows32, hipStream_t st) {
+  const int panels = cdiv(cols, 32);
+  const int64_t blocks = (rows32 + 63) / 64 * panels;
+  const int vec = ((uintptr_t)from & 15) == 0 && ldf % 8 == 0;
+  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, st, from, ldf, rows,
+                     cols, to, rows32, panels, vec);
   MTX_LAUNCHED();
   return MTX_OK;
 }

@@ -19,13 +19,15 @@ __global__ __launch_bounds__(1024) void count_kernel(const int64_t* __restrict__
                                                      float* __restrict__ inv) {
   __shared__ int part[16];
   int c = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) c += labels[i] >= 0 && labels[i] < V;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < n; i += 1024) c += (uint64_t)labels[i] < (uint64_t)V;
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) c += __shfl_xor(c, m, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = c;
   __syncthreads();
   if (threadIdx.x == 0) {
     int t = 0;
+#pragma unroll
     for (int k = 0; k < 16; ++k) t += part[k];
     *inv = 1.0f / (float)(t > 0 ? t : 1);
   }
@@ -36,12 +38,14 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ ro
                                                     const float* __restrict__ inv, float* __restrict__ loss) {
   __shared__ float part[16];
   float s = 0.f;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < n; i += 1024) s += row_loss[i];
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     float t = 0.f;
+#pragma unroll
     for (int k = 0; k < 16; ++k) t += part[k];
     *loss = t * *inv;
   }
@@ -56,86 +60,279 @@ __global__ __launch_bounds__(256) void zero_kernel(void* p, int size, int64_t sr
   }
 }
 
-// pieces: 0 no gradient, -1 dz in place of z (fp32), 1 or 3 bf16 pieces of dz.
+// ---------------------------------------------------------------------------
+// The rows' statistics and losses and, in place of the logits or beside them, their
+// gradients.
+//
+// MODE: 0 no gradient; 1 dz = (p - onehot) / labels in place of z, fp32; 2 and 3 p -
+// onehot as one or three bf16 pieces (of 8 bits each: three hold all 24), in panels of
+// 32 columns, the factor 1 / labels left to the products: rounded to bf16, it would be
+// off by the same amount in every row.
+// ---------------------------------------------------------------------------
 struct RowArgs {
   float* z;
-  int64_t ldz;
+  int64_t ldz;  // a multiple of 32; what lies behind V is anything
   const int64_t* labels;
   const float* inv;
   float *row_loss, *lse;
   bf16_t* dz;
-  int64_t ldd, piece;
-  float* db;  // partial column sums, a row of ldz per workgroup; or nullptr
-  int rows, V, pieces;
+  int64_t rows32, piece;  // rows of a panel, values of a piece
+  float* db;  // partial column sums of p - onehot, a row of ldz per workgroup; or nullptr
+  int rows, V;
   bool first;  // the partial sums start here
 };
 
-__global__ __launch_bounds__(256) void row_kernel(const RowArgs a) {
-  __shared__ float part[8];
-  const int tid = threadIdx.x;
-  float* db = a.db ? a.db + (int64_t)blockIdx.x * a.ldz : nullptr;
-  if (db && a.first)
-    for (int v = tid; v < a.V; v += 256) db[v] = 0.f;
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    float* z = a.z + r * a.ldz;
-    float m = -INFINITY;
-    for (int v = tid; v < a.V; v += 256) m = fmaxf(m, z[v]);
-    m = wave_max(m);
-    __syncthreads();
-    if ((tid & 63) == 0) part[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    const float from = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-    for (int v = tid; v < a.V; v += 256) s += expf(z[v] - from);
-    s = wave_sum(s);
-    if ((tid & 63) == 0) part[4 + (tid >> 6)] = s;
-    __syncthreads();
-    s = (part[4] + part[5]) + (part[6] + part[7]);
-    const int64_t y = a.labels[r];
-    const bool some = y >= 0 && y < a.V;
-    if (tid == 0) {
-      const float l = m + logf(s);
-      a.lse[r] = l;
-      const float zy = some ? z[y] : 0.f;
-      a.row_loss[r] = !some ? 0.f : zy == -INFINITY && l == -INFINITY ? INFINITY : l - zy;
-    }
-    if (a.pieces == 0) continue;
-    __syncthreads();  // z[y] is read before it is overwritten
-    const float inv = *a.inv, rs = s == 0.f ? 0.f : 1.0f / s;
-    for (int v = tid; v < a.ldd; v += 256) {
-      float d = 0.f;
-      if (some && v < a.V) d = (expf(z[v] - from) * rs - (v == y ? 1.f : 0.f)) * inv;
-      if (a.pieces < 0) {
-        z[v] = d;
-      } else {
-        bf16_t* q = a.dz + r * a.ldd + v;
-        float rest = d;
-        for (int p = 0; p < a.pieces; ++p) {
-          const bf16_t h = f2bf(rest);
-          q[p * a.piece] = h;
-          rest -= bf2f(h);
-        }
-      }
-      if (db && v < a.V) db[v] += d;
+// d = p - onehot of row r's columns v0 + 4 sub ..  + 3 (v0 a multiple of 32, the same
+// for all lanes), where they lie before ldz
+template <int MODE>
+__device__ __forceinline__ void put_grad(const RowArgs& a, int64_t r, int v0, int sub, f32x4 d, float inv) {
+  if (v0 + 4 * sub >= a.ldz) return;
+  if constexpr (MODE == 1) {
+    char* p = reinterpret_cast<char*>(a.z + r * a.ldz + v0);
+    *reinterpret_cast<f32x4*>(p + 16u * sub) = f32x4{d[0] * inv, d[1] * inv, d[2] * inv, d[3] * inv};
+  } else {
+    // (32 bits: 2^18 rows of 128 panels)
+    char* p = reinterpret_cast<char*>(a.dz + ((int64_t)(v0 >> 5) * a.rows32 + r) * 32);
+    const uint32_t at = (uint32_t)(sub >> 3) * ((uint32_t)a.rows32 * 64u) + (sub & 7) * 8u;
+    uint2 h, m, l;
+    if constexpr (MODE == 2) {
+      *reinterpret_cast<uint2*>(p + at) = make_uint2(pk_bf16(d[0], d[1]), pk_bf16(d[2], d[3]));
+    } else {
+      split3(d, h, m, l);
+      *reinterpret_cast<uint2*>(p + at) = h;
+      *reinterpret_cast<uint2*>(p + 2 * a.piece + at) = m;
+      *reinterpret_cast<uint2*>(p + 4 * a.piece + at) = l;
     }
   }
 }
 
-// db = the column sums of the workgroups' partial ones, in their order
-__global__ __launch_bounds__(256) void bias_kernel(const float* __restrict__ part, int64_t ld, int n, int V,
-                                                   float* __restrict__ db) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= V) return;
-  float s = 0.f;
-  for (int i = 0; i < n; ++i) s += part[i * ld + v];
-  db[v] = s;
+// The rows' (m, s): maximum and sum of exp(z - m), to the label's loss
+__device__ __forceinline__ void put_loss(const RowArgs& a, int64_t r, float m, float s, bool some, float zy) {
+  const float l = m + logf(s);
+  a.lse[r] = l;
+  a.row_loss[r] = !some ? 0.f : zy == -INFINITY && l == -INFINITY ? INFINITY : l - zy;
 }
 
-constexpr int kRowWgs = 1024;
+// T threads a row, NV vectors of four columns each, all in registers: a row is read
+// once.  T = 64: a wave a row, four of them a workgroup; else a workgroup a row, whose
+// waves exchange their (maximum, sum) once.  Without column sums the next row is
+// requested while one is worked on; with them their registers are taken.
+template <int T, int NV, int MODE, bool DB>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void row_kernel(const RowArgs a) {
+  constexpr int kRows = T == 64 ? 4 : 1, kW = T / 64;
+  constexpr bool kNext = !DB && NV <= 8;
+  __shared__ float part[2][2][kW];
+  const int sub = threadIdx.x % T, lane = threadIdx.x & 63, w = threadIdx.x / 64 % kW;
+  const int step = gridDim.x * kRows;
+  f32x4 db[DB ? NV : 1];
+  if constexpr (DB)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) db[i] = zero4();
+  int r = blockIdx.x * kRows + (T == 64 ? threadIdx.x / T : 0);
+  if constexpr (T == 64) r = __builtin_amdgcn_readfirstlane(r);
+  const float inv = MODE == 1 ? *a.inv : 1.f;
+  f32x4 z[NV], next[kNext ? NV : 1];
+  auto request = [&](int row, f32x4* to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    float* p = a.z + (int64_t)row * a.ldz;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int left = max(0, (int)a.ldz - 4 * T * i) * 4;  // what lies behind reads as zeros
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(p + 4 * T * i, (short)0, left, 0x00020000);
+      to[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * sub, 0, 0));
+    }
+#endif
+  };
+  if constexpr (kNext)
+    if (r < a.rows) request(r, next);
+  int par = 0;
+  for (; r < a.rows; r += step, par ^= 1) {
+    const int64_t y = a.labels[r];
+    const bool some = (uint64_t)y < (uint64_t)a.V;
+    const float zy = some ? a.z[(int64_t)r * a.ldz + y] : 0.f;
+    if constexpr (kNext) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) z[i] = next[i];
+    } else {
+      request(r, z);
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (4 * T * (i + 1) > a.V)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (4 * (sub + T * i) + j >= a.V) z[i][j] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = fmaxf(m, z[i][j]);
+    }
+    m = wave_max(m);
+    if constexpr (kNext)
+      if (r + step < a.rows) request(r + step, next);
+    const float from = m == -INFINITY ? 0.f : m * kLog2e;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        z[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j], kLog2e, -from));
+        s += z[i][j];
+      }
+    s = wave_sum(s);
+    float mine = 1.f;  // what this wave's exponentials lack: exp(its maximum - the row's)
+    if constexpr (kW > 1) {
+      if (lane == 0) {
+        part[par][0][w] = m;
+        part[par][1][w] = s;
+      }
+      __syncthreads();
+      float M = -INFINITY, S = 0.f;
+#pragma unroll
+      for (int k = 0; k < kW; ++k) M = fmaxf(M, part[par][0][k]);
+      const float top = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int k = 0; k < kW; ++k) S += part[par][1][k] * __builtin_amdgcn_exp2f((part[par][0][k] - top) * kLog2e);
+      mine = __builtin_amdgcn_exp2f((m - top) * kLog2e);
+      m = M;
+      s = S;
+    }
+    if (sub == 0) put_loss(a, r, m, s, some, zy);
+    if constexpr (MODE != 0) {
+      const float f = s == 0.f ? 0.f : mine / s;
+      const int own = (int)y - 4 * sub;  // the label's column from this lane's first one
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        f32x4 d = zero4();
+        if (some) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[j] = z[i][j] * f - (own == 4 * T * i + j ? 1.f : 0.f);
+          // (behind V the exponentials are 0; if f is NaN, the products are not)
+          if (4 * T * (i + 1) > a.V)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (4 * (sub + T * i) + j >= a.V) d[j] = 0.f;
+          if constexpr (DB) db[i] += d;
+        }
+        put_grad<MODE>(a, r, 4 * T * i, sub, d, inv);
+      }
+    }
+  }
+  if constexpr (MODE >= 2) {  // the panels' rows behind the last one
+    for (int64_t q = a.rows + r % step; q < a.rows32; q += step)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) put_grad<MODE>(a, q, 4 * T * i, sub, zero4(), inv);
+  }
+  if constexpr (DB) {
+    float* out = a.db + (int64_t)blockIdx.x * a.ldz;
+    if constexpr (T == 64) {
+      __shared__ f32x4 sums[3][NV * 64];
+      const int k = threadIdx.x / 64;
+      if (k)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) sums[k - 1][sub + 64 * i] = db[i];
+      __syncthreads();
+      if (k) return;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) db[i] = ((db[i] + sums[0][sub + 64 * i]) + sums[1][sub + 64 * i]) + sums[2][sub + 64 * i];
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = 4 * (sub + T * i);
+      if (v >= a.ldz) continue;
+      f32x4* p = reinterpret_cast<f32x4*>(out + v);
+      *p = a.first ? db[i] : *p + db[i];
+    }
+  }
+}
+
+// Rows that no workgroup's registers hold: read twice, by 1024 threads.
+template <int MODE, bool DB>
+__global__ __launch_bounds__(1024) void long_row_kernel(const RowArgs a) {
+  __shared__ float part[2][16];
+  const int tid = threadIdx.x;
+  const float inv = MODE == 1 ? *a.inv : 1.f;
+  float* db = DB ? a.db + (int64_t)blockIdx.x * a.ldz : nullptr;
+  if constexpr (DB)
+    if (a.first)
+      for (int v = tid; v < a.ldz; v += 1024) db[v] = 0.f;
+  for (int64_t r = blockIdx.x; r < (MODE >= 2 ? a.rows32 : a.rows); r += gridDim.x) {
+    if (r >= a.rows) {
+      for (int v0 = 0; v0 < a.ldz; v0 += 4096) put_grad<MODE>(a, r, v0, tid, zero4(), inv);
+      continue;
+    }
+    const float* z = a.z + r * a.ldz;
+    const int64_t y = a.labels[r];
+    const bool some = (uint64_t)y < (uint64_t)a.V;
+    const float zy = some ? z[y] : 0.f;
+    float m = -INFINITY, s = 0.f;
+    for (int v0 = tid; v0 < a.V; v0 += 8192) {
+      float x[8], t = m;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = v0 + 1024 * j < a.V ? z[v0 + 1024 * j] : -INFINITY;
+        t = fmaxf(t, x[j]);
+      }
+      const float from = t == -INFINITY ? 0.f : t;
+      s *= __builtin_amdgcn_exp2f((m - from) * kLog2e);
+      m = t;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f((x[j] - from) * kLog2e);
+    }
+    const float wm = wave_max(m);
+    s = wave_sum(s * __builtin_amdgcn_exp2f((m - (wm == -INFINITY ? 0.f : wm)) * kLog2e));
+    __syncthreads();
+    if ((tid & 63) == 0) {
+      part[0][tid >> 6] = wm;
+      part[1][tid >> 6] = s;
+    }
+    __syncthreads();
+    m = -INFINITY;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) m = fmaxf(m, part[0][k]);
+    const float top = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += part[1][k] * __builtin_amdgcn_exp2f((part[0][k] - top) * kLog2e);
+    if (tid == 0) put_loss(a, r, m, s, some, zy);
+    if constexpr (MODE == 0) continue;
+    const float f = s == 0.f ? 0.f : 1.0f / s;
+    for (int v0 = 0; v0 < a.ldz; v0 += 4096) {
+      const int v = v0 + 4 * tid;
+      f32x4 d = zero4();
+      if (some && v < a.ldz) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(z + v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (v + j < a.V) d[j] = __builtin_amdgcn_exp2f((x[j] - top) * kLog2e) * f;
+          if (v + j == (int)y) d[j] -= 1.f;
+        }
+        if constexpr (DB) *reinterpret_cast<f32x4*>(db + v) += d;
+      }
+      put_grad<MODE>(a, r, v0, tid, d, inv);
+    }
+  }
+}
+
+// db = scale times the column sums of the workgroups' partial ones, in a fixed order:
+// 64 columns a workgroup, whose 16 waves take every 16th partial row
+__global__ __launch_bounds__(1024) void bias_kernel(const float* __restrict__ part, int64_t ld, int n, int V,
+                                                    const float* __restrict__ inv, float* __restrict__ db) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, v = blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (v < V)
+#pragma unroll 8
+    for (int i = w; i < n; i += 16) s += part[i * ld + v];
+  sums[w][lane] = s;
+  __syncthreads();
+  if (w || v >= V) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) s += sums[k][lane];
+  db[v] = s * *inv;
+}
 
 struct Plan {
-  int64_t ldz;
+  int64_t ldz, rows32;
   int rows, wgs, pieces;
   bool pack_x, pack_w;
   size_t z, dz, db, dw, x, w, gemm, bytes;  // offsets, and the whole
@@ -143,38 +340,47 @@ struct Plan {
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// From so many rows on the operands are copied into panels (gemm_bf16.h) also where the
+// products could take them as they are.
+constexpr int64_t kPackRows = 1024;
+
 // Whether rows of `cols` bf16 values at p, ld values apart, are whole 16-byte vectors
 // that the products can take as they are.
 bool whole(const void* p, int64_t ld, int cols) {
   return cols % 8 == 0 && ld % 8 == 0 && ld < kGemmBf16MaxLd && ((uintptr_t)p & 15) == 0;
 }
 
+// Row kernels' workgroups: about as many as the chip holds at once (as many partial
+// column sums are added up at the end).
+int row_wgs(int rows, int V) { return V <= 1024 ? std::min(cdiv(rows, 4), 1024) : std::min(rows, V <= 4096 ? 1024 : V <= 16384 ? 512 : 256); }
+
 // The rows whose logits are kept at a time are as many as have logits_bytes of them.
 // The query for the workspace's size does not know where the operands lie and counts
 // their copies (pack_x, pack_w) in.
 Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logits_bytes, bool pack_x, bool pack_w) {
   Plan p{};
-  p.ldz = (V + 7) / 8 * 8;
-  const int64_t fit = std::max<int64_t>(logits_bytes / (4 * p.ldz), 1);
+  p.ldz = (V + 31) / 32 * 32;
+  const int64_t fit = std::min<int64_t>(std::max<int64_t>(logits_bytes / (4 * p.ldz), 1), 1 << 18);
   p.rows = (int)std::min(n, fit < 256 ? fit : fit / 256 * 256);
-  p.wgs = std::min(p.rows, kRowWgs);
+  p.rows32 = (p.rows + 31) / 32 * 32;
+  p.wgs = row_wgs(p.rows, V);
   p.pieces = grads < 0 ? 0 : dtype == MTX_F32 ? -1 : grads == MTX_F32 ? 3 : 1;
   size_t at = 256;  // 1 / labels
   p.z = at;
   at += up((size_t)p.rows * p.ldz * 4);
   p.dz = at;
-  if (p.pieces > 0) at += up((size_t)p.pieces * p.rows * p.ldz * 2);
+  if (p.pieces > 0) at += up((size_t)p.pieces * p.rows32 * p.ldz * 2);
   p.db = at;
   if (p.pieces && bias) at += up((size_t)p.wgs * p.ldz * 4);
   p.dw = at;  // a bf16 gradient of the weights is summed over blocks of rows in fp32
   if (p.pieces == 1 && p.rows < n) at += up((size_t)C * V * 4);
   p.pack_x = dtype == MTX_BF16 && pack_x;
   p.pack_w = dtype == MTX_BF16 && pack_w;
-  const int64_t c8 = (C + 7) / 8 * 8, longer = std::max<int64_t>(C * p.ldz, V * c8);
+  const int64_t c32 = (C + 31) / 32 * 32;
   p.x = at;
-  if (p.pack_x) at += up((size_t)p.rows * c8 * 2);
+  if (p.pack_x) at += up((size_t)p.rows32 * c32 * 2);
   p.w = at;
-  if (p.pack_w) at += up((size_t)longer * 2);
+  if (p.pack_w) at += up((size_t)c32 * p.ldz * 2);
   p.gemm = at;
   size_t most = 0;
   for (int r : {p.rows, (int)(n % p.rows)}) {
@@ -197,6 +403,20 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   }
   p.bytes = at + up(most);
   return p;
+}
+
+template <int MODE, bool DB>
+void rows(const RowArgs& a, int wgs, hipStream_t st) {
+  auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(wgs), dim3(threads), 0, st, a); };
+  if (a.V <= 256) go(row_kernel<64, 1, MODE, DB>, 256);
+  else if (a.V <= 512) go(row_kernel<64, 2, MODE, DB>, 256);
+  else if (a.V <= 1024) go(row_kernel<64, 4, MODE, DB>, 256);
+  else if (a.V <= 4096) go(row_kernel<256, 4, MODE, DB>, 256);
+  else if (a.V <= 8192) go(row_kernel<256, 8, MODE, DB>, 256);
+  else if (a.V <= 16384) go(row_kernel<512, 8, MODE, DB>, 512);
+  else if (a.V <= 32768) go(row_kernel<1024, 8, MODE, DB>, 1024);
+  else if (a.V <= (DB ? 40960 : 65536)) go(row_kernel<1024, DB ? 10 : 16, MODE, DB>, 1024);
+  else go(long_row_kernel<MODE, DB>, 1024);
 }
 
 bool known(int dtype) { return dtype == MTX_F32 || dtype == MTX_BF16; }
@@ -238,7 +458,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   const bool wv = swv == 1 && swc >= V;
   const int64_t ldw = wv ? swc : swv;
   const Plan p = plan(dtype, grad ? grad_dtype : -1, std::max<int64_t>(n, 1), C, V, db != nullptr, logits_bytes,
-                      !whole(x, ldx, C), !whole(w, ldw, wv ? V : C));
+                      n >= kPackRows || !whole(x, ldx, C), n >= kPackRows || !whole(w, ldw, wv ? V : C));
   MTX_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
                 "linear_xent: workspace of %zu bytes, need %zu aligned to 256", workspace_bytes, p.bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -252,8 +472,8 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   bf16_t* wp = reinterpret_cast<bf16_t*>(ws + p.w);
   void* gws = ws + p.gemm;
   const size_t gbytes = workspace_bytes - p.gemm;
-  const int64_t piece = (int64_t)p.rows * p.ldz;
-  const int c8 = (C + 7) / 8 * 8;
+  const int64_t piece = p.rows32 * p.ldz;
+  const int c8 = (C + 7) / 8 * 8, v8 = (V + 7) / 8 * 8, c32 = (C + 31) / 32 * 32;
 
   hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, st, labels, n, V, inv);
   MTX_LAUNCHED();
@@ -265,35 +485,33 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
     }
   }
   // the weights as the bf16 products take them
-  const bf16_t* wb = static_cast<const bf16_t*>(w);
-  int64_t ldwb = ldw;
+  Bf16Matrix wm = bf16_rows(static_cast<const bf16_t*>(w), wv ? C : V, wv ? V : C, ldw);
   if (p.pack_w && n) {
-    ldwb = wv ? p.ldz : c8;
-    if (int rc = pack_bf16(wb, ldw, wv ? C : V, wv ? V : C, wp, ldwb, st)) return rc;
-    wb = wp;
+    const int64_t rows32 = wv ? c32 : p.ldz;
+    if (int rc = pack_bf16(wm.p, ldw, wv ? C : V, wv ? V : C, wp, rows32, st)) return rc;
+    wm = bf16_panels(wp, rows32, (wv ? p.ldz : c32) / 32, 0);
   }
   for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
     const int r = (int)std::min<int64_t>(p.rows, n - r0);
     const bool first = r0 == 0, last = r0 + r == n;
     const float* xf = static_cast<const float*>(x) + r0 * ldx;
     const bf16_t* xb = static_cast<const bf16_t*>(x) + r0 * ldx;
-    int64_t ldxb = ldx;
+    const int64_t r32 = (r + 31) / 32 * 32;
     int rc;
+    Bf16Matrix xm = bf16_rows(xb, r, C, ldx);
     if (p.pack_x) {
-      ldxb = c8;
-      if ((rc = pack_bf16(xb, ldx, r, C, xp, ldxb, st))) return rc;
-      xb = xp;
+      if ((rc = pack_bf16(xb, ldx, r, C, xp, r32, st))) return rc;
+      xm = bf16_panels(xp, r32, c32 / 32, 0);
     }
+    const Bf16Matrix dm = bf16_panels(dz, r32, p.ldz / 32, piece);
     if (dtype == MTX_F32) {
       rc = mtx_gemm_f32(r, V, C, 1, 1.f, xf, ldx, 1, 0, static_cast<const float*>(w), swc, swv, 0, 0.f, z, p.ldz, 1, 0,
                         bias, gws, gbytes, stream);
     } else {
       GemmBf16 g{};
-      g.a = xb;
-      g.lda = ldxb;
+      g.a = xm;
       g.a_k = true;
-      g.b = wb;
-      g.ldb = ldwb;
+      g.b = wm;
       g.b_k = !wv;
       g.pieces = 1;
       g.c = z;
@@ -302,13 +520,15 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       g.M = r;
       g.N = V;
       g.K = c8;  // behind C: zeros in x
-      g.kb = wv ? C : 0;
       rc = gemm_bf16(g, gws, st);
     }
     if (rc) return rc;
-    const RowArgs a{z, p.ldz, labels + r0, inv, row_loss + r0, lse + r0, dz, p.ldz, piece, db ? part : nullptr, r, V,
-                    p.pieces, first};
-    hipLaunchKernelGGL(row_kernel, dim3(first ? p.wgs : std::min(r, p.wgs)), dim3(256), 0, st, a);
+    const RowArgs a{z, p.ldz, labels + r0, inv, row_loss + r0, lse + r0, dz, r32, piece, db ? part : nullptr, r, V, first};
+    const int wgs = first ? p.wgs : std::min(p.wgs, row_wgs(r, V));
+    if (p.pieces == 0) rows<0, false>(a, wgs, st);
+    else if (p.pieces < 0) db ? rows<1, true>(a, wgs, st) : rows<1, false>(a, wgs, st);
+    else if (p.pieces == 1) db ? rows<2, true>(a, wgs, st) : rows<2, false>(a, wgs, st);
+    else db ? rows<3, true>(a, wgs, st) : rows<3, false>(a, wgs, st);
     MTX_LAUNCHED();
     if (dx) {
       if (dtype == MTX_F32) {
@@ -316,21 +536,18 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
                           static_cast<float*>(dx) + r0 * lddx, lddx, 1, 0, nullptr, gws, gbytes, stream);
       } else {
         GemmBf16 g{};
-        g.a = dz;
-        g.lda = p.ldz;
-        g.pa = piece;
+        g.a = dm;
         g.a_k = true;
-        g.b = wb;
-        g.ldb = ldwb;
+        g.b = wm;
         g.b_k = wv;
         g.pieces = p.pieces;
         g.c = static_cast<char*>(dx) + r0 * lddx * (grad_dtype == MTX_F32 ? 4 : 2);
         g.ldc = lddx;
         g.c_bf16 = grad_dtype == MTX_BF16;
+        g.scale = inv;
         g.M = r;
         g.N = C;
-        g.K = (int)p.ldz;  // behind V: zeros in dz, and zeros or nothing in W
-        g.kb = wv ? 0 : V;
+        g.K = v8;  // behind V: zeros in dz
         rc = gemm_bf16(g, gws, st);
       }
       if (rc) return rc;
@@ -348,12 +565,9 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
                           0, nullptr, gws, gbytes, stream);
       } else {
         GemmBf16 g{};
-        g.a = rows ? xb : dz;
-        g.lda = rows ? ldxb : p.ldz;
-        g.pa = rows ? 0 : piece;
-        g.b = rows ? dz : xb;
-        g.ldb = rows ? p.ldz : ldxb;
-        g.pb = rows ? piece : 0;
+        g.a = rows ? xm : dm;
+        g.b = rows ? dm : xm;
+        g.scale = inv;
         g.pieces = p.pieces;
         g.M = M;
         g.N = N;
@@ -373,7 +587,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
     }
   }
   if (db) {
-    hipLaunchKernelGGL(bias_kernel, dim3(cdiv(V, 256)), dim3(256), 0, st, part, p.ldz, n ? p.wgs : 0, V, db);
+    hipLaunchKernelGGL(bias_kernel, dim3(cdiv(V, 64)), dim3(1024), 0, st, part, p.ldz, n ? p.wgs : 0, V, inv, db);
     MTX_LAUNCHED();
   }
   hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, n, inv, loss);
