@@ -328,7 +328,9 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     // rows through a resource that begins at the pair's first row and ends with the
     // output: rows behind it are dropped, a column behind it has an offset that is
-    constexpr int kSize = OUT >= 2 ? 2 : 4;
+    // (fp32 results are large and not read again here: they pass the caches. The 1.6 GB
+    // of 8192 x 50021: 1120 -> 1060 us)
+    constexpr int kSize = OUT >= 2 ? 2 : 4, kNt = 2;
     uint32_t oo[NI], ao[NI];
     float bias[NI];
     const float scale = g.scale ? *g.scale : 1.f;
@@ -367,17 +369,13 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
 #pragma unroll
           for (int y = 0; y < NI; ++y) {
             if constexpr (OUT >= 2) __builtin_amdgcn_raw_buffer_store_b16(f2bf(v[i][y]), rc, (int)oo[y], 0, 0);
-            else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[i][y]), rc, (int)oo[y], 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[i][y]), rc, (int)oo[y], 0, kNt);
           }
         }
       }
 #endif
   }
 }
-
-struct __attribute__((aligned(16))) Pack8 {
-  bf16_t v[8];
-};
 
 // The tiles that were taken in ranges of k: the ranges' sums in order, then the
 // epilogue.
@@ -406,28 +404,41 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   }
 }
 
-// A thread a row's eight columns: whole 16 bytes of the panel.
+// 64 rows x 128 columns a workgroup and step, four rows' eight columns a thread: whole 16
+// bytes of a panel.  (Rows that are not aligned are read in 16 bytes all the same.)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 __global__ __launch_bounds__(256) void pack_kernel(const bf16_t* __restrict__ from, int64_t ldf, int64_t rows, int cols,
-                                                   bf16_t* __restrict__ to, int64_t rows32, int panels, int vec) {
-  // 64 rows x 32 columns a workgroup and step
-  const int64_t blocks = (rows32 + 63) / 64 * panels;
+                                                   bf16_t* __restrict__ to, int64_t rows32, int panels) {
+  const int across = (panels + 3) / 4;
+  const int64_t blocks = (rows32 + 63) / 64 * across;
   for (int64_t i = blockIdx.x; i < blocks; i += gridDim.x) {
-    const int panel = (int)(i % panels);
-    const int64_t r = i / panels * 64 + threadIdx.x / 4;
-    const int c = panel * 32 + threadIdx.x % 4 * 8;
-    if (r >= rows32) continue;
-    Pack8 q{};
-    if (r < rows) {
-      const bf16_t* p = from + r * ldf + c;
-      if (vec && c + 8 <= cols) {
-        q = *reinterpret_cast<const Pack8*>(p);
-      } else {
+    const int64_t r0 = i / across * 64, r = r0 + threadIdx.x / 16;
+    const int c0 = (int)(i % across) * 128, panel = c0 / 32 + threadIdx.x % 16 / 4, in = threadIdx.x % 4 * 8;
+    const int c = panel * 32 + in;
+    const bf16_t* p = from + r * ldf + c;
+    u32x4 q[4];
+    if (c0 + 128 <= cols && r0 + 64 <= rows) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c + j < cols) q.v[j] = p[j];
+      for (int k = 0; k < 4; ++k) q[k] = *reinterpret_cast<const u32x4_any*>(p + 16 * k * ldf);
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        bf16_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = r + 16 * k < rows && c + j < cols ? p[16 * k * ldf + j] : 0;
+        const u32x4 x = {v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16,
+                         v[6] | (uint32_t)v[7] << 16};
+        q[0] = k == 0 ? x : q[0];
+        q[1] = k == 1 ? x : q[1];
+        q[2] = k == 2 ? x : q[2];
+        q[3] = x;
       }
     }
-    *reinterpret_cast<Pack8*>(to + (panel * rows32 + r) * 32 + threadIdx.x % 4 * 8) = q;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (panel < panels && r + 16 * k < rows32)
+        *reinterpret_cast<u32x4*>(to + (panel * rows32 + r + 16 * k) * 32 + in) = q[k];
   }
 }
 
@@ -451,11 +462,12 @@ Plan plan(int M, int N, int K, int pieces) {
   const int rest = tiles % kWgs;
   p.whole = tiles - rest;
   // the number of ranges, of at least 8 stages each, after which the last round ends
-  // soonest; each costs its partial tile's way through memory
+  // soonest, in us: 0.5 a stage, 0.05 for a partial tile's way to memory and back, 5 for
+  // the launch that joins them
   p.split = 1;
   double best = 1e30;
   for (int s = 1; rest && s <= std::min(16, std::max(1, p.ksteps / 8)); ++s) {
-    const double cost = (double)cdiv(rest * s, kWgs) / s + (s > 1 ? 0.02 * s : 0.0);
+    const double cost = 0.5 * p.ksteps / s * cdiv(rest * s, kWgs) + (s > 1 ? 0.05 * rest * s + 5 : 0.0);
     if (cost < best) {
       best = cost;
       p.split = s;
@@ -515,10 +527,9 @@ int gemm_bf16(const GemmBf16& g, void* workspace, hipStream_t st) {
 
 int pack_bf16(const bf16_t* from, int64_t ldf, int64_t rows, int cols, bf16_t* to, int64_t rows32, hipStream_t st) {
   const int panels = cdiv(cols, 32);
-  const int64_t blocks = (rows32 + 63) / 64 * panels;
-  const int vec = ((uintptr_t)from & 15) == 0 && ldf % 8 == 0;
+  const int64_t blocks = (rows32 + 63) / 64 * cdiv(panels, 4);
   hipLaunchKernelGGL(pack_kernel, dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(256), 0, st, from, ldf, rows,
-                     cols, to, rows32, panels, vec);
+                     cols, to, rows32, panels);
   MTX_LAUNCHED();
   return MTX_OK;
 }

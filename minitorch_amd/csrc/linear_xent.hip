@@ -33,21 +33,37 @@ __global__ __launch_bounds__(1024) void count_kernel(const int64_t* __restrict__
   }
 }
 
-// loss = inv * sum of the rows' losses, in a fixed order.
-__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ row_loss, int64_t n,
-                                                    const float* __restrict__ inv, float* __restrict__ loss) {
+// loss = the mean of the rows' losses over those that have a label, summed in a fixed
+// order.
+__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ row_loss,
+                                                    const int64_t* __restrict__ labels, int64_t n, int V,
+                                                    float* __restrict__ loss) {
   __shared__ float part[16];
+  __shared__ int count[16];
   float s = 0.f;
+  int c = 0;
 #pragma unroll 8
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += row_loss[i];
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    s += row_loss[i];
+    c += (uint64_t)labels[i] < (uint64_t)V;
+  }
   s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) c += __shfl_xor(c, m, 64);
+  if ((threadIdx.x & 63) == 0) {
+    part[threadIdx.x >> 6] = s;
+    count[threadIdx.x >> 6] = c;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
     float t = 0.f;
+    int k = 0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) t += part[k];
-    *loss = t * *inv;
+    for (int i = 0; i < 16; ++i) {
+      t += part[i];
+      k += count[i];
+    }
+    *loss = t / (float)(k > 0 ? k : 1);
   }
 }
 
@@ -139,7 +155,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row_kernel(const RowArgs a)
     for (int i = 0; i < NV; ++i) {
       const int left = max(0, (int)a.ldz - 4 * T * i) * 4;  // what lies behind reads as zeros
       const auto rs = __builtin_amdgcn_make_buffer_rsrc(p + 4 * T * i, (short)0, left, 0x00020000);
-      to[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * sub, 0, 0));
+      to[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * sub, 0, MODE >= 2 ? 2 : 0));
     }
 #endif
   };
@@ -340,9 +356,10 @@ struct Plan {
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// From so many rows on the operands are copied into panels (gemm_bf16.h) also where the
-// products could take them as they are.
-constexpr int64_t kPackRows = 1024;
+// x is copied into panels (gemm_bf16.h), where the products could take it as it is, if
+// its copy is small beside them: 8192 x 1024 and a vocabulary of 50021 take 3284 us with
+// it (13 of them the copy) and 3355 without; the copy of W (62 us) gains nothing.
+constexpr int64_t kPanelRows = 2048, kPanelCols = 16384;
 
 // Whether rows of `cols` bf16 values at p, ld values apart, are whole 16-byte vectors
 // that the products can take as they are.
@@ -458,7 +475,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   const bool wv = swv == 1 && swc >= V;
   const int64_t ldw = wv ? swc : swv;
   const Plan p = plan(dtype, grad ? grad_dtype : -1, std::max<int64_t>(n, 1), C, V, db != nullptr, logits_bytes,
-                      n >= kPackRows || !whole(x, ldx, C), n >= kPackRows || !whole(w, ldw, wv ? V : C));
+                      (n >= kPanelRows && V >= kPanelCols) || !whole(x, ldx, C), !whole(w, ldw, wv ? V : C));
   MTX_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
                 "linear_xent: workspace of %zu bytes, need %zu aligned to 256", workspace_bytes, p.bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -475,8 +492,10 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   const int64_t piece = p.rows32 * p.ldz;
   const int c8 = (C + 7) / 8 * 8, v8 = (V + 7) / 8 * 8, c32 = (C + 31) / 32 * 32;
 
-  hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, st, labels, n, V, inv);
-  MTX_LAUNCHED();
+  if (grad) {
+    hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, st, labels, n, V, inv);
+    MTX_LAUNCHED();
+  }
   if (n == 0) {
     if (dw) {
       hipLaunchKernelGGL(zero_kernel, dim3((unsigned)std::min<int64_t>(((int64_t)C * V + 255) / 256, 16384)), dim3(256), 0,
@@ -590,7 +609,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
     hipLaunchKernelGGL(bias_kernel, dim3(cdiv(V, 64)), dim3(1024), 0, st, part, p.ldz, n ? p.wgs : 0, V, inv, db);
     MTX_LAUNCHED();
   }
-  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, n, inv, loss);
+  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, labels, n, V, loss);
   MTX_LAUNCHED();
   return MTX_OK;
 }
