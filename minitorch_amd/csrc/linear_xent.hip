@@ -483,7 +483,9 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   float* inv = reinterpret_cast<float*>(ws);
   float* z = reinterpret_cast<float*>(ws + p.z);
   bf16_t* dz = reinterpret_cast<bf16_t*>(ws + p.dz);
-  float* part = reinterpret_cast<float*>(ws + p.db);
+  // fp32: the bias' gradient comes with the weights', where their rows are contiguous
+  const bool sums = dtype == MTX_F32 && db && dw && sdv == 1;
+  float* part = db && !sums ? reinterpret_cast<float*>(ws + p.db) : nullptr;
   float* sum = reinterpret_cast<float*>(ws + p.dw);
   bf16_t* xp = reinterpret_cast<bf16_t*>(ws + p.x);
   bf16_t* wp = reinterpret_cast<bf16_t*>(ws + p.w);
@@ -542,12 +544,12 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       rc = gemm_bf16(g, gws, st);
     }
     if (rc) return rc;
-    const RowArgs a{z, p.ldz, labels + r0, inv, row_loss + r0, lse + r0, dz, r32, piece, db ? part : nullptr, r, V, first};
+    const RowArgs a{z, p.ldz, labels + r0, inv, row_loss + r0, lse + r0, dz, r32, piece, part, r, V, first};
     const int wgs = first ? p.wgs : std::min(p.wgs, row_wgs(r, V));
     if (p.pieces == 0) rows<0, false>(a, wgs, st);
-    else if (p.pieces < 0) db ? rows<1, true>(a, wgs, st) : rows<1, false>(a, wgs, st);
-    else if (p.pieces == 1) db ? rows<2, true>(a, wgs, st) : rows<2, false>(a, wgs, st);
-    else db ? rows<3, true>(a, wgs, st) : rows<3, false>(a, wgs, st);
+    else if (p.pieces < 0) part ? rows<1, true>(a, wgs, st) : rows<1, false>(a, wgs, st);
+    else if (p.pieces == 1) part ? rows<2, true>(a, wgs, st) : rows<2, false>(a, wgs, st);
+    else part ? rows<3, true>(a, wgs, st) : rows<3, false>(a, wgs, st);
     MTX_LAUNCHED();
     if (dx) {
       if (dtype == MTX_F32) {
@@ -580,8 +582,13 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       if (dtype == MTX_F32) {
         const float *a = rows ? xf : z, *b = rows ? z : xf;
         const int64_t lda = rows ? ldx : p.ldz, ldb = rows ? p.ldz : ldx;
-        rc = mtx_gemm_f32(M, N, r, 1, 1.f, a, 1, lda, 0, b, ldb, 1, 0, first ? 0.f : 1.f, static_cast<float*>(dw), ld, 1,
-                          0, nullptr, gws, gbytes, stream);
+        float* out = static_cast<float*>(dw);
+        if (sums)
+          rc = mtx_gemm_wgrad_f32(M, N, r, a, 1, lda, b, ldb, 1, first ? 0.f : 1.f, out, ld, 1, db, !first, gws, gbytes,
+                                  stream);
+        else
+          rc = mtx_gemm_f32(M, N, r, 1, 1.f, a, 1, lda, 0, b, ldb, 1, 0, first ? 0.f : 1.f, out, ld, 1, 0, nullptr, gws,
+                            gbytes, stream);
       } else {
         GemmBf16 g{};
         g.a = rows ? xm : dm;
@@ -605,7 +612,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       if (rc) return rc;
     }
   }
-  if (db) {
+  if (part || (db && n == 0)) {
     hipLaunchKernelGGL(bias_kernel, dim3(cdiv(V, 64)), dim3(1024), 0, st, part, p.ldz, n ? p.wgs : 0, V, inv, db);
     MTX_LAUNCHED();
   }

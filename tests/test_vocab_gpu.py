@@ -459,13 +459,15 @@ def test_linear_xent_same_bits_every_time(dev, dtype, out):
 def test_linear_xent_wanted_gradients_alone(dev, dtype, out):
     from minitorch_amd import kernels as K
 
-    args, db, _ = check_xent(50, 40, 210, dtype, out)
+    args, db, r = check_xent(50, 40, 210, dtype, out)
     full_ = [empty((50, 40), out), empty((40, 210), out), empty((210,))]
     K.linear_xent(*args, bias=db, dx=full_[0], dw=full_[1], db=full_[2])
     for i, name in enumerate(("dx", "dw")):
         g = empty(full_[i].shape, out)
         K.linear_xent(*args, bias=db, **{name: g})
         assert np.array_equal(host(g), host(full_[i]))
+    # db alone may be added up in another order: two sums of the 50 rows' terms, each off
+    # by at most 52 roundings of their magnitudes
     d = empty((210,))
     K.linear_xent(*args, bias=db, db=d)
-    assert np.array_equal(host(d), host(full_[2]))
+    inside(host(d), host(full_[2]), 2 * 52 * U * np.abs(r["dz"]).sum(0))
