@@ -40,10 +40,17 @@ struct GemmBf16 {
   const float* bias;   // or nullptr
   const float* scale;  // one value on the device, or nullptr
   int M, N, K;
+  // Instead of C (c = nullptr): of each row and each 64 columns the maximum and the sum
+  // of exp(C - maximum), stats[column / 64][m], and chosen[m] = C[m][columns[m]], for
+  // columns within N.
+  float2* stats;
+  const int64_t* columns;
+  float* chosen;
 };
 // Strides must be smaller than this (byte offsets within a tile are 32 bits): an
 // operand's rows', its panels' and a result's.
 constexpr int64_t kGemmBf16MaxLd = 1 << 22, kGemmBf16MaxPanel = (int64_t)1 << 28, kGemmBf16MaxLdc = 1 << 26;
+// (0 for products that give statistics)
 size_t gemm_bf16_workspace_bytes(int M, int N, int K, int pieces);
 int gemm_bf16(const GemmBf16& g, void* workspace, hipStream_t st);
 

@@ -176,7 +176,9 @@ __device__ __forceinline__ int here(int x) {
   return x;
 }
 
-// OUT: 0 fp32, 1 fp32 plus add, 2 bf16, 3 bf16 of the sum with add
+// OUT: 0 fp32, 1 fp32 plus add, 2 bf16, 3 bf16 of the sum with add; 4 the rows'
+// statistics: there the products are taken transposed, so that a lane holds 32 columns
+// of a row and only two lanes have to meet
 template <int MI, bool AK, bool BKC, int OUT>
 __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
   constexpr int BM = 64 * MI, BN = 128, NI = 2;
@@ -305,7 +307,8 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
         for (int x = 0; x < MI; ++x)
 #pragma unroll
           for (int y = 0; y < NI; ++y)
-            acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[x], fb[y], acc[x][y], 0, 0, 0);
+            acc[x][y] = OUT == 4 ? __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[y], fa[x], acc[x][y], 0, 0, 0)
+                                 : __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[x], fb[y], acc[x][y], 0, 0, 0);
       };
       products(std::integral_constant<int, 0>());
       products(std::integral_constant<int, 1>());
@@ -323,6 +326,45 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
         for (int e = 0; e < 16; ++e)
 #pragma unroll
           for (int y = 0; y < NI; ++y) p[(32 * x + 8 * (e / 4) + 4 * lh + e % 4) * BN + 32 * y + lr] = acc[x][y][e];
+      continue;
+    }
+    if constexpr (OUT == 4) {
+      // acc[x][y][e] = row 32 x + lane % 32, column 32 y + 8 (e / 4) + 4 (lane / 32) + e % 4
+      float bias[NI][16];
+#pragma unroll
+      for (int y = 0; y < NI; ++y)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int n = nw + 32 * y + 8 * (e / 4) + 4 * lh + e % 4;
+          bias[y][e] = g.bias && n < g.N ? g.bias[n] : 0.f;
+        }
+#pragma unroll
+      for (int x = 0; x < MI; ++x) {
+        const int m = mw + 32 * x + lr;
+        const int64_t t = m < g.M ? g.columns[m] : -1;
+        const int at = t >= nw && t < nw + 64 && t < g.N ? (int)(t - nw) : -1;
+        const int own = at >= 0 && ((at >> 2) & 1) == lh ? (at >> 5) * 16 + ((at & 31) >> 3) * 4 + (at & 3) : -1;
+        float top = -INFINITY, sum = 0.f, pick = 0.f;
+#pragma unroll
+        for (int y = 0; y < NI; ++y)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            acc[x][y][e] += bias[y][e];
+            // (behind N there may be anything)
+            if (nw + 64 > g.N && nw + 32 * y + 8 * (e / 4) + 4 * lh + e % 4 >= g.N) acc[x][y][e] = -INFINITY;
+            top = fmaxf(top, acc[x][y][e]);
+            pick = own == 16 * y + e ? acc[x][y][e] : pick;
+          }
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float from = top == -INFINITY ? 0.f : top * kLog2e;
+#pragma unroll
+        for (int y = 0; y < NI; ++y)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[x][y][e], kLog2e, -from));
+        sum += __shfl_xor(sum, 32, 64);
+        if (m < g.M && nw < g.N && lh == 0) g.stats[(int64_t)(nw / 64) * g.M + m] = make_float2(top, sum);
+        if (own >= 0) g.chosen[m] = pick;
+      }
       continue;
     }
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -451,7 +493,7 @@ struct Plan {
 };
 // Tiles that fill whole rounds of the chip are taken whole; those of the last round,
 // where it is not full, in ranges of k that fill it.
-Plan plan(int M, int N, int K, int pieces) {
+Plan plan(int M, int N, int K, int pieces, bool stats = false) {
   Plan p{};
   p.ksteps = (K + BK - 1) / BK * pieces;
   p.wide = (int64_t)cdiv(M, 256) * cdiv(N, 128) >= kWgs / 2;
@@ -466,7 +508,7 @@ Plan plan(int M, int N, int K, int pieces) {
   // the launch that joins them
   p.split = 1;
   double best = 1e30;
-  for (int s = 1; rest && s <= std::min(16, std::max(1, p.ksteps / 8)); ++s) {
+  for (int s = 1; rest && !stats && s <= std::min(16, std::max(1, p.ksteps / 8)); ++s) {
     const double cost = 0.5 * p.ksteps / s * cdiv(rest * s, kWgs) + (s > 1 ? 0.05 * rest * s + 5 : 0.0);
     if (cost < best) {
       best = cost;
@@ -486,11 +528,12 @@ void launch_out(const Args& a, int wgs, hipStream_t st) {
   const dim3 grid(wgs), block(kThreads);
   if (a.g.a_k && a.g.b_k) hipLaunchKernelGGL((gemm_bf16_kernel<MI, true, true, OUT>), grid, block, 0, st, a);
   else if (a.g.a_k) hipLaunchKernelGGL((gemm_bf16_kernel<MI, true, false, OUT>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((gemm_bf16_kernel<MI, false, false, OUT>), grid, block, 0, st, a);
+  else if constexpr (OUT != 4) hipLaunchKernelGGL((gemm_bf16_kernel<MI, false, false, OUT>), grid, block, 0, st, a);
 }
 template <int MI>
 void launch(const Args& a, int wgs, hipStream_t st) {
-  if (a.g.c_bf16) a.g.add ? launch_out<MI, 3>(a, wgs, st) : launch_out<MI, 2>(a, wgs, st);
+  if (a.g.stats) launch_out<MI, 4>(a, wgs, st);
+  else if (a.g.c_bf16) a.g.add ? launch_out<MI, 3>(a, wgs, st) : launch_out<MI, 2>(a, wgs, st);
   else a.g.add ? launch_out<MI, 1>(a, wgs, st) : launch_out<MI, 0>(a, wgs, st);
 }
 
@@ -502,12 +545,12 @@ size_t gemm_bf16_workspace_bytes(int M, int N, int K, int pieces) {
 
 int gemm_bf16(const GemmBf16& g, void* workspace, hipStream_t st) {
   if (g.M == 0 || g.N == 0) return MTX_OK;
-  const Plan p = plan(g.M, g.N, g.K, g.pieces);
+  const Plan p = plan(g.M, g.N, g.K, g.pieces, g.stats != nullptr);
   auto bad = [](const Bf16Matrix& m) {
     return ((uintptr_t)m.p & 15) || (m.row | m.panel | m.piece | m.size) % 8 || m.row >= kGemmBf16MaxLd ||
            m.panel >= kGemmBf16MaxPanel;
   };
-  MTX_CHECK_ARG(g.K > 0 && (g.a_k || !g.b_k) && (!g.a_k || g.K % 8 == 0) && !bad(g.a) && !bad(g.b) &&
+  MTX_CHECK_ARG(g.K > 0 && (g.a_k || (!g.b_k && !g.stats)) && (!g.a_k || g.K % 8 == 0) && !bad(g.a) && !bad(g.b) &&
                     g.ldc < kGemmBf16MaxLdc && g.ldadd < kGemmBf16MaxLdc,
                 "bf16 product: operand layout");
   const Args a{g, p.gx, p.gy, p.whole, p.split, p.units, p.ksteps, p.per, static_cast<float*>(workspace)};

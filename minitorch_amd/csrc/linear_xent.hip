@@ -329,6 +329,36 @@ __global__ __launch_bounds__(1024) void long_row_kernel(const RowArgs a) {
   }
 }
 
+// The losses from the statistics of 64 columns each: 16 rows a workgroup, 64 threads a
+// row.  (The logits themselves are never stored: 500 rows of 50021 took 88 us of
+// products and 23 of the rows' pass with them.)
+__global__ __launch_bounds__(1024) void stats_kernel(const float2* __restrict__ stats, int parts, const RowArgs a,
+                                                     const float* __restrict__ chosen) {
+  __shared__ float2 all[64][17];
+  const int row = threadIdx.x % 16, k0 = threadIdx.x / 16, r = blockIdx.x * 16 + row;
+  float m = -INFINITY, s = 0.f;
+  auto join = [](float& m, float& s, float2 o) {
+    const float top = fmaxf(m, o.x), from = top == -INFINITY ? 0.f : top;
+    s = s * __builtin_amdgcn_exp2f((m - from) * kLog2e) + o.y * __builtin_amdgcn_exp2f((o.x - from) * kLog2e);
+    m = top;
+  };
+  if (r < a.rows)
+#pragma unroll 4
+    for (int k = k0; k < parts; k += 64) join(m, s, stats[(int64_t)k * a.rows + r]);
+  all[k0][row] = make_float2(m, s);
+  __syncthreads();
+  for (int h = 32; h >= 1; h >>= 1) {
+    if (k0 < h) {
+      join(m, s, all[k0 + h][row]);
+      all[k0][row] = make_float2(m, s);
+    }
+    __syncthreads();
+  }
+  if (k0 || r >= a.rows) return;
+  const bool some = (uint64_t)a.labels[r] < (uint64_t)a.V;
+  put_loss(a, r, m, s, some, some ? chosen[r] : 0.f);
+}
+
 // db = scale times the column sums of the workgroups' partial ones, in a fixed order:
 // 64 columns a workgroup, whose 16 waves take every 16th partial row
 __global__ __launch_bounds__(1024) void bias_kernel(const float* __restrict__ part, int64_t ld, int n, int V,
@@ -383,8 +413,8 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   p.wgs = row_wgs(p.rows, V);
   p.pieces = grads < 0 ? 0 : dtype == MTX_F32 ? -1 : grads == MTX_F32 ? 3 : 1;
   size_t at = 256;  // 1 / labels
-  p.z = at;
-  at += up((size_t)p.rows * p.ldz * 4);
+  p.z = at;  // without gradients bf16 logits are never stored: their statistics are
+  at += p.pieces == 0 && dtype == MTX_BF16 ? up((size_t)p.rows * (cdiv(V, 64) * 8 + 4)) : up((size_t)p.rows * p.ldz * 4);
   p.dz = at;
   if (p.pieces > 0) at += up((size_t)p.pieces * p.rows32 * p.ldz * 2);
   p.db = at;
@@ -541,10 +571,22 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       g.M = r;
       g.N = V;
       g.K = c8;  // behind C: zeros in x
+      if (!grad) {
+        g.c = nullptr;
+        g.stats = reinterpret_cast<float2*>(z);
+        g.columns = labels + r0;
+        g.chosen = z + (int64_t)r * cdiv(V, 64) * 2;
+      }
       rc = gemm_bf16(g, gws, st);
     }
     if (rc) return rc;
     const RowArgs a{z, p.ldz, labels + r0, inv, row_loss + r0, lse + r0, dz, r32, piece, part, r, V, first};
+    if (!grad && dtype == MTX_BF16) {
+      hipLaunchKernelGGL(stats_kernel, dim3(cdiv(r, 16)), dim3(1024), 0, st, reinterpret_cast<const float2*>(z),
+                         cdiv(V, 64), a, z + (int64_t)r * cdiv(V, 64) * 2);
+      MTX_LAUNCHED();
+      continue;
+    }
     const int wgs = first ? p.wgs : std::min(p.wgs, row_wgs(r, V));
     if (p.pieces == 0) rows<0, false>(a, wgs, st);
     else if (p.pieces < 0) part ? rows<1, true>(a, wgs, st) : rows<1, false>(a, wgs, st);
