@@ -108,14 +108,31 @@ constexpr int kPiece = 32;  // sorted tokens a piece; rows of more are added in 
 constexpr int kWaves = 16, kMaxRows = 512;  // 32 KB of counts
 constexpr int kAhead = 16, kHeld = 32;  // groups of 64 ids that a wave requests at once, and holds
 
-// The tokens of the workgroup's `rows` table rows from v0 on.  cnt: [wave][R] in
-// LDS.  row(r, first, count) is called by one thread a row, with the row's place in
-// the sorted order of all tokens; put(r, at, i) by one lane a token, in order.
-// Returns where the range's tokens begin.
-template <typename Row, typename Put>
-__device__ __forceinline__ uint32_t sort_range(const int64_t* __restrict__ ids, int64_t n, int64_t v0, uint32_t rows,
-                                               int R, uint32_t* cnt, Row row, Put put) {
+struct SortArgs {
+  const int64_t* ids;
+  int64_t n, V;
+  int R;            // rows of the table a workgroup
+  uint2* span;      // [V] out: (first place in the sorted order, tokens)
+  uint32_t* order;  // [tokens] out: the sorted tokens' places
+  uint32_t* key;    // [tokens] out: and rows
+  uint32_t* tokens;  // out: how many they are
+  uint32_t* starts;  // [pieces] out: the row of more than a piece that begins there
+  // Rows without a token are set to 0 here, while the sorting waits for its memory (205
+  // MB of 50021 x 1024 rows, three quarters of them: XXX); nullptr: they are left alone
+  float* dw;
+  int64_t lddw;
+  int C, vec;
+};
+
+__global__ __launch_bounds__(64 * kWaves) void sort_kernel(const SortArgs a) {
   __shared__ uint32_t below[kWaves], sums[kWaves];
+  extern __shared__ uint32_t cnt[];  // [wave][R], then the rows' tokens
+  const int64_t* ids = a.ids;
+  const int64_t n = a.n;
+  const int R = a.R;
+  uint32_t* count = cnt + kWaves * R;
+  const int64_t v0 = (int64_t)blockIdx.x * R;
+  const uint32_t rows = (uint32_t)min<int64_t>(R, a.V - v0);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t part = (n + 64 * kWaves - 1) / (64 * kWaves) * 64;
   const int64_t beg = min(n, w * part), end = min(n, beg + part);
@@ -161,7 +178,6 @@ __device__ __forceinline__ uint32_t sort_range(const int64_t* __restrict__ ids, 
   uint32_t base = 0, total = 0;
 #pragma unroll
   for (int k = 0; k < kWaves; ++k) base += below[k];
-  const uint32_t begin = base;
   uint32_t c[kWaves];
   if (tid < R)
 #pragma unroll
@@ -176,7 +192,12 @@ __device__ __forceinline__ uint32_t sort_range(const int64_t* __restrict__ ids, 
   __syncthreads();
   for (int k = 0; k < w; ++k) base += sums[k];
   uint32_t at = base + run - total;
-  if (tid < (int)rows) row((uint32_t)tid, at, total);
+  if (tid < (int)rows) {
+    a.span[v0 + tid] = make_uint2(at, total);
+    if (v0 + tid == a.V - 1) *a.tokens = at + total;
+    if (total > kPiece) a.starts[at / kPiece] = (uint32_t)v0 + tid;  // at most one in a piece
+    count[tid] = total;
+  }
   if (tid < R)
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) {
@@ -184,6 +205,15 @@ __device__ __forceinline__ uint32_t sort_range(const int64_t* __restrict__ ids, 
       at += c[k];
     }
   __syncthreads();
+  if (a.dw)
+    for (uint32_t r = w; r < rows; r += kWaves)
+      if (count[r] == 0) {
+        float* p = a.dw + (v0 + r) * a.lddw;
+        if (a.vec)
+          for (int k = 4 * lane; k < a.C; k += 256) *reinterpret_cast<f32x4*>(p + k) = zero4();
+        else
+          for (int k = lane; k < a.C; k += 64) p[k] = 0.f;
+      }
   for (int64_t i0 = beg; i0 < end; i0 += 64 * kHeld) {
     if (!once) request(i0);
 #pragma unroll
@@ -193,32 +223,16 @@ __device__ __forceinline__ uint32_t sort_range(const int64_t* __restrict__ ids, 
         const uint32_t r = __builtin_amdgcn_readlane(t[k], __builtin_ctzll(left));
         const uint64_t same = __ballot(t[k] == r);
         const uint32_t to = mine[r];
-        if (t[k] == r) put(r, to + __builtin_popcountll(same & ((1ull << lane) - 1)), (uint32_t)(i0 + 64 * k + lane));
+        if (t[k] == r) {
+          const uint32_t place = to + __builtin_popcountll(same & ((1ull << lane) - 1));
+          a.order[place] = (uint32_t)(i0 + 64 * k + lane);
+          a.key[place] = (uint32_t)v0 + r;
+        }
         mine[r] = to + __builtin_popcountll(same);  // by every lane, so that each reads its own write
         left &= ~same;
       }
     }
   }
-  return begin;
-}
-
-__global__ __launch_bounds__(64 * kWaves) void sort_kernel(const int64_t* __restrict__ ids, int64_t n, int64_t V, int R,
-                                                           uint2* __restrict__ span, uint32_t* __restrict__ order,
-                                                           uint32_t* __restrict__ key, uint32_t* __restrict__ tokens,
-                                                           uint32_t* __restrict__ starts) {
-  extern __shared__ uint32_t cnt[];
-  const int64_t v0 = (int64_t)blockIdx.x * R;
-  sort_range(
-      ids, n, v0, (uint32_t)min<int64_t>(R, V - v0), R, cnt,
-      [&](uint32_t r, uint32_t first, uint32_t count) {
-        span[v0 + r] = make_uint2(first, count);
-        if (v0 + r == V - 1) *tokens = first + count;
-        if (count > kPiece) starts[first / kPiece] = (uint32_t)v0 + r;  // at most one in a piece
-      },
-      [&](uint32_t r, uint32_t at, uint32_t i) {
-        order[at] = i;
-        key[at] = (uint32_t)v0 + r;
-      });
 }
 
 // ---------------------------------------------------------------------------
@@ -302,7 +316,8 @@ __device__ __forceinline__ void store_row(const GradArgs& a, int64_t v, int c0, 
 
 // A wave's `rows` table rows from v0 on.  Their tokens follow each other in the sorted
 // order: up to eight tokens' values are requested at once, whichever rows they are
-// for, and a row is stored where its tokens end.  A wave a row, one row's
+// for, and a row is stored where its tokens end (one without a token was set to 0 by
+// the sort).  A wave a row, one row's
 // values at a time, took 83 us for 50021 rows of 1024 and 29500 bf16 tokens, this 66.
 template <typename T, int VEC, int U>
 __device__ __forceinline__ void add_range(const GradArgs& a, int64_t v0, int rows, int c0) {
@@ -328,7 +343,7 @@ __device__ __forceinline__ void add_range(const GradArgs& a, int64_t v0, int row
   // store the rows that end at token k
   auto flush = [&] {
     while (k == end && r < rows) {
-      if (some || !a.accumulate) store_row<VEC, 64, U>(a, v0 + r, c0, acc);
+      if (some) store_row<VEC, 64, U>(a, v0 + r, c0, acc);
       clear();
       some = false;
       ++r;
@@ -392,7 +407,7 @@ __global__ __launch_bounds__(256) void add_kernel(const GradArgs a) {
         add_range<T, VEC, U>(a, v0, (int)min<int64_t>(a.rows, a.V - v0), c0);
       } else {
         const uint2 s = a.span[item];
-        if (s.y > kPiece || (s.y == 0 && a.accumulate)) continue;
+        if (s.y > kPiece || s.y == 0) continue;
         add_rows<T, VEC, LPR, U>(a, a.order + s.x, (int)s.y, c0, acc);
         store_row<VEC, LPR, U>(a, item, c0, acc);
       }
@@ -472,48 +487,92 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(const GradArgs a, int
   }
 }
 
-// The whole gradient in one launch, for few tokens: each workgroup sorts its range
-// and adds it up, a wave a row; a long row by all waves, in contiguous parts.
+// The whole gradient in one launch, for few tokens.  A workgroup takes R rows of the
+// table, a wave every 16th of them; the ids lie in LDS, and a row's tokens are found by
+// comparing 64 of them at a time.  Rows of more than kPiece tokens are left to the end:
+// each wave takes a contiguous part of the ids, and the parts' sums are added in order.
+constexpr int kSmallTokens = 4096;
 template <typename T, int VEC, int U>
 __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, int R) {
-  // the counts [wave][R] and, once they are done with, the parts' sums; the rows'
-  // spans; the order
-  extern __shared__ uint32_t cnt[];
   constexpr int kCols = 64 * VEC * U;
-  float* sums = reinterpret_cast<float*>(cnt);
-  uint2* span = reinterpret_cast<uint2*>(cnt + kWaves * max(R, kCols));
-  uint32_t* order = reinterpret_cast<uint32_t*>(span + R);
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ uint32_t key[kSmallTokens];
+  __shared__ float sums[kWaves][kCols];
+  __shared__ uint32_t longs[kSmallTokens / kPiece];
+  __shared__ uint32_t many;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = (int)a.n;
   const int64_t v0 = (int64_t)blockIdx.x * R;
   const uint32_t rows = (uint32_t)min<int64_t>(R, a.V - v0);
-  // (places in the order of all tokens: the range's begin is subtracted below)
-  __shared__ uint32_t begin;
-  sort_range(
-      a.ids, a.n, v0, rows, R, cnt,
-      [&](uint32_t r, uint32_t first, uint32_t count) {
-        span[r] = make_uint2(first, count);
-        if (r == 0) begin = first;
-      },
-      [&](uint32_t, uint32_t at, uint32_t i) { order[at - begin] = i; });
+  const int groups = (n + 63) / 64;
+  if (threadIdx.x == 0) many = 0;
+#pragma unroll
+  for (int k = 0; k < kSmallTokens / 1024; ++k) {
+    const int i = threadIdx.x + 1024 * k;
+    if (i >= 64 * groups) break;
+    const uint2 id = i < n ? reinterpret_cast<const uint2*>(a.ids)[i] : make_uint2(~0u, ~0u);
+    const uint32_t off = id.x - (uint32_t)v0;
+    key[i] = id.y == 0 && off < rows ? off : ~0u;
+  }
   __syncthreads();
+  const T* g = static_cast<const T*>(a.g);
+  // acc = the tokens of row r among the ids of groups g0 to g1, for columns from c0 on
+  auto add = [&](uint32_t r, int g0, int g1, int c0, float (&acc)[U][VEC]) {
+    constexpr int N = sizeof(T);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[u][j] = 0.f;
+    uint32_t o[N];
+    int held = 0;
+    auto put = [&](auto count) {
+      constexpr int M = decltype(count)::value;
+      add_some<T, VEC, 64, U, M>(a, o, c0, acc);
+    };
+    for (int q = g0; q < g1; ++q) {
+      uint64_t left = __ballot(key[64 * q + lane] == r);
+      while (left) {
+        const uint32_t i = 64 * q + __builtin_ctzll(left);
+        left &= left - 1;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[k] = held == k ? i : o[k];
+        if (++held == N) {
+          put(std::integral_constant<int, N>());
+          held = 0;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k + 1 < N; ++k)
+      if (k < held) {
+        const uint32_t one[1] = {o[k]};
+        add_some<T, VEC, 64, U, 1>(a, one, c0, acc);
+      }
+  };
   float acc[U][VEC];
-  for (int c0 = lane * VEC; c0 - lane * VEC < a.C; c0 += kCols) {
-    for (uint32_t r = w; r < rows; r += kWaves) {
-      const uint2 s = span[r];
-      if (s.y > kPiece || (s.y == 0 && a.accumulate)) continue;
-      add_rows<T, VEC, 64, U, sizeof(T)>(a, order + (s.x - begin), (int)s.y, c0, acc);
+  for (uint32_t r = w; r < rows; r += kWaves) {
+    int count = 0;
+    for (int q = 0; q < groups; ++q) count += __builtin_popcountll(__ballot(key[64 * q + lane] == r));
+    if (count > kPiece) {
+      if (lane == 0) longs[atomicAdd(&many, 1u)] = r;
+      continue;
+    }
+    if (count == 0 && a.accumulate) continue;
+    for (int c0 = lane * VEC; c0 - lane * VEC < a.C; c0 += kCols) {
+      add(r, 0, count ? groups : 0, c0, acc);
       store_row<VEC, 64, U>(a, v0 + r, c0, acc);
     }
-    for (uint32_t r = 0; r < rows; ++r) {
-      const uint2 s = span[r];
-      if (s.y <= kPiece) continue;
-      const int per = ((int)s.y + kWaves - 1) / kWaves, b = min((int)s.y, w * per), e = min((int)s.y, b + per);
-      add_rows<T, VEC, 64, U, sizeof(T)>(a, order + (s.x - begin) + b, e - b, c0, acc);
+  }
+  __syncthreads();
+  // (the order in which the long rows come does not matter: each is added up by itself)
+  for (uint32_t k = 0; k < many; ++k) {
+    const uint32_t r = longs[k];
+    const int per = (groups + kWaves - 1) / kWaves, g0 = min(groups, w * per), g1 = min(groups, g0 + per);
+    for (int c0 = lane * VEC; c0 - lane * VEC < a.C; c0 += kCols) {
+      add(r, g0, g1, c0, acc);
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) sums[(w * U + u) * 64 * VEC + lane * VEC + j] = acc[u][j];
+        for (int j = 0; j < VEC; ++j) sums[w][(u * 64 + lane) * VEC + j] = acc[u][j];
       __syncthreads();
       if (w != 0) continue;
 #pragma unroll 1
@@ -521,10 +580,61 @@ __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, in
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[u][j] += sums[(m * U + u) * 64 * VEC + lane * VEC + j];
+          for (int j = 0; j < VEC; ++j) acc[u][j] += sums[m][(u * 64 + lane) * VEC + j];
       store_row<VEC, 64, U>(a, v0 + r, c0, acc);
     }
   }
+}
+
+// Small tables under many tokens: a workgroup holds a column slice of the whole table in
+// LDS, a column a thread, and adds a chunk of the tokens to it one after another; a
+// second launch adds the chunks' tables up in order.  Nothing is sorted.
+template <typename T>
+__global__ __launch_bounds__(512) void table_kernel(const GradArgs a, int chunk, float* __restrict__ part) {
+  extern __shared__ float tab[];  // [V][columns]
+  const int W = blockDim.x, c = blockIdx.y * W + threadIdx.x, V = (int)a.V;
+  const int i0 = blockIdx.x * chunk, i1 = (int)min<int64_t>(a.n, (int64_t)i0 + chunk);
+  float* col = tab + threadIdx.x;
+  for (int v = 0; v < V; ++v) col[v * W] = 0.f;
+  // (a thread reads and writes its own column alone: no barrier)
+  const T* g = static_cast<const T*>(a.g) + min(c, a.C - 1);
+  constexpr int kAhead = 8;
+  for (int i = i0; i < i1; i += kAhead) {
+    float x[kAhead];
+    int64_t id[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int at = min(i + k, i1 - 1);
+      id[k] = i + k < i1 ? a.ids[at] : -1;
+      x[k] = Elem<T>::to_f(g[at * a.ldg]);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if ((uint64_t)id[k] < (uint64_t)V) col[(int)id[k] * W] += x[k];
+  }
+  if (c >= a.C) return;
+  float* out = part + (int64_t)blockIdx.x * V * a.C + c;
+#pragma unroll 8
+  for (int v = 0; v < V; ++v) out[(int64_t)v * a.C] = col[v * W];
+}
+
+// dW (+)= scale times the sum of the chunks' tables: 64 values a workgroup, whose 16
+// waves take contiguous runs of chunks
+__global__ __launch_bounds__(64 * kWaves) void table_sum_kernel(const GradArgs a, int chunks, const float* __restrict__ part) {
+  __shared__ float sums[kWaves][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, size = (int)a.V * a.C, e = blockIdx.x * 64 + lane;
+  const int per = (chunks + kWaves - 1) / kWaves, b = w * per, end = min(chunks, b + per);
+  float t = 0.f;
+  if (e < size)
+#pragma unroll 16
+    for (int k = b; k < end; ++k) t += part[(int64_t)k * size + e];
+  sums[w][lane] = t;
+  __syncthreads();
+  if (w || e >= size) return;
+#pragma unroll
+  for (int k = 1; k < kWaves; ++k) t += sums[k][lane];
+  float* p = a.dw + (int64_t)(e / a.C) * a.lddw + e % a.C;
+  *p = a.accumulate ? *p + a.scale * t : a.scale * t;
 }
 
 bool known(int dtype) { return dtype == MTX_F32 || dtype == MTX_BF16; }
@@ -568,23 +678,36 @@ int lookup(const void* w, int64_t ldw, int64_t V, const int64_t* ids, int64_t n,
   return MTX_OK;
 }
 
-// The gradient's workspace: where the tables begin, and its size.
+// How a gradient is worked out, its workspace's tables and size.
 struct Plan {
   int R;           // table rows a sorting workgroup
   unsigned sorts;  // sorting workgroups
-  bool small;
+  bool small, table;
+  int width, chunk, chunks;  // table: columns a workgroup, tokens a chunk
   size_t span, order, key, starts, part, bytes;
 };
-// Few tokens in one launch: as long as one workgroup may have to read all their rows.
-constexpr int64_t kSmallTokens = 4096, kSmallBytes = 1 << 20;
 
 Plan plan(int dtype, int64_t n, int64_t V, int C) {
   Plan p{};
+  const int size = dtype == MTX_F32 ? 4 : 2;
   p.R = (int)std::min<int64_t>((V + 255) / 256, kMaxRows);
   p.sorts = (unsigned)((V + p.R - 1) / p.R);
-  p.small = n <= kSmallTokens && n * C * (dtype == MTX_F32 ? 4 : 2) <= kSmallBytes;
+  // Few tokens, as long as one workgroup may have to read all their rows
+  p.small = n <= kSmallTokens && n * C * size <= (1 << 20);
   if (p.small) return p;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+  // Tables of which 64 columns fit in a quarter of a compute unit's LDS, under tokens
+  // enough for 64 chunks that are longer than the table
+  p.chunk = std::max<int>(64, (int)std::min<int64_t>(V, 1 << 20));
+  p.table = V <= 160 && n / p.chunk >= 64 && n <= ((int64_t)1 << 22) && V * C <= (1 << 22);
+  if (p.table) {
+    p.width = (int)std::min<int64_t>(512, (65536 / 4 / V) / 64 * 64);
+    const int slices = cdiv(C, p.width);
+    p.width = (cdiv(C, slices) + 63) / 64 * 64;
+    p.chunks = (int)((n + p.chunk - 1) / p.chunk);
+    p.bytes = up((size_t)p.chunks * V * C * 4);
+    return p;
+  }
   p.span = 256;
   p.order = p.span + up((size_t)V * sizeof(uint2));
   p.key = p.order + up((size_t)n * 4);
@@ -595,23 +718,40 @@ Plan plan(int dtype, int64_t n, int64_t V, int C) {
 }
 
 template <typename T>
-int grad(GradArgs a, const Plan& p, hipStream_t st) {
+int grad(GradArgs a, const Plan& p, char* ws, hipStream_t st) {
   constexpr int kVec = 16 / sizeof(T), kU = sizeof(T) == 4 ? 2 : 1;
   const bool vec = whole(a.g, a.ldg, a.C, kVec, sizeof(T)) && whole(a.dw, a.lddw, a.C, kVec, 4);
   if (p.small) {
-    auto go = [&](auto kernel, int columns) {
-      const size_t lds = (size_t)kWaves * std::max(p.R, columns) * 4 + (size_t)p.R * 8 + (size_t)a.n * 4;
-      hipLaunchKernelGGL(kernel, dim3(p.sorts), dim3(64 * kWaves), lds, st, a, p.R);
-    };
-    if (vec) go(small_kernel<T, kVec, 1>, 64 * kVec);
-    else go(small_kernel<T, 1, 4>, 256);
+    const dim3 grid(p.sorts), block(64 * kWaves);
+    if (vec) hipLaunchKernelGGL((small_kernel<T, kVec, 1>), grid, block, 0, st, a, p.R);
+    else hipLaunchKernelGGL((small_kernel<T, 1, 4>), grid, block, 0, st, a, p.R);
     MTX_LAUNCHED();
     return MTX_OK;
   }
-  hipLaunchKernelGGL(sort_kernel, dim3(p.sorts), dim3(64 * kWaves), (size_t)kWaves * p.R * 4, st, a.ids, a.n, a.V, p.R,
-                     const_cast<uint2*>(a.span), const_cast<uint32_t*>(a.order), const_cast<uint32_t*>(a.key),
-                     const_cast<uint32_t*>(a.tokens), const_cast<uint32_t*>(a.starts));
+  if (p.table) {
+    float* part = reinterpret_cast<float*>(ws);
+    hipLaunchKernelGGL((table_kernel<T>), dim3(p.chunks, cdiv(a.C, p.width)), dim3(p.width),
+                       (size_t)a.V * p.width * sizeof(float), st, a, p.chunk, part);
+    MTX_LAUNCHED();
+    hipLaunchKernelGGL(table_sum_kernel, dim3(cdiv((int)(a.V * a.C), 64)), dim3(64 * kWaves), 0, st, a, p.chunks, part);
+    MTX_LAUNCHED();
+    return MTX_OK;
+  }
+  uint32_t* tokens = reinterpret_cast<uint32_t*>(ws);
+  uint2* span = reinterpret_cast<uint2*>(ws + p.span);
+  uint32_t* order = reinterpret_cast<uint32_t*>(ws + p.order);
+  uint32_t* key = reinterpret_cast<uint32_t*>(ws + p.key);
+  uint32_t* starts = reinterpret_cast<uint32_t*>(ws + p.starts);
+  const SortArgs sa{a.ids, a.n, a.V, p.R, span, order, key, tokens, starts, a.accumulate ? nullptr : a.dw, a.lddw, a.C,
+                    whole(a.dw, a.lddw, a.C, 4, 4)};
+  hipLaunchKernelGGL(sort_kernel, dim3(p.sorts), dim3(64 * kWaves), (size_t)(kWaves + 1) * p.R * 4, st, sa);
   MTX_LAUNCHED();
+  a.tokens = tokens;
+  a.span = span;
+  a.order = order;
+  a.key = key;
+  a.starts = starts;
+  a.part = a.n > kPiece ? reinterpret_cast<float*>(ws + p.part) : nullptr;
   const int lpr = lanes(vec ? a.C / kVec : a.C);
   auto go = [&](auto kernel, int columns) {
     a.slices = (a.C + columns - 1) / columns;
@@ -678,7 +818,6 @@ extern "C" int mtx_embedding_grad(int dtype, const int64_t* ids, int64_t n, cons
   const Plan p = plan(dtype, n, V, C);
   MTX_CHECK_ARG(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0),
                 "embedding_grad: workspace of %zu bytes, need %zu aligned to 256", workspace_bytes, p.bytes);
-  char* ws = static_cast<char*>(workspace);
   GradArgs a{};
   a.ids = ids;
   a.g = grad_;
@@ -690,12 +829,7 @@ extern "C" int mtx_embedding_grad(int dtype, const int64_t* ids, int64_t n, cons
   a.n = n;
   a.C = C;
   a.accumulate = accumulate ? 1 : 0;
-  a.tokens = reinterpret_cast<uint32_t*>(ws);
-  a.span = reinterpret_cast<uint2*>(ws + p.span);
-  a.order = reinterpret_cast<uint32_t*>(ws + p.order);
-  a.key = reinterpret_cast<uint32_t*>(ws + p.key);
-  a.starts = reinterpret_cast<uint32_t*>(ws + p.starts);
-  a.part = n > kPiece ? reinterpret_cast<float*>(ws + p.part) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == MTX_F32 ? grad<float>(a, p, st) : grad<bf16_t>(a, p, st);
+  return dtype == MTX_F32 ? grad<float>(a, p, static_cast<char*>(workspace), st)
+                          : grad<bf16_t>(a, p, static_cast<char*>(workspace), st);
 }
