@@ -591,26 +591,54 @@ __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, in
 // second launch adds the chunks' tables up in order.  Nothing is sorted.
 template <typename T>
 __global__ __launch_bounds__(512) void table_kernel(const GradArgs a, int chunk, float* __restrict__ part) {
-  extern __shared__ float tab[];  // [V][columns]
+  extern __shared__ float tab[];  // [V + 1][columns]
   const int W = blockDim.x, c = blockIdx.y * W + threadIdx.x, V = (int)a.V;
   const int i0 = blockIdx.x * chunk, i1 = (int)min<int64_t>(a.n, (int64_t)i0 + chunk);
   float* col = tab + threadIdx.x;
-  for (int v = 0; v < V; ++v) col[v * W] = 0.f;
+#pragma unroll 8
+  for (int v = 0; v <= V; ++v) col[v * W] = 0.f;
   // (a thread reads and writes its own column alone: no barrier)
   const T* g = static_cast<const T*>(a.g) + min(c, a.C - 1);
-  constexpr int kAhead = 8;
-  for (int i = i0; i < i1; i += kAhead) {
-    float x[kAhead];
-    int64_t id[kAhead];
+  // Eight tokens at a time: their rows' sums are read at once (one after another they
+  // wait 200 cycles each), a row that comes twice takes the sum of the time before, and
+  // the last one to write it has it all.  Tokens that are none go to a row behind the
+  // table.
+  constexpr int N = 8;
+  const int lane = threadIdx.x & 63;
+  for (int b = i0; b < i1; b += 64) {
+    const int64_t v = a.ids[min(b + lane, i1 - 1)];
+    const int ids = b + lane < i1 && (uint64_t)v < (uint64_t)V ? (int)v : V;
+    const int count = min(64, i1 - b);
+    float all[64];  // requested at once: one wait for memory
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int at = min(i + k, i1 - 1);
-      id[k] = i + k < i1 ? a.ids[at] : -1;
-      x[k] = Elem<T>::to_f(g[at * a.ldg]);
+    for (int k = 0; k < 64; ++k) all[k] = Elem<T>::to_f(g[(int64_t)(b + min(k, count - 1)) * a.ldg]);
+#pragma unroll
+    for (int k = 0; k < 64; ++k) asm volatile("" : "+v"(all[k]));  // (the loads stay where they are)
+#pragma unroll
+    for (int k0 = 0; k0 < 64; k0 += N) {
+      if (k0 >= count) break;
+      float x[N], t[N];
+      int id[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = all[k0 + k];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        id[k] = __builtin_amdgcn_readlane(ids, k0 + k);
+        t[k] = col[id[k] * W];
+      }
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+#pragma unroll
+        for (int m = 0; m < k; ++m) {
+          float before = t[m];
+          asm("" : "+v"(before));  // a plain select; from an array the compiler makes an index
+          t[k] = id[m] == id[k] ? before : t[k];
+        }
+        t[k] += x[k];
+      }
+#pragma unroll
+      for (int k = 0; k < N; ++k) col[id[k] * W] = t[k];
     }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if ((uint64_t)id[k] < (uint64_t)V) col[(int)id[k] * W] += x[k];
   }
   if (c >= a.C) return;
   float* out = part + (int64_t)blockIdx.x * V * a.C + c;
@@ -696,12 +724,12 @@ Plan plan(int dtype, int64_t n, int64_t V, int C) {
   p.small = n <= kSmallTokens && n * C * size <= (1 << 20);
   if (p.small) return p;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
-  // Tables of which 64 columns fit in a quarter of a compute unit's LDS, under tokens
-  // enough for 64 chunks that are longer than the table
-  p.chunk = std::max<int>(64, (int)std::min<int64_t>(V, 1 << 20));
-  p.table = V <= 160 && n / p.chunk >= 64 && n <= ((int64_t)1 << 22) && V * C <= (1 << 22);
+  // Tables of which 64 columns fit in 64 KB of LDS, under tokens enough for 64 chunks of
+  // half the table or more
+  p.chunk = V <= 128 ? 64 : 128;
+  p.table = V < 256 && n / p.chunk >= 64 && n <= ((int64_t)1 << 22) && V * C <= (1 << 22);
   if (p.table) {
-    p.width = (int)std::min<int64_t>(512, (65536 / 4 / V) / 64 * 64);
+    p.width = (int)std::min<int64_t>(512, (65536 / 4 / (V + 1)) / 64 * 64);
     const int slices = cdiv(C, p.width);
     p.width = (cdiv(C, slices) + 63) / 64 * 64;
     p.chunks = (int)((n + p.chunk - 1) / p.chunk);
@@ -731,7 +759,7 @@ int grad(GradArgs a, const Plan& p, char* ws, hipStream_t st) {
   if (p.table) {
     float* part = reinterpret_cast<float*>(ws);
     hipLaunchKernelGGL((table_kernel<T>), dim3(p.chunks, cdiv(a.C, p.width)), dim3(p.width),
-                       (size_t)a.V * p.width * sizeof(float), st, a, p.chunk, part);
+                       (size_t)(a.V + 1) * p.width * sizeof(float), st, a, p.chunk, part);
     MTX_LAUNCHED();
     hipLaunchKernelGGL(table_sum_kernel, dim3(cdiv((int)(a.V * a.C), 64)), dim3(64 * kWaves), 0, st, a, p.chunks, part);
     MTX_LAUNCHED();
