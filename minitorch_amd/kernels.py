@@ -1421,11 +1421,6 @@ def dropout(x, p: float, seed: int, offset: int = 0, residual=None, out=None, su
     return out
 
 
-def dropout_calls(x) -> int:
-    """How far a dropout of x moves its generator's offset on."""
-    return (x.numel() + 3) // 4
-
-
 def _either_order(name, spec, shape):
     """(row stride, column stride, dtype) of a matrix that is contiguous along
     its rows or its columns."""

@@ -171,6 +171,43 @@ def test_lookup_grad_same_bits_every_time(dev, n, V, C):
         assert np.array_equal(host(K.embedding_grad(ids, g, empty((V, C)))), first)
 
 
+# tokens, table rows, width: few tokens of wide and narrow rows and the borders where that
+# ends, small tables up to their largest and to their shortest batch, and what lies behind
+GRAD_WAYS = [(4096, 3, 64), (4097, 3, 64), (2048, 40, 128), (2048, 40, 129), (100, 9, 2621), (100, 9, 2622), (4096, 50000, 1),
+             (4096, 127, 70), (8192, 255, 40), (8191, 255, 40), (12001, 200, 515), (8200, 256, 24), (5000, 128, 1030)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n,V,C", GRAD_WAYS)
+def test_lookup_grad_borders(dev, n, V, C, dtype):
+    """Added up and written; NaN and infinities reach the row of their own token alone;
+    no token at all."""
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(n + V + C)
+    g, ids = rounded(rng.standard_normal((n, C)), dtype), tokens(rng, n, V)
+    counts = np.bincount(ids[(ids >= 0) & (ids < V)], minlength=V)[:, None]
+    want, size = ref.lookup_grad(ids, g, V, 0.5)
+    bound = (counts + 2) * U * size
+    dg, di = dev_array(g, dtype), dev_array(ids, "int64")
+    inside(host(K.embedding_grad(di, dg, full((V, C), 7.0), scale=0.5)), want, bound)
+    old = rng.standard_normal((V, C)).astype(np.float32)
+    got = host(K.embedding_grad(di, dg, dev_array(old), scale=0.5, accumulate=True))
+    inside(got, want + old, bound + U * (np.abs(want + old) + bound))
+    assert np.array_equal(got[counts[:, 0] == 0], old[counts[:, 0] == 0])
+    plain = host(K.embedding_grad(di, dg, empty((V, C))))
+    at = np.nonzero((ids >= 0) & (ids < V))[0][:2]
+    bad = g.copy()
+    bad[at[0]], bad[at[1], 0] = np.nan, np.inf
+    got = host(K.embedding_grad(di, dev_array(bad, dtype), empty((V, C))))
+    rest = np.setdiff1d(np.arange(V), ids[at])
+    assert np.array_equal(got[rest], plain[rest])
+    assert np.isnan(got[ids[at[0]]]).all() and not np.isfinite(got[ids[at[1]], 0])
+    none = dev_array(np.full(n, -1), "int64")
+    assert not host(K.embedding_grad(none, dg, full((V, C), 7.0))).any()
+    assert np.array_equal(host(K.embedding_grad(none, dg, dev_array(old), accumulate=True)), old)
+
+
 # ---------------------------------------------------------------------------
 # dropout
 # ---------------------------------------------------------------------------
@@ -269,10 +306,14 @@ def xent_bounds(x, w, bias, r, dtype, out):
     fin = np.where(np.isfinite(r["lse"]), np.abs(r["lse"]), 0.0)
     lse = e + 4 * U * (fin + mag)
     row = lse + ez + 4 * U * (fin + mag)
-    count = max(1, int((r["row_loss"] != 0).sum()))
+    # Rows with a label: some entry of theirs has a gradient.  Not entry by entry: the
+    # label's own is p - 1, exactly 0 in float64 once 1 - p < 2^-54, and a p that is off
+    # by p (2 e + 8 u) is off by that beside 1 too.
+    named = (r["dz"] != 0).any(1)
+    count = max(1, int(named.sum()))
     loss = row.sum() / count + (n + 4) * U * np.where(np.isfinite(r["row_loss"]), r["row_loss"], 0).sum() / count
     d = np.abs(r["dz"])
-    ed = r["p"] * (2 * e + 8 * U)[:, None] * (d != 0) / count + 4 * U * d
+    ed = r["p"] * (2 * e + 8 * U)[:, None] * named[:, None] / count + 4 * U * d
     ed = ed + (B if out == "bfloat16" else U) * d if dtype == "bfloat16" else ed
     size = B if out == "bfloat16" else U
     dx = ed @ w.T + ((V + 2) * U + cut) * (d @ w.T)
@@ -324,6 +365,22 @@ XENTS = [
 @pytest.mark.parametrize("n,C,V", XENTS)
 def test_linear_xent(dev, n, C, V, tied, dtype, out):
     check_xent(n, C, V, dtype, out, tied=tied, bias=n % 2 == 1)
+
+
+@pytest.mark.parametrize("dtype,out", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("V", [256, 512, 513, 1024, 1025, 4096, 4097, 8192, 8193, 16384, 16385, 32768, 32769, 40960,
+                               40961, 65536, 65537])
+def test_linear_xent_lengths_of_rows(dev, V, bias, dtype, out):
+    """Where one way to walk a row ends and the next begins."""
+    check_xent(5, 6, V, dtype, out, tied=True, bias=bias)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n,C,V", [(1, 70, 5003), (2, 64, 4113), (17, 130, 9000), (64, 33, 20001), (65, 33, 20001)])
+def test_linear_xent_few_rows(dev, n, C, V, dtype):
+    for tied in (False, True):
+        check_xent(n, C, V, dtype, tied=tied)
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
@@ -472,3 +529,73 @@ def test_linear_xent_wanted_gradients_alone(dev, dtype, out):
     d = empty((210,))
     K.linear_xent(*args, bias=db, db=d)
     inside(host(d), host(full_[2]), 2 * 52 * U * np.abs(r["dz"]).sum(0))
+
+
+# ---------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------
+
+def step_of(K, ids, labels, w, wt, x, y, dx, dw, db, b, dt, p, seed):
+    """Lookup, dropout, projection with its loss, and the gradients back into the table."""
+    K.embedding_lookup(w, ids, scale=2.0, out=x)
+    K.dropout(x, p, seed, 0, out=y)
+    loss, row, lse = K.linear_xent(y, wt, labels, bias=b, dx=dx, dw=dw, db=db)
+    K.dropout(dx, p, seed, 0, out=dx)
+    K.embedding_grad(ids, dx, dt, scale=2.0)
+    return loss, row, lse
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n,C,V", [(50, 24, 70), (4500, 32, 100), (5000, 16, 900)])
+def test_a_recorded_step_is_the_eager_one(dev, n, C, V, dtype):
+    """Two recorded steps over buffers of their own, replayed in turn with other tokens
+    each time and eager calls between: every replay has the bits of the eager step."""
+    from minitorch_amd import graphs
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(n)
+    w = rounded(rng.standard_normal((V, C)), dtype)
+    wd, b = dev_array(w, dtype), dev_array(rng.standard_normal(V))
+
+    def memory():
+        return dict(ids=dev_array(np.zeros(n), "int64"), labels=dev_array(np.zeros(n), "int64"), w=wd, wt=wd.t(),
+                    x=empty((n, C), dtype), y=empty((n, C), dtype), dx=empty((n, C), dtype),
+                    dw=empty((V, C), dtype).t(), db=empty((V,)), b=b, dt=empty((V, C)), p=0.3, seed=12)
+
+    def values(m, outs):
+        return [host(t).copy() for t in (*outs, m["x"], m["y"], m["dx"], m["dw"].t(), m["db"], m["dt"])]
+
+    eager, sets = memory(), [memory(), memory()]
+    step_of(K, **eager)
+    recorded = []
+    for m in sets:
+        g = graphs.Graph()
+        with g.capture():
+            outs = step_of(K, **m)
+        recorded.append((g, m, outs))
+    for turn in range(3):
+        for g, m, outs in recorded:
+            ids, labels = tokens(rng, n, V), tokens(rng, n, V)
+            for t in (eager, m):
+                t["ids"].copy_(ids)
+                t["labels"].copy_(labels)
+            want = values(eager, step_of(K, **eager))
+            g.replay()
+            K.embedding_grad(eager["ids"], eager["dx"], empty((V, C)))  # eager work behind the replay
+            assert all(np.array_equal(a, c, equal_nan=True) for a, c in zip(want, values(m, outs)))
+            assert np.isfinite(want[0]).all()
+        # the whole against float64, from the values the step itself stored
+        keep = ref.keep((n, C), 0.3, 12)
+        inside(want[3], ref.lookup(w, ids, 2.0), (U if dtype == "float32" else B) * np.abs(ref.lookup(w, ids, 2.0)))
+        y = rounded(np.where(keep, want[3] * np.float32(1 / 0.7), np.float32(0)), dtype)
+        assert np.array_equal(want[4], y)
+        r = ref.linear_xent(y, w.T, labels, host(b))
+        bd = xent_bounds(y, w.T, host(b), r, dtype, dtype)
+        inside(want[2], r["lse"], bd[0])
+        inside(want[6], r["dw"].T, bd[4].T)
+        gx = np.where(keep, r["dx"] / 0.7, 0)
+        got = want[5]
+        inside(got, gx, np.where(keep, (bd[3] + (U if dtype == "float32" else B) * 2 * (np.abs(gx) + bd[3])) / 0.7, 0))
+        dt, size = ref.lookup_grad(ids, got, V, 2.0)
+        counts = np.bincount(ids[(ids >= 0) & (ids < V)], minlength=V)[:, None]
+        inside(want[8], dt, (counts + 2) * U * size)
