@@ -1,4 +1,4 @@
-// Embedding lookup with scaling, and its gradient by sorted tokens (fp32, bf16).
+// Embedding lookup with scaling, and its gradient without atomics on values (fp32, bf16).
 //
 //   out[i][c] = scale * W[t_i][c]                      (0 where t_i is no token)
 //   dW[v][c] (+)= scale * sum over i with t_i = v of g[i][c], in token order
@@ -6,11 +6,17 @@
 // A token outside [0, V) is none: padding.  Its row comes out as zeros and its
 // gradient goes nowhere.
 //
-// The gradient: one launch sorts the tokens (every workgroup takes a range of the
-// table and looks through all ids for its own, so no workgroup waits for
-// another), one adds up (a group of lanes per table row; rows of more than kPiece
-// tokens in pieces of the sorted order, by as many groups), one joins the pieces.
-// Nothing is added by atomics: the sums have one order.
+// The gradient's sums have one order, in one of three ways, by the sizes:
+//   few tokens     one launch; a workgroup finds the tokens of its table rows by
+//                  comparing (small_kernel)
+//   small tables   the table in LDS, a chunk of the tokens a workgroup, then the
+//                  chunks' tables added up (table_kernel, table_sum_kernel)
+//   all others     one launch sorts the tokens (every workgroup takes a range of the
+//                  table and looks through all ids for its own, so no workgroup waits
+//                  for another) and sets rows without one to 0, one adds up (rows of
+//                  more than kPiece tokens in pieces of the sorted order), one joins
+//                  the pieces (sort_kernel, add_kernel, join_kernel)
+// Bound by memory: the gradient's rows are read and the table written, once each.
 #include "mtx_common.h"
 
 #include <type_traits>
@@ -56,7 +62,9 @@ __device__ __forceinline__ void store_f(T* __restrict__ p, const float (&f)[N]) 
 }
 
 // LPR lanes take a row, VEC values at a time, and kLookRows rows one after another:
-// their ids, then their values, are requested before the first is needed.
+// their ids, then their values, are requested before the first is needed.  Bound by
+// memory; where the rows are too few to fill the chip, the columns are dealt out too
+// (5 rows of 1838 fp32 values: 3.0 us, 8 by one workgroup).
 constexpr int kLookRows = 4;
 template <typename T, typename O, int VEC, int LPR>
 __global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ w, int64_t ldw, int64_t V,
@@ -72,7 +80,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ w, in
       const int64_t i = i0 + k * (256 / LPR);
       t[k] = i < n ? ids[i] : -1;
     }
-    for (int c = sub; c < nv; c += LPR) {
+    for (int c = sub + (int)blockIdx.y * LPR; c < nv; c += LPR * (int)gridDim.y) {
       float f[kLookRows][VEC];
 #pragma unroll
       for (int k = 0; k < kLookRows; ++k) {
@@ -117,8 +125,9 @@ struct SortArgs {
   uint32_t* key;    // [tokens] out: and rows
   uint32_t* tokens;  // out: how many they are
   uint32_t* starts;  // [pieces] out: the row of more than a piece that begins there
-  // Rows without a token are set to 0 here, while the sorting waits for its memory (205
-  // MB of 50021 x 1024 rows, three quarters of them: XXX); nullptr: they are left alone
+  // Rows without a token are set to 0 here, while the sorting waits for its memory: of
+  // 50021 x 1024 rows (205 MB) three quarters are, which makes this launch 36 us instead
+  // of 16 and the adding up 30 instead of 66.  nullptr: they are left alone
   float* dw;
   int64_t lddw;
   int C, vec;
@@ -488,22 +497,26 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(const GradArgs a, int
 }
 
 // The whole gradient in one launch, for few tokens.  A workgroup takes R rows of the
-// table, a wave every 16th of them; the ids lie in LDS, and a row's tokens are found by
-// comparing 64 of them at a time.  Rows of more than kPiece tokens are left to the end:
+// table, a wave every 16th of them; the ids lie in LDS with the rows' counts, and a row's
+// tokens are found by comparing 64 of them at a time.  Rows of more than kPiece tokens are left to the end:
 // each wave takes a contiguous part of the ids, and the parts' sums are added in order.
-constexpr int kSmallTokens = 4096;
+// 300 tokens of 384 fp32 values, a table of 5003 rows (7.7 MB): 9 us; 1339 bf16 tokens of
+// 256, 42338 rows (43 MB): 20, and 27 where every row's tokens were counted by comparing.
+constexpr int kSmallTokens = 4096, kScan = 4;  // groups of ids looked at together
 template <typename T, int VEC, int U>
 __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, int R) {
   constexpr int kCols = 64 * VEC * U;
   __shared__ uint32_t key[kSmallTokens];
   __shared__ float sums[kWaves][kCols];
-  __shared__ uint32_t longs[kSmallTokens / kPiece];
+  __shared__ uint32_t count[kMaxRows], longs[kSmallTokens / kPiece];
   __shared__ uint32_t many;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = (int)a.n;
   const int64_t v0 = (int64_t)blockIdx.x * R;
   const uint32_t rows = (uint32_t)min<int64_t>(R, a.V - v0);
   const int groups = (n + 63) / 64;
   if (threadIdx.x == 0) many = 0;
+  if (threadIdx.x < kMaxRows) count[threadIdx.x] = 0;
+  __syncthreads();
 #pragma unroll
   for (int k = 0; k < kSmallTokens / 1024; ++k) {
     const int i = threadIdx.x + 1024 * k;
@@ -511,6 +524,7 @@ __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, in
     const uint2 id = i < n ? reinterpret_cast<const uint2*>(a.ids)[i] : make_uint2(~0u, ~0u);
     const uint32_t off = id.x - (uint32_t)v0;
     key[i] = id.y == 0 && off < rows ? off : ~0u;
+    if (id.y == 0 && off < rows) atomicAdd(&count[off], 1u);
   }
   __syncthreads();
   const T* g = static_cast<const T*>(a.g);
@@ -527,16 +541,22 @@ __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, in
       constexpr int M = decltype(count)::value;
       add_some<T, VEC, 64, U, M>(a, o, c0, acc);
     };
-    for (int q = g0; q < g1; ++q) {
-      uint64_t left = __ballot(key[64 * q + lane] == r);
-      while (left) {
-        const uint32_t i = 64 * q + __builtin_ctzll(left);
-        left &= left - 1;
+    for (int q0 = g0; q0 < g1; q0 += kScan) {
+      uint32_t keys[kScan];
 #pragma unroll
-        for (int k = 0; k < N; ++k) o[k] = held == k ? i : o[k];
-        if (++held == N) {
-          put(std::integral_constant<int, N>());
-          held = 0;
+      for (int h = 0; h < kScan; ++h) keys[h] = key[64 * min(q0 + h, g1 - 1) + lane];
+#pragma unroll
+      for (int h = 0; h < kScan; ++h) {
+        uint64_t left = q0 + h < g1 ? __ballot(keys[h] == r) : 0;
+        while (left) {
+          const uint32_t i = 64 * (q0 + h) + __builtin_ctzll(left);
+          left &= left - 1;
+#pragma unroll
+          for (int k = 0; k < N; ++k) o[k] = held == k ? i : o[k];
+          if (++held == N) {
+            put(std::integral_constant<int, N>());
+            held = 0;
+          }
         }
       }
     }
@@ -549,15 +569,14 @@ __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, in
   };
   float acc[U][VEC];
   for (uint32_t r = w; r < rows; r += kWaves) {
-    int count = 0;
-    for (int q = 0; q < groups; ++q) count += __builtin_popcountll(__ballot(key[64 * q + lane] == r));
-    if (count > kPiece) {
+    const uint32_t some = __builtin_amdgcn_readfirstlane(count[r]);
+    if (some > kPiece) {
       if (lane == 0) longs[atomicAdd(&many, 1u)] = r;
       continue;
     }
-    if (count == 0 && a.accumulate) continue;
+    if (some == 0 && a.accumulate) continue;
     for (int c0 = lane * VEC; c0 - lane * VEC < a.C; c0 += kCols) {
-      add(r, 0, count ? groups : 0, c0, acc);
+      add(r, 0, some ? groups : 0, c0, acc);
       store_row<VEC, 64, U>(a, v0 + r, c0, acc);
     }
   }
@@ -688,9 +707,10 @@ int lookup(const void* w, int64_t ldw, int64_t V, const int64_t* ids, int64_t n,
   const int lpr = lanes(vec ? C / kVec : C);
   const int64_t rows = 256 / lpr * kLookRows;
   const unsigned blocks = (unsigned)std::min<int64_t>((n + rows - 1) / rows, 1 << 20);
+  const unsigned slices = std::min<unsigned>(cdiv(vec ? C / kVec : C, lpr), std::max(1u, 512 / blocks));
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, st, static_cast<const T*>(w), ldw, V, ids, n, C, scale,
-                       static_cast<O*>(out), ldo);
+    hipLaunchKernelGGL(kernel, dim3(blocks, slices), dim3(256), 0, st, static_cast<const T*>(w), ldw, V, ids, n, C,
+                       scale, static_cast<O*>(out), ldo);
   };
   switch ((vec ? 100 : 0) + lpr) {
     case 108: go(lookup_kernel<T, O, kVec, 8>); break;
