@@ -8,8 +8,17 @@
 //
 // The rows are taken in blocks whose logits fit the workspace: a block's
 // gradients are worked out while its logits are there, so each logit is computed
-// once.
+// once.  Three ways, by sizes and types:
+//   many rows and a small vocabulary: the logits stay in registers (narrow_xent.hip);
+//   bf16 without gradients: the product's epilogue keeps a row's statistics of 64
+//     columns each, and no logit is stored;
+//   else: the product z, a pass over its rows that puts dz in z's place (fp32) or
+//     beside it as bf16 pieces, the products dx and dW.  fp32 products are those of
+//     mtx_gemm_f32, bf16 ones gemm_bf16's.
+// (8192, 1024) x (1024, 50021) in bf16: z 1.0-1.25 ms, the rows' pass 0.55 (2.5 GB, 4.4
+// TB/s), dx 0.82, dW 0.83-0.92: bound by the products, at 1.0 PFLOP/s.
 #include "gemm_bf16.h"
+#include "narrow_xent.h"
 
 namespace mtx {
 namespace {
@@ -19,7 +28,7 @@ __global__ __launch_bounds__(1024) void count_kernel(const int64_t* __restrict__
                                                      float* __restrict__ inv) {
   __shared__ int part[16];
   int c = 0;
-#pragma unroll 8
+#pragma unroll 16
   for (int64_t i = threadIdx.x; i < n; i += 1024) c += (uint64_t)labels[i] < (uint64_t)V;
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) c += __shfl_xor(c, m, 64);
@@ -42,7 +51,7 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ ro
   __shared__ int count[16];
   float s = 0.f;
   int c = 0;
-#pragma unroll 8
+#pragma unroll 16
   for (int64_t i = threadIdx.x; i < n; i += 1024) {
     s += row_loss[i];
     c += (uint64_t)labels[i] < (uint64_t)V;
@@ -380,7 +389,7 @@ __global__ __launch_bounds__(1024) void bias_kernel(const float* __restrict__ pa
 struct Plan {
   int64_t ldz, rows32;
   int rows, wgs, pieces;
-  bool pack_x, pack_w;
+  bool pack_x, pack_w, narrow;
   size_t z, dz, db, dw, x, w, gemm, bytes;  // offsets, and the whole
 };
 
@@ -397,6 +406,19 @@ bool whole(const void* p, int64_t ld, int cols) {
   return cols % 8 == 0 && ld % 8 == 0 && ld < kGemmBf16MaxLd && ((uintptr_t)p & 15) == 0;
 }
 
+// Whether a block of so many rows is faster in narrow_xent, with
+// (rows, C, V)          here, fp32 and bf16   there
+// (16384, 384, 65)      95    83              63    62 us
+// (16384, 1024, 65)     181   99              104   106
+// (16384, 384, 96)      86    78              70    72
+// (16384, 1024, 96)     158   94              119   124
+// (16384, 384, 128)     84    79              99    101
+// (2048, 384, 65)       57    53              43    45
+// (300, 2048, 65)       50    50              124   133
+bool narrow_is_faster(int dtype, int rows, int C, int V) {
+  return V <= (dtype == MTX_F32 ? kNarrowV : 80) && rows >= 4LL * C;
+}
+
 // Row kernels' workgroups: about as many as the chip holds at once (as many partial
 // column sums are added up at the end).
 int row_wgs(int rows, int V) { return V <= 1024 ? std::min(cdiv(rows, 4), 1024) : std::min(rows, V <= 4096 ? 1024 : V <= 16384 ? 512 : 256); }
@@ -404,25 +426,30 @@ int row_wgs(int rows, int V) { return V <= 1024 ? std::min(cdiv(rows, 4), 1024) 
 // The rows whose logits are kept at a time are as many as have logits_bytes of them.
 // The query for the workspace's size does not know where the operands lie and counts
 // their copies (pack_x, pack_w) in.
-Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logits_bytes, bool pack_x, bool pack_w) {
+// near: strides that narrow_xent takes.
+Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logits_bytes, bool pack_x, bool pack_w,
+          bool near) {
   Plan p{};
   p.ldz = (V + 31) / 32 * 32;
   const int64_t fit = std::min<int64_t>(std::max<int64_t>(logits_bytes / (4 * p.ldz), 1), 1 << 18);
   p.rows = (int)std::min(n, fit < 256 ? fit : fit / 256 * 256);
   p.rows32 = (p.rows + 31) / 32 * 32;
+  p.narrow = near && narrow_is_faster(dtype, p.rows, C, V);
   p.wgs = row_wgs(p.rows, V);
   p.pieces = grads < 0 ? 0 : dtype == MTX_F32 ? -1 : grads == MTX_F32 ? 3 : 1;
   size_t at = 256;  // 1 / labels
   p.z = at;  // without gradients bf16 logits are never stored: their statistics are
-  at += p.pieces == 0 && dtype == MTX_BF16 ? up((size_t)p.rows * (cdiv(V, 64) * 8 + 4)) : up((size_t)p.rows * p.ldz * 4);
+  // narrow: dz alone, where the logits would be, and dW's ranges
+  if (p.narrow) at += p.pieces ? up((size_t)p.rows * p.ldz * 4) : 0;
+  else at += p.pieces == 0 && dtype == MTX_BF16 ? up((size_t)p.rows * (cdiv(V, 64) * 8 + 4)) : up((size_t)p.rows * p.ldz * 4);
   p.dz = at;
-  if (p.pieces > 0) at += up((size_t)p.pieces * p.rows32 * p.ldz * 2);
+  if (p.pieces > 0 && !p.narrow) at += up((size_t)p.pieces * p.rows32 * p.ldz * 2);
   p.db = at;
-  if (p.pieces && bias) at += up((size_t)p.wgs * p.ldz * 4);
+  if (p.pieces && bias && !p.narrow) at += up((size_t)p.wgs * p.ldz * 4);
   p.dw = at;  // a bf16 gradient of the weights is summed over blocks of rows in fp32
   if (p.pieces == 1 && p.rows < n) at += up((size_t)C * V * 4);
-  p.pack_x = dtype == MTX_BF16 && pack_x;
-  p.pack_w = dtype == MTX_BF16 && pack_w;
+  p.pack_x = dtype == MTX_BF16 && !p.narrow && pack_x;
+  p.pack_w = dtype == MTX_BF16 && !p.narrow && pack_w;
   const int64_t c32 = (C + 31) / 32 * 32;
   p.x = at;
   if (p.pack_x) at += up((size_t)p.rows32 * c32 * 2);
@@ -432,6 +459,10 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   size_t most = 0;
   for (int r : {p.rows, (int)(n % p.rows)}) {
     if (!r) continue;
+    if (p.narrow) {
+      if (p.pieces) most = std::max(most, narrow_grad_workspace_bytes(r, C, V));
+      continue;
+    }
     auto bytes = [&](int M, int N, int K) {
       most = std::max(most, dtype == MTX_F32 ? mtx_gemm_workspace_bytes(M, N, K, 1)
                                              : gemm_bf16_workspace_bytes(M, N, K, N == V && M == r ? 1 : p.pieces));
@@ -480,7 +511,10 @@ using namespace mtx;
 extern "C" size_t mtx_linear_xent_workspace_bytes(int dtype, int grad_dtype, int64_t n, int C, int V, int bias,
                                                   int64_t logits_bytes) {
   if (n < 0 || C < 1 || V < 1 || n >= (1LL << 31)) return 0;
-  return plan(dtype, grad_dtype, std::max<int64_t>(n, 1), C, V, bias != 0, logits_bytes, true, true).bytes;
+  auto bytes = [&](bool near) {
+    return plan(dtype, grad_dtype, std::max<int64_t>(n, 1), C, V, bias != 0, logits_bytes, true, true, near).bytes;
+  };
+  return std::max(bytes(true), bytes(false));
 }
 
 extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int V, const void* x, int64_t ldx,
@@ -508,8 +542,9 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   // W's rows in memory: of V values, or of C
   const bool wv = swv == 1 && swc >= V;
   const int64_t ldw = wv ? swc : swv;
+  const bool near = std::max({n ? ldx : 0, ldw, dx ? lddx : 0}) < kNarrowLd;
   const Plan p = plan(dtype, grad ? grad_dtype : -1, std::max<int64_t>(n, 1), C, V, db != nullptr, logits_bytes,
-                      (n >= kPanelRows && V >= kPanelCols) || !whole(x, ldx, C), !whole(w, ldw, wv ? V : C));
+                      (n >= kPanelRows && V >= kPanelCols) || !whole(x, ldx, C), !whole(w, ldw, wv ? V : C), near);
   MTX_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
                 "linear_xent: workspace of %zu bytes, need %zu aligned to 256", workspace_bytes, p.bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -519,7 +554,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   bf16_t* dz = reinterpret_cast<bf16_t*>(ws + p.dz);
   // fp32: the bias' gradient comes with the weights', where their rows are contiguous
   const bool sums = dtype == MTX_F32 && db && dw && sdv == 1;
-  float* part = db && !sums ? reinterpret_cast<float*>(ws + p.db) : nullptr;
+  float* part = db && !sums && !p.narrow ? reinterpret_cast<float*>(ws + p.db) : nullptr;
   float* sum = reinterpret_cast<float*>(ws + p.dw);
   bf16_t* xp = reinterpret_cast<bf16_t*>(ws + p.x);
   bf16_t* wp = reinterpret_cast<bf16_t*>(ws + p.w);
@@ -559,6 +594,31 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       xm = bf16_panels(xp, r32, c32 / 32, 0);
     }
     const Bf16Matrix dm = bf16_panels(dz, r32, p.ldz / 32, piece);
+    if (p.narrow) {
+      const void* xr = dtype == MTX_F32 ? static_cast<const void*>(xf) : xb;
+      const bool half = grad_dtype == MTX_BF16;
+      if ((rc = narrow_xent({dtype, xr, ldx, w, swc, swv, bias, labels + r0, inv, row_loss + r0, lse + r0, r, C, V,
+                             dx ? static_cast<char*>(dx) + r0 * lddx * (half ? 2 : 4) : nullptr, lddx, half,
+                             dw || db ? z : nullptr, p.ldz}, st)))
+        return rc;
+      if (!dw && !db) continue;
+      // blocks of rows are added up in fp32, the sum is rounded once
+      const bool apart = half && p.rows < n;
+      NarrowGrad g{dtype, xr, ldx, z, p.ldz, r, C, V, dw, sdc, sdv, half, static_cast<const float*>(dw), sdc, sdv, db, first};
+      if (apart) {
+        g.sum = sum;
+        g.sum_c = V;
+        g.sum_v = 1;
+        if (!last) {
+          g.dw = dw ? sum : nullptr;
+          g.sdc = V;
+          g.sdv = 1;
+          g.dw_bf16 = false;
+        }
+      }
+      if ((rc = narrow_grad(g, gws, st))) return rc;
+      continue;
+    }
     if (dtype == MTX_F32) {
       rc = mtx_gemm_f32(r, V, C, 1, 1.f, xf, ldx, 1, 0, static_cast<const float*>(w), swc, swv, 0, 0.f, z, p.ldz, 1, 0,
                         bias, gws, gbytes, stream);

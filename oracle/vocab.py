@@ -69,5 +69,5 @@ def linear_xent(x, w, labels, bias=None):
     dz[rows, at] -= 1.0
     dz[~some] = 0.0
     dz /= count
-    return dict(z=z, lse=lse, p=p, row_loss=row_loss, loss=row_loss.sum() / count, dz=dz, dx=dz @ w.T, dw=x.T @ dz,
+    return dict(z=z, lse=lse, p=p, some=some, row_loss=row_loss, loss=row_loss.sum() / count, dz=dz, dx=dz @ w.T, dw=x.T @ dz,
                 db=dz.sum(0))

@@ -306,10 +306,10 @@ def xent_bounds(x, w, bias, r, dtype, out):
     fin = np.where(np.isfinite(r["lse"]), np.abs(r["lse"]), 0.0)
     lse = e + 4 * U * (fin + mag)
     row = lse + ez + 4 * U * (fin + mag)
-    # Rows with a label: some entry of theirs has a gradient.  Not entry by entry: the
-    # label's own is p - 1, exactly 0 in float64 once 1 - p < 2^-54, and a p that is off
-    # by p (2 e + 8 u) is off by that beside 1 too.
-    named = (r["dz"] != 0).any(1)
+    # All entries of a row with a label, not those alone whose gradient is not 0: the
+    # label's own is p - 1, exactly 0 in float64 once 1 - p < 2^-54 (or V is 1), and a p
+    # that is off by p (2 e + 8 u) is off by that beside 1 too.
+    named = r["some"]
     count = max(1, int(named.sum()))
     loss = row.sum() / count + (n + 4) * U * np.where(np.isfinite(r["row_loss"]), r["row_loss"], 0).sum() / count
     d = np.abs(r["dz"])
@@ -374,6 +374,89 @@ def test_linear_xent(dev, n, C, V, tied, dtype, out):
 def test_linear_xent_lengths_of_rows(dev, V, bias, dtype, out):
     """Where one way to walk a row ends and the next begins."""
     check_xent(5, 6, V, dtype, out, tied=True, bias=bias)
+
+
+# many rows and a small vocabulary: one to six chunks of C, the borders of the tiles of
+# 16 entries, rows that fill no group of 16 or 64, and what lies beside
+NARROW = [(4, 1, 1), (20, 5, 3), (19, 5, 3), (63, 8, 16), (130, 32, 17), (300, 64, 32), (300, 65, 33), (515, 128, 64),
+          (1030, 129, 65), (1025, 200, 65), (2000, 384, 65), (700, 130, 80), (129, 32, 81), (640, 33, 96), (515, 100, 96),
+          (640, 130, 95), (640, 130, 97), (4100, 70, 65)]
+
+
+@pytest.mark.parametrize("dtype,out", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("n,C,V", NARROW)
+def test_linear_xent_small_vocabularies(dev, n, C, V, tied, dtype, out):
+    check_xent(n, C, V, dtype, out, tied=tied, bias=n % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype,out", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+def test_linear_xent_small_vocabulary_strides_and_blocks(dev, dtype, out):
+    for tied in (False, True):
+        for pad, at in ((8, 0), (4, 4), (3, 1)):
+            check_xent(210, 44, 65, dtype, out, tied=tied, pad=pad, at=at)
+            check_xent(210, 37, 20, dtype, out, tied=tied, pad=pad, at=at)
+        check_xent(1000, 40, 65, dtype, out, tied=tied, logits_bytes=256 * 96 * 4)
+        check_xent(700, 20, 30, dtype, out, tied=tied, logits_bytes=100 * 32 * 4)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_linear_xent_small_vocabulary_rows_far_apart(dev, dtype):
+    """Rows of the weights 2^22 values apart."""
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(3)
+    n, C, V, ld = 30, 3, 7, 1 << 22
+    x, w = rounded(rng.standard_normal((n, C)), dtype), rounded(rng.standard_normal((C, V)), dtype)
+    labels = tokens(rng, n, V)
+    r = ref.linear_xent(x, w, labels)
+    bd = xent_bounds(x, w, None, r, dtype, "float32")
+    dx, dw = empty((n, C)), empty((C, V))
+    loss, row, lse = K.linear_xent(dev_array(x, dtype), wide(w, dtype, ld - V), dev_array(labels, "int64"), dx=dx,
+                                   dw=dw)
+    for got, want, b in ((lse, r["lse"], bd[0]), (row, r["row_loss"], bd[1]), (dx, r["dx"], bd[3]), (dw, r["dw"], bd[4])):
+        inside(host(got), want, b)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_linear_xent_small_vocabulary_hidden_entries_and_rows(dev, dtype):
+    """Entries hidden by a bias of -inf, all of a row's, rows without a label that hold
+    anything finite; gradients wanted one at a time; the same bits every time."""
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(8)
+    n, C, V = 300, 40, 65
+    x, w = rounded(rng.standard_normal((n, C)), dtype), rounded(rng.standard_normal((C, V)) / 6, dtype)
+    b = np.where(rng.random(V) < 0.4, -np.inf, 0.0).astype(np.float32)
+    b[0] = 0.0
+    labels = np.where(rng.random(n) < 0.3, -1, 0)
+    x[labels < 0] = rounded(1e38, dtype)
+    seen = x.copy()
+    seen[labels < 0] = 0.0
+    r = ref.linear_xent(seen, w, labels, b)
+    bd = xent_bounds(seen, w, np.where(b == -np.inf, 0.0, b), r, dtype, "float32")
+    args = [dev_array(x, dtype), dev_array(w, dtype), dev_array(labels, "int64")]
+    first = None
+    for _ in range(3):
+        dx, dw, db = empty((n, C)), empty((C, V)), empty((V,))
+        loss, row, lse = K.linear_xent(*args, bias=dev_array(b), dx=dx, dw=dw, db=db)
+        now = [host(t) for t in (loss, row, dx, dw, db)]
+        first = first or now
+        assert all(np.array_equal(p, q) for p, q in zip(first, now))
+    inside(host(lse)[labels >= 0], r["lse"][labels >= 0], bd[0][labels >= 0])
+    for got, want, bound in zip(now, ([r["loss"]], r["row_loss"], r["dx"], r["dw"], r["db"]), (bd[2], bd[1], *bd[3:])):
+        inside(got, np.asarray(want), bound)
+    assert (now[4][b == -np.inf] == 0).all()
+    for name, like, want in (("dx", (n, C), now[2]), ("dw", (C, V), now[3]), ("db", (V,), now[4])):
+        g = empty(like)
+        K.linear_xent(*args, bias=dev_array(b), **{name: g})
+        assert np.array_equal(host(g), want)
+    none = dev_array(np.full(V, -np.inf))
+    dx, dw, db = empty((n, C)), empty((C, V)), empty((V,))
+    args[0] = dev_array(seen, dtype)
+    loss, row, lse = K.linear_xent(*args, bias=none, dx=dx, dw=dw, db=db)
+    assert (host(lse) == -np.inf).all() and np.array_equal(host(row), np.where(labels < 0, 0, np.inf))
+    assert abs(host(db)[0] + 1) <= (n + 2) * U and not host(db)[1:].any()
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
