@@ -865,8 +865,10 @@ int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void* logits, i
  * lse -inf, row_loss +inf and, as gradient, its label's own term alone.  Infinities
  * and NaN in x or w give NaN (fp32: in every logit that they meet).
  * The rows are worked through in blocks whose logits (fp32) fill at most logits_bytes
- * (one row at least); fewer, larger blocks are faster.  bf16 gradients are products of the logits' gradient rounded to bf16,
- * fp32 ones of all its 24 bits; either way sums are fp32, rounded once.
+ * (one row at least, 2^18 at most); fewer, larger blocks are faster.  bf16 gradients
+ * are products of the logits' gradient rounded to bf16 (small vocabularies: of all its
+ * bits), fp32 ones of all its 24 bits; either way sums are fp32, rounded once.  No
+ * output may overlap an input or another output.
  * n < 2^31, C <= 2^20, V <= 2^27; bf16: V < 2^22, and rows of dx and dw less than 2^26
  * values apart.  Deterministic.
  */
@@ -890,15 +892,16 @@ int mtx_embedding_bwd_f32(const int64_t* idx, int64_t n, const float* grad, int6
 /*
  * Scaled lookup: out[i, :] = scale * weight[ids[i], :] (layers.py:102-104), zeros
  * where ids[i] is outside [0, V): no token, padding.  Table and output are fp32 or
- * bf16 each, the product is rounded once.  n, V < 2^31.
+ * bf16 each, the product is rounded once.  n, V < 2^31.  out may not overlap weight.
  */
 int mtx_embedding_lookup(int dtype, int out_dtype, const void* weight, int64_t ldw, int64_t V, const int64_t* ids,
                          int64_t n, int C, float scale, void* out, int64_t ldo, void* stream);
 /*
- * Its gradient by sorted tokens: dweight[v, :] (+)= scale * the sum of the rows
- * grad[i, :] (fp32 or bf16) with ids[i] = v (np.add.at, tensor.py:382), in fp32 and
- * in token order.  Tokens outside [0, V) add to nothing.  Without accumulate every row of dweight
- * is written, with it only those that have tokens.  Deterministic.
+ * Its gradient: dweight[v, :] (+)= scale * the sum of the rows grad[i, :] (fp32 or
+ * bf16) with ids[i] = v (np.add.at, tensor.py:382), in fp32: few tokens in token order,
+ * many in runs of consecutive ones whose sums are added in order.  Tokens outside
+ * [0, V) add to nothing.  Without accumulate every row of dweight is written, with it
+ * only those that have tokens.  dweight may not overlap grad.  Deterministic.
  */
 size_t mtx_embedding_grad_workspace_bytes(int dtype, int64_t n, int64_t V, int C);
 int mtx_embedding_grad(int dtype, const int64_t* ids, int64_t n, const void* grad, int64_t ldg, float scale,

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const DropArgs a) {
 
 // Rows of whole 16-byte vectors (all values as one row where they lie side by side), a
 // vector a thread.  Memory bounds it: 16384 x 384 fp32 with a residual 11.8 us (6.4
-// TB/s, one value at a time 25.0), 32768 x 2048 bf16 52 us (5.2 TB/s; 106); the
+// TB/s, one value at a time 25.0), 32768 x 2048 bf16 45 us (5.9 TB/s; 106); the
 // generator's 20 wide products for four values run beside it.  Two and four vectors a
 // thread took 53 and 58 us.
 template <typename T, bool RES, bool FLAT>

@@ -547,6 +547,12 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
                       (n >= kPanelRows && V >= kPanelCols) || !whole(x, ldx, C), !whole(w, ldw, wv ? V : C), near);
   MTX_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
                 "linear_xent: workspace of %zu bytes, need %zu aligned to 256", workspace_bytes, p.bytes);
+  {
+    const void* in[] = {x, w, bias};
+    const void* out[] = {dx, dw, db, loss, row_loss, lse};
+    for (const void* o : out)
+      for (const void* i : in) MTX_CHECK_ARG(!o || n == 0 || o != i, "linear_xent: an output is an input");
+  }
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   float* inv = reinterpret_cast<float*>(ws);

@@ -526,8 +526,8 @@ def embedding(weight, idx, scale=1.0):
     """scale * weight[idx] for a (V, C) table (Embedding.forward, layers.py:102-104,
     times a constant), (*idx.shape, C).  A negative id has no row: zeros, and no
     gradient (padding); device-resident ids outside the table count as that too.
-    The gradient adds the rows up by token, in token order, from the tokens sorted
-    on the device (mtx_embedding_lookup, mtx_embedding_grad)."""
+    The gradient adds the rows up by token, in a fixed order, without looking
+    through all tokens for every row (mtx_embedding_lookup, mtx_embedding_grad)."""
     V, C = weight.shape
     if not isinstance(idx, DeviceArray):
         idx = np.asarray(idx)

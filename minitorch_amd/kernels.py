@@ -1364,7 +1364,7 @@ def _grad_plan(ids, grad, dweight):
 
 def embedding_grad(ids, grad, dweight, scale: float = 1.0, accumulate: bool = False):
     """dweight (V, C) fp32 = (with accumulate: +=) scale * the rows of grad (n, C),
-    fp32 or bf16, added up by their int64 (n,) ids in token order
+    fp32 or bf16, added up by their int64 (n,) ids in a fixed order
     (mtx_embedding_grad).  Rows whose id is outside [0, V) add to nothing."""
     if not (ids.is_cuda and grad.is_cuda and dweight.is_cuda):
         _on_device(ids, grad, dweight)
@@ -1407,6 +1407,8 @@ def dropout(x, p: float, seed: int, offset: int = 0, residual=None, out=None, su
         out = dev.empty_buf(x.shape, _dt(x))
     if not (x.is_cuda and out.is_cuda):
         _on_device(x, out)
+    if residual is not None:
+        _on_device(residual)
     code, rows, cols, (ldx, ldr, ldo) = _dropout_plan((x.shape, x.stride(), x.dtype), _spec(residual),
                                                       (out.shape, out.stride(), out.dtype))
     if base is not None:
@@ -1479,7 +1481,8 @@ def linear_xent(x, w, labels, bias=None, loss=None, row_loss=None, lse=None, dx=
     [0, V): none; bias fp32 (V,).  Returns (loss (1,): the mean over the rows that
     have a label, row_loss (n,), lse (n,)), fp32.  dx (n, C), dw (C, V) and db (V,),
     where given, receive the gradients of loss: fp32, dx and dw also bf16 with bf16
-    inputs.  The logits of as many rows as fill logits_bytes are kept at a time."""
+    inputs.  The logits of as many rows as fill logits_bytes are kept at a time.  No
+    output may overlap an input or another output."""
     if logits_bytes < 1:
         raise ValueError(f"logits_bytes must be positive (got {logits_bytes})")
     n = x.shape[0]
@@ -1487,6 +1490,7 @@ def linear_xent(x, w, labels, bias=None, loss=None, row_loss=None, lse=None, dx=
     row_loss, lse = (dev.empty_buf((n,), "float32") if t is None else t for t in (row_loss, lse))
     if not (x.is_cuda and w.is_cuda and labels.is_cuda and loss.is_cuda and row_loss.is_cuda and lse.is_cuda):
         _on_device(x, w, labels, loss, row_loss, lse)
+    _on_device(*(t for t in (bias, dx, dw, db) if t is not None))
     sizes, ldx, sw, lddx, sd, ws_bytes = _xent_plan(
         (x.shape, x.stride(), x.dtype), (w.shape, w.stride(), w.dtype), (labels.shape, labels.stride(), labels.dtype),
         _spec(bias), (loss.shape, loss.stride(), loss.dtype), (row_loss.shape, row_loss.stride(), row_loss.dtype),

@@ -279,3 +279,61 @@ def test_greedy_decoding_refuses_scaled_tables(dev):
     model.tok_emb = mt.Embedding(cfg.vocab, cfg.n_embd, scale=8.0)
     with pytest.raises(NotImplementedError):
         model.generate_greedy(np.zeros((1, 4), np.int64), 3)
+
+
+@pytest.mark.parametrize("first", [0, 1])
+def test_a_transposed_table_with_two_uses(dev, first):
+    """Its gradient arrives in the table's layout from one use and row by row from
+    the other, in either order."""
+    import minitorch_amd as mt
+    from minitorch_amd import F
+
+    rng = np.random.default_rng(12)
+    table = mt.Tensor(rng.standard_normal((30, 8)).astype(np.float32), requires_grad=True)
+    x = mt.Tensor(rng.standard_normal((20, 8)).astype(np.float32), requires_grad=True)
+    labels = rng.integers(0, 30, 20)
+    F.set_dropout_seed(4)
+    w = table.transpose()
+    uses = [lambda: F.linear_cross_entropy(x, w, None, labels), lambda: F.dropout(w, 0.5).sum()]
+    a, b = uses[first](), uses[1 - first]()
+    (a + b).backward()
+    keep = ref.keep((1, 240), 0.5, 4, 0, subsequence=1).reshape(8, 30)
+    r = ref.linear_xent(x.numpy(), table.numpy().T, labels)
+    bound = xent_bounds(x.numpy(), table.numpy().T, None, r, "float32", "float32")[4].T
+    want = (r["dw"] + 2.0 * keep).T
+    inside(table.grad.numpy(), want, bound + 2 * U * (np.abs(want) + bound))
+
+
+def test_shapes_at_the_ends(dev):
+    """No rows, one row without a batch axis, 0-d values, transposed inputs."""
+    import minitorch_amd as mt
+    from minitorch_amd import F
+
+    rng = np.random.default_rng(13)
+    w = mt.Tensor(rng.standard_normal((8, 30)).astype(np.float32), requires_grad=True)
+    x = mt.Tensor(np.zeros((0, 8), np.float32), requires_grad=True)
+    loss = F.linear_cross_entropy(x, w, None, np.zeros(0, np.int64))
+    loss.backward()
+    assert float(loss) == 0 and not w.grad.numpy().any() and x.grad.numpy().shape == (0, 8)
+    assert F.embedding(w, np.zeros((0,), np.int64)).shape == (0, 30)
+    assert F.dropout(mt.Tensor(np.zeros((0, 3), np.float32)), 0.5).shape == (0, 3)
+    one = rng.standard_normal(8).astype(np.float32)
+    t = mt.Tensor(one, requires_grad=True)
+    F.linear_cross_entropy(t, w, None, np.array([3])).backward()
+    r = ref.linear_xent(one[None], w.numpy(), np.array([3]))
+    inside(t.grad.numpy(), r["dx"][0], xent_bounds(one[None], w.numpy(), None, r, "float32", "float32")[3][0])
+    w.grad = None
+    y = F.embedding(w, np.array(2), scale=2.0)
+    y.sum().backward()
+    assert np.array_equal(y.numpy().ravel(), 2 * w.numpy()[2])
+    assert np.array_equal(w.grad.numpy(), np.where(np.arange(8)[:, None] == 2, 2.0, 0.0) * np.ones(30))
+    s = mt.Tensor(np.float32(3), requires_grad=True)
+    F.set_dropout_seed(1)
+    F.dropout(s, 0.5).backward()
+    assert s.grad.numpy().item() in (0.0, 2.0)
+    xt = rng.standard_normal((8, 20)).astype(np.float32)
+    labels = rng.integers(0, 30, 20)
+    tx = mt.Tensor(xt, requires_grad=True)
+    F.linear_cross_entropy(tx.transpose(), w, None, labels).backward()
+    r = ref.linear_xent(xt.T, w.numpy(), labels)
+    inside(tx.grad.numpy(), r["dx"].T, xent_bounds(xt.T, w.numpy(), None, r, "float32", "float32")[3].T)

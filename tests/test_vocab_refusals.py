@@ -215,11 +215,32 @@ def test_xent_wrapper_refuses(monkeypatch, over, frag):
         K.linear_xent(**{**dict(x=Fake((4, 8)), w=Fake((8, 10)), labels=Fake((4,), "int64")), **over})
 
 
+@pytest.mark.parametrize("fn,over,frag", [
+    (lookup, dict(), "out is the table"),
+    (grad, dict(), "dweight is grad"),
+    (xent, dict(), "an output is an input"),
+    (xent, dict(x=p(32), w=p(48), bias=p(64), dw=p(48)), "an output is an input"),
+    (xent, dict(x=p(32), w=p(48), bias=p(64), loss=p(64)), "an output is an input"),
+])
+def test_outputs_in_place_of_inputs(fn, over, frag):
+    rc, msg = fn(over)
+    assert rc == L.MTX_ERR_ARG and frag in msg
+
+
 def test_wrappers_refuse_host_arrays(monkeypatch):
     K = _kernels(monkeypatch)
     host = Fake((4, 8))
     host.is_cuda = False
-    for f in (lambda: K.dropout(host, 0.5, 1), lambda: K.embedding_lookup(host, Fake((4,), "int64")),
+    vec = Fake((10,))
+    vec.is_cuda = False
+    wide = Fake((8, 10))
+    wide.is_cuda = False
+    args = Fake((4, 8)), Fake((8, 10)), Fake((4,), "int64")
+    for f in (lambda: K.dropout(Fake((4, 8)), 0.5, 1, residual=host), lambda: K.dropout(Fake((4, 8)), 0.5, 1, out=host),
+              lambda: K.linear_xent(*args, bias=vec), lambda: K.linear_xent(*args, dx=host),
+              lambda: K.linear_xent(*args, dw=wide), lambda: K.linear_xent(*args, bias=Fake((10,)), db=vec),
+              lambda: K.embedding_grad(Fake((4,), "int64"), Fake((4, 8)), wide),
+              lambda: K.dropout(host, 0.5, 1), lambda: K.embedding_lookup(host, Fake((4,), "int64")),
               lambda: K.embedding_grad(Fake((4,), "int64"), host, Fake((10, 8))),
               lambda: K.linear_xent(host, Fake((8, 10)), Fake((4,), "int64"))):
         with pytest.raises(ValueError, match="device arrays"):
