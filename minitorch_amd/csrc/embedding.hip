@@ -501,7 +501,8 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(const GradArgs a, int
 // table, a wave every 16th of them; the ids lie in LDS with the rows' counts, and a row's
 // tokens are found by comparing 64 of them at a time.  Rows of more than kPiece tokens are left to the end:
 // each wave takes a contiguous part of the ids, and the parts' sums are added in order.
-// 300 tokens of 384 fp32 values, a table of 5003 rows (7.7 MB): 9 us; 1339 bf16 tokens of
+// 300 tokens of 384 fp32 values, a table of 5003 rows (7.7 MB): 7.4 us (9.7 with all of a
+// row's columns by one workgroup; 208 tokens of 2248, 4 rows: 10 and 36); 1339 bf16 tokens of
 // 256, 42338 rows (43 MB): 20, and 27 where every row's tokens were counted by comparing.
 constexpr int kSmallTokens = 4096, kScan = 4;  // groups of ids looked at together
 template <typename T, int VEC, int U>
@@ -514,7 +515,7 @@ __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, in
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = (int)a.n;
   const int64_t v0 = (int64_t)blockIdx.x * R;
   const uint32_t rows = (uint32_t)min<int64_t>(R, a.V - v0);
-  const int groups = (n + 63) / 64;
+  const int groups = (n + 63) / 64, from = (int)blockIdx.y * kCols + lane * VEC;
   if (threadIdx.x == 0) many = 0;
   if (threadIdx.x < kMaxRows) count[threadIdx.x] = 0;
   __syncthreads();
@@ -576,7 +577,7 @@ __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, in
       continue;
     }
     if (some == 0 && a.accumulate) continue;
-    for (int c0 = lane * VEC; c0 - lane * VEC < a.C; c0 += kCols) {
+    for (int c0 = from; c0 - lane * VEC < a.C; c0 += kCols * (int)gridDim.y) {
       add(r, 0, some ? groups : 0, c0, acc);
       store_row<VEC, 64, U>(a, v0 + r, c0, acc);
     }
@@ -586,7 +587,7 @@ __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, in
   for (uint32_t k = 0; k < many; ++k) {
     const uint32_t r = longs[k];
     const int per = (groups + kWaves - 1) / kWaves, g0 = min(groups, w * per), g1 = min(groups, g0 + per);
-    for (int c0 = lane * VEC; c0 - lane * VEC < a.C; c0 += kCols) {
+    for (int c0 = from; c0 - lane * VEC < a.C; c0 += kCols * (int)gridDim.y) {
       add(r, g0, g1, c0, acc);
       __syncthreads();
 #pragma unroll
@@ -775,7 +776,9 @@ int grad(GradArgs a, const Plan& p, char* ws, hipStream_t st) {
   constexpr int kVec = 16 / sizeof(T), kU = sizeof(T) == 4 ? 2 : 1;
   const bool vec = whole(a.g, a.ldg, a.C, kVec, sizeof(T)) && whole(a.dw, a.lddw, a.C, kVec, 4);
   if (p.small) {
-    const dim3 grid(p.sorts), block(64 * kWaves);
+    // columns beside each other too, where there are few table rows
+    const int cols = vec ? 64 * kVec : 256;
+    const dim3 grid(p.sorts, std::min<unsigned>(cdiv(a.C, cols), std::max(1u, 512 / p.sorts))), block(64 * kWaves);
     if (vec) hipLaunchKernelGGL((small_kernel<T, kVec, 1>), grid, block, 0, st, a, p.R);
     else hipLaunchKernelGGL((small_kernel<T, 1, 4>), grid, block, 0, st, a, p.R);
     MTX_LAUNCHED();
