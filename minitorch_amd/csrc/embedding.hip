@@ -499,8 +499,9 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(const GradArgs a, int
 
 // The whole gradient in one launch, for few tokens.  A workgroup takes R rows of the
 // table, a wave every 16th of them; the ids lie in LDS with the rows' counts, and a row's
-// tokens are found by comparing 64 of them at a time.  Rows of more than kPiece tokens are left to the end:
-// each wave takes a contiguous part of the ids, and the parts' sums are added in order.
+// tokens are found by comparing 64 of them at a time.  Rows of more than kPiece tokens
+// are left to the end: each wave takes a contiguous part of the ids, and the parts' sums
+// are added in order.
 // 300 tokens of 384 fp32 values, a table of 5003 rows (7.7 MB): 7.4 us (9.7 with all of a
 // row's columns by one workgroup; 208 tokens of 2248, 4 rows: 10 and 36); 1339 bf16 tokens of
 // 256, 42338 rows (43 MB): 20, and 27 where every row's tokens were counted by comparing.
@@ -746,8 +747,10 @@ Plan plan(int dtype, int64_t n, int64_t V, int C) {
   const int size = dtype == MTX_F32 ? 4 : 2;
   p.R = (int)std::min<int64_t>((V + 255) / 256, kMaxRows);
   p.sorts = (unsigned)((V + p.R - 1) / p.R);
-  // Few tokens, as long as one workgroup may have to read all their rows
-  p.small = n <= kSmallTokens && n * C * size <= (1 << 20);
+  // Few tokens, as long as one workgroup may have to read all their rows, 64 or 128 vectors
+  // of them at a time (1024 tokens of 1856 fp32 values, 9 rows: 8.5 us here, 25 sorted; of
+  // 1024, all of one row: 16 and 19; 600 bf16 tokens of 4096, 5003 rows: 25 and 32)
+  p.small = n <= 1024 || (n <= kSmallTokens && n * C * size <= (1 << 20));
   if (p.small) return p;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
   // Tables of which 64 columns fit in 64 KB of LDS, under tokens enough for 64 chunks of
@@ -776,9 +779,10 @@ int grad(GradArgs a, const Plan& p, char* ws, hipStream_t st) {
   constexpr int kVec = 16 / sizeof(T), kU = sizeof(T) == 4 ? 2 : 1;
   const bool vec = whole(a.g, a.ldg, a.C, kVec, sizeof(T)) && whole(a.dw, a.lddw, a.C, kVec, 4);
   if (p.small) {
-    // columns beside each other too, where there are few table rows
+    // columns beside each other too (600 bf16 tokens of 4096, 5003 rows: 25 us with up to
+    // 2048 workgroups, 43 with 512)
     const int cols = vec ? 64 * kVec : 256;
-    const dim3 grid(p.sorts, std::min<unsigned>(cdiv(a.C, cols), std::max(1u, 512 / p.sorts))), block(64 * kWaves);
+    const dim3 grid(p.sorts, std::min<unsigned>(cdiv(a.C, cols), std::max(1u, 2048 / p.sorts))), block(64 * kWaves);
     if (vec) hipLaunchKernelGGL((small_kernel<T, kVec, 1>), grid, block, 0, st, a, p.R);
     else hipLaunchKernelGGL((small_kernel<T, 1, 4>), grid, block, 0, st, a, p.R);
     MTX_LAUNCHED();

@@ -174,7 +174,8 @@ def test_lookup_grad_same_bits_every_time(dev, n, V, C):
 # tokens, table rows, width: few tokens of wide and narrow rows and the borders where that
 # ends, small tables up to their largest and to their shortest batch, and what lies behind
 GRAD_WAYS = [(4096, 3, 64), (4097, 3, 64), (2048, 40, 128), (2048, 40, 129), (100, 9, 2621), (100, 9, 2622), (4096, 50000, 1),
-             (4096, 127, 70), (8192, 255, 40), (8191, 255, 40), (12001, 200, 515), (8200, 256, 24), (5000, 128, 1030)]
+             (4096, 127, 70), (8192, 255, 40), (8191, 255, 40), (12001, 200, 515), (8200, 256, 24), (5000, 128, 1030),
+             (1024, 9, 300), (1025, 9, 300), (1000, 700, 1300), (1024, 1, 520)]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
