@@ -42,39 +42,7 @@ __global__ __launch_bounds__(1024) void count_kernel(const int64_t* __restrict__
   }
 }
 
-// loss = the mean of the rows' losses over those that have a label, summed in a fixed
-// order.
-__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ row_loss,
-                                                    const int64_t* __restrict__ labels, int64_t n, int V,
-                                                    float* __restrict__ loss) {
-  __shared__ float part[16];
-  __shared__ int count[16];
-  float s = 0.f;
-  int c = 0;
-#pragma unroll 16
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    s += row_loss[i];
-    c += (uint64_t)labels[i] < (uint64_t)V;
-  }
-  s = wave_sum(s);
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) c += __shfl_xor(c, m, 64);
-  if ((threadIdx.x & 63) == 0) {
-    part[threadIdx.x >> 6] = s;
-    count[threadIdx.x >> 6] = c;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float t = 0.f;
-    int k = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      t += part[i];
-      k += count[i];
-    }
-    *loss = t / (float)(k > 0 ? k : 1);
-  }
-}
+__global__ __launch_bounds__(1024) void loss_kernel(const MeanLoss a) { mean_loss(a); }
 
 // rows x cols values of `size` bytes = 0
 __global__ __launch_bounds__(256) void zero_kernel(void* p, int size, int64_t sr, int64_t sc, int rows, int cols) {
@@ -610,7 +578,8 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       if (!dw && !db) continue;
       // blocks of rows are added up in fp32, the sum is rounded once
       const bool apart = half && p.rows < n;
-      NarrowGrad g{dtype, xr, ldx, z, p.ldz, r, C, V, dw, sdc, sdv, half, static_cast<const float*>(dw), sdc, sdv, db, first};
+      NarrowGrad g{dtype, xr, ldx, z, p.ldz, r, C, V, dw, sdc, sdv, half, static_cast<const float*>(dw), sdc, sdv, db, first,
+                   {row_loss, labels, n, V, last ? loss : nullptr}};
       if (apart) {
         g.sum = sum;
         g.sum_c = V;
@@ -728,7 +697,8 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
     hipLaunchKernelGGL(bias_kernel, dim3(cdiv(V, 64)), dim3(1024), 0, st, part, p.ldz, n ? p.wgs : 0, V, inv, db);
     MTX_LAUNCHED();
   }
-  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, labels, n, V, loss);
+  if (n && p.narrow && (dw || db)) return MTX_OK;  // (narrow_grad has it)
+  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, MeanLoss{row_loss, labels, n, V, loss});
   MTX_LAUNCHED();
   return MTX_OK;
 }

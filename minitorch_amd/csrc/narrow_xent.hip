@@ -491,9 +491,13 @@ __global__ __launch_bounds__(256, 2) void narrow_grad_kernel(const NarrowGrad a,
 }
 
 // The ranges' sums, added in order: 64 values a workgroup, whose 16 waves take contiguous
-// runs of ranges
+// runs of ranges.  The mean of the losses by one more, if wanted: its 4 us pass beside.
 __global__ __launch_bounds__(1024) void narrow_sum_kernel(const NarrowGrad a, int ranges, const float* __restrict__ part) {
   __shared__ float sums[16][64];
+  if (a.mean.loss && blockIdx.x == gridDim.x - 1) {
+    mean_loss(a.mean);
+    return;
+  }
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t size = (int64_t)(a.C + 1) * a.V, e = (a.dw ? 0 : (int64_t)a.C * a.V) + (int64_t)blockIdx.x * 64 + lane;
   const int per = (ranges + 15) / 16, b = w * per, end = min(ranges, b + per);
@@ -573,7 +577,8 @@ int narrow_grad(const NarrowGrad& a, void* workspace, hipStream_t st) {
   else run<bf16_t>(a, per, grid, part, st);
   MTX_LAUNCHED();
   const int64_t values = a.dw ? (int64_t)(a.C + 1) * a.V : a.V;
-  hipLaunchKernelGGL(narrow_sum_kernel, dim3((unsigned)((values + 63) / 64)), dim3(1024), 0, st, a, ranges, part);
+  const unsigned wgs = (unsigned)((values + 63) / 64) + (a.mean.loss ? 1 : 0);
+  hipLaunchKernelGGL(narrow_sum_kernel, dim3(wgs), dim3(1024), 0, st, a, ranges, part);
   MTX_LAUNCHED();
   return MTX_OK;
 }
