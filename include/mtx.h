@@ -858,7 +858,8 @@ int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void* logits, i
  *   lse[r] = log sum exp z[r];  row_loss[r] = lse[r] - z[r][labels[r]];
  *   loss[0] = the mean of row_loss over the rows that have a label.
  * A label outside [0, V) is none: row_loss 0, no gradient; loss is 0 if no row has
- * one.  dx (n x C), dw (C x V, strides sdc, sdv, one of them 1) and db (V) receive
+ * one.  (With dw, such a row's x must be finite all the same, its logits need not be:
+ * dw adds 0 times it.)  dx (n x C), dw (C x V, strides sdc, sdv, one of them 1) and db (V) receive
  * the gradients of loss; those that are NULL are not worked out.  dx and dw are
  * fp32, or bf16 with bf16 inputs (grad_dtype; not looked at without gradients);
  * db is fp32.  A logit of -inf has probability 0; a row of nothing else has
@@ -901,7 +902,8 @@ int mtx_embedding_lookup(int dtype, int out_dtype, const void* weight, int64_t l
  * bf16) with ids[i] = v (np.add.at, tensor.py:382), in fp32: few tokens in token order,
  * many in runs of consecutive ones whose sums are added in order.  Tokens outside
  * [0, V) add to nothing.  Without accumulate every row of dweight is written, with it
- * only those that have tokens.  dweight may not overlap grad.  Deterministic.
+ * only those that have tokens.  dweight may not overlap grad.  n < 2^31, V <= 2^31 -
+ * 1024.  Deterministic.
  */
 size_t mtx_embedding_grad_workspace_bytes(int dtype, int64_t n, int64_t V, int C);
 int mtx_embedding_grad(int dtype, const int64_t* ids, int64_t n, const void* grad, int64_t ldg, float scale,

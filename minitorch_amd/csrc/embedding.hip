@@ -691,6 +691,9 @@ __global__ __launch_bounds__(64 * kWaves) void table_sum_kernel(const GradArgs a
   *p = a.accumulate ? *p + a.scale * t : a.scale * t;
 }
 
+// (a launch has fewer than 2^32 threads: 1024 for kMaxRows rows of the table)
+constexpr int64_t kMaxTable = (1LL << 31) - 2 * kMaxRows;
+
 bool known(int dtype) { return dtype == MTX_F32 || dtype == MTX_BF16; }
 
 // whether rows of C values at p, ld values apart, are whole 16-byte vectors of vec
@@ -864,7 +867,7 @@ extern "C" int mtx_embedding_lookup(int dtype, int out_dtype, const void* weight
 }
 
 extern "C" size_t mtx_embedding_grad_workspace_bytes(int dtype, int64_t n, int64_t V, int C) {
-  if (n < 0 || n >= (1LL << 31) || V < 1 || V >= (1LL << 31) || C < 1) return 0;
+  if (n < 0 || n >= (1LL << 31) || V < 1 || V > kMaxTable || C < 1) return 0;
   return plan(dtype, n, V, C).bytes;
 }
 
@@ -872,8 +875,8 @@ extern "C" int mtx_embedding_grad(int dtype, const int64_t* ids, int64_t n, cons
                                   float* dweight, int64_t lddw, int64_t V, int C, int accumulate, void* workspace,
                                   size_t workspace_bytes, void* stream) {
   if (!known(dtype)) return fail(MTX_ERR_DTYPE, "embedding_grad: unsupported dtype %d", dtype);
-  MTX_CHECK_SHAPE(n >= 0 && n < (1LL << 31) && V >= 1 && V < (1LL << 31) && C >= 1 && C <= (1 << 30),
-                  "embedding_grad: need 0 <= n < 2^31, 1 <= V < 2^31, 1 <= C <= 2^30");
+  MTX_CHECK_SHAPE(n >= 0 && n < (1LL << 31) && V >= 1 && V <= kMaxTable && C >= 1 && C <= (1 << 30),
+                  "embedding_grad: need 0 <= n < 2^31, 1 <= V <= 2^31 - 1024, 1 <= C <= 2^30");
   MTX_CHECK_ARG(lddw >= C && (n == 0 || ldg >= C), "embedding_grad: rows of grad or dweight overlap");
   MTX_CHECK_ARG(dweight && (n == 0 || (ids && grad_)), "embedding_grad: null pointer");
   const Plan p = plan(dtype, n, V, C);

@@ -1478,7 +1478,7 @@ def linear_xent(x, w, labels, bias=None, loss=None, row_loss=None, lse=None, dx=
     """Softmax cross-entropy of the logits x @ w + bias, and its gradients, without
     the logits in memory (mtx_linear_xent).  x (n, C) and w (C, V), contiguous along
     either axis (a (V, C) table's .t()), fp32 or bf16; labels int64 (n,), one outside
-    [0, V): none; bias fp32 (V,).  Returns (loss (1,): the mean over the rows that
+    [0, V): none (with dw, x must be finite there too); bias fp32 (V,).  Returns (loss (1,): the mean over the rows that
     have a label, row_loss (n,), lse (n,)), fp32.  dx (n, C), dw (C, V) and db (V,),
     where given, receive the gradients of loss: fp32, dx and dw also bf16 with bf16
     inputs.  The logits of as many rows as fill logits_bytes are kept at a time.  No

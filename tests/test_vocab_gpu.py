@@ -615,6 +615,96 @@ def test_linear_xent_wanted_gradients_alone(dev, dtype, out):
     inside(host(d), host(full_[2]), 2 * 52 * U * np.abs(r["dz"]).sum(0))
 
 
+@pytest.mark.parametrize("dtype,out", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("n,C,V", [(70, 40, 300), (500, 40, 65)])
+def test_linear_xent_gradient_in_the_other_order(dev, n, C, V, dtype, out):
+    """The weights' gradient laid out as the transpose of the weights."""
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(n)
+    x, w = rounded(rng.standard_normal((n, C)), dtype), rounded(rng.standard_normal((C, V)) / 6, dtype)
+    labels = tokens(rng, n, V)
+    r = ref.linear_xent(x, w, labels)
+    bound = xent_bounds(x, w, None, r, dtype, out)[4]
+    for tied in (False, True):
+        wd = dev_array(w.T, dtype).t() if tied else dev_array(w, dtype)
+        dw = empty((C, V), out) if tied else empty((V, C), out).t()
+        K.linear_xent(dev_array(x, dtype), wd, dev_array(labels, "int64"), dw=dw)
+        inside(host(dw) if tied else host(dw.t()).T, r["dw"], bound)
+
+
+# ---------------------------------------------------------------------------
+# more than 2^32 bytes and values
+# ---------------------------------------------------------------------------
+
+def test_lookup_and_gradient_far_into_a_table(dev):
+    from minitorch_amd import kernels as K
+
+    V, C = (1 << 25) + 77, 132  # 4.4e9 values
+    rng = np.random.default_rng(1)
+    far = np.array([0, 5, V // 2, V - 2, V - 1])
+    rows = rounded(rng.standard_normal((len(far), C)), "bfloat16")
+    table = empty((V, C), "bfloat16")
+    for i, v in enumerate(far):
+        table[int(v):int(v) + 1].copy_(dev_array(rows[i:i + 1], "bfloat16"))
+    at = rng.integers(0, len(far), 3000)
+    ids = dev_array(far[at], "int64")
+    assert np.array_equal(host(K.embedding_lookup(table, ids, scale=2.0)), rounded(2.0 * rows[at], "bfloat16"))
+    del table
+    dw = empty((V, C))  # 17.7 GB, of which the rows looked at are set
+    for v in far:
+        dw[int(v):int(v) + 1].copy_(np.ones((1, C), np.float32))
+    for n in (1000, 3000):  # in one launch, and sorted
+        g = rng.integers(-4, 5, (n, C)).astype(np.float32)  # sums are exact
+        K.embedding_grad(dev_array(far[at[:n]], "int64"), dev_array(g), dw, accumulate=True)
+        for i, v in enumerate(far):
+            want = 1 + g[at[:n] == i].sum(0) if n == 1000 else before[i] + g[at[:n] == i].sum(0)
+            assert np.array_equal(host(dw[int(v):int(v) + 1])[0], want)
+        before = [host(dw[int(v):int(v) + 1])[0].copy() for v in far]
+
+
+def test_dropout_of_more_than_32_bits_of_values(dev):
+    from minitorch_amd import kernels as K
+
+    rows, cols = (1 << 20) + 3, 4100
+    x = full((rows, cols), 1.0, "bfloat16")
+    y = K.dropout(x, 0.5, 3, 11, out=x)
+    for r in (0, rows // 2, rows - 5):
+        part = K.dropout(full((5, cols), 1.0, "bfloat16"), 0.5, 3, 11 + r * cols // 4)
+        assert np.array_equal(host(y[r:r + 5]), host(part))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_linear_xent_logits_of_more_than_32_bits_of_bytes(dev, dtype):
+    """All logits at once (4.8 GB, and as much or more of their gradients) and 1024 rows
+    at a time: each is off by at most its bounds, so they differ by at most twice those."""
+    from minitorch_amd import kernels as K
+
+    n, C, V = 40000, 16, 30011
+    rng = np.random.default_rng(5)
+    x = rounded(rng.uniform(-1, 1, (n, C)) * np.linspace(0.1, 4, n)[:, None], dtype)
+    w = rounded(rng.uniform(-1, 1, (C, V)), dtype)
+    labels = tokens(rng, n, V, 0.1)
+    args = dev_array(x, dtype), dev_array(w, dtype), dev_array(labels, "int64")
+    got = []
+    for size in (1 << 33, 1024 * 30016 * 4):
+        dx, dw = empty((n, C)), empty((C, V))
+        loss, row, lse = K.linear_xent(*args, dx=dx, dw=dw, logits_bytes=size)
+        got.append([host(t).copy() for t in (lse, row, dx)])
+        assert np.isfinite(host(dw)).all()
+    some = rng.choice(n, 60, replace=False)
+    some[:4] = 0, 1, n - 2, n - 1
+    r = ref.linear_xent(x[some], w, labels[some])
+    bd = xent_bounds(x[some], w, None, r, dtype, "float32")
+    count = ((labels >= 0) & (labels < V)).sum()
+    mine = max(1, r["some"].sum())
+    for lse, row, dx in got:
+        inside(lse[some], r["lse"], bd[0])
+        inside(row[some], r["row_loss"], bd[1])
+        inside(dx[some], r["dx"] * mine / count, (bd[3] + 2 * U * np.abs(r["dx"])) * mine / count)
+    assert np.abs(got[0][0] - got[1][0]).max() <= 2 * bd[0].max() and np.isfinite(got[0][2]).all()
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------

@@ -58,6 +58,7 @@ def xent(over):
     (lookup, dict(out=None), L.MTX_ERR_ARG, "null"),
     (grad, dict(dtype=2), L.MTX_ERR_DTYPE, "dtype"),
     (grad, dict(n=-1), L.MTX_ERR_SHAPE, "n"),
+    (grad, dict(V=(1 << 31) - 1023), L.MTX_ERR_SHAPE, "1024"),
     (grad, dict(n=1 << 31), L.MTX_ERR_SHAPE, "2^31"),
     (grad, dict(V=0), L.MTX_ERR_SHAPE, "V"),
     (grad, dict(C=0), L.MTX_ERR_SHAPE, "C"),
