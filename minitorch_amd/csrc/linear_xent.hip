@@ -403,8 +403,10 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   p.rows = (int)std::min(n, fit < 256 ? fit : fit / 256 * 256);
   p.rows32 = (p.rows + 31) / 32 * 32;
   p.narrow = near && narrow_is_faster(dtype, p.rows, C, V);
-  p.wgs = row_wgs(p.rows, V);
   p.pieces = grads < 0 ? 0 : dtype == MTX_F32 ? -1 : grads == MTX_F32 ? 3 : 1;
+  // (rows of panels behind the last one are set to 0 by workgroups of their own: 2 rows of
+  // 27453 in three pieces 44 us by two workgroups, 14 by 32)
+  p.wgs = row_wgs(p.pieces > 0 ? (int)p.rows32 : p.rows, V);
   size_t at = 256;  // 1 / labels
   p.z = at;  // without gradients bf16 logits are never stored: their statistics are
   // narrow: dz alone, where the logits would be, and dW's ranges
@@ -626,7 +628,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       MTX_LAUNCHED();
       continue;
     }
-    const int wgs = first ? p.wgs : std::min(p.wgs, row_wgs(r, V));
+    const int wgs = first ? p.wgs : std::min(p.wgs, row_wgs(p.pieces > 0 ? (int)r32 : r, V));
     if (p.pieces == 0) rows<0, false>(a, wgs, st);
     else if (p.pieces < 0) part ? rows<1, true>(a, wgs, st) : rows<1, false>(a, wgs, st);
     else if (p.pieces == 1) part ? rows<2, true>(a, wgs, st) : rows<2, false>(a, wgs, st);
