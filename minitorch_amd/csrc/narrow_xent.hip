@@ -6,9 +6,9 @@
 // its gradient stay in the registers of 16 lanes: x is read once and dx written once by
 // one launch, and only dz (for the second launch, dW) passes through memory.  All products
 // are fp32 ones (mfma_f32_16x16x4f32): nothing of the operands is cut.  (16384, 384) x
-// (384, 65), fp32: 30 us (16 of them before dx), dW 21, and 62 with the counts and sums,
-// where products, softmax and gradients in five launches took 95.  Bound by the matrix
-// cores, at 60 % of their fp32 rate (7 us a product): a SIMD has but one or two waves.
+// (384, 65), fp32: 30 us (16 of them before dx), dW 21, and 57.5 with the count and the
+// sums, where products, softmax and gradients in five launches took 91.  Bound by the
+// matrix cores, half busy (7 us a product at their fp32 rate): a SIMD has but one wave.
 // A wave's rows are worked on one chunk of k after another, so few rows of many k are slow:
 // 300 x 2048 takes 124 us, the general way 50.
 #include "narrow_xent.h"
