@@ -406,7 +406,7 @@ template <typename T, int VEC, int LPR, int U>
 __global__ __launch_bounds__(256) void add_kernel(const GradArgs a) {
   constexpr int kPer = 256 / LPR;
   const int64_t ranges = (a.V + a.rows - 1) / a.rows;
-  const int64_t total = (ranges + (a.part ? (a.n + kPiece - 1) / kPiece : 0)) * a.slices;
+  const int64_t total = (ranges + (a.n + kPiece - 1) / kPiece) * a.slices;
   for (int64_t q = (int64_t)blockIdx.x * kPer + threadIdx.x / LPR; q < total; q += (int64_t)gridDim.x * kPer) {
     const int64_t item = q / a.slices;
     const int c0 = (int)(q - item * a.slices) * LPR * VEC * U + (threadIdx.x % LPR) * VEC;
@@ -750,9 +750,10 @@ Plan plan(int dtype, int64_t n, int64_t V, int C) {
   const int size = dtype == MTX_F32 ? 4 : 2;
   p.R = (int)std::min<int64_t>((V + 255) / 256, kMaxRows);
   p.sorts = (unsigned)((V + p.R - 1) / p.R);
-  // Few tokens, as long as one workgroup may have to read all their rows, 64 or 128 vectors
-  // of them at a time (1024 tokens of 1856 fp32 values, 9 rows: 8.5 us here, 25 sorted; of
-  // 1024, all of one row: 16 and 19; 600 bf16 tokens of 4096, 5003 rows: 25 and 32)
+  // Few tokens, as long as one workgroup may have to read all their rows, 64 vectors or
+  // 256 values of each at a time (1024 tokens of 1856 fp32 values, 9 rows: 8.5 us here, 25
+  // sorted; of 1024, all of one row: 16 and 19; 600 bf16 tokens of 4096, 5003 rows: 25 and
+  // 32)
   p.small = n <= 1024 || (n <= kSmallTokens && n * C * size <= (1 << 20));
   if (p.small) return p;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -773,7 +774,7 @@ Plan plan(int dtype, int64_t n, int64_t V, int C) {
   p.key = p.order + up((size_t)n * 4);
   p.starts = p.key + up((size_t)n * 4);
   p.part = p.starts + up((size_t)(n + kPiece - 1) / kPiece * 4);
-  p.bytes = p.part + (n > kPiece ? up((size_t)((n + kPiece - 1) / kPiece) * 2 * C * 4) : 0);
+  p.bytes = p.part + up((size_t)((n + kPiece - 1) / kPiece) * 2 * C * 4);
   return p;
 }
 
@@ -814,12 +815,12 @@ int grad(GradArgs a, const Plan& p, char* ws, hipStream_t st) {
   a.order = order;
   a.key = key;
   a.starts = starts;
-  a.part = a.n > kPiece ? reinterpret_cast<float*>(ws + p.part) : nullptr;
+  a.part = reinterpret_cast<float*>(ws + p.part);
   const int lpr = lanes(vec ? a.C / kVec : a.C);
   auto go = [&](auto kernel, int columns) {
     a.slices = (a.C + columns - 1) / columns;
     a.rows = lpr < 64 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(8, a.V * a.slices / 8192));
-    const int64_t items = ((a.V + a.rows - 1) / a.rows + (a.part ? (a.n + kPiece - 1) / kPiece : 0)) * a.slices;
+    const int64_t items = ((a.V + a.rows - 1) / a.rows + (a.n + kPiece - 1) / kPiece) * a.slices;
     const int64_t blocks = (items * lpr + 255) / 256;
     hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(blocks, 1 << 23)), dim3(256), 0, st, a);
   };
@@ -834,7 +835,6 @@ int grad(GradArgs a, const Plan& p, char* ws, hipStream_t st) {
     default: go(add_kernel<T, 1, 64, 4>, 256); break;
   }
   MTX_LAUNCHED();
-  if (!a.part) return MTX_OK;
   const int64_t wgs = (a.n + kPiece * kWaves - 1) / (kPiece * kWaves);
   const int chunks = a.C <= 64 ? 1 : a.C <= 128 ? 2 : 4;
   hipLaunchKernelGGL(join_kernel, dim3((unsigned)std::min<int64_t>(wgs, 4096), std::min(cdiv(a.C, 64 * chunks), 64)),

@@ -25,7 +25,7 @@ inline Bf16Matrix bf16_panels(const bf16_t* p, int64_t rows, int64_t panels, int
 // up to K where they are k (K a multiple of 8), else up to whole 32; its rows up to
 // whole tiles, as far as its size goes; what lies behind reads as zeros.  So where the
 // one's columns are k, and K is rounded up over zeros, the other's rows may end earlier.
-// C and add are contiguous along n; add may be C itself.
+// C and add are contiguous along n; add (with A as (K, M) only) may be C itself.
 struct GemmBf16 {
   Bf16Matrix a;
   bool a_k;

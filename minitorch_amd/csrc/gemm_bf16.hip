@@ -555,9 +555,14 @@ Plan plan(int M, int N, int K, int pieces, bool stats = false) {
 template <int MI, int OUT>
 void launch_out(const Args& a, int wgs, hipStream_t st) {
   const dim3 grid(wgs), block(kThreads);
-  if (a.g.a_k && a.g.b_k) hipLaunchKernelGGL((gemm_bf16_kernel<MI, true, true, OUT>), grid, block, 0, st, a);
-  else if (a.g.a_k) hipLaunchKernelGGL((gemm_bf16_kernel<MI, true, false, OUT>), grid, block, 0, st, a);
-  else if constexpr (OUT != 4) hipLaunchKernelGGL((gemm_bf16_kernel<MI, false, false, OUT>), grid, block, 0, st, a);
+  if constexpr (OUT == 0 || OUT == 2 || OUT == 4) {  // (only products over rows are added up)
+    if (a.g.a_k) {
+      if (a.g.b_k) hipLaunchKernelGGL((gemm_bf16_kernel<MI, true, true, OUT>), grid, block, 0, st, a);
+      else hipLaunchKernelGGL((gemm_bf16_kernel<MI, true, false, OUT>), grid, block, 0, st, a);
+      return;
+    }
+  }
+  if constexpr (OUT != 4) hipLaunchKernelGGL((gemm_bf16_kernel<MI, false, false, OUT>), grid, block, 0, st, a);
 }
 template <int MI>
 void launch(const Args& a, int wgs, hipStream_t st) {
@@ -579,7 +584,7 @@ int gemm_bf16(const GemmBf16& g, void* workspace, hipStream_t st) {
     return ((uintptr_t)m.p & 15) || (m.row | m.panel | m.piece | m.size) % 8 || m.row >= kGemmBf16MaxLd ||
            m.panel >= kGemmBf16MaxPanel;
   };
-  MTX_CHECK_ARG(g.K > 0 && (g.a_k || (!g.b_k && !g.stats)) && (!g.a_k || g.K % 8 == 0) && !bad(g.a) && !bad(g.b) &&
+  MTX_CHECK_ARG(g.K > 0 && (g.a_k ? !g.add : !g.b_k && !g.stats) && (!g.a_k || g.K % 8 == 0) && !bad(g.a) && !bad(g.b) &&
                     g.ldc < kGemmBf16MaxLdc && g.ldadd < kGemmBf16MaxLdc,
                 "bf16 product: operand layout");
   const Args a{g, p.gx, p.gy, p.whole, p.split, p.units, p.ksteps, p.per, static_cast<float*>(workspace)};
