@@ -374,15 +374,16 @@ bool whole(const void* p, int64_t ld, int cols) {
   return cols % 8 == 0 && ld % 8 == 0 && ld < kGemmBf16MaxLd && ((uintptr_t)p & 15) == 0;
 }
 
-// Whether a block of so many rows is faster in narrow_xent, with
-// (rows, C, V)          here, fp32 and bf16   there
-// (16384, 384, 65)      95    83              63    62 us
-// (16384, 1024, 65)     181   99              104   106
-// (16384, 384, 96)      86    78              70    72
-// (16384, 1024, 96)     158   94              119   124
-// (16384, 384, 128)     84    79              99    101
-// (2048, 384, 65)       57    53              43    45
-// (300, 2048, 65)       50    50              124   133
+// Whether a block of so many rows is faster in narrow_xent.  Measured, with a bias and all
+// gradients, in us, fp32 and bf16:
+// (rows, C, V)          the general way   narrow_xent
+// (16384, 384, 65)      95    83          60    58
+// (16384, 1024, 65)     181   99          104   104
+// (16384, 384, 96)      86    78          65    72
+// (16384, 1024, 96)     158   94          117   124
+// (16384, 384, 128)     84    79          99    101
+// (2048, 384, 65)       57    53          41    43
+// (300, 2048, 65)       50    50          124   133
 bool narrow_is_faster(int dtype, int rows, int C, int V) {
   return V <= (dtype == MTX_F32 ? kNarrowV : 80) && rows >= 4LL * C;
 }
