@@ -53,6 +53,13 @@ __global__ __launch_bounds__(256) void zero_kernel(void* p, int size, int64_t sr
   }
 }
 
+// to = the (rows x cols) matrix `from`, and zeros in the rows behind it
+__global__ __launch_bounds__(256) void pad_kernel(const float* __restrict__ from, int64_t ldf, int rows, int cols,
+                                                  float* __restrict__ to, int64_t ldt, int all) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, r = e / cols, c = e - r * cols;
+  if (r < all) to[r * ldt + c] = r < rows ? from[r * ldf + c] : 0.f;
+}
+
 // ---------------------------------------------------------------------------
 // The rows' statistics and losses and, in place of the logits or beside them, their
 // gradients.
@@ -358,6 +365,7 @@ struct Plan {
   int64_t ldz, rows32;
   int rows, wgs, pieces;
   bool pack_x, pack_w, narrow;
+  bool pad;  // fp32: x and dx in 128 rows
   size_t z, dz, db, dw, x, w, gemm, bytes;  // offsets, and the whole
 };
 
@@ -404,6 +412,10 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   p.rows = (int)std::min(n, fit < 256 ? fit : fit / 256 * 256);
   p.rows32 = (p.rows + 31) / 32 * 32;
   p.narrow = near && narrow_is_faster(dtype, p.rows, C, V);
+  // Below 128 rows the fp32 products leave the matrix cores; above 64 they pay for 128 on
+  // the vector units.  With all gradients 72 rows, C = 1370, V = 37387: 553 us so, 326 as 128
+  // rows; 100, 512, 20001: 141 and 112; but 65, 128, 5003: 48 and 77.
+  p.pad = dtype == MTX_F32 && n > 64 && n < 128 && p.rows == n && C >= 128 && (int64_t)C * V >= 1 << 23;
   p.pieces = grads < 0 ? 0 : dtype == MTX_F32 ? -1 : grads == MTX_F32 ? 3 : 1;
   // (rows of panels behind the last one are set to 0 by workgroups of their own: 2 rows of
   // 27453 in three pieces 44 us by two workgroups, 14 by 32)
@@ -412,7 +424,7 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   p.z = at;  // without gradients bf16 logits are never stored: their statistics are
   // narrow: dz alone, where the logits would be, and dW's ranges
   if (p.narrow) at += p.pieces ? up((size_t)p.rows * p.ldz * 4) : 0;
-  else at += p.pieces == 0 && dtype == MTX_BF16 ? up((size_t)p.rows * (cdiv(V, 64) * 8 + 4)) : up((size_t)p.rows * p.ldz * 4);
+  else at += p.pieces == 0 && dtype == MTX_BF16 ? up((size_t)p.rows * (cdiv(V, 64) * 8 + 4)) : up((size_t)(p.pad ? 128 : p.rows) * p.ldz * 4);
   p.dz = at;
   if (p.pieces > 0 && !p.narrow) at += up((size_t)p.pieces * p.rows32 * p.ldz * 2);
   p.db = at;
@@ -424,6 +436,7 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   const int64_t c32 = (C + 31) / 32 * 32;
   p.x = at;
   if (p.pack_x) at += up((size_t)p.rows32 * c32 * 2);
+  if (p.pad) at += up((size_t)2 * 128 * C * 4);  // x, dx
   p.w = at;
   if (p.pack_w) at += up((size_t)c32 * p.ldz * 2);
   p.gemm = at;
@@ -438,10 +451,11 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
       most = std::max(most, dtype == MTX_F32 ? mtx_gemm_workspace_bytes(M, N, K, 1)
                                              : gemm_bf16_workspace_bytes(M, N, K, N == V && M == r ? 1 : p.pieces));
     };
-    bytes(r, V, C);
+    const int m = p.pad ? 128 : r;
+    bytes(m, V, C);
     if (!p.pieces) continue;
     if (dtype == MTX_F32) {
-      bytes(r, C, V);
+      bytes(m, C, V);
       // Few rows and a long V: the product cuts V into up to 64 ranges only if it finds
       // room for as many as it first asks for, before it rounds them to whole slices (1 row,
       // C = 896, V = 24763: dx 1480 us without that room, 46 with it)
@@ -535,6 +549,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   float* sum = reinterpret_cast<float*>(ws + p.dw);
   bf16_t* xp = reinterpret_cast<bf16_t*>(ws + p.x);
   bf16_t* wp = reinterpret_cast<bf16_t*>(ws + p.w);
+  float* padded = reinterpret_cast<float*>(ws + p.x);
   void* gws = ws + p.gemm;
   const size_t gbytes = workspace_bytes - p.gemm;
   const int64_t piece = p.rows32 * p.ldz;
@@ -598,8 +613,12 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
       continue;
     }
     if (dtype == MTX_F32) {
-      rc = mtx_gemm_f32(r, V, C, 1, 1.f, xf, ldx, 1, 0, static_cast<const float*>(w), swc, swv, 0, 0.f, z, p.ldz, 1, 0,
-                        bias, gws, gbytes, stream);
+      if (p.pad) {
+        hipLaunchKernelGGL(pad_kernel, dim3(cdiv(128 * C, 256)), dim3(256), 0, st, xf, ldx, r, C, padded, C, 128);
+        MTX_LAUNCHED();
+      }
+      rc = mtx_gemm_f32(p.pad ? 128 : r, V, C, 1, 1.f, p.pad ? padded : xf, p.pad ? C : ldx, 1, 0,
+                        static_cast<const float*>(w), swc, swv, 0, 0.f, z, p.ldz, 1, 0, bias, gws, gbytes, stream);
     } else {
       GemmBf16 g{};
       g.a = xm;
@@ -637,8 +656,13 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
     MTX_LAUNCHED();
     if (dx) {
       if (dtype == MTX_F32) {
-        rc = mtx_gemm_f32(r, C, V, 1, 1.f, z, p.ldz, 1, 0, static_cast<const float*>(w), swv, swc, 0, 0.f,
-                          static_cast<float*>(dx) + r0 * lddx, lddx, 1, 0, nullptr, gws, gbytes, stream);
+        float* to = p.pad ? padded + 128 * (int64_t)C : static_cast<float*>(dx) + r0 * lddx;
+        rc = mtx_gemm_f32(p.pad ? 128 : r, C, V, 1, 1.f, z, p.ldz, 1, 0, static_cast<const float*>(w), swv, swc, 0, 0.f, to,
+                          p.pad ? C : lddx, 1, 0, nullptr, gws, gbytes, stream);
+        if (!rc && p.pad) {  // (what the rows behind give is left there)
+          hipLaunchKernelGGL(pad_kernel, dim3(cdiv(r * C, 256)), dim3(256), 0, st, to, C, r, C, static_cast<float*>(dx), lddx, r);
+          MTX_LAUNCHED();
+        }
       } else {
         GemmBf16 g{};
         g.a = dm;

@@ -461,7 +461,8 @@ def test_linear_xent_small_vocabulary_hidden_entries_and_rows(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("n,C,V", [(1, 70, 5003), (2, 64, 4113), (17, 130, 9000), (64, 33, 20001), (65, 33, 20001)])
+@pytest.mark.parametrize("n,C,V", [(1, 70, 5003), (2, 64, 4113), (17, 130, 9000), (64, 33, 20001), (65, 33, 20001), (65, 128, 65537),
+                                   (72, 1031, 8201), (127, 420, 20003), (128, 130, 4999)])
 def test_linear_xent_few_rows(dev, n, C, V, dtype):
     for tied in (False, True):
         check_xent(n, C, V, dtype, tied=tied)
