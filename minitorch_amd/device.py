@@ -420,7 +420,7 @@ class DevBuf:
         if not self.is_contiguous():
             raise ValueError("fill_ of non-float arrays needs a contiguous array")
         word = np.zeros(1, np.uint64)
-        word.view(_HOST[self.dtype])[0] = value
+        word.view(_HOST[self.dtype])[0] = host_array(value, self.dtype).item()  # (bfloat16: its bits)
         L.call("mtx_fill", C.c_void_p(self.data_ptr()), self.numel(), int(word[0]), self.element_size(),
                L.stream_handle())
         return self

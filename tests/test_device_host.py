@@ -148,3 +148,20 @@ def test_dtype_name_of_an_object_that_cannot_be_hashed():
             return "somewhere.float32"
 
     assert dev.dtype_name(Odd()) == "float32"
+
+
+@pytest.mark.parametrize("dtype,value,word", [
+    ("bfloat16", 1.0, 0x3F80), ("bfloat16", -2.5, 0xC020), ("bfloat16", 1.0 + 2.0 ** -8, 0x3F80),  # ties to even
+    ("bfloat16", 0, 0), ("bfloat16", float("-inf"), 0xFF80), ("int32", -3, 0xFFFFFFFD), ("int64", 1 << 40, 1 << 40),
+    ("uint8", 200, 200),
+])
+def test_fill_writes_the_dtype_s_bits(monkeypatch, dtype, value, word):
+    buf = dev.DevBuf.__new__(dev.DevBuf)
+    seen = []
+    monkeypatch.setattr(dev.L, "call", lambda name, *args: seen.append((name, args)))
+    monkeypatch.setattr(dev.L, "stream_handle", lambda: None)
+    for name, result in (("is_contiguous", True), ("data_ptr", 16), ("numel", 5), ("element_size", 1)):
+        monkeypatch.setattr(dev.DevBuf, name, lambda self, r=result: r)
+    buf.dtype = dtype
+    buf.fill_(value)
+    assert seen[0][0] == "mtx_fill" and seen[0][1][2] == word
