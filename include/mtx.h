@@ -259,7 +259,7 @@ int mtx_dropout_keep_philox(uint8_t* keep, int64_t rows, int cols, int64_t ld, f
  * values.
  */
 int mtx_dropout(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y, int64_t ldy,
-                int64_t rows, int cols, float p, float scale, uint64_t seed, uint64_t offset, uint32_t subsequence,
+                int64_t rows, int64_t cols, float p, float scale, uint64_t seed, uint64_t offset, uint32_t subsequence,
                 const uint64_t* base, void* stream);
 
 /*

@@ -70,8 +70,7 @@ __global__ __launch_bounds__(256) void keep_philox_kernel(uint8_t* __restrict__ 
 struct DropArgs {
   const void *x, *res;  // res: nullptr for none
   void* y;
-  int64_t ldx, ldr, ldy, n;  // n: values
-  int cols;
+  int64_t ldx, ldr, ldy, n, cols;  // n: values
   uint32_t below;  // kept: words above it
   float scale;
   uint32_t k0, k1, sub;
@@ -99,8 +98,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const DropArgs a) {
   if (e0 >= a.n) return;
   const U4 r = draw(a, a.offset + (a.base ? *a.base : 0), t);
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-  int64_t row = e0 / a.cols;
-  int col = (int)(e0 - row * a.cols);
+  int64_t row = e0 / a.cols, col = e0 - row * a.cols;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (e0 + i < a.n) {
@@ -177,10 +175,11 @@ void dropout(DropArgs a, int64_t rows, hipStream_t st) {
 using namespace mtx;
 
 extern "C" int mtx_dropout(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y,
-                           int64_t ldy, int64_t rows, int cols, float p, float scale, uint64_t seed, uint64_t offset,
-                           uint32_t subsequence, const uint64_t* base, void* stream) {
+                           int64_t ldy, int64_t rows, int64_t cols, float p, float scale, uint64_t seed,
+                           uint64_t offset, uint32_t subsequence, const uint64_t* base, void* stream) {
   if (dtype != MTX_F32 && dtype != MTX_BF16) return fail(MTX_ERR_DTYPE, "dropout: unsupported dtype %d", dtype);
-  MTX_CHECK_SHAPE(rows >= 0 && cols >= 1, "dropout: rows=%lld, cols=%d: need rows >= 0, cols >= 1", (long long)rows, cols);
+  MTX_CHECK_SHAPE(rows >= 0 && cols >= 1, "dropout: rows=%lld, cols=%lld: need rows >= 0, cols >= 1", (long long)rows,
+                  (long long)cols);
   MTX_CHECK_ARG(p >= 0.f && p < 1.f, "dropout: p=%g must be in [0, 1)", (double)p);
   MTX_CHECK_ARG(ldx >= cols && ldy >= cols && (!residual || ldr >= cols), "dropout: rows overlap");
   if (rows == 0) return MTX_OK;
@@ -189,7 +188,7 @@ extern "C" int mtx_dropout(int dtype, const void* x, int64_t ldx, const void* re
   MTX_CHECK_SHAPE(rows <= ((int64_t)1 << 33) / cols, "dropout: more than 2^33 values");
   // u > p with u = (w >> 8) 2^-24: w >= 256 (floor(2^24 p) + 1)
   const uint32_t below = (uint32_t)((((uint64_t)((double)p * 0x1p24)) + 1) * 256 - 1);
-  const DropArgs a{x, residual, y, ldx, ldr, ldy, rows * (int64_t)cols, cols, below, scale, (uint32_t)seed,
+  const DropArgs a{x, residual, y, ldx, ldr, ldy, rows * cols, cols, below, scale, (uint32_t)seed,
                    (uint32_t)(seed >> 32), subsequence, offset, base};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == MTX_F32) residual ? dropout<float, true>(a, rows, st) : dropout<float, false>(a, rows, st);

@@ -1,0 +1,31 @@
+"""What the operators of training with a large vocabulary take and refuse at the ends
+of their ranges.  No GPU: every check runs before any HIP call."""
+import pytest
+from test_vocab_refusals import Fake, _kernels, dropout, p
+
+from minitorch_amd import _lib as L
+
+
+@pytest.mark.parametrize("over,code,frag", [
+    (dict(rows=1, cols=(1 << 32) + 8), L.MTX_ERR_ARG, "overlap"),  # rows of 8 values in between
+    (dict(rows=1, cols=(1 << 33) + 8, ldx=1 << 34, ldy=1 << 34), L.MTX_ERR_SHAPE, "2^33"),
+    (dict(rows=3, cols=(1 << 32) - 8, ldx=1 << 32, ldy=1 << 32), L.MTX_ERR_SHAPE, "2^33"),
+    # up to there the next check is reached
+    (dict(rows=1, cols=1 << 33, ldx=1 << 33, ldy=1 << 33, x=None), L.MTX_ERR_ARG, "null"),
+    (dict(rows=1, cols=1 << 31, ldx=1 << 31, ldy=1 << 31, base=p(12)), L.MTX_ERR_ARG, "aligned"),
+])
+def test_dropout_of_rows_longer_than_32_bits(over, code, frag):
+    rc, msg = dropout(over)
+    assert rc == code and frag in msg, (rc, msg)
+
+
+def test_dropout_wrapper_passes_all_columns(monkeypatch):
+    K = _kernels(monkeypatch)
+    seen = []
+    monkeypatch.setattr(Fake, "data_ptr", lambda self: 16)
+    monkeypatch.setattr(L, "call", lambda name, *args: seen.append((name, args)))
+    n = (1 << 32) + 8
+    K.dropout(Fake((1, n)), 0.5, 1, out=Fake((1, n)))
+    name, args = seen[0]
+    types = L.SIGNATURES[name][1]
+    assert name == "mtx_dropout" and [t(a).value for t, a in zip(types, args)][7:9] == [1, n]
