@@ -1318,6 +1318,13 @@ def _matrix(name, spec, shape=None):
     return (rows, cols), ld, _dt(dtype)
 
 
+def _int32(**sizes):
+    """Sizes that the library takes as 32-bit numbers, to which a call would wrap them."""
+    for name, size in sizes.items():
+        if size >= 1 << 31:
+            raise ValueError(f"{name} must be below 2^31 (got {size})")
+
+
 @functools.lru_cache(maxsize=512)
 def _lookup_plan(weight, ids, out):
     (V, C), ldw, dtype = _matrix("weight", weight)
@@ -1326,6 +1333,7 @@ def _lookup_plan(weight, ids, out):
     _, ldo, odt = _matrix("out", out, (n, C))
     if not V or not C:
         raise ValueError(f"weight of shape {(V, C)} has no rows")
+    _int32(C=C)
     dev.device()
     return (_code(dtype), _code(odt)), (ldw, V), (n, C), ldo
 
@@ -1355,6 +1363,7 @@ def _grad_plan(ids, grad, dweight):
         raise ValueError("dweight must be fp32")
     if not V or not C:
         raise ValueError(f"dweight of shape {(V, C)} has no rows")
+    _int32(C=C)
     n = ids[0][0] if len(ids[0]) == 1 else -1
     _vector("ids", ids, n, "int64")
     _, ldg, dtype = _matrix("grad", grad, (n, C))
@@ -1449,6 +1458,7 @@ def _xent_plan(x, w, labels, bias, loss, row_loss, lse, dx, dw, db, logits_bytes
     V = w[0][1]
     if w[0][0] != C or wdt != dtype or not C or not V:
         raise ValueError(f"w must be ({C}, V) {dtype} like x, got {tuple(w[0])} {wdt}")
+    _int32(C=C, V=V)
     _vector("labels", labels, n, "int64")
     for name, t, size in (("bias", bias, V), ("loss", loss, 1), ("row_loss", row_loss, n), ("lse", lse, n),
                           ("db", db, V)):

@@ -29,3 +29,21 @@ def test_dropout_wrapper_passes_all_columns(monkeypatch):
     name, args = seen[0]
     types = L.SIGNATURES[name][1]
     assert name == "mtx_dropout" and [t(a).value for t, a in zip(types, args)][7:9] == [1, n]
+
+
+FAR = (1 << 32) + 8  # wrapped to 32 bits: 8
+
+
+@pytest.mark.parametrize("call,frag", [
+    (lambda K: K.embedding_lookup(Fake((3, FAR)), Fake((4,), "int64"), out=Fake((4, FAR))), "C must"),
+    (lambda K: K.embedding_grad(Fake((4,), "int64"), Fake((4, FAR)), Fake((3, FAR))), "C must"),
+    (lambda K: K.linear_xent(Fake((4, FAR)), Fake((FAR, 10)), Fake((4,), "int64")), "C must"),
+    (lambda K: K.linear_xent(Fake((4, 8)), Fake((8, FAR)), Fake((4,), "int64")), "V must"),
+    (lambda K: K.linear_xent(Fake((4, 8)), Fake((8, 1 << 31)), Fake((4,), "int64")), "V must"),
+])
+def test_sizes_that_the_library_takes_as_32_bits(monkeypatch, call, frag):
+    K = _kernels(monkeypatch)
+    monkeypatch.setattr(L, "call", lambda *args: pytest.fail("wrapped and passed on"))
+    monkeypatch.setattr(Fake, "data_ptr", lambda self: 16)
+    with pytest.raises(ValueError, match=frag):
+        call(K)
