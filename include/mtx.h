@@ -46,6 +46,9 @@ enum mtx_status {
 
 enum mtx_dtype { MTX_F32 = 0, MTX_BF16 = 1 };
 
+/* Added to MTX_BF16 as mtx_linear_xent's grad_dtype. */
+enum mtx_grad_flag { MTX_GRAD_ONE_PIECE = 256 };
+
 /* Thread-local description of the last failure on this thread. */
 const char* mtx_last_error(void);
 
@@ -867,8 +870,10 @@ int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void* logits, i
  * and NaN in x or w give NaN (fp32: in every logit that they meet).
  * The rows are worked through in blocks whose logits (fp32) fill at most logits_bytes
  * (one row at least, 2^18 at most); fewer, larger blocks are faster.  bf16 gradients
- * are products of the logits' gradient rounded to bf16 (small vocabularies: of all its
- * bits), fp32 ones of all its 24 bits; either way sums are fp32, rounded once.  No
+ * are products of the logits' gradient to 2^-18 of each entry, fp32 ones of all its 24
+ * bits; either way sums are fp32, rounded once.  With grad_dtype MTX_BF16 |
+ * MTX_GRAD_ONE_PIECE the logits' gradient is rounded to bf16 first (2^-9 of each entry;
+ * small vocabularies: not at all), which saves the products the second piece.  No
  * output may overlap an input or another output.
  * n < 2^31, C <= 2^20, V <= 2^27; bf16: V < 2^22, and rows of dx and dw less than 2^26
  * values apart.  Deterministic.

@@ -20,6 +20,7 @@ LIB_PATH = _PKG / "libmtx_hip.so"
 
 MTX_OK, MTX_ERR_ARG, MTX_ERR_SHAPE, MTX_ERR_DTYPE, MTX_ERR_HIP = range(5)
 MTX_F32, MTX_BF16 = 0, 1
+MTX_GRAD_ONE_PIECE = 256
 MTX_GEMM_FP32, MTX_GEMM_BF16X3 = 0, 1
 ATTN_SCRATCH_BYTES = 8 << 20  # MTX_ATTN_SCRATCH_BYTES (include/mtx.h)
 ATTN_BWD_DELTA, ATTN_BWD_DKDV, ATTN_BWD_DQ, ATTN_BWD_ALL = 1, 2, 4, 7

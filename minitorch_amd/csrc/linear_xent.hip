@@ -64,10 +64,16 @@ __global__ __launch_bounds__(256) void pad_kernel(const float* __restrict__ from
 // The rows' statistics and losses and, in place of the logits or beside them, their
 // gradients.
 //
-// MODE: 0 no gradient; 1 dz = (p - onehot) / labels in place of z, fp32; 2 and 3 p -
-// onehot as one or three bf16 pieces (of 8 bits each: three hold all 24), in panels of
-// 32 columns, the factor 1 / labels left to the products: rounded to bf16, it would be
+// MODE: 0 no gradient; 1 dz = (p - onehot) / labels in place of z, fp32; 2, 3 and 4 p -
+// onehot as one, two or three bf16 pieces (of 8 bits each: three hold all 24), in panels
+// of 32 columns, the factor 1 / labels left to the products: rounded to bf16, it would be
 // off by the same amount in every row.
+//
+// bf16 gradients take two pieces: what these lack, 2^-18 of a term, is less than the fp32
+// sums lose, so that the rounding of the result is all that counts.  One piece costs 2^-9
+// more in every term: of 8192 x 1024 and a vocabulary of 50021, 1.86e-3 of the gradients'
+// norm in place of 1.66e-3; it is what a caller asks for who wants the time (kOnePiece),
+// 3.1 ms in place of 5.1.
 // ---------------------------------------------------------------------------
 struct RowArgs {
   float* z;
@@ -97,6 +103,10 @@ __device__ __forceinline__ void put_grad(const RowArgs& a, int64_t r, int v0, in
     uint2 h, m, l;
     if constexpr (MODE == 2) {
       *reinterpret_cast<uint2*>(p + at) = make_uint2(pk_bf16(d[0], d[1]), pk_bf16(d[2], d[3]));
+    } else if constexpr (MODE == 3) {
+      split2(d, h, m);
+      *reinterpret_cast<uint2*>(p + at) = h;
+      *reinterpret_cast<uint2*>(p + 2 * a.piece + at) = m;
     } else {
       split3(d, h, m, l);
       *reinterpret_cast<uint2*>(p + at) = h;
@@ -361,6 +371,9 @@ __global__ __launch_bounds__(1024) void bias_kernel(const float* __restrict__ pa
   db[v] = s * *inv;
 }
 
+// grad_dtype: bf16, from the logits' gradient in one piece
+constexpr int kOnePiece = MTX_BF16 | MTX_GRAD_ONE_PIECE;
+
 struct Plan {
   int64_t ldz, rows32;
   int rows, wgs, pieces;
@@ -416,7 +429,7 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   // the vector units.  With all gradients 72 rows, C = 1370, V = 37387: 553 us so, 326 as 128
   // rows; 100, 512, 20001: 141 and 112; but 65, 128, 5003: 48 and 77.
   p.pad = dtype == MTX_F32 && n > 64 && n < 128 && p.rows == n && C >= 128 && (int64_t)C * V >= 1 << 23;
-  p.pieces = grads < 0 ? 0 : dtype == MTX_F32 ? -1 : grads == MTX_F32 ? 3 : 1;
+  p.pieces = grads < 0 ? 0 : dtype == MTX_F32 ? -1 : grads == MTX_F32 ? 3 : grads == kOnePiece ? 1 : 2;
   // (rows of panels behind the last one are set to 0 by workgroups of their own: 2 rows of
   // 27453 in three pieces 44 us by two workgroups, 14 by 32)
   p.wgs = row_wgs(p.pieces > 0 ? (int)p.rows32 : p.rows, V);
@@ -430,7 +443,7 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   p.db = at;
   if (p.pieces && bias && !p.narrow) at += up((size_t)p.wgs * p.ldz * 4);
   p.dw = at;  // a bf16 gradient of the weights is summed over blocks of rows in fp32
-  if (p.pieces == 1 && p.rows < n) at += up((size_t)C * V * 4);
+  if ((p.pieces == 1 || p.pieces == 2) && p.rows < n) at += up((size_t)C * V * 4);
   p.pack_x = dtype == MTX_BF16 && !p.narrow && pack_x;
   p.pack_w = dtype == MTX_BF16 && !p.narrow && pack_w;
   const int64_t c32 = (C + 31) / 32 * 32;
@@ -509,8 +522,9 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
                                void* stream) {
   if (!known(dtype)) return fail(MTX_ERR_DTYPE, "linear_xent: unsupported dtype %d", dtype);
   const bool grad = dx || dw || db;
-  if (grad && (!known(grad_dtype) || (dtype == MTX_F32 && grad_dtype != MTX_F32)))
+  if (grad && ((!known(grad_dtype) && grad_dtype != kOnePiece) || (dtype == MTX_F32 && grad_dtype != MTX_F32)))
     return fail(MTX_ERR_DTYPE, "linear_xent: gradients must be fp32, or bf16 like the inputs (got %d)", grad_dtype);
+  const bool half = grad && grad_dtype != MTX_F32;  // bf16 gradients
   MTX_CHECK_SHAPE(n >= 0 && n < (1LL << 31) && C >= 1 && C <= (1 << 20) && V >= 1 && V <= (1 << 27),
                   "linear_xent: need 0 <= n < 2^31, 1 <= C <= 2^20, 1 <= V <= 2^27");
   MTX_CHECK_ARG(loss && w && (n == 0 || (x && labels && row_loss && lse)), "linear_xent: null pointer");
@@ -562,7 +576,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   if (n == 0) {
     if (dw) {
       hipLaunchKernelGGL(zero_kernel, dim3((unsigned)std::min<int64_t>(((int64_t)C * V + 255) / 256, 16384)), dim3(256), 0,
-                         st, dw, grad_dtype == MTX_F32 ? 4 : 2, sdc, sdv, C, V);
+                         st, dw, half ? 2 : 4, sdc, sdv, C, V);
       MTX_LAUNCHED();
     }
   }
@@ -588,7 +602,6 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
     const Bf16Matrix dm = bf16_panels(dz, r32, p.ldz / 32, piece);
     if (p.narrow) {
       const void* xr = dtype == MTX_F32 ? static_cast<const void*>(xf) : xb;
-      const bool half = grad_dtype == MTX_BF16;
       if ((rc = narrow_xent({dtype, xr, ldx, w, swc, swv, bias, labels + r0, inv, row_loss + r0, lse + r0, r, C, V,
                              dx ? static_cast<char*>(dx) + r0 * lddx * (half ? 2 : 4) : nullptr, lddx, half,
                              dw || db ? z : nullptr, p.ldz}, st)))
@@ -652,7 +665,8 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
     if (p.pieces == 0) rows<0, false>(a, wgs, st);
     else if (p.pieces < 0) part ? rows<1, true>(a, wgs, st) : rows<1, false>(a, wgs, st);
     else if (p.pieces == 1) part ? rows<2, true>(a, wgs, st) : rows<2, false>(a, wgs, st);
-    else part ? rows<3, true>(a, wgs, st) : rows<3, false>(a, wgs, st);
+    else if (p.pieces == 2) part ? rows<3, true>(a, wgs, st) : rows<3, false>(a, wgs, st);
+    else part ? rows<4, true>(a, wgs, st) : rows<4, false>(a, wgs, st);
     MTX_LAUNCHED();
     if (dx) {
       if (dtype == MTX_F32) {
@@ -670,9 +684,9 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
         g.b = wm;
         g.b_k = wv;
         g.pieces = p.pieces;
-        g.c = static_cast<char*>(dx) + r0 * lddx * (grad_dtype == MTX_F32 ? 4 : 2);
+        g.c = static_cast<char*>(dx) + r0 * lddx * (half ? 2 : 4);
         g.ldc = lddx;
-        g.c_bf16 = grad_dtype == MTX_BF16;
+        g.c_bf16 = half;
         g.scale = inv;
         g.M = r;
         g.N = C;
@@ -707,13 +721,12 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
         g.N = N;
         g.K = r;
         // blocks of rows are added up in fp32, the sum is rounded once
-        const bool narrow = grad_dtype == MTX_BF16;
-        g.c_bf16 = narrow && last;
-        g.c = narrow && !last ? static_cast<void*>(sum) : dw;
-        g.ldc = narrow && !last ? N : ld;
+        g.c_bf16 = half && last;
+        g.c = half && !last ? static_cast<void*>(sum) : dw;
+        g.ldc = half && !last ? N : ld;
         if (!first) {
-          g.add = narrow ? sum : static_cast<const float*>(dw);
-          g.ldadd = narrow ? N : ld;
+          g.add = half ? sum : static_cast<const float*>(dw);
+          g.ldadd = half ? N : ld;
         }
         rc = gemm_bf16(g, gws, st);
       }

@@ -197,6 +197,14 @@ __device__ __forceinline__ uint32_t pk_bf16(float x, float y) {
   return u;
 }
 
+// x = h + m (+ 2^-18 |x|), for four values, each plane as four bf16
+__device__ __forceinline__ void split2(f32x4 v, uint2& h, uint2& m) {
+  h.x = pk_bf16(v[0], v[1]);
+  h.y = pk_bf16(v[2], v[3]);
+  m.x = pk_bf16(v[0] - __uint_as_float(h.x << 16), v[1] - __uint_as_float(h.x & 0xffff0000u));
+  m.y = pk_bf16(v[2] - __uint_as_float(h.y << 16), v[3] - __uint_as_float(h.y & 0xffff0000u));
+}
+
 // x = h + m + l (+ 2^-24 |x|), for four values, each plane as four bf16
 __device__ __forceinline__ void split3(f32x4 v, uint2& h, uint2& m, uint2& l) {
   h.x = pk_bf16(v[0], v[1]);

@@ -1,7 +1,7 @@
 """What the operators of training with a large vocabulary take and refuse at the ends
 of their ranges.  No GPU: every check runs before any HIP call."""
 import pytest
-from test_vocab_refusals import Fake, _kernels, dropout, p
+from test_vocab_refusals import Fake, _kernels, dropout, p, xent
 
 from minitorch_amd import _lib as L
 
@@ -47,3 +47,24 @@ def test_sizes_that_the_library_takes_as_32_bits(monkeypatch, call, frag):
     monkeypatch.setattr(Fake, "data_ptr", lambda self: 16)
     with pytest.raises(ValueError, match=frag):
         call(K)
+
+
+@pytest.mark.parametrize("over", [dict(gdt=256), dict(dtype=0, gdt=257), dict(gdt=258), dict(gdt=513)])
+def test_one_piece_is_for_bf16_gradients(over):
+    rc, msg = xent(over)
+    assert rc == L.MTX_ERR_DTYPE and "gradients" in msg
+
+
+def test_one_piece_wrapper_refuses(monkeypatch):
+    K = _kernels(monkeypatch)
+    args = Fake((4, 8), "bfloat16"), Fake((8, 10), "bfloat16"), Fake((4,), "int64")
+    for grads in ({}, dict(dx=Fake((4, 8))), dict(bias=Fake((10,)), db=Fake((10,)))):
+        with pytest.raises(ValueError, match="one_piece"):
+            K.linear_xent(*args, one_piece=True, **grads)
+
+
+def test_one_piece_takes_less_workspace():
+    f = L.lib().mtx_linear_xent_workspace_bytes
+    one, two, three = (f(1, g, 4096, 64, 1000, 1, 1 << 30) for g in (257, 1, 0))
+    # 4096 x 1024 values of two bytes a piece
+    assert two - one >= 1 << 23 and three - two >= 1 << 23

@@ -3,7 +3,9 @@ against the float64 forms (oracle.vocab)."""
 import numpy as np
 import pytest
 from devarrays import T as dev_array, empty, full
-from test_vocab_gpu import host
+from test_vocab_gpu import B, host, inside, rounded, tokens
+
+from oracle import vocab as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +42,66 @@ def test_dropout_function_of_more_than_32_bits_of_values(dev):
         part = host(K.dropout(full((1, 64), 1.0), 0.5, 9, e // 4, subsequence=1))[0]
         assert np.array_equal(host(y.data.t[e:e + 64]), part)
         assert np.array_equal(host(x.grad.t[e:e + 64]), 3 * part)
+
+
+# ---------------------------------------------------------------------------
+# projection and cross-entropy: the bits of bf16 gradients
+# ---------------------------------------------------------------------------
+
+def _bf16_case(n, C, V, seed=0):
+    rng = np.random.default_rng(seed + n + C + V)
+    x = rounded(rng.standard_normal((n, C)), "bfloat16")
+    w = rounded(rng.standard_normal((C, V)) * 2 / np.sqrt(C), "bfloat16")
+    return x, w, tokens(rng, n, V)
+
+
+def _bf16_bounds(x, w, r):
+    """xent_bounds of bf16 outputs whose logits' gradient is off by 2^-18 of each entry
+    in place of 2^-8: what fp32 gradients of the same call are off by, with 2^-18 of
+    the entries, and the rounding of the result, 2^-8."""
+    from test_vocab_gpu import xent_bounds
+
+    dx, dw = xent_bounds(x, w, None, r, "bfloat16", "float32")[3:5]
+    d = np.abs(r["dz"])
+    dx, dw = dx + 2.0 ** -18 * (d @ np.abs(w).T), dw + 2.0 ** -18 * (np.abs(x).T @ d)
+    return dx + B * (np.abs(r["dx"]) + dx), dw + B * (np.abs(r["dw"]) + dw)
+
+
+# a wave a row, a workgroup a row, the longest rows; one block of rows and several; the
+# small vocabularies' way
+@pytest.mark.parametrize("n,C,V,more", [(60, 64, 40, {}), (130, 96, 700, {}), (300, 40, 5003, {}), (20, 24, 70001, {}),
+                                        (300, 64, 136, dict(logits_bytes=100 * 136 * 4)), (600, 64, 65, {})])
+def test_bf16_gradients_are_off_by_their_own_rounding(dev, n, C, V, more):
+    from minitorch_amd import kernels as K
+
+    x, w, labels = _bf16_case(n, C, V)
+    r = ref.linear_xent(x, w, labels)
+    bx, bw = _bf16_bounds(x, w, r)
+    for tied in (False, True):
+        args = dev_array(x, "bfloat16"), dev_array(w.T, "bfloat16").t() if tied else dev_array(w, "bfloat16")
+        dx, dw = empty((n, C), "bfloat16"), empty((V, C) if tied else (C, V), "bfloat16")
+        K.linear_xent(*args, dev_array(labels, "int64"), dx=dx, dw=dw.t() if tied else dw, **more)
+        inside(host(dx), r["dx"], bx)
+        inside(host(dw).T if tied else host(dw), r["dw"], bw)
+
+
+def test_bf16_gradients_of_one_piece(dev):
+    """On request from the logits' gradient in bf16: other values, inside the bounds that
+    grant its rounding too."""
+    from minitorch_amd import kernels as K
+    from test_vocab_gpu import xent_bounds
+
+    n, C, V = 130, 96, 700
+    x, w, labels = _bf16_case(n, C, V)
+    r = ref.linear_xent(x, w, labels)
+    bounds = xent_bounds(x, w, None, r, "bfloat16", "bfloat16")[3:5]
+    got = {}
+    for one in (False, True):
+        for more in ({}, dict(logits_bytes=64 * 704 * 4)):
+            dx, dw = empty((n, C), "bfloat16"), empty((C, V), "bfloat16")
+            K.linear_xent(dev_array(x, "bfloat16"), dev_array(w, "bfloat16"), dev_array(labels, "int64"), dx=dx, dw=dw,
+                          one_piece=one, **more)
+            inside(host(dx), r["dx"], bounds[0])
+            inside(host(dw), r["dw"], bounds[1])
+        got[one] = host(dx)
+    assert not np.array_equal(got[False], got[True])
