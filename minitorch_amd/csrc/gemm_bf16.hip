@@ -368,11 +368,12 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(const Args a) {
             pick = own == 16 * y + e ? acc[x][y][e] : pick;
           }
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float from = top == -INFINITY ? 0.f : top * kLog2e;
+        // (the difference first: top log2(e) may be infinite for a finite top)
+        const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int y = 0; y < NI; ++y)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[x][y][e], kLog2e, -from));
+          for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f((acc[x][y][e] - from) * kLog2e);
         sum += __shfl_xor(sum, 32, 64);
         if (m < g.M && nw < g.N && lh == 0) g.stats[(int64_t)(nw / 64) * g.M + m] = make_float2(top, sum);
         if (own >= 0) g.chosen[m] = pick;

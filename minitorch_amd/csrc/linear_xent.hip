@@ -116,11 +116,12 @@ __device__ __forceinline__ void put_grad(const RowArgs& a, int64_t r, int v0, in
   }
 }
 
-// The rows' (m, s): maximum and sum of exp(z - m), to the label's loss
+// The rows' (m, s): maximum and sum of exp(z - m), to the label's loss, as the distance
+// from the maximum and log s: their sum lse may be too large to hold log s
 __device__ __forceinline__ void put_loss(const RowArgs& a, int64_t r, float m, float s, bool some, float zy) {
-  const float l = m + logf(s);
-  a.lse[r] = l;
-  a.row_loss[r] = !some ? 0.f : zy == -INFINITY && l == -INFINITY ? INFINITY : l - zy;
+  const float l = logf(s);
+  a.lse[r] = m + l;
+  a.row_loss[r] = !some ? 0.f : zy == -INFINITY && m == -INFINITY ? INFINITY : (m - zy) + l;
 }
 
 // T threads a row, NV vectors of four columns each, all in registers: a row is read
@@ -179,13 +180,15 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row_kernel(const RowArgs a)
     m = wave_max(m);
     if constexpr (kNext)
       if (r + step < a.rows) request(r + step, next);
-    const float from = m == -INFINITY ? 0.f : m * kLog2e;
+    // (the difference first: m log2(e) is infinite for a finite m beyond 2.36e38, as where a
+    // row's entries all hold the type's lowest value)
+    const float from = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        z[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][j], kLog2e, -from));
+        z[i][j] = __builtin_amdgcn_exp2f((z[i][j] - from) * kLog2e);
         s += z[i][j];
       }
     s = wave_sum(s);

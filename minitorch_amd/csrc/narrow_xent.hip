@@ -251,11 +251,12 @@ __global__ __launch_bounds__(256, 2) void narrow_kernel(const NarrowXent a) {
   });
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float from = m[i] == -INFINITY ? 0.f : m[i] * kLog2e;
+    // (the difference first: m log2(e) may be infinite for a finite m)
+    const float from = m[i] == -INFINITY ? 0.f : m[i];
     sum[i] = 0.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      sum[i] += acc[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[t][i], kLog2e, -from));
+      sum[i] += acc[t][i] = __builtin_amdgcn_exp2f((acc[t][i] - from) * kLog2e);
   }
   row16([&](auto dpp) {
 #pragma unroll
@@ -265,9 +266,9 @@ __global__ __launch_bounds__(256, 2) void narrow_kernel(const NarrowXent a) {
   for (int i = 0; i < 4; ++i) {
     const int row = row0 + 4 * g + i;
     if (c != i || row >= a.rows) continue;  // (a lane a row)
-    const float l = m[i] + logf(sum[i]);
-    a.lse[row] = l;
-    a.row_loss[row] = y[i] < 0 ? 0.f : zy[i] == -INFINITY && l == -INFINITY ? INFINITY : l - zy[i];
+    const float l = logf(sum[i]);
+    a.lse[row] = m[i] + l;
+    a.row_loss[row] = y[i] < 0 ? 0.f : zy[i] == -INFINITY && m[i] == -INFINITY ? INFINITY : (m[i] - zy[i]) + l;
   }
   if (!a.dx && !a.dz) return;
   const float inv = *a.inv;

@@ -105,3 +105,53 @@ def test_bf16_gradients_of_one_piece(dev):
             inside(host(dw), r["dw"], bounds[1])
         got[one] = host(dx)
     assert not np.array_equal(got[False], got[True])
+
+
+# ---------------------------------------------------------------------------
+# projection and cross-entropy: logits as large as fp32 holds
+# ---------------------------------------------------------------------------
+
+# the small vocabularies' way, a wave a row, a workgroup a row, the longest rows
+ROW_WAYS = [(300, 40, 65), (40, 24, 200), (20, 24, 3000), (20, 16, 10000), (9, 16, 30000), (9, 16, 50000), (9, 16, 70001)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("kind", ["lowest", "highest", "both"])
+@pytest.mark.parametrize("n,C,V", ROW_WAYS)
+def test_linear_xent_of_logits_at_the_ends_of_fp32(dev, n, C, V, kind, dtype):
+    """A mask of the type's lowest value that leaves nothing, logits near the highest,
+    and both in one row.  Beside a bias of 3e38 the products vanish (its steps are 2e31):
+    the k entries that hold the maximum have probability 1 / k, the others 0, exactly but
+    for the rounding of 1 / k and of the steps to dz."""
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(n + V)
+    x, w = rounded(rng.standard_normal((n, C)), dtype), rounded(rng.standard_normal((C, V)), dtype)
+    low = float(np.finfo(np.float32).min)
+    b = {"lowest": np.full(V, low), "highest": np.full(V, 3e38),
+         "both": np.where(np.arange(V) % 3 == 1, low, 3e38)}[kind].astype(np.float32)
+    labels = tokens(rng, n, V)
+    some = (labels >= 0) & (labels < V)
+    labels = np.where(some, labels // 3 * 3, labels)  # of the entries that are seen
+    top = b.max()
+    k = int((b == top).sum())
+    dx, dw, db = empty((n, C)), empty((C, V)), empty((V,))
+    args = [dev_array(x, dtype), dev_array(w, dtype), dev_array(labels, "int64")]
+    U = 2.0 ** -24
+    for grads in (dict(), dict(dx=dx, dw=dw, db=db)):
+        loss, row, lse = K.linear_xent(*args, bias=dev_array(b), **grads)
+        inside(host(lse), float(top) + np.log(k), 2 * U * abs(float(top)))
+        # log k: the log's rounding and that of a sum of k ones, which is exact
+        inside(host(row), np.where(some, np.log(k), 0.0), 4 * U * np.log(k))
+        inside(host(loss), np.array([np.log(k)]), (n + 8) * U * np.log(k))
+    count = some.sum()
+    dz = np.where(b == top, 1.0 / k, 0.0) * np.ones((n, 1))
+    dz[np.nonzero(some)[0], labels[some]] -= 1.0
+    dz[~some] = 0.0
+    dz /= count
+    cut = 2.0 ** -22 if dtype == "float32" else 0.0
+    size, xa, wa = np.abs(dz), np.abs(x.astype(np.float64)), np.abs(w.astype(np.float64))
+    ed = 6 * U * (size + 1.0 / k / count)  # beside 1, 1 / k is off by a step of 1
+    inside(host(dx), dz @ w.astype(np.float64).T, ed @ wa.T + ((V + 4) * U + cut) * (size @ wa.T))
+    inside(host(dw), x.astype(np.float64).T @ dz, xa.T @ ed + ((n + 4) * U + cut) * (xa.T @ size))
+    inside(host(db), dz.sum(0), ed.sum(0) + (n + 4) * U * size.sum(0))
