@@ -757,14 +757,31 @@ Plan plan(int dtype, int64_t n, int64_t V, int C) {
   p.small = n <= 1024 || (n <= kSmallTokens && n * C * size <= (1 << 20));
   if (p.small) return p;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
-  // Tables of which 64 columns fit in 64 KB of LDS, under tokens enough for 64 chunks of
-  // half the table or more
+  // Small tables (64 columns of V + 1 rows in 64 KB of LDS, at most kTableValues values)
+  // under tokens enough for 64 chunks of half the table or more: a chunk has 64 or 128 tokens,
+  // and more where the workgroups would be more than the chip holds at once, whose tables
+  // would only be written and read again.  In us, here and sorted:
+  //     V, C        tokens    fp32            bf16
+  //     65, 384     32768     24.8   36.3     24.5   31.9
+  //                 131072    64.6   111      62.3   94.7
+  //                 1048576   388    884      372    742
+  //     255, 128    131072    51.4   82.7     50.5   78.5
+  //     128, 256    131072    55.6   92.6     50.5   86.5
+  //     200, 200    131072    82     92       81     86
+  //     255, 160    131072    111    86       110    83
+  //     128, 1024   131072    220    195      220    129
+  // (131072 tokens of 384, V = 65, took 109 with 64 a chunk, and a workspace of 204 MB
+  // where 34 do now.)  2^22 tokens at most: a column's sum of a chunk is one chain.
+  constexpr int64_t kTableValues = 36864;
   p.chunk = V <= 128 ? 64 : 128;
-  p.table = V < 256 && n / p.chunk >= 64 && n <= ((int64_t)1 << 22) && V * C <= (1 << 22);
+  p.table = V < 256 && n / p.chunk >= 64 && n <= ((int64_t)1 << 22) && V * C <= kTableValues;
   if (p.table) {
     p.width = (int)std::min<int64_t>(512, (65536 / 4 / (V + 1)) / 64 * 64);
     const int slices = cdiv(C, p.width);
     p.width = (cdiv(C, slices) + 63) / 64 * 64;
+    // (256 compute units of 160 KB of LDS)
+    const int64_t held = 256 * std::min<int64_t>(8, 163840 / ((V + 1) * p.width * 4));
+    p.chunk = (int)std::max<int64_t>(p.chunk, (n * slices / held + 63) / 64 * 64);
     p.chunks = (int)((n + p.chunk - 1) / p.chunk);
     p.bytes = up((size_t)p.chunks * V * C * 4);
     return p;

@@ -68,3 +68,16 @@ def test_one_piece_takes_less_workspace():
     one, two, three = (f(1, g, 4096, 64, 1000, 1, 1 << 30) for g in (257, 1, 0))
     # 4096 x 1024 values of two bytes a piece
     assert two - one >= 1 << 23 and three - two >= 1 << 23
+
+
+@pytest.mark.parametrize("V,C", [(10, 384), (65, 384), (128, 256), (255, 128), (255, 256), (128, 1024), (255, 4096)])
+def test_small_tables_workspace_does_not_grow_with_the_tokens(V, C):
+    """The chunks' tables of as many workgroups as the chip's LDS holds (256 x 160 KB) and
+    one more chunk's, or the sorted way's pieces and lists: a quarter of the gradient's
+    rows in fp32, twelve bytes a token and eight a table row."""
+    f = L.lib().mtx_embedding_grad_workspace_bytes
+    for n in (1 << 15, 1 << 17, 1 << 20, 1 << 22):
+        for dtype in (0, 1):
+            most = max(256 * 163840 + V * C * 4, (n // 32 + 1) * 8 * C + 12 * n + 8 * V + 2048)
+            assert f(dtype, n, V, C) <= most, (n, dtype)
+    assert f(0, 1 << 22, V, C) == f(1, 1 << 22, V, C)

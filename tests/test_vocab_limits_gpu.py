@@ -155,3 +155,35 @@ def test_linear_xent_of_logits_at_the_ends_of_fp32(dev, n, C, V, kind, dtype):
     inside(host(dx), dz @ w.astype(np.float64).T, ed @ wa.T + ((V + 4) * U + cut) * (size @ wa.T))
     inside(host(dw), x.astype(np.float64).T @ dz, xa.T @ ed + ((n + 4) * U + cut) * (xa.T @ size))
     inside(host(db), dz.sum(0), ed.sum(0) + (n + 4) * U * size.sum(0))
+
+
+# ---------------------------------------------------------------------------
+# the table's gradient: small tables under many tokens
+# ---------------------------------------------------------------------------
+
+# chunks of one and of several groups of 64 tokens, the last one short; tables of as many
+# values as take this way, and of more
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n,V,C", [(140000, 65, 5), (140001, 10, 70), (200063, 128, 24), (70000, 255, 130), (66000, 65, 300),
+                                   (40000, 192, 192), (40000, 193, 192)])
+def test_lookup_grad_of_many_tokens(dev, n, V, C, dtype):
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(n + V + C)
+    ids = tokens(rng, n, V)
+    g = rounded(rng.standard_normal((n, C)).astype(np.float32), dtype)
+    counts = np.bincount(ids[(ids >= 0) & (ids < V)], minlength=V)[:, None]
+    want, size = ref.lookup_grad(ids, g, V, 0.5)
+    bound = (counts + 2) * 2.0 ** -24 * size
+    dg, di = dev_array(g, dtype), dev_array(ids, "int64")
+    first = host(K.embedding_grad(di, dg, full((V, C), 7.0), scale=0.5))
+    inside(first, want, bound)
+    assert np.array_equal(host(K.embedding_grad(di, dg, empty((V, C)), scale=0.5)), first)
+    old = rng.standard_normal((V, C)).astype(np.float32)
+    got = host(K.embedding_grad(di, dg, dev_array(old), scale=0.5, accumulate=True))
+    inside(got, want + old, bound + 2.0 ** -24 * (np.abs(want + old) + bound))
+    bad = int(np.nonzero((ids >= 0) & (ids < V))[0][-1])  # NaN stays in its token's row
+    g[bad] = np.nan
+    got = host(K.embedding_grad(di, dev_array(g, dtype), empty((V, C)), scale=0.5))
+    rest = np.arange(V) != ids[bad]
+    assert np.array_equal(got[rest], first[rest]) and np.isnan(got[ids[bad]]).all()
