@@ -398,18 +398,37 @@ bool whole(const void* p, int64_t ld, int cols) {
   return cols % 8 == 0 && ld % 8 == 0 && ld < kGemmBf16MaxLd && ((uintptr_t)p & 15) == 0;
 }
 
-// Whether a block of so many rows is faster in narrow_xent.  Measured, with a bias and all
-// gradients, in us, fp32 and bf16:
-// (rows, C, V)          the general way   narrow_xent
-// (16384, 384, 65)      95    83          60    58
-// (16384, 1024, 65)     181   99          104   104
-// (16384, 384, 96)      86    78          65    72
-// (16384, 1024, 96)     158   94          117   124
-// (16384, 384, 128)     84    79          99    101
-// (2048, 384, 65)       57    53          41    43
-// (300, 2048, 65)       50    50          124   133
-bool narrow_is_faster(int dtype, int rows, int C, int V) {
-  return V <= (dtype == MTX_F32 ? kNarrowV : 80) && rows >= 4LL * C;
+// Whether a block of so many rows is faster in narrow_xent, where every wave goes through
+// all of C for its 16 rows; bf16 values take the fp32 matrix cores there, so that wide rows
+// are faster the general way however many they are.  Measured in us, the general way and
+// narrow_xent; with gradients: bias and all of them, bf16 ones from bf16:
+//   rows, C, V        fp32         fp32, none   bf16         bf16, none
+//   16384, 384, 65    91    58     42    19     76    57     25    20
+//   65536, 384, 65    263   154    114   57     153   152    51    57
+//   16384, 1024, 65   184   101    87    34     95    103    34    35
+//   4096, 1024, 65    73    82     32    33     62    86     30    34
+//   2048, 384, 65     57    41     27    17     48    43     21    17
+//   300, 384, 65      34    39     20    16     49    41     21    17
+//   600, 256, 64      40    29     22    17     43    30     21    17
+//   3000, 512, 80     59    50     29    20     54    52     20    21
+//   3000, 768, 80     72    67     39    26     57    70     23    27
+//   3000, 768, 64     48    58     22    22     55    60     23    24
+//   6000, 512, 64     60    50     29    18     60    52     20    19
+//   3000, 256, 96     48    39     20    17     49    41     20    18
+//   4096, 384, 96     54    51     25    20     57    53     18    20
+//   6000, 512, 96     71    64     32    24     63    67     20    25
+//   1500, 1024, 32    49    42     22    18     52    45     26    19
+//   3000, 2048, 32    66    76     27    30     62    80     39    32
+//   12000, 2048, 32   128   92     56    33     103   96     43    35
+//   30000, 2048, 32   294   212    129   57     167   158    52    56
+bool narrow_is_faster(int dtype, bool grads, int rows, int C, int V) {
+  if (V > kNarrowV) return false;
+  const bool half = dtype == MTX_BF16;
+  if (V <= 32) return C <= 1024 || (half && !grads ? C <= 2048 && rows <= 16384 : rows >= 4LL * C);
+  const bool many = rows >= (grads && C > 512 ? 6LL : 4LL) * C;
+  if (!half) return C <= (grads ? 256 : 512) || many;
+  return C <= 256 || (V <= 80 && C <= 384 && (grads || rows <= 32768)) ||
+         (C <= 512 && rows <= 16384 && (V <= 64 || (V <= 80 && many)));
 }
 
 // Row kernels' workgroups: about as many as the chip holds at once (as many partial
@@ -427,7 +446,7 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   const int64_t fit = std::min<int64_t>(std::max<int64_t>(logits_bytes / (4 * p.ldz), 1), 1 << 18);
   p.rows = (int)std::min(n, fit < 256 ? fit : fit / 256 * 256);
   p.rows32 = (p.rows + 31) / 32 * 32;
-  p.narrow = near && narrow_is_faster(dtype, p.rows, C, V);
+  p.narrow = near && narrow_is_faster(dtype, grads >= 0, p.rows, C, V);
   // Below 128 rows the fp32 products leave the matrix cores; above 64 they pay for 128 on
   // the vector units.  With all gradients 72 rows, C = 1370, V = 37387: 553 us so, 326 as 128
   // rows; 100, 512, 20001: 141 and 112; but 65, 128, 5003: 48 and 77.

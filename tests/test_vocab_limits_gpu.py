@@ -187,3 +187,16 @@ def test_lookup_grad_of_many_tokens(dev, n, V, C, dtype):
     got = host(K.embedding_grad(di, dev_array(g, dtype), empty((V, C)), scale=0.5))
     rest = np.arange(V) != ids[bad]
     assert np.array_equal(got[rest], first[rest]) and np.isnan(got[ids[bad]]).all()
+
+
+# ---------------------------------------------------------------------------
+# projection and cross-entropy: either side of the small vocabularies' borders
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,out", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("n,C,V", [(1, 1024, 32), (5, 1025, 32), (40, 256, 33), (40, 257, 96), (300, 384, 80), (300, 385, 80),
+                                   (70, 512, 64), (70, 513, 64), (3100, 513, 70), (50, 384, 81), (4200, 1030, 20)])
+def test_linear_xent_where_the_small_vocabularies_way_ends(dev, n, C, V, dtype, out):
+    from test_vocab_gpu import check_xent
+
+    check_xent(n, C, V, dtype, out, tied=n % 2 == 0)
