@@ -1331,6 +1331,18 @@ struct Plan {
   int bm, bn, ksplit, kchunk;  // tile rows and columns, K split
 };
 
+// Ranges of K that t tiles are to be cut into: up to 64 for K >= 4096 (partials: as many
+// M x N floats), each of MTX_SPLIT_MINK or more; for skinny products (decode steps: M =
+// sequences), whose tiles are too few to cover the CUs, of 64 or more.
+int wanted_ranges(int64_t t, int K) {
+  if (t < 256 && K >= 1024) {
+    const int want = (int)std::min<int64_t>(K >= 4096 ? 64 : 16, (MTX_SPLIT_TARGET + t - 1) / t);
+    return std::min(want, std::max(1, K / MTX_SPLIT_MINK));
+  }
+  if (t < 64 && K >= 128) return std::min((int)std::min<int64_t>(16, (256 + t - 1) / t), K / 64);
+  return 1;
+}
+
 // Pick the tile and the K split for a problem so that the launch has enough
 // workgroups to fill 256 CUs, splitting K only when it is long.
 Plan plan_gemm(int M, int N, int K, int batch, size_t ws_bytes) {
@@ -1347,28 +1359,12 @@ Plan plan_gemm(int M, int N, int K, int batch, size_t ws_bytes) {
   const int64_t t128 = tiles(128, 128);
   if (!longk && (t128 < 512 || t128 % 256 != 0)) { p.bm = 64; p.bn = 64; }
   const int64_t t = tiles(p.bm, p.bn);
-  if (t < 256 && K >= 1024) {
-    // up to 64 splits for K >= 4096 (partials: want x M x N floats)
-    int want = (int)std::min<int64_t>(K >= 4096 ? 64 : 16, (MTX_SPLIT_TARGET + t - 1) / t);
-    // each split keeps >= MTX_SPLIT_MINK of K
-    want = std::min(want, std::max(1, K / MTX_SPLIT_MINK));
-    const size_t need = (size_t)want * batch * (size_t)(M + 1) * N * sizeof(float);
-    if (want > 1 && need <= ws_bytes) {
-      p.ksplit = want;
-      p.kchunk = cdiv(cdiv(K, want), BK) * BK;
-      p.ksplit = cdiv(K, p.kchunk);
-    }
-  } else if (t < 64 && K >= 128) {
-    // skinny products (decode steps: M = sequences): too few output tiles to
-    // cover the CUs, so split K into chunks of >= 64
-    int want = (int)std::min<int64_t>(16, (256 + t - 1) / t);
-    want = std::min(want, K / 64);
-    const size_t need = (size_t)want * batch * (size_t)M * N * sizeof(float);
-    if (want > 1 && need <= ws_bytes) {
-      p.ksplit = want;
-      p.kchunk = cdiv(cdiv(K, want), BK) * BK;
-      p.ksplit = cdiv(K, p.kchunk);
-    }
+  const int want = wanted_ranges(t, K);
+  // (the long products' room has the column sums of mtx_gemm_wgrad_f32 beside it)
+  const size_t need = (size_t)want * batch * (size_t)(M + (t < 256 && K >= 1024 ? 1 : 0)) * N * sizeof(float);
+  if (want > 1 && need <= ws_bytes) {
+    p.kchunk = cdiv(cdiv(K, want), BK) * BK;
+    p.ksplit = cdiv(K, p.kchunk);
   }
   return p;
 }
@@ -1512,6 +1508,16 @@ int launch_x3(const GemmArgs& g, int bn, bool ak, bool bn1, hipStream_t st) {
 }
 
 }  // namespace
+}  // namespace mtx
+
+namespace mtx {
+size_t gemm_room_bytes(int M, int N, int K) {
+  const bool long128 = K >= 4096 && M >= 128 && N >= 128;  // (as plan_gemm: tiles of 128 x 128)
+  const int64_t t = long128 ? (int64_t)cdiv(M, 128) * cdiv(N, 128) : (int64_t)cdiv(M, 64) * cdiv(N, 64);
+  const int want = wanted_ranges(t, K);
+  const size_t room = want > 1 ? (size_t)want * (size_t)(M + 1) * N * sizeof(float) : 0;
+  return std::max(room, mtx_gemm_workspace_bytes(M, N, K, 1));
+}
 }  // namespace mtx
 
 using namespace mtx;

@@ -483,7 +483,7 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
       continue;
     }
     auto bytes = [&](int M, int N, int K) {
-      most = std::max(most, dtype == MTX_F32 ? mtx_gemm_workspace_bytes(M, N, K, 1)
+      most = std::max(most, dtype == MTX_F32 ? gemm_room_bytes(M, N, K)
                                              : gemm_bf16_workspace_bytes(M, N, K, N == V && M == r ? 1 : p.pieces));
     };
     const int m = p.pad ? 128 : r;
@@ -491,10 +491,6 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
     if (!p.pieces) continue;
     if (dtype == MTX_F32) {
       bytes(m, C, V);
-      // Few rows and a long V: the product cuts V into up to 64 ranges only if it finds
-      // room for as many as it first asks for, before it rounds them to whole slices (1 row,
-      // C = 896, V = 24763: dx 1480 us without that room, 46 with it)
-      if (r <= 64) most = std::max(most, (size_t)64 * (r + 1) * C * 4);
       bytes(C, V, r);
       bytes(V, C, r);
     } else {

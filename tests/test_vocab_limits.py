@@ -81,3 +81,14 @@ def test_small_tables_workspace_does_not_grow_with_the_tokens(V, C):
             most = max(256 * 163840 + V * C * 4, (n // 32 + 1) * 8 * C + 12 * n + 8 * V + 2048)
             assert f(dtype, n, V, C) <= most, (n, dtype)
     assert f(0, 1 << 22, V, C) == f(1, 1 << 22, V, C)
+
+
+@pytest.mark.parametrize("n,C,V", [(12000, 64, 100), (6000, 100, 120), (9000, 40, 500), (3001, 64, 97)])
+def test_fp32_weights_gradients_have_room_for_all_ranges_of_the_rows(n, C, V):
+    """The product dW = x^T dz asks for this many ranges of the rows (the fp32 tiles' rule),
+    each with its C + 1 rows of V sums, and is not cut at all without the room."""
+    tiles = -(-C // 64) * -(-V // 64)
+    ranges = min(64 if n >= 4096 else 16, -(-768 // tiles), n // 256)
+    kept = n * (-(-V // 32) * 32) * 4  # the logits
+    f = L.lib().mtx_linear_xent_workspace_bytes
+    assert f(0, 0, n, C, V, 0, 1 << 30) >= kept + ranges * (C + 1) * V * 4
