@@ -387,10 +387,20 @@ struct Plan {
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// x is copied into panels (gemm_bf16.h), where the products could take it as it is, if
-// its copy is small beside them: 8192 x 1024 and a vocabulary of 50021 take 3284 us with
-// it (13 of them the copy) and 3355 without; the copy of W (62 us) gains nothing.
-constexpr int64_t kPanelRows = 2048, kPanelCols = 16384;
+// Whether x is copied into panels (gemm_bf16.h) where the products could take it as it is:
+// a copy that is small beside them, for long vocabularies.  In us, as it is and with the
+// copy, without gradients and with bf16 ones:
+//   rows, C, V          none          bf16
+//   8192, 1024, 50021   899   846     5183  5138
+//   16384, 2048, 32768  2330  2106    12574 12254
+//   2048, 1024, 32768   153   149     917   896
+//   8192, 256, 32768    224   220     1566  1565
+//   2048, 256, 50021    97    101     634   630
+//   8192, 256, 16384    119   119     780   776
+//   16384, 1024, 4096   159   159     850   843
+//   8192, 1024, 4096    85    86      436   442
+// (The copy of W, 62 us of the first, gains nothing.)
+bool panels_pay(int64_t n, int C, int V) { return V >= 16384 && (double)n * C * V >= 0x1p36; }
 
 // Whether rows of `cols` bf16 values at p, ld values apart, are whole 16-byte vectors
 // that the products can take as they are.
@@ -561,7 +571,7 @@ extern "C" int mtx_linear_xent(int dtype, int grad_dtype, int64_t n, int C, int 
   const int64_t ldw = wv ? swc : swv;
   const bool near = std::max({n ? ldx : 0, ldw, dx ? lddx : 0}) < kNarrowLd;
   const Plan p = plan(dtype, grad ? grad_dtype : -1, std::max<int64_t>(n, 1), C, V, db != nullptr, logits_bytes,
-                      (n >= kPanelRows && V >= kPanelCols) || !whole(x, ldx, C), !whole(w, ldw, wv ? V : C), near);
+                      panels_pay(n, C, V) || !whole(x, ldx, C), !whole(w, ldw, wv ? V : C), near);
   MTX_CHECK_ARG(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
                 "linear_xent: workspace of %zu bytes, need %zu aligned to 256", workspace_bytes, p.bytes);
   {
