@@ -550,15 +550,34 @@ def embedding(weight, idx, scale=1.0):
 
 
 # Where F.dropout's generator stands: Philox4x32-10 keyed by the seed.  Eager calls
-# draw from its subsequence 1, one after another; every recorded graph has a
-# subsequence of its own (graphs.Graph); attention_keep_mask's masks are in
-# subsequence 0.
-_LAYER_RNG = {"seed": 0, "offset": 0}
+# draw from its subsequence 1, one after another; a recorded graph gets a subsequence
+# of its own, from 2 on, with the first call in it that draws (graphs.Graph);
+# attention_keep_mask's masks are in subsequence 0.
+_LAYER_RNG = {"seed": 0, "offset": 0, "graphs": 0}
 
 
 def set_dropout_seed(seed: int) -> None:
-    """Restart F.dropout's generator (a graph recorded before keeps its own)."""
-    _LAYER_RNG.update(seed=int(seed), offset=0)
+    """Restart F.dropout's generator: what is drawn, and recorded, from here on draws
+    the same numbers after the same seed.  A graph recorded before keeps its own; it
+    shares them with one recorded after a restart with its seed."""
+    _LAYER_RNG.update(seed=int(seed), offset=0, graphs=0)
+
+
+def _draw(calls):
+    """Where the next `calls` calls of the generator begin, as kernels.dropout takes it."""
+    from . import _lib
+
+    graph = _lib._GRAPH[0]
+    if graph is None:
+        at = dict(seed=_LAYER_RNG["seed"], offset=_LAYER_RNG["offset"], subsequence=1)
+        _LAYER_RNG["offset"] += calls
+        return at
+    if graph.subsequence is None:
+        _LAYER_RNG["graphs"] += 1
+        graph.seed, graph.subsequence = _LAYER_RNG["seed"], 1 + _LAYER_RNG["graphs"]
+    at = dict(seed=graph.seed, offset=graph.draws, subsequence=graph.subsequence, base=graph.base)
+    graph.draws += calls
+    return at
 
 
 def dropout(x, p=0.5, residual=None):
@@ -567,8 +586,6 @@ def dropout(x, p=0.5, residual=None):
     in one pass each way.  The mask comes from the device generator and is drawn
     again, not read, in the backward (mtx_dropout); set_dropout_seed restarts it.
     In a recorded step every replay draws other masks."""
-    from . import _lib
-
     if not 0.0 <= p < 1.0:
         raise ValueError(f"dropout probability must be in [0, 1) (got {p})")
     if residual is not None and tuple(residual.shape) != tuple(x.shape):
@@ -576,14 +593,7 @@ def dropout(x, p=0.5, residual=None):
     if p == 0.0:
         return x if residual is None else residual + x
     flat = lambda a: a.contiguous().t.reshape(1, -1)  # noqa: E731
-    calls = (x.data.size + 3) // 4
-    graph = _lib._GRAPH[0]
-    if graph is not None:
-        at = dict(seed=_LAYER_RNG["seed"], offset=graph.draws, subsequence=graph.subsequence, base=graph.base)
-        graph.draws += calls
-    else:
-        at = dict(seed=_LAYER_RNG["seed"], offset=_LAYER_RNG["offset"], subsequence=1)
-        _LAYER_RNG["offset"] += calls
+    at = _draw((x.data.size + 3) // 4)
     data = DeviceArray(_empty(x.shape, x.data.t.dtype))
     K.dropout(flat(x.data), p, residual=None if residual is None else flat(residual.data), out=flat(data), **at)
     prev = (x,) if residual is None else (x, residual)

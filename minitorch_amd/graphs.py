@@ -48,12 +48,13 @@ class Graph:
     """One recorded HIP graph.  ``with g.capture(): ...`` records every launch
     the block issues (none of them runs); ``g.replay()`` runs them all."""
 
-    _recorded = 0  # graphs recorded by this process
-
     def __init__(self):
         self._h = None
-        self.draws = 0  # calls of F.dropout's generator in one replay
-        self.replays = 0
+        # F.dropout's numbers: a recorded call's lie at `base`, in device memory, plus
+        # what the step drew before it, in the subsequence that the first of them gets
+        # here; replay() moves base on by the step's draws
+        self.base, self.draws, self.replays = None, 0, 0
+        self.seed = self.subsequence = None
 
     @contextmanager
     def capture(self):
@@ -61,11 +62,7 @@ class Graph:
             raise RuntimeError("this graph is already recorded")
         if L.capturing():
             raise RuntimeError("a capture is already in progress")
-        # F.dropout's numbers: a recorded call's lie at `base` plus what the step drew
-        # before it, in a subsequence of this graph's own; replay() moves base on
-        self.base, self.draws, self.replays = dev.zeros((1,), "int64").t, 0, 0
-        Graph._recorded += 1
-        self.subsequence = 1 + Graph._recorded
+        self.base, self.draws, self.replays, self.subsequence = dev.zeros((1,), "int64").t, 0, 0, None
         dev.synchronize()
         s = _capture_stream()
         L.call("mtx_graph_begin", s)
