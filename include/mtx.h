@@ -249,6 +249,13 @@ int mtx_attn_bwd_dropout(int dtype, int B, int H, int Tq, int Tk, int D,
  */
 int mtx_dropout_keep_philox(uint8_t* keep, int64_t rows, int cols, int64_t ld, float p,
                             uint64_t seed, uint64_t offset, void* stream);
+/*
+ * The same with `subsequence` as the counter's third word, from counter offset + base[0]
+ * on (base, device memory: NULL counts as 0), as mtx_dropout draws: a recorded call draws
+ * another mask in every replay if base[0] changes in between.
+ */
+int mtx_dropout_keep(uint8_t* keep, int64_t rows, int cols, int64_t ld, float p, uint64_t seed, uint64_t offset,
+                     uint32_t subsequence, const uint64_t* base, void* stream);
 
 /*
  * Dropout whose mask is never stored (Dropout.forward, layers.py:113-126):

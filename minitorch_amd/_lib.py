@@ -89,6 +89,7 @@ SIGNATURES = {
                                   _P, _I64P, _P, _I64P, _P, _I64P,
                                   _P, _SZ, _F, _I, _I, _P, _I64, _F, _P]),
     "mtx_dropout_keep_philox": (_I, [_P, _I64, _I, _I64, _F, C.c_uint64, C.c_uint64, _P]),
+    "mtx_dropout_keep": (_I, [_P, _I64, _I, _I64, _F, C.c_uint64, C.c_uint64, C.c_uint32, _P, _P]),
     "mtx_dropout": (_I, [_I, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _F, _F, C.c_uint64, C.c_uint64, C.c_uint32, _P,
                          _P]),
     "mtx_pack3_f32": (_I, [_P, _P, _P, _I64, _I64, _P, _P]),

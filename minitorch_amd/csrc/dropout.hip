@@ -39,13 +39,13 @@ __device__ __forceinline__ U4 philox4x32_10(U4 c, uint32_t k0, uint32_t k1) {
 // array; element (i, j) is stored at keep[i * ld + j]
 __global__ __launch_bounds__(256) void keep_philox_kernel(uint8_t* __restrict__ keep, int64_t rows, int cols,
                                                           int64_t ld, float p, uint32_t k0, uint32_t k1,
-                                                          uint64_t offset) {
+                                                          uint64_t offset, uint32_t sub, const uint64_t* base) {
   const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t n = rows * (int64_t)cols;
   const int64_t e0 = 4 * t;
   if (e0 >= n) return;
-  const uint64_t ctr = offset + (uint64_t)t;
-  const U4 r = philox4x32_10(U4{(uint32_t)ctr, (uint32_t)(ctr >> 32), 0u, 0u}, k0, k1);
+  const uint64_t ctr = offset + (base ? *base : 0) + (uint64_t)t;
+  const U4 r = philox4x32_10(U4{(uint32_t)ctr, (uint32_t)(ctr >> 32), sub, 0u}, k0, k1);
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
   int64_t row = e0 / cols;
   int col = (int)(e0 - row * cols);
@@ -197,18 +197,24 @@ extern "C" int mtx_dropout(int dtype, const void* x, int64_t ldx, const void* re
   return MTX_OK;
 }
 
-extern "C" int mtx_dropout_keep_philox(uint8_t* keep, int64_t rows, int cols, int64_t ld, float p,
-                                       uint64_t seed, uint64_t offset, void* stream) {
+extern "C" int mtx_dropout_keep(uint8_t* keep, int64_t rows, int cols, int64_t ld, float p, uint64_t seed,
+                                uint64_t offset, uint32_t subsequence, const uint64_t* base, void* stream) {
   MTX_CHECK_ARG(rows >= 0 && cols >= 1, "rows=%lld, cols=%d: need rows >= 0, cols >= 1", (long long)rows, cols);
   MTX_CHECK_ARG(ld >= cols, "ld=%lld must be >= cols=%d", (long long)ld, cols);
   MTX_CHECK_ARG(p >= 0.f && p < 1.f, "p=%g must be in [0, 1)", (double)p);
   if (rows == 0) return MTX_OK;
   MTX_CHECK_ARG(keep != nullptr, "keep: null pointer");
+  MTX_CHECK_ARG((reinterpret_cast<uintptr_t>(base) & 7) == 0, "dropout_keep: base must be 8-byte aligned");
+  MTX_CHECK_SHAPE(rows <= (int64_t)0x7fffffff * 1024 / cols, "mask too large");
   const int64_t calls = (rows * (int64_t)cols + 3) / 4;
-  MTX_CHECK_SHAPE(calls <= (int64_t)0x7fffffff * 256, "mask too large");
   const unsigned blocks = (unsigned)((calls + 255) / 256);
   hipLaunchKernelGGL(keep_philox_kernel, dim3(blocks), dim3(256), 0, static_cast<hipStream_t>(stream), keep, rows,
-                     cols, ld, p, (uint32_t)seed, (uint32_t)(seed >> 32), offset);
+                     cols, ld, p, (uint32_t)seed, (uint32_t)(seed >> 32), offset, subsequence, base);
   MTX_LAUNCHED();
   return MTX_OK;
+}
+
+extern "C" int mtx_dropout_keep_philox(uint8_t* keep, int64_t rows, int cols, int64_t ld, float p,
+                                       uint64_t seed, uint64_t offset, void* stream) {
+  return mtx_dropout_keep(keep, rows, cols, ld, p, seed, offset, 0, nullptr, stream);
 }

@@ -405,18 +405,23 @@ def set_attention_dropout_rng(mode: str = "host", seed: int = 0) -> None:
     _DROPOUT_RNG.update(mode=mode, seed=int(seed), offset=0)
 
 
-def attention_keep_mask(shape, p: float):
+def attention_keep_mask(shape, p: float, rng="host"):
     """Keep-mask of a (B, H, Tq, Tk) attention matrix for drop probability p,
     as the fused kernels take it (uint8 (B, H, Tq, ld), ld = Tk rounded up to
-    a multiple of 4).  Returns (mask, keep_scale)."""
+    a multiple of 4).  rng "host": drawn where set_attention_dropout_rng says;
+    "device": from F.dropout's generator, in a recorded step another mask in
+    every replay.  Returns (mask, keep_scale)."""
     from . import _lib
 
+    B, H, Tq, Tk = (int(x) for x in shape)
+    keep_scale = float(np.float32(1.0 / (1.0 - p)))
+    if rng == "device":
+        return K.dropout_keep_philox((B, H, Tq, Tk), p, **_draw((B * H * Tq * Tk + 3) // 4))[0], keep_scale
     if _lib.capturing():
         # a recorded step would replay this draw (host mask or Philox
         # offset) unchanged on every call
-        raise RuntimeError("attention dropout masks cannot be drawn inside a recorded (captured) step")
-    B, H, Tq, Tk = (int(x) for x in shape)
-    keep_scale = float(np.float32(1.0 / (1.0 - p)))
+        raise RuntimeError("attention dropout masks cannot be drawn inside a recorded (captured) step, but by "
+                           'a module with dropout_rng="device"')
     if _DROPOUT_RNG["mode"] == "device":
         mask, _DROPOUT_RNG["offset"] = K.dropout_keep_philox(
             (B, H, Tq, Tk), p, _DROPOUT_RNG["seed"], _DROPOUT_RNG["offset"])
@@ -552,7 +557,7 @@ def embedding(weight, idx, scale=1.0):
 # Where F.dropout's generator stands: Philox4x32-10 keyed by the seed.  Eager calls
 # draw from its subsequence 1, one after another; a recorded graph gets a subsequence
 # of its own, from 2 on, with the first call in it that draws (graphs.Graph);
-# attention_keep_mask's masks are in subsequence 0.
+# set_attention_dropout_rng's masks are in subsequence 0.
 _LAYER_RNG = {"seed": 0, "offset": 0, "graphs": 0}
 
 

@@ -80,18 +80,19 @@ def keep_ld(Tk: int) -> int:
     return (Tk + 3) // 4 * 4
 
 
-def dropout_keep_philox(shape, p: float, seed: int, offset: int, out=None):
+def dropout_keep_philox(shape, p: float, seed: int, offset: int, out=None, subsequence: int = 0, base=None):
     """Keep-mask (B, H, Tq, keep_ld(Tk)) uint8 for dropout probability p, from
-    the device Philox4x32-10 generator (mtx_dropout_keep_philox): element
-    e of the logical (B*H*Tq, Tk) array uses output word e % 4 of counter
-    offset + e // 4.  Returns (mask, next offset)."""
+    the device Philox4x32-10 generator (mtx_dropout_keep): element e of the
+    logical (B*H*Tq, Tk) array uses output word e % 4 of counter offset + e // 4
+    in the generator's `subsequence`.  base: a device int64 (1,) array that is
+    added to offset when the kernel runs.  Returns (mask, next offset)."""
     B, H, Tq, Tk = (int(x) for x in shape)
     ld = keep_ld(Tk)
     if out is None:
         out = dev.empty_buf((B, H, Tq, ld), "uint8").fill_(0)
     rows = B * H * Tq
-    L.call("mtx_dropout_keep_philox", L.ptr(out), rows, Tk, ld, float(p), int(seed) & (2**64 - 1),
-           int(offset) & (2**64 - 1), L.stream_handle())
+    L.call("mtx_dropout_keep", L.ptr(out), rows, Tk, ld, float(p), int(seed) & (2**64 - 1),
+           int(offset) & (2**64 - 1), int(subsequence) & (2**32 - 1), _ptr(base), L.stream_handle())
     return out, offset + (rows * Tk + 3) // 4
 
 

@@ -54,7 +54,7 @@ def _linear_ln_into(x, lin, out, ln):
 
 
 class MultiHeadAttention(Module):
-    def __init__(self, n_embd, n_head, dropout=0.0):
+    def __init__(self, n_embd, n_head, dropout=0.0, dropout_rng="host"):
         super().__init__()
         assert n_embd % n_head == 0, "n_embd must be divisible by n_head"
         self.n_head = n_head
@@ -63,7 +63,7 @@ class MultiHeadAttention(Module):
         self.k_proj = Linear(n_embd, n_embd)
         self.v_proj = Linear(n_embd, n_embd)
         self.out_proj = Linear(n_embd, n_embd)
-        self.attn_drop = Dropout(dropout)
+        self.attn_drop = Dropout(dropout, dropout_rng)
         self._qkv = None  # fused q/k/v projection for decode steps (fuse_qkv)
 
     def _split_heads(self, x, B, T):
@@ -80,7 +80,7 @@ class MultiHeadAttention(Module):
             # attn_drop (transformer.py:43) inside the fused kernel: the mask
             # is drawn where the reference draws it (no other draw happens
             # between the projections and the softmax)
-            keep, ks = F.attention_keep_mask((B, self.n_head, T, T), self.attn_drop.p)
+            keep, ks = F.attention_keep_mask((B, self.n_head, T, T), self.attn_drop.p, self.attn_drop.rng)
             drop = {"keep": keep, "keep_scale": ks}
         scale = 1.0 / math.sqrt(self.head_dim)
         projs = (self.q_proj, self.k_proj, self.v_proj)
@@ -257,12 +257,12 @@ class MultiHeadAttention(Module):
 
 class TransformerBlock(Module):
     """Pre-norm block: x + attn(ln1(x)), then x + mlp(ln2(x)).  dropout_rng: where
-    the MLP's dropout draws (Dropout)."""
+    the attention's and the MLP's dropout draw (Dropout)."""
 
     def __init__(self, n_embd, n_head, dropout=0.0, dropout_rng="host"):
         super().__init__()
         self.ln1 = LayerNorm(n_embd)
-        self.attn = MultiHeadAttention(n_embd, n_head, dropout)
+        self.attn = MultiHeadAttention(n_embd, n_head, dropout, dropout_rng)
         self.ln2 = LayerNorm(n_embd)
         self.mlp = Sequential(
             Linear(n_embd, 4 * n_embd),

@@ -1,7 +1,7 @@
 """What the operators of training with a large vocabulary take and refuse at the ends
 of their ranges.  No GPU: every check runs before any HIP call."""
 import pytest
-from test_vocab_refusals import Fake, _kernels, dropout, p, xent
+from test_vocab_refusals import Fake, _kernels, call, dropout, p, xent
 
 from minitorch_amd import _lib as L
 
@@ -92,3 +92,14 @@ def test_fp32_weights_gradients_have_room_for_all_ranges_of_the_rows(n, C, V):
     kept = n * (-(-V // 32) * 32) * 4  # the logits
     f = L.lib().mtx_linear_xent_workspace_bytes
     assert f(0, 0, n, C, V, 0, 1 << 30) >= kept + ranges * (C + 1) * V * 4
+
+
+@pytest.mark.parametrize("over,code,frag", [
+    (dict(rows=-1), L.MTX_ERR_ARG, "rows"), (dict(cols=0), L.MTX_ERR_ARG, "cols"), (dict(ld=7), L.MTX_ERR_ARG, "ld"),
+    (dict(p=1.0), L.MTX_ERR_ARG, "p="), (dict(keep=None), L.MTX_ERR_ARG, "null"), (dict(base=p(12)), L.MTX_ERR_ARG, "aligned"),
+    (dict(rows=1 << 60), L.MTX_ERR_SHAPE, "large"),
+])
+def test_dropout_keep_refusals(over, code, frag):
+    rc, msg = call("mtx_dropout_keep", dict(keep=p(16), rows=4, cols=8, ld=8, p=0.5, seed=1, offset=0, sub=0, base=None,
+                                            stream=None), over)
+    assert rc == code and frag in msg, (rc, msg)
