@@ -557,8 +557,10 @@ def embedding(weight, idx, scale=1.0):
 # Where F.dropout's generator stands: Philox4x32-10 keyed by the seed.  Eager calls
 # draw from its subsequence 1, one after another; a recorded graph gets a subsequence
 # of its own, from 2 on, with the first call in it that draws (graphs.Graph);
-# set_attention_dropout_rng's masks are in subsequence 0.
-_LAYER_RNG = {"seed": 0, "offset": 0, "graphs": 0}
+# set_attention_dropout_rng's masks are in subsequence 0.  Without set_dropout_seed the
+# first call draws the seed from NumPy's global RNG, which the host's masks come from:
+# processes side by side draw different masks, and np.random.seed settles both.
+_LAYER_RNG = {"seed": None, "offset": 0, "graphs": 0}
 
 
 def set_dropout_seed(seed: int) -> None:
@@ -572,6 +574,8 @@ def _draw(calls):
     """Where the next `calls` calls of the generator begin, as kernels.dropout takes it."""
     from . import _lib
 
+    if _LAYER_RNG["seed"] is None:
+        set_dropout_seed(np.random.randint(0, 1 << 63, dtype=np.uint64))
     graph = _lib._GRAPH[0]
     if graph is None:
         at = dict(seed=_LAYER_RNG["seed"], offset=_LAYER_RNG["offset"], subsequence=1)
