@@ -101,6 +101,8 @@ class Embedding(Module):
     out times that constant, negative ids are padding, and the gradient goes by
     sorted tokens (F.embedding)."""
 
+    scale = None  # of a subclass with an __init__ of its own
+
     def __init__(self, num_embeddings, embed_dim, scale=None):
         super().__init__()
         assert num_embeddings > 0 and embed_dim > 0, "sizes must be positive"
@@ -121,6 +123,8 @@ class Dropout(Module):
     p == 0 (the same Tensor is returned).  The keep-mask is drawn on the host
     from NumPy's global RNG, as the reference draws it, or, with rng="device",
     on the device where it is used (F.dropout)."""
+
+    rng = "host"  # of a subclass with an __init__ of its own
 
     def __init__(self, p=0.5, rng="host"):
         super().__init__()

@@ -80,7 +80,8 @@ class MultiHeadAttention(Module):
             # attn_drop (transformer.py:43) inside the fused kernel: the mask
             # is drawn where the reference draws it (no other draw happens
             # between the projections and the softmax)
-            keep, ks = F.attention_keep_mask((B, self.n_head, T, T), self.attn_drop.p, self.attn_drop.rng)
+            keep, ks = F.attention_keep_mask((B, self.n_head, T, T), self.attn_drop.p,
+                                               getattr(self.attn_drop, "rng", "host"))
             drop = {"keep": keep, "keep_scale": ks}
         scale = 1.0 / math.sqrt(self.head_dim)
         projs = (self.q_proj, self.k_proj, self.v_proj)
@@ -462,7 +463,8 @@ class GPT(Module):
             idx = np.asarray(idx)
         B, T = idx.shape
         assert T <= self.block_size, f"sequence length {T} exceeds block_size {self.block_size}"
-        tok = F.embedding(self.tok_emb.weight, idx, 1.0 if self.tok_emb.scale is None else self.tok_emb.scale)
+        scale = getattr(self.tok_emb, "scale", None)
+        tok = F.embedding(self.tok_emb.weight, idx, 1.0 if scale is None else scale)
         return F.linear_cross_entropy(self._trunk(tok, T), self.lm_head.weight, self.lm_head.bias, targets)
 
     def generate_greedy(self, idx, max_new_tokens, return_margins=False, graph=True):
@@ -495,7 +497,7 @@ class GPT(Module):
         Tmax = T0 + n
         if Tmax > self.block_size:
             raise ValueError(f"prompt + new tokens = {Tmax} exceeds block_size {self.block_size}")
-        if any(e.scale not in (None, 1.0) for e in (self.tok_emb, self.pos_emb)):
+        if any(getattr(e, "scale", None) not in (None, 1.0) for e in (self.tok_emb, self.pos_emb)):
             raise NotImplementedError("greedy decode steps read embedding tables without a scale (use generate())")
         if n < 1:
             return (idx.copy(), np.empty((B, 0))) if return_margins else idx.copy()
