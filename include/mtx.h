@@ -263,10 +263,10 @@ int mtx_dropout_keep(uint8_t* keep, int64_t rows, int cols, int64_t ld, float p,
  * over rows x cols values of fp32 or bf16, row strides ldx, ldr, ldy; x, residual
  * and y may be one array.  keep is mtx_dropout_keep_philox's: element e has word
  * e % 4 of counter offset + base[0] + e/4 (base, device memory: NULL counts as 0)
- * with `subsequence` as the counter's third word.  The gradient is the same call on the
- * upstream gradient; with residual = y it is added.  A recorded call draws other
- * numbers in every replay if base[0] changes in between.  0 <= p < 1.  At most 2^33
- * values.
+ * with `subsequence` as the counter's third word; p = 0 keeps every value, where that
+ * mask lacks the uniform 0.  The gradient is the same call on the upstream gradient; with
+ * residual = y it is added.  A recorded call draws other numbers in every replay if
+ * base[0] changes in between.  0 <= p < 1.  At most 2^33 values.
  */
 int mtx_dropout(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y, int64_t ldy,
                 int64_t rows, int64_t cols, float p, float scale, uint64_t seed, uint64_t offset, uint32_t subsequence,

@@ -72,6 +72,7 @@ struct DropArgs {
   void* y;
   int64_t ldx, ldr, ldy, n, cols;  // n: values
   uint32_t below;  // kept: words above it
+  bool all;        // p = 0: every value, where the uniform is 0 too
   float scale;
   uint32_t k0, k1, sub;
   uint64_t offset;
@@ -79,6 +80,7 @@ struct DropArgs {
 };
 
 __device__ __forceinline__ U4 draw(const DropArgs& a, uint64_t from, uint64_t call) {
+  if (a.all) return U4{~0u, ~0u, ~0u, ~0u};
   const uint64_t ctr = from + call;
   return philox4x32_10(U4{(uint32_t)ctr, (uint32_t)(ctr >> 32), a.sub, 0u}, a.k0, a.k1);
 }
@@ -188,8 +190,8 @@ extern "C" int mtx_dropout(int dtype, const void* x, int64_t ldx, const void* re
   MTX_CHECK_SHAPE(rows <= ((int64_t)1 << 33) / cols, "dropout: more than 2^33 values");
   // u > p with u = (w >> 8) 2^-24: w >= 256 (floor(2^24 p) + 1)
   const uint32_t below = (uint32_t)((((uint64_t)((double)p * 0x1p24)) + 1) * 256 - 1);
-  const DropArgs a{x, residual, y, ldx, ldr, ldy, rows * cols, cols, below, scale, (uint32_t)seed,
-                   (uint32_t)(seed >> 32), subsequence, offset, base};
+  const DropArgs a{x, residual, y, ldx, ldr, ldy, rows * cols, cols, below, p == 0.f, scale,
+                   (uint32_t)seed, (uint32_t)(seed >> 32), subsequence, offset, base};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == MTX_F32) residual ? dropout<float, true>(a, rows, st) : dropout<float, false>(a, rows, st);
   else residual ? dropout<bf16_t, true>(a, rows, st) : dropout<bf16_t, false>(a, rows, st);

@@ -1408,9 +1408,10 @@ def _dropout_plan(x, residual, out):
 def dropout(x, p: float, seed: int, offset: int = 0, residual=None, out=None, subsequence: int = 0, base=None):
     """(residual +) x * keep / (1 - p) over a (rows, cols) view, fp32 or bf16, the
     keep-mask drawn where it is used (mtx_dropout): dropout_keep_philox's at
-    (seed, offset), with the generator's `subsequence`.  The gradient is the same
-    call on the upstream gradient; out may be x or residual.  base: a device int64
-    (1,) array that is added to offset when the kernel runs.  Returns out."""
+    (seed, offset), with the generator's `subsequence`; p = 0 keeps everything.  The
+    gradient is the same call on the upstream gradient; out may be x or residual.  base:
+    a device int64 (1,) array that is added to offset when the kernel runs.  Returns
+    out."""
     if not 0.0 <= p < 1.0:
         raise ValueError(f"dropout probability must be in [0, 1) (got {p})")
     if out is None:

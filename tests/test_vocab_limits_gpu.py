@@ -200,3 +200,32 @@ def test_linear_xent_where_the_small_vocabularies_way_ends(dev, n, C, V, dtype, 
     from test_vocab_gpu import check_xent
 
     check_xent(n, C, V, dtype, out, tied=n % 2 == 0)
+
+
+# ---------------------------------------------------------------------------
+# dropout: probability 0
+# ---------------------------------------------------------------------------
+
+# Philox's output words below 256, whose uniform is 0: (seed, counter, word)
+ZEROS = [(5, 2920362, 1), (6, 2977858, 3)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("seed,counter,word", ZEROS)
+def test_dropout_of_probability_0_is_the_identity(dev, seed, counter, word, dtype):
+    """Where the uniform is 0 too: in whole vectors, value by value, with a residual."""
+    from minitorch_amd import kernels as K
+
+    rng = np.random.default_rng(seed)
+    x, r = (rounded(rng.standard_normal((2, 64)), dtype) for _ in range(2))
+    # (the oracle's mask lacks that value: the case is the one it is meant to be)
+    assert (~ref.keep((2, 64), 0.0, seed, counter - 3)).nonzero()[1].tolist() == [12 + word]
+    for cols in (64, 63):
+        dx = dev_array(x, dtype)[:, :cols]
+        got = K.dropout(dx, 0.0, seed, counter - 3, out=empty((2, 64), dtype)[:, :cols])
+        assert np.array_equal(host(got), x[:, :cols])
+        got = K.dropout(dx, 0.0, seed, counter - 3, residual=dev_array(r, dtype)[:, :cols], out=empty((2, 64), dtype)[:, :cols])
+        assert np.array_equal(host(got), rounded(r + x, dtype)[:, :cols])
+    # and the smallest probabilities drop it, and no other
+    got = host(K.dropout(full((2, 64), 1.0, dtype), 2.0 ** -30, seed, counter - 3))
+    assert np.argwhere(got == 0).tolist() == [[0, 12 + word]]
