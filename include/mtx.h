@@ -861,8 +861,8 @@ int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void* logits, i
 
 /*
  * The vocabulary projection and the softmax cross-entropy (transformer.py:91,
- * layers.py:31-37, loss.py:17-27) with their gradients, without the logits in
- * memory as a whole.  x (n x C, row stride ldx) and w (C x V, strides swc, swv, one
+ * layers.py:31-37, loss.py:17-27) with their gradients, a block of rows'
+ * logits at a time.  x (n x C, row stride ldx) and w (C x V, strides swc, swv, one
  * of them 1: a Linear's weight, or a (V, C) table transposed) are fp32 or bf16,
  * bias fp32 (V) or NULL.  With z = x w + bias:
  *   lse[r] = log sum exp z[r];  row_loss[r] = lse[r] - z[r][labels[r]];
@@ -876,7 +876,12 @@ int mtx_token_logprobs_bwd(int dtype, int64_t rows, int V, const void* logits, i
  * lse -inf, row_loss +inf and, as gradient, its label's own term alone.  Infinities
  * and NaN in x or w give NaN (fp32: in every logit that they meet).
  * The rows are worked through in blocks whose logits (fp32) fill at most logits_bytes
- * (one row at least, 2^18 at most); fewer, larger blocks are faster.  bf16 gradients
+ * (one row at least, 2^18 at most); fewer, larger blocks are faster, and logits that fit are
+ * there all at once.  The workspace holds them and, for bf16 inputs, half as much again for
+ * each bf16 piece of their gradient (two for bf16 gradients, three for fp32 ones), copies of
+ * x and w that the products cannot take as they are, and sums of ranges.  (bf16 without
+ * gradients: 8 bytes for 64 logits alone; small vocabularies: the gradient in place of the
+ * logits, which stay in registers.)  bf16 gradients
  * are products of the logits' gradient to 2^-18 of each entry, fp32 ones of all its 24
  * bits; either way sums are fp32, rounded once.  With grad_dtype MTX_BF16 |
  * MTX_GRAD_ONE_PIECE the logits' gradient is rounded to bf16 first (2^-9 of each entry;

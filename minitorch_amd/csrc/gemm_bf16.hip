@@ -7,7 +7,8 @@
 // one's epilogue runs beside the other's products.
 //
 // (8192, 1024) x (1024, 50021), 839 GFLOP: 0.96 ms with 1.6 GB of fp32 results, 0.80 for
-// the product over 8192 rows, 0.82 for the one over 50021 columns (a library's products of
+// the product over 8192 rows, 0.82 for the one over 50021 columns, of one piece each; 1.6 and
+// 1.5 of two (a library's products of
 // these shapes, with bf16 results: 0.70, 0.84, 0.68 ms).  The matrix cores are 60 % busy
 // (42 % in the first, whose results' way out is what bounds it), at a clock that falls to
 // 1.5 GHz under this load.

@@ -1,5 +1,5 @@
 // A vocabulary projection with its softmax cross entropy and the gradients of
-// both, without keeping the logits.
+// both, a block of rows' logits at a time.
 //
 //   z = x W + b;  lse_n = log sum_v exp z_nv;  l_n = lse_n - z_n[y_n]
 //   loss = 1/M sum_n l_n over the M rows that have a label
@@ -15,8 +15,9 @@
 //   else: the product z, a pass over its rows that puts dz in z's place (fp32) or
 //     beside it as bf16 pieces, the products dx and dW.  fp32 products are those of
 //     mtx_gemm_f32, bf16 ones gemm_bf16's.
-// (8192, 1024) x (1024, 50021) in bf16: z 1.0-1.25 ms, the rows' pass 0.55 (2.5 GB, 4.4
-// TB/s), dx 0.82, dW 0.83-0.92: bound by the products, at 1.0 PFLOP/s.
+// (8192, 1024) x (1024, 50021) in bf16 with bf16 gradients, 5.1 ms: z 0.96-1.1, the rows'
+// pass 0.87 (3.3 GB, 3.8 TB/s), dx 1.5 and dW 1.6 of two pieces each: bound by the products,
+// at 1.0 PFLOP/s.  Of one piece, 3.1 ms: 0.55 (2.5 GB), 0.82 and 0.80.
 #include "gemm_bf16.h"
 #include "narrow_xent.h"
 

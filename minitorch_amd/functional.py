@@ -18,7 +18,7 @@ conv.py:66-95):
                                the device where it is used and never stored
   linear_cross_entropy(x, W, b, labels)
                                a projection and its cross entropy, with the
-                               gradients, without keeping the logits
+                               gradients, a block of rows' logits at a time
 """
 from __future__ import annotations
 
@@ -627,8 +627,10 @@ def linear_cross_entropy(x, weight, bias, labels, logits_bytes=1 << 31):
     that have one: a negative label has none (padding), nor has a device-resident
     one outside the vocabulary.  x (..., C), weight (C, V) (a table's transpose
     too), bias (V,) or None.  Where gradients are wanted they are worked out here,
-    while a block of rows' logits is there (mtx_linear_xent), and the backward
-    scales them by its upstream gradient."""
+    while a block of rows' logits is there, of at most logits_bytes
+    (mtx_linear_xent), and the backward scales them by its upstream gradient.  A row
+    without a label adds 0 times its x to the weight's gradient: x must be finite
+    there too."""
     C, V = weight.shape
     if x.shape[-1] != C:
         raise AssertionError(f"Linear expects last dim {C}, got {x.shape[-1]}")

@@ -1489,17 +1489,18 @@ def _xent_plan(x, w, labels, bias, loss, row_loss, lse, dx, dw, db, logits_bytes
 
 def linear_xent(x, w, labels, bias=None, loss=None, row_loss=None, lse=None, dx=None, dw=None, db=None,
                 logits_bytes: int = 1 << 31, one_piece: bool = False):
-    """Softmax cross-entropy of the logits x @ w + bias, and its gradients, without
-    the logits in memory (mtx_linear_xent).  x (n, C) and w (C, V), contiguous along
+    """Softmax cross-entropy of the logits x @ w + bias, and its gradients, a block of
+    rows' logits at a time (mtx_linear_xent).  x (n, C) and w (C, V), contiguous along
     either axis (a (V, C) table's .t()), fp32 or bf16; labels int64 (n,), one outside
-    [0, V): none (with dw, x must be finite there too); bias fp32 (V,).  Returns (loss (1,): the mean over the rows that
-    have a label, row_loss (n,), lse (n,)), fp32.  dx (n, C), dw (C, V) and db (V,),
-    where given, receive the gradients of loss: fp32, dx and dw also bf16 with bf16
-    inputs.  bf16 gradients are off by the rounding of the result; with one_piece the
+    [0, V): none (with dw, x must be finite there too); bias fp32 (V,).  Returns (loss
+    (1,): the mean over the rows that have a label, row_loss (n,), lse (n,)), fp32.
+    dx (n, C), dw (C, V) and db (V,), where given, receive the gradients of loss: fp32,
+    dx and dw also bf16 with bf16 inputs.  bf16 gradients are off by the rounding of the result; with one_piece the
     logits' gradient is rounded to bf16 too (small vocabularies: not), for less time
     (8192 x 1024, V = 50021: 3.1 ms in place of 5.1, an error of 1.86e-3 of the norm in
-    place of 1.66e-3).  The logits of as many rows as fill logits_bytes are kept at a
-    time.  No output may overlap an input or another output."""
+    place of 1.66e-3).  A block's logits fill at most
+    logits_bytes; beside them bf16 inputs take as much again for bf16 gradients, half
+    of it more for fp32 ones.  No output may overlap an input or another output."""
     if logits_bytes < 1:
         raise ValueError(f"logits_bytes must be positive (got {logits_bytes})")
     n = x.shape[0]

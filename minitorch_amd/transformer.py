@@ -455,7 +455,8 @@ class GPT(Module):
     def loss(self, idx, targets):
         """Mean cross-entropy of the logits after idx (B, T) against targets (B, T)
         -- cross_entropy_loss(model(idx), targets), char_transformer.py:70-77 -- for
-        vocabularies of any size: the logits are never kept (F.linear_cross_entropy)
+        vocabularies of any size: in blocks of rows whose logits fill at most 2 GiB
+        (F.linear_cross_entropy), of which none is kept for the backward,
         and the token table's gradient goes by sorted tokens (F.embedding).
         Negative ids are padding: such a token is embedded as zeros, such a target
         counts nowhere."""

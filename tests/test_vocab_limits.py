@@ -103,3 +103,19 @@ def test_dropout_keep_refusals(over, code, frag):
     rc, msg = call("mtx_dropout_keep", dict(keep=p(16), rows=4, cols=8, ld=8, p=0.5, seed=1, offset=0, sub=0, base=None,
                                             stream=None), over)
     assert rc == code and frag in msg, (rc, msg)
+
+
+@pytest.mark.parametrize("n", [8192, 100000])
+@pytest.mark.parametrize("grads,pieces", [(257, 1), (1, 2), (0, 3)])
+def test_workspace_is_what_the_documents_say(n, grads, pieces):
+    """The logits, half as much again for a piece of their gradient, copies of x and w, a
+    sum of dw where there are several blocks, and the sums of ranges of the last tiles, for
+    these sizes fewer than four tiles of 256 x 128 for each of the 512 places."""
+    C, V = 1024, 50021
+    f = L.lib().mtx_linear_xent_workspace_bytes
+    for logits in (1 << 28, 1 << 31):
+        rows = min(n, logits // (4 * 50048) // 256 * 256)
+        kept = rows * 50048 * 4
+        got = f(1, grads, n, C, V, 0, logits)
+        copies = 2 * (rows + 50048) * C + (4 * C * V if rows < n and grads != 0 else 0)
+        assert kept * (1 + pieces / 2) <= got <= kept * (1 + pieces / 2) + copies + 4 * 512 * 256 * 128 * 4, (got, kept)
