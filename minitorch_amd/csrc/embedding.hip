@@ -65,7 +65,7 @@ __device__ __forceinline__ void store_f(T* __restrict__ p, const float (&f)[N]) 
 // their ids, then their values, are requested before the first is needed.  Bound by
 // memory (32768 rows of 1024 bf16 values, words: 17 us, 67 MB written); where the rows
 // are too few to fill the chip, the columns are dealt out too (5 rows of 1838 fp32
-// values: 3.0 us, 8 by one workgroup).
+// values: 4.7 us a call, 11.5 by one workgroup).
 constexpr int kLookRows = 4;
 template <typename T, typename O, int VEC, int LPR>
 __global__ __launch_bounds__(256) void lookup_kernel(const T* __restrict__ w, int64_t ldw, int64_t V,
@@ -127,7 +127,7 @@ struct SortArgs {
   uint32_t* tokens;  // out: how many they are
   uint32_t* starts;  // [pieces] out: the row of more than a piece that begins there
   // Rows without a token are set to 0 here, while the sorting waits for its memory: of
-  // 50021 x 1024 rows (205 MB) three quarters are, which makes this launch 36 us instead
+  // 50021 x 1024 rows (205 MB) three quarters are, which makes this launch 43 us instead
   // of 16 and the adding up 30 instead of 66.  nullptr: they are left alone
   float* dw;
   int64_t lddw;
@@ -327,8 +327,7 @@ __device__ __forceinline__ void store_row(const GradArgs& a, int64_t v, int c0, 
 // A wave's `rows` table rows from v0 on.  Their tokens follow each other in the sorted
 // order: up to eight tokens' values are requested at once, whichever rows they are
 // for, and a row is stored where its tokens end (one without a token was set to 0 by
-// the sort).  A wave a row, one row's
-// values at a time, took 83 us for 50021 rows of 1024 and 29500 bf16 tokens, this 66.
+// the sort).
 template <typename T, int VEC, int U>
 __device__ __forceinline__ void add_range(const GradArgs& a, int64_t v0, int rows, int c0) {
   const T* g = static_cast<const T*>(a.g);
@@ -502,9 +501,9 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(const GradArgs a, int
 // tokens are found by comparing 64 of them at a time.  Rows of more than kPiece tokens
 // are left to the end: each wave takes a contiguous part of the ids, and the parts' sums
 // are added in order.
-// 300 tokens of 384 fp32 values, a table of 5003 rows (7.7 MB): 7.4 us (9.7 with all of a
-// row's columns by one workgroup; 208 tokens of 2248, 4 rows: 10 and 36); 1339 bf16 tokens of
-// 256, 42338 rows (43 MB): 20, and 27 where every row's tokens were counted by comparing.
+// 300 tokens of 384 fp32 values, a table of 5003 rows (7.7 MB): 5.9 us (7.6 with all of a
+// row's columns by one workgroup; 208 tokens of 2248, 4 rows: 6.3 and 34); 1339 bf16 tokens of
+// 256, 42338 rows (43 MB): 19, and 29 sorted.
 constexpr int kSmallTokens = 4096, kScan = 4;  // groups of ids looked at together
 template <typename T, int VEC, int U>
 __global__ __launch_bounds__(64 * kWaves) void small_kernel(const GradArgs a, int R) {
@@ -751,9 +750,9 @@ Plan plan(int dtype, int64_t n, int64_t V, int C) {
   p.R = (int)std::min<int64_t>((V + 255) / 256, kMaxRows);
   p.sorts = (unsigned)((V + p.R - 1) / p.R);
   // Few tokens, as long as one workgroup may have to read all their rows, 64 vectors or
-  // 256 values of each at a time (1024 tokens of 1856 fp32 values, 9 rows: 8.5 us here, 25
-  // sorted; of 1024, all of one row: 16 and 19; 600 bf16 tokens of 4096, 5003 rows: 25 and
-  // 32)
+  // 256 values of each at a time (1024 tokens of 1856 fp32 values, 9 rows: 8.1 us here, 25
+  // sorted; of 1024, all of one row: 16 and 18; 600 bf16 tokens of 4096, 5003 rows: 26 and
+  // 30)
   p.small = n <= 1024 || (n <= kSmallTokens && n * C * size <= (1 << 20));
   if (p.small) return p;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -800,7 +799,7 @@ int grad(GradArgs a, const Plan& p, char* ws, hipStream_t st) {
   constexpr int kVec = 16 / sizeof(T), kU = sizeof(T) == 4 ? 2 : 1;
   const bool vec = whole(a.g, a.ldg, a.C, kVec, sizeof(T)) && whole(a.dw, a.lddw, a.C, kVec, 4);
   if (p.small) {
-    // columns beside each other too (600 bf16 tokens of 4096, 5003 rows: 25 us with up to
+    // columns beside each other too (600 bf16 tokens of 4096, 5003 rows: 26 us with up to
     // 2048 workgroups, 43 with 512)
     const int cols = vec ? 64 * kVec : 256;
     const dim3 grid(p.sorts, std::min<unsigned>(cdiv(a.C, cols), std::max(1u, 2048 / p.sorts))), block(64 * kWaves);

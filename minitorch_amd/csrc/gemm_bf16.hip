@@ -535,8 +535,8 @@ Plan plan(int M, int N, int K, int pieces, bool stats = false) {
   p.whole = tiles - rest;
   // the number of ranges, of at least 8 stages each, after which the last round ends
   // soonest, in us: 0.5 a stage, 0.05 for a partial tile's way to memory and back, 5 for
-  // the launch that joins them (2 rows, C = 384, over 27453 columns in three pieces: 81 us
-  // in 16 ranges, 33 in 64)
+  // the launch that joins them (linear cross entropy of 2 rows, C = 384, over 27453 columns, dx
+  // in three pieces: 113 us in 16 ranges, 68 in 64)
   p.split = 1;
   double best = 1e30;
   for (int s = 1; rest && !stats && s <= std::min(64, std::max(1, p.ksteps / 8)); ++s) {

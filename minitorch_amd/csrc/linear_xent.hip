@@ -459,12 +459,12 @@ Plan plan(int dtype, int grads, int64_t n, int C, int V, bool bias, int64_t logi
   p.rows32 = (p.rows + 31) / 32 * 32;
   p.narrow = near && narrow_is_faster(dtype, grads >= 0, p.rows, C, V);
   // Below 128 rows the fp32 products leave the matrix cores; above 64 they pay for 128 on
-  // the vector units.  With all gradients 72 rows, C = 1370, V = 37387: 553 us so, 326 as 128
-  // rows; 100, 512, 20001: 141 and 112; but 65, 128, 5003: 48 and 77.
+  // the vector units.  With all gradients 72 rows, C = 1370, V = 37387: 556 us so, 308 as 128
+  // rows; 100, 512, 20001: 138 and 107; but 65, 128, 5003: 48 and 78.
   p.pad = dtype == MTX_F32 && n > 64 && n < 128 && p.rows == n && C >= 128 && (int64_t)C * V >= 1 << 23;
   p.pieces = grads < 0 ? 0 : dtype == MTX_F32 ? -1 : grads == MTX_F32 ? 3 : grads == kOnePiece ? 1 : 2;
-  // (rows of panels behind the last one are set to 0 by workgroups of their own: 2 rows of
-  // 27453 in three pieces 44 us by two workgroups, 14 by 32)
+  // (rows of panels behind the last one are set to 0 by workgroups of their own: 2 rows, C =
+  // 384, V = 27453, bf16 with fp32 dx: 99 us by two workgroups, 68 by 32)
   p.wgs = row_wgs(p.pieces > 0 ? (int)p.rows32 : p.rows, V);
   size_t at = 256;  // 1 / labels
   p.z = at;  // without gradients bf16 logits are never stored: their statistics are

@@ -399,7 +399,8 @@ _DROPOUT_RNG = {"mode": "host", "seed": 0, "offset": 0}
 
 def set_attention_dropout_rng(mode: str = "host", seed: int = 0) -> None:
     """Choose where attention dropout masks come from ("host" or "device");
-    "device" restarts the Philox stream at (seed, offset 0)."""
+    "device" restarts the Philox stream at (seed, offset 0).  The masks of modules
+    with dropout_rng="device" come from F.dropout's generator instead."""
     if mode not in ("host", "device"):
         raise ValueError(f"unknown dropout RNG mode {mode!r}")
     _DROPOUT_RNG.update(mode=mode, seed=int(seed), offset=0)

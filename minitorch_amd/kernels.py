@@ -88,9 +88,13 @@ def dropout_keep_philox(shape, p: float, seed: int, offset: int, out=None, subse
     added to offset when the kernel runs.  Returns (mask, next offset)."""
     B, H, Tq, Tk = (int(x) for x in shape)
     ld = keep_ld(Tk)
+    if base is not None:
+        _on_device(base)
+        _vector("base", _spec(base), 1, "int64")
     if out is None:
         out = dev.empty_buf((B, H, Tq, ld), "uint8").fill_(0)
     rows = B * H * Tq
+    _int32(Tk=Tk)
     L.call("mtx_dropout_keep", L.ptr(out), rows, Tk, ld, float(p), int(seed) & (2**64 - 1),
            int(offset) & (2**64 - 1), int(subsequence) & (2**32 - 1), _ptr(base), L.stream_handle())
     return out, offset + (rows * Tk + 3) // 4

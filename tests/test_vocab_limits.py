@@ -119,3 +119,11 @@ def test_workspace_is_what_the_documents_say(n, grads, pieces):
         got = f(1, grads, n, C, V, 0, logits)
         copies = 2 * (rows + 50048) * C + (4 * C * V if rows < n and grads != 0 else 0)
         assert kept * (1 + pieces / 2) <= got <= kept * (1 + pieces / 2) + copies + 4 * 512 * 256 * 128 * 4, (got, kept)
+
+
+@pytest.mark.parametrize("base,frag", [(Fake((1,), "int32"), "base"), (Fake((2,), "int64"), "base")])
+def test_keep_mask_wrapper_refuses(monkeypatch, base, frag):
+    K = _kernels(monkeypatch)
+    monkeypatch.setattr(Fake, "fill_", lambda self, value: self, raising=False)
+    with pytest.raises(ValueError, match=frag):
+        K.dropout_keep_philox((1, 2, 3, 4), 0.5, 1, 0, base=base)
