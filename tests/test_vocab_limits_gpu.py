@@ -229,3 +229,12 @@ def test_dropout_of_probability_0_is_the_identity(dev, seed, counter, word, dtyp
     # and the smallest probabilities drop it, and no other
     got = host(K.dropout(full((2, 64), 1.0, dtype), 2.0 ** -30, seed, counter - 3))
     assert np.argwhere(got == 0).tolist() == [[0, 12 + word]]
+
+
+@pytest.mark.parametrize("dtype,out", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("n,C,V,rows", [(5, 40, 65, 1), (22, 40, 65, 7), (530, 70, 20, 256), (262144 + 77, 8, 20, 1 << 30)])
+def test_linear_xent_small_vocabularies_in_blocks_of_few_rows(dev, n, C, V, rows, dtype, out):
+    """Blocks of one row, of a few, of as many as there may be (2^18)."""
+    from test_vocab_gpu import check_xent
+
+    check_xent(n, C, V, dtype, out, tied=n % 2 == 1, logits_bytes=rows * (-(-V // 32) * 32) * 4)
